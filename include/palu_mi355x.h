@@ -21,7 +21,7 @@
 extern "C" {
 #endif
 
-#define PALU_ABI_VERSION 16
+#define PALU_ABI_VERSION 17
 
 #define PALU_OK 0
 #define PALU_EINVAL 1       /* arguments outside the op's envelope */
@@ -414,6 +414,80 @@ int palu_prefill_attention(const void* qkv, long long ld, int users, int seq, in
 
 /* Workspace bytes of palu_prefill_attention (0 for invalid shapes): the rebuilt keys and values as operand tiles. */
 size_t palu_prefill_workspace_bytes(int users, int seq, int n_heads, int n_kv, int n_groups, int r_k, int r_v);
+
+/* ---- Packed batches over page pools -------------------------------------------------------------------
+ * Sequences of different lengths in one call: the new rows of `batch` sequences lie one after another, sequence b's at
+ * cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (int32 [batch + 1], device memory, not decreasing, from 0); rows past
+ * cu_seqlens[batch] belong to no sequence: their outputs keep what they hold. Pages, tables and layouts as for
+ * palu_flash_decode_paged. No counterparts in the reference (its caches are contiguous, its prefill one prompt). */
+
+/* Causal attention of packed sequences over full K and V, each over its own rows: row i of a sequence sees its rows 0 .. i.
+ *   q [rows][n_q][128], k [rows][n_kv][128], v [rows][n_kv][head_dim_v] bf16, rows and heads at the element strides given
+ *   (multiples of 8; head_dim_v a multiple of 16 up to 128); out [rows][n_q][head_dim_v] bf16, dense, not overlapping them.
+ * Head h reads KV head h / (n_q / n_kv). fp32 scores, statistics and sums; probabilities rounded to bf16 for their
+ * product with V. A NaN or infinity in K or V reaches the rows that see it and no others. workspace:
+ * palu_flash_prefill_workspace_bytes with max_keys = rows; calls that share one must be ordered on one stream. */
+int palu_flash_prefill(const void* q, long long q_row_stride, long long q_head_stride, const void* k, long long k_row_stride,
+                       long long k_head_stride, const void* v, long long v_row_stride, long long v_head_stride,
+                       const int32_t* cu_seqlens, void* out, float scale, int rows, int batch, int n_q, int n_kv,
+                       int head_dim_v, void* workspace, size_t workspace_bytes, palu_stream_t stream);
+
+/* The same over page pools k_pages [num_pages][n_kv][page_size][128], v_pages [..][head_dim_v]: row i of sequence b stands
+ * at position start_pos[b] + i (start_pos NULL: i) and sees positions 0 .. that of the sequence's pages, which hold the new
+ * rows' keys and values already (palu_latent_fill_paged). A row at a negative position sees nothing and gets zeros; one past
+ * the table's max_pages_per_seq * page_size positions sees those. Page ids are clamped into the pool. workspace as
+ * above with max_keys = max_pages_per_seq * page_size: the keys of few rows are split among workgroups. */
+int palu_flash_prefill_paged(const void* q, long long q_row_stride, long long q_head_stride, const void* k_pages,
+                             const void* v_pages, const int32_t* cu_seqlens, const int32_t* start_pos,
+                             const int32_t* page_table, void* out, float scale, int rows, int batch, int n_q, int n_kv,
+                             int num_pages, int page_size, int max_pages_per_seq, int head_dim_v, int cache_layout,
+                             void* workspace, size_t workspace_bytes, palu_stream_t stream);
+
+/* Workspace bytes of palu_flash_prefill / _paged (0 when no keys are split, and for invalid shapes). */
+size_t palu_flash_prefill_workspace_bytes(int rows, int batch, int n_q, int n_kv, int max_keys, int head_dim_v);
+
+/* Packed rows into a page pool [num_pages][n_groups][page_size][width] (cache_layout PALU_LAYOUT_ROWS, _TILED or _TILED_V):
+ * row i of sequence b to position start_pos[b] + i (start_pos NULL: i), from rows + (cu_seqlens[b] + i) * row_stride + g *
+ * group_stride (multiples of 8). Positions outside the table and page ids outside the pool are skipped; every other
+ * position of the pool keeps what it holds. width: a multiple of 8 (16 when tiled) up to 512. */
+int palu_latent_fill_paged(void* cache_pages, const void* rows, long long row_stride, long long group_stride,
+                           const int32_t* cu_seqlens, const int32_t* start_pos, const int32_t* page_table, int n_rows,
+                           int batch, int n_groups, int num_pages, int page_size, int max_pages_per_seq, int width,
+                           int cache_layout, palu_stream_t stream);
+
+/* Forks, ends, cuts and grows the rows of a page table in one step. Row b becomes a copy of row parents[b] as it was
+ * (parents NULL: of itself; an index outside the batch: of an empty row), cut or grown to new_lengths[b] positions (NULL: as
+ * long as the parent), at most max_pages_per_seq * page_size. A page is in use where one of a row's first ceil(length /
+ * page_size) entries names it; nothing else is kept, so a row of length 0 holds nothing. Whole kept pages are shared. The
+ * page that a row writes next, which its kept positions end inside, becomes its own: of the rows that would write a page the
+ * first keeps it, unless another row holds it whole; the others get a copy of it in every pool. New pages are the
+ * lowest free ones in the order of rows and slots; where they run out, lengths_out[b] is what the row's pages hold.
+ * Entries past a row's pages become -1. Ids outside the pool are kept as entries and name no page.
+ *   page_table, page_table_out [batch][max_pages_per_seq], lengths, lengths_out [batch] int32: separate memory
+ *   pools: n_pools device pointers (host array) to pools of num_pages pages of page_bytes[i] bytes (a multiple of 16)
+ * At most 4096 rows; the bits of num_pages pages and the rows' data fit 156 KB of LDS (a million pages for small batches).
+ * workspace: palu_pages_workspace_bytes, 16-byte aligned. */
+int palu_pages_update(const int32_t* page_table, const int32_t* lengths, const int32_t* parents, const int32_t* new_lengths,
+                      int32_t* page_table_out, int32_t* lengths_out, void* const* pools, const long long* page_bytes,
+                      int n_pools, int batch, int num_pages, int page_size, int max_pages_per_seq, void* workspace,
+                      size_t workspace_bytes, palu_stream_t stream);
+
+/* Moves the pages in use to the front of every pool: with n of them, those at n or above go, in order, to the free ones
+ * below n. page_table_out is the table over the new places (entries past a row's pages -1), n_live [1] int32 receives n. */
+int palu_pages_compact(const int32_t* page_table, const int32_t* lengths, int32_t* page_table_out, int32_t* n_live,
+                       void* const* pools, const long long* page_bytes, int n_pools, int batch, int num_pages, int page_size,
+                       int max_pages_per_seq, void* workspace, size_t workspace_bytes, palu_stream_t stream);
+
+/* Workspace bytes of palu_pages_update and palu_pages_compact (0 for invalid counts). */
+size_t palu_pages_workspace_bytes(int batch, int num_pages);
+
+/* Log probabilities of row r's token tokens[r] under softmax(logits[r]), the entropy of that distribution in nats, and its
+ * `top` largest entries (0 .. 64, at most n): log probabilities and ids, the lower id first among equal logits, NaN above
+ * every number. logits [rows][n], rows ld elements apart, fp32 or bf16 (PALU_DTYPE_*). A negative token (padding) gets 0,
+ * one past the row NaN; a row with a NaN or +infinity, or of -infinity alone, gives NaN. The reference's generation loop
+ * (generate.py:53-62) has the greedy pick only. */
+int palu_token_logprobs(const void* logits, long long ld, int dtype, const int64_t* tokens, int rows, int n, int top,
+                        float* logprob, float* entropy, float* top_logprobs, int64_t* top_ids, palu_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,131 @@
+"""Refusals of the packed-batch entry points (prompts' attention, page fills, page tables, token log probabilities) without a GPU:
+the C-ABI checks its arguments before any launch, the Python layer before any call."""
+import ctypes
+
+import pytest
+import torch
+
+from palu_tt import _build, _native, decoder_ops, fused
+from palu_tt.pages import PagePools
+
+P = 4096                                                     # a 16-byte aligned address that no refused call reads
+
+
+@pytest.fixture(scope="module")
+def lib():
+    if not _build.library_path().exists():
+        _build.build_native()
+    return _native.load()
+
+
+def _refused(lib, rc, code, what):
+    assert rc == code and what in lib.palu_last_error().decode(), (rc, lib.palu_last_error().decode())
+
+
+@pytest.mark.parametrize("kw,code,what", [
+    (dict(q=None), _native.PALU_EINVAL, "null"), (dict(cu=None), _native.PALU_EINVAL, "null"),
+    (dict(rows=0), _native.PALU_EINVAL, "must be positive"), (dict(batch=-1), _native.PALU_EINVAL, "must be positive"),
+    (dict(n_q=6, n_kv=4), _native.PALU_EINVAL, "multiple of the KV head"), (dict(dv=24), _native.PALU_EUNSUPPORTED, "head_dim_v"),
+    (dict(dv=144), _native.PALU_EUNSUPPORTED, "head_dim_v"), (dict(rows=1 << 28, n_q=8), _native.PALU_EUNSUPPORTED, "grid"),
+    (dict(q_st=1028), _native.PALU_EINVAL, "strides"), (dict(v_sh=-8), _native.PALU_EINVAL, "strides"),
+    (dict(k=P + 8), _native.PALU_EINVAL, "16-byte"), (dict(out=P + 2), _native.PALU_EINVAL, "16-byte")])
+def test_flash_prefill_refusals(lib, kw, code, what):
+    a = dict(q=P, q_st=1024, q_sh=128, k=P, k_st=256, k_sh=128, v=P, v_st=128, v_sh=64, cu=P, out=P, scale=0.1, rows=5, batch=1, n_q=8,
+             n_kv=2, dv=64, ws=None, bytes=0, stream=None)
+    a.update(kw)
+    _refused(lib, lib.palu_flash_prefill(*a.values()), code, what)
+
+
+@pytest.mark.parametrize("kw,code,what", [
+    (dict(pt=None), _native.PALU_EINVAL, "page_table is null"), (dict(page=48), _native.PALU_EINVAL, "power of two"),
+    (dict(pages=0), _native.PALU_EINVAL, "num_pages"), (dict(slots=2048), _native.PALU_EUNSUPPORTED, "65536"),
+    (dict(layout=2), _native.PALU_EINVAL, "cache layout"), (dict(layout=3), _native.PALU_EINVAL, "cache layout"),
+    (dict(v=None), _native.PALU_EINVAL, "null"), (dict(dv=40), _native.PALU_EUNSUPPORTED, "head_dim_v"),
+    (dict(q_sh=4), _native.PALU_EINVAL, "strides"), (dict(slots=512), _native.PALU_EINVAL, "workspace"),
+    (dict(slots=512, ws=P + 8, bytes=1 << 40), _native.PALU_EINVAL, "workspace"),
+    (dict(slots=512, ws=P, bytes=64), _native.PALU_EINVAL, "workspace")])
+def test_flash_prefill_paged_refusals(lib, kw, code, what):
+    a = dict(q=P, q_st=1024, q_sh=128, k=P, v=P, cu=P, start=P, pt=P, out=P, scale=0.1, rows=5, batch=1, n_q=8, n_kv=2, pages=9, page=64,
+             slots=4, dv=64, layout=0, ws=None, bytes=0, stream=None)
+    a.update(kw)
+    _refused(lib, lib.palu_flash_prefill_paged(*a.values()), code, what)
+
+
+def test_flash_prefill_workspace(lib):
+    """None where the tiles fill the chip or the keys are few; a slot per tile, KV head and split else."""
+    f = lib.palu_flash_prefill_workspace_bytes
+    assert f(8192, 1, 32, 8, 8192, 128) == 0 and f(24, 1, 32, 8, 24, 128) == 0 and f(1, 1, 32, 8, 256, 128) == 0
+    need = f(1, 1, 32, 8, 32768, 128)
+    assert need > 0 and need % (8 * 128 * 130 * 4) == 0
+    assert f(0, 1, 32, 8, 100, 128) == 0 and f(5, 1, 7, 2, 100, 128) == 0 and f(5, 1, 8, 2, -1, 128) == 0
+
+
+@pytest.mark.parametrize("kw,code,what", [
+    (dict(cache=None), _native.PALU_EINVAL, "null"), (dict(pt=None), _native.PALU_EINVAL, "page_table"),
+    (dict(n=0), _native.PALU_EINVAL, "must be positive"), (dict(groups=0), _native.PALU_EINVAL, "must be positive"),
+    (dict(layout=3), _native.PALU_EINVAL, "cache layout"), (dict(width=20), _native.PALU_EINVAL, "multiple of 8"),
+    (dict(width=24, layout=1), _native.PALU_EINVAL, "multiple of 16"), (dict(width=520), _native.PALU_EINVAL, "up to 512"),
+    (dict(st=100), _native.PALU_EINVAL, "strides"), (dict(rows=P + 4), _native.PALU_EINVAL, "16-byte"),
+    (dict(page=16), _native.PALU_EINVAL, "power of two"), (dict(groups=70000), _native.PALU_EUNSUPPORTED, "grid")])
+def test_fill_refusals(lib, kw, code, what):
+    a = dict(cache=P, rows=P, st=128, sg=64, cu=P, start=None, pt=P, n=5, batch=1, groups=2, pages=9, page=64, slots=4, width=64, layout=0,
+             stream=None)
+    a.update(kw)
+    _refused(lib, lib.palu_latent_fill_paged(*a.values()), code, what)
+
+
+def _pools(n, ptr=P, size=4096):
+    return (ctypes.c_void_p * n)(*[ptr] * n), (ctypes.c_longlong * n)(*[size] * n)
+
+
+@pytest.mark.parametrize("kw,code,what", [
+    (dict(table=None), _native.PALU_EINVAL, "null"), (dict(out=P), _native.PALU_EINVAL, "old one's memory"),
+    (dict(len_out=2 * P), _native.PALU_EINVAL, "memory of its own"), (dict(batch=0), _native.PALU_EINVAL, "batch"),
+    (dict(pages=0), _native.PALU_EINVAL, "num_pages"), (dict(page=33), _native.PALU_EINVAL, "power of two"),
+    (dict(slots=4096), _native.PALU_EUNSUPPORTED, "65536"), (dict(ws=None), _native.PALU_EINVAL, "workspace"),
+    (dict(bytes=91), _native.PALU_EINVAL, "workspace"), (dict(batch=5000), _native.PALU_EUNSUPPORTED, "4096"),
+    (dict(pages=1_400_000), _native.PALU_EUNSUPPORTED, "LDS"), (dict(pools=_pools(2, P + 4)), _native.PALU_EINVAL, "pool 0"),
+    (dict(pools=_pools(1, P, 40)), _native.PALU_EINVAL, "pool 0"), (dict(pools=(None, None)), _native.PALU_EINVAL, "pools")])
+def test_update_refusals(lib, kw, code, what):
+    a = dict(table=P, len=2 * P, parents=None, new=None, out=3 * P, len_out=4 * P, pools=_pools(2), batch=3, pages=9, page=64, slots=4,
+             ws=P, bytes=1 << 30)
+    a.update(kw)
+    pools, sizes = a.pop("pools")
+    rc = lib.palu_pages_update(a["table"], a["len"], None, None, a["out"], a["len_out"], pools, sizes, 2 if pools is None else len(pools),
+                               a["batch"], a["pages"], a["page"], a["slots"], a["ws"], a["bytes"], None)
+    _refused(lib, rc, code, what)
+
+
+def test_compact_refusals(lib):
+    pools, sizes = _pools(1)
+    call = lambda table=P, n=5 * P, pages=9, ws=P: lib.palu_pages_compact(table, 2 * P, 3 * P, n, pools, sizes, 1, 3, pages, 64, 4, ws,
+                                                                          1 << 30, None)
+    _refused(lib, call(table=None), _native.PALU_EINVAL, "null")
+    _refused(lib, call(n=None), _native.PALU_EINVAL, "null")
+    _refused(lib, call(ws=None), _native.PALU_EINVAL, "workspace")
+    _refused(lib, call(pages=1_400_000), _native.PALU_EUNSUPPORTED, "LDS")
+    assert lib.palu_pages_workspace_bytes(0, 5) == 0 and lib.palu_pages_workspace_bytes(3, 100) >= 16 + 4 * (2 * 51 + 100)
+
+
+@pytest.mark.parametrize("kw,code,what", [
+    (dict(x=None), _native.PALU_EINVAL, "null"), (dict(top_id=None), _native.PALU_EINVAL, "null"), (dict(rows=0), _native.PALU_EINVAL, "positive"),
+    (dict(n=0), _native.PALU_EINVAL, "positive"), (dict(dtype=2), _native.PALU_EINVAL, "dtype"), (dict(top=65), _native.PALU_EINVAL, "top"),
+    (dict(n=3, top=4), _native.PALU_EINVAL, "top"), (dict(top=-1), _native.PALU_EINVAL, "top"),
+    (dict(n=(1 << 30) + 1), _native.PALU_EUNSUPPORTED, "logits")])
+def test_token_logprobs_refusals(lib, kw, code, what):
+    a = dict(x=P, ld=100, dtype=1, tokens=P, rows=2, n=100, top=5, lp=P, ent=P, top_lp=P, top_id=P, stream=None)
+    a.update(kw)
+    _refused(lib, lib.palu_token_logprobs(*a.values()), code, what)
+
+
+def test_cpu_tensors_are_refused():
+    t = lambda *s: torch.zeros(*s, dtype=torch.bfloat16)
+    ints = lambda x: torch.tensor(x, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="GPU"):
+        fused.flash_prefill(t(4, 4, 128), t(4, 2, 128), t(4, 2, 64), ints([0, 4]))
+    with pytest.raises(RuntimeError, match="GPU"):
+        fused.paged_fill_cache(t(3, 2, 32, 64), t(4, 2, 64), ints([0, 4]), ints([[0]]))
+    with pytest.raises(RuntimeError, match="GPU"):
+        PagePools([t(3, 2, 32, 64)])
+    with pytest.raises(RuntimeError, match="GPU"):
+        decoder_ops.token_logprobs(t(4, 10), ints([0, 1, 2, 3]))

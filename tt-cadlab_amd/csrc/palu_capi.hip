@@ -23,21 +23,6 @@ unsigned long long next_epoch() {
   return CHUNK_TAG | (((calls.fetch_add(1) + 1) & 0xFFFFFFFFull) << 16);
 }
 
-}  // namespace palu
-
-namespace {
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
-int check_layout(int layout, int seq_len, const char* who) {
-  if (layout != PALU_LAYOUT_ROWS && layout != PALU_LAYOUT_TILED)
-    return fail(PALU_EINVAL, "%s: cache layout must be PALU_LAYOUT_ROWS or PALU_LAYOUT_TILED, got %d", who, layout);
-  if (layout == PALU_LAYOUT_TILED && seq_len % 32 != 0)
-    return fail(PALU_EINVAL, "%s: a tiled cache holds whole 32-position blocks; seq_len %d is not a multiple of 32", who,
-                seq_len);
-  return PALU_OK;
-}
-
 // Paged pools: page_size a power of two in 32..4096 (whole 32-position blocks per page), at least one
 // page, a page table of max_pages_per_seq entries per row. Returns log2(page_size / 32) in *shift.
 int check_pages(const int32_t* page_table, int num_pages, int page_size, int max_pages, int* shift, const char* who) {
@@ -53,6 +38,21 @@ int check_pages(const int32_t* page_table, int num_pages, int page_size, int max
   int s = 0;
   while ((32 << s) < page_size) ++s;
   *shift = s;
+  return PALU_OK;
+}
+
+}  // namespace palu
+
+namespace {
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+int check_layout(int layout, int seq_len, const char* who) {
+  if (layout != PALU_LAYOUT_ROWS && layout != PALU_LAYOUT_TILED)
+    return fail(PALU_EINVAL, "%s: cache layout must be PALU_LAYOUT_ROWS or PALU_LAYOUT_TILED, got %d", who, layout);
+  if (layout == PALU_LAYOUT_TILED && seq_len % 32 != 0)
+    return fail(PALU_EINVAL, "%s: a tiled cache holds whole 32-position blocks; seq_len %d is not a multiple of 32", who,
+                seq_len);
   return PALU_OK;
 }
 

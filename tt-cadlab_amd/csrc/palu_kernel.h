@@ -150,6 +150,9 @@ int flash_setup(DecodeArgs& a, const void* q, const void* k, const void* v, cons
                 float scale, int batch, int n_q, int n_kv, int seq_len, int head_dim_v, int out_dtype, int cache_layout,
                 int deterministic, void* workspace, size_t workspace_bytes, const char* who);
 
+// Checks a page table and its pool; log2(page_size / 32) in *shift (defined in palu_capi.hip).
+int check_pages(const int32_t* page_table, int num_pages, int page_size, int max_pages, int* shift, const char* who);
+
 // Waves per workgroup: 8 (two per SIMD) where the kernel fits 256 registers, else 4 (one per SIMD,
 // which lets the compiler use the full 512-entry register file instead of spilling).
 template <int RK, int RV, bool KFULL, bool TILED>

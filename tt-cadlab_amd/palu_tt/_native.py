@@ -15,7 +15,7 @@ from palu_tt._build import library_path
 PALU_OK, PALU_EINVAL, PALU_EUNSUPPORTED, PALU_EHIP = 0, 1, 2, 3
 DTYPE_F32, DTYPE_BF16 = 0, 1
 OUT_TILED_ROWS = 0x100      # PALU_OUT_TILED_ROWS, OR'ed into palu_sdpa_decode's out_dtype
-ABI_VERSION = 16
+ABI_VERSION = 17
 LAYOUT_ROWS, LAYOUT_TILED, LAYOUT_TILED_V, LAYOUT_TILED_GROUPED = 0, 1, 2, 3
 
 _vp, _i, _f, _sz, _ll = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_size_t, ctypes.c_longlong
@@ -62,6 +62,15 @@ _SIGNATURES = {
     "palu_naive_decode": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _f, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _vp,
                                _sz, _vp]),
     "palu_naive_workspace_bytes": (_sz, [_i, _i, _i, _i]),
+    "palu_flash_prefill": (_i, [_vp, _ll, _ll, _vp, _ll, _ll, _vp, _ll, _ll, _vp, _vp, _f, _i, _i, _i, _i, _i, _vp, _sz, _vp]),
+    "palu_flash_prefill_paged": (_i, [_vp, _ll, _ll, _vp, _vp, _vp, _vp, _vp, _vp, _f, _i, _i, _i, _i, _i, _i, _i, _i, _i,
+                                      _vp, _sz, _vp]),
+    "palu_flash_prefill_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i]),
+    "palu_latent_fill_paged": (_i, [_vp, _vp, _ll, _ll, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _vp]),
+    "palu_pages_update": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _sz, _vp]),
+    "palu_pages_compact": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _sz, _vp]),
+    "palu_pages_workspace_bytes": (_sz, [_i, _i]),
+    "palu_token_logprobs": (_i, [_vp, _ll, _i, _vp, _i, _i, _i, _vp, _vp, _vp, _vp, _vp]),
     "palu_prefill_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i]),
 }
 EXPORTED = tuple(_SIGNATURES)
@@ -102,6 +111,16 @@ def check(status: int) -> None:
 
 def ptr(t) -> int:
     return 0 if t is None else t.data_ptr()
+
+
+def launch(name: str, device, *args) -> None:
+    """check(palu_<name>(*args, the current stream of `device`)) with that device current."""
+    fn = getattr(load(), "palu_" + name)
+    if torch._C._cuda_getDevice() == device.index:
+        check(fn(*args, stream_handle(device)))
+    else:
+        with torch.cuda.device(device):
+            check(fn(*args, stream_handle(device)))
 
 
 def stream_handle(device) -> int:

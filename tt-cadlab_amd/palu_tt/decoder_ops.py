@@ -78,6 +78,35 @@ def argmax_rows(x: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Te
     return out
 
 
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0):
+    """(logprob [rows], entropy [rows], top_logprobs [rows, top], top_ids [rows, top]) of logits [rows, n] (bf16 or fp32, a
+    row-strided view): the log probability of each row's token tokens [rows] (integers; a negative one, padding, gets 0, one
+    past the row NaN), the entropy of the row's distribution in nats, and its `top` (0 .. 64) most probable entries, the lower id
+    first among equal ones. fp32 and int64; computed in fp32."""
+    if not (isinstance(logits, torch.Tensor) and logits.is_cuda and logits.dtype in (torch.bfloat16, torch.float32)):
+        raise RuntimeError("logits must be a bf16 or fp32 tensor on the GPU")
+    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise RuntimeError("logits must be a row-strided [rows, n] view")
+    rows, n = logits.shape
+    dev = logits.device
+    if not isinstance(tokens, torch.Tensor) or tokens.is_floating_point() or tokens.shape != (rows,):
+        raise RuntimeError(f"tokens must be an integer tensor [{rows}]")
+    if n < 1 or not 0 <= top <= min(64, n):
+        raise RuntimeError(f"top must be in 0 .. {min(64, n)}, got {top}")
+    if torch.is_grad_enabled() and logits.requires_grad:
+        raise RuntimeError("token_logprobs has no backward pass: call it under torch.no_grad()")
+    t = tokens if tokens.device == dev and tokens.dtype == torch.int64 else tokens.to(device=dev, dtype=torch.int64)
+    t = t.contiguous()
+    lp, ent = torch.empty(2, rows, dtype=torch.float32, device=dev)
+    top_lp = torch.empty(rows, top, dtype=torch.float32, device=dev)
+    ids = torch.empty(rows, top, dtype=torch.int64, device=dev)
+    if rows:
+        _native.launch("token_logprobs", dev, logits.data_ptr(), logits.stride(0) if rows > 1 else n,
+                       _native.DTYPE_BF16 if logits.dtype == torch.bfloat16 else _native.DTYPE_F32, t.data_ptr(), rows, n, top,
+                       lp.data_ptr(), ent.data_ptr(), top_lp.data_ptr(), ids.data_ptr())
+    return lp, ent, top_lp, ids
+
+
 def swiglu(gu: torch.Tensor, out: Optional[torch.Tensor] = None, tiled_out: bool = False) -> torch.Tensor:
     """silu(g) * u for gu = [g | u] of shape [rows, 2 ffn]; returns [rows, ffn], or with tiled_out a
     [64, ffn] buffer in the tiled activation layout (rows <= 64)."""

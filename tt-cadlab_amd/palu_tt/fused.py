@@ -470,6 +470,124 @@ def naive_decode(q, k_latent, u_k, cos, sin, v_latent, cur_pos_tensor, recon_len
     return out
 
 
+def _seq_ints(t, name: str, n: Optional[int], device) -> torch.Tensor:
+    """A contiguous int32 vector on the device (of n entries), converted where it is another integer type or elsewhere."""
+    if not isinstance(t, torch.Tensor) or t.is_floating_point() or t.dim() != 1 or (n is not None and t.numel() != n):
+        raise RuntimeError(f"{name} must be an integer tensor [{'B + 1' if n is None else n}]")
+    if t.device != device or t.dtype != torch.int32:
+        t = t.to(device=device, dtype=torch.int32)
+    return t.contiguous()
+
+
+def _strided_rows(t, name: str, width: Optional[int], device=None):
+    """(row stride, head stride) of a packed [rows, heads, width] bf16 view: heads of contiguous elements, 16-byte aligned."""
+    if not (isinstance(t, torch.Tensor) and t.dim() == 3 and (width is None or t.shape[2] == width)):
+        raise RuntimeError(f"{name} must be [rows, heads, {width or 'width'}], got {tuple(getattr(t, 'shape', ()))}")
+    if not t.is_cuda or t.dtype != torch.bfloat16 or (device is not None and t.device != device):
+        raise RuntimeError(f"{name} must be a torch.bfloat16 tensor on {device or 'the GPU'}, got {t.dtype} on {t.device}")
+    st = t.stride(0) if t.shape[0] > 1 else 0
+    sh = t.stride(1) if t.shape[1] > 1 else 0
+    if (t.stride(2) != 1 and t.shape[2] > 1) or st % 8 or sh % 8 or t.data_ptr() % 16:
+        raise RuntimeError(f"{name} must have contiguous heads, row and head strides in multiples of 8, and start 16-byte aligned")
+    return st, sh
+
+
+def _no_grad_wanted(what: str, *tensors) -> None:
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad()")
+
+
+def flash_prefill(q, k, v, cu_seqlens, *, scale=None, head_dim_v=None, out=None, workspace=None, page_table_tensor=None,
+                  start_pos=None) -> torch.Tensor:
+    """Causal attention of packed sequences of different lengths over full rotated K and V, the prompts' counterpart of
+    flash_decode. q [T, n_q, 128]: sequence b's new rows are cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (int32 [B + 1] on the
+    device). Without page_table_tensor, k [T, n_kv, 128] and v [T, n_kv, head_dim_v] are the same rows' (q, k and v may be
+    column views of one projection's rows). With it, k and v are page pools [n_pages, n_kv, page_size, width] (tensors or
+    LatentCache) that hold the new rows already (paged_update_cache, paged_fill_cache), and row i of sequence b
+    stands at position start_pos[b] + i (int32 [B]; None: i) behind the positions cached before. Query head h reads KV head
+    h // (n_q // n_kv). head_dim_v: multiples of 16 up to 128. Returns [T, n_q, head_dim_v] bf16; rows past
+    cu_seqlens[B] are not written (``out``, which must not overlap the inputs, keeps what it held there). workspace: a uint8
+    device tensor of palu_flash_prefill_workspace_bytes(...) bytes, else one from torch's caching allocator where needed."""
+    q_st, q_sh = _strided_rows(q, "q", HEAD_DIM)
+    dev = q.device
+    T, n_q = q.shape[:2]
+    cu = _seq_ints(cu_seqlens, "cu_seqlens", None, dev)
+    B = cu.numel() - 1
+    if B < 1:
+        raise RuntimeError("cu_seqlens must hold at least one sequence")
+    _no_grad_wanted("flash_prefill", q, *(t for t in (k, v) if isinstance(t, torch.Tensor)))
+    if page_table_tensor is None:
+        if start_pos is not None:
+            raise RuntimeError("start_pos needs page_table_tensor: packed rows attend to themselves from position 0")
+        k_st, k_sh = _strided_rows(k, "k", HEAD_DIM, dev)
+        v_st, v_sh = _strided_rows(v, "v", None, dev)
+        n_kv, dv = v.shape[1:]
+        if k.shape[:2] != (T, n_kv) or v.shape[0] != T:
+            raise RuntimeError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must have the {T} rows of q and the same heads")
+        max_keys = T
+    else:
+        k_store, k_shape, layout = _cache_arg(k, "k", dev, "k")
+        v_store, v_shape, v_layout = _cache_arg(v, "v", dev, "v")
+        if layout != v_layout or layout == _native.LAYOUT_TILED_GROUPED:
+            raise RuntimeError("k and v must use the same cache layout (row-major or LatentCache pools)")
+        n_pages, n_kv, page_size, hd = k_shape
+        if hd != HEAD_DIM or tuple(v_shape[:3]) != (n_pages, n_kv, page_size):
+            raise RuntimeError(f"k must be a pool [n_pages, n_kv, page_size, {HEAD_DIM}] and v match it, got {k_shape}, {v_shape}")
+        dv = v_shape[3]
+        pt = _page_table(page_table_tensor, B, dev)
+        start = None if start_pos is None else _seq_ints(start_pos, "start_pos", B, dev)
+        max_keys = pt.shape[1] * page_size
+    if head_dim_v is not None and int(head_dim_v) != dv:
+        raise RuntimeError(f"head_dim_v {head_dim_v} != V width {dv}")
+    if out is None:
+        out = torch.empty(T, n_q, dv, dtype=torch.bfloat16, device=dev)
+    else:
+        _as_dev(out, "out", torch.bfloat16, dev)
+        if tuple(out.shape) != (T, n_q, dv):
+            raise RuntimeError(f"out must be [{T}, {n_q}, {dv}]")
+    if T == 0:
+        return out
+    need = _native.load().palu_flash_prefill_workspace_bytes(T, B, n_q, n_kv, max_keys, dv)
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    elif not (workspace.device == dev and workspace.numel() * workspace.element_size() >= need):
+        raise RuntimeError(f"workspace must hold {need} bytes on {dev}")
+    sc = float(HEAD_DIM ** -0.5 if scale is None else scale)
+    if page_table_tensor is None:
+        _native.launch("flash_prefill", dev, q.data_ptr(), q_st, q_sh, k.data_ptr(), k_st, k_sh, v.data_ptr(), v_st, v_sh,
+                       cu.data_ptr(), out.data_ptr(), sc, T, B, n_q, n_kv, dv, _native.ptr(workspace), need)
+    else:
+        _native.launch("flash_prefill_paged", dev, q.data_ptr(), q_st, q_sh, k_store.data_ptr(), v_store.data_ptr(),
+                       cu.data_ptr(), _native.ptr(start), pt.data_ptr(), out.data_ptr(), sc, T, B, n_q, n_kv, n_pages,
+                       page_size, pt.shape[1], dv, layout, _native.ptr(workspace), need)
+    return out
+
+
+def paged_fill_cache(cache, rows: torch.Tensor, cu_seqlens, page_table, start_pos=None) -> None:
+    """The rows of packed sequences into a page pool (paged_update_cache for whole prompts): row i of sequence b, rows
+    [T, n_groups, width] bf16 (a strided view such as columns of a projection), goes to position start_pos[b] + i (int32 [B];
+    None: i) of its pages, page_table[b, position // page_size]. ``cache`` is a [n_pages, n_groups, page_size, width] tensor or a
+    LatentCache pool. Positions outside the table and page ids outside the pool are skipped; the rest of the pool
+    keeps what it holds. Sequences of one call must not share the pages that they write."""
+    if isinstance(cache, GroupedLatentCache):
+        raise RuntimeError("a GroupedLatentCache is contiguous")
+    st, sg = _strided_rows(rows, "rows", None)
+    dev = rows.device
+    store, (n_pages, G, page_size, width), layout = _cache_arg(cache, "cache", dev)
+    if tuple(rows.shape[1:]) != (G, width):
+        raise RuntimeError(f"rows must be [T, {G}, {width}] for this cache, got {tuple(rows.shape)}")
+    cu = _seq_ints(cu_seqlens, "cu_seqlens", None, dev)
+    B = cu.numel() - 1
+    if B < 1:
+        raise RuntimeError("cu_seqlens must hold at least one sequence")
+    pt = _page_table(page_table, B, dev)
+    start = None if start_pos is None else _seq_ints(start_pos, "start_pos", B, dev)
+    if rows.shape[0] == 0:
+        return
+    _native.launch("latent_fill_paged", dev, store.data_ptr(), rows.data_ptr(), st, sg, cu.data_ptr(), _native.ptr(start),
+                   pt.data_ptr(), rows.shape[0], B, G, n_pages, page_size, pt.shape[1], width, layout)
+
+
 def scaled_dot_product_attention_decode(q, k, v, cur_pos_tensor, scale=None, **_):
     """Name-compatible alias of the stock decode op (full K and V, head_dim_v = 128)."""
     return flash_decode(q, k, v, cur_pos_tensor, scale=scale)

@@ -125,14 +125,18 @@ __device__ __forceinline__ Tile find_tile(const FlashPrefillArgs& a, int w) {
 }
 
 // dv = V width (a multiple of 16), DV32 its 32-wide tiles; row-major V rows stand DVP wide in LDS.
+//
+// LDS: K in the order of the caches' K tiles (kilobyte (block, half-block c, dim block kb): slot 16 g + n is key 8 (n / 4) + 4 c +
+// n % 4 and dims 32 kb + 8 g .. + 7), V in that of their V tiles or, from rows, in lines of rows 4 apart: the four
+// consecutive keys that a transposing read wants are a kilobyte and 64 bytes apart, so that they meet different banks.
 template <Source SRC, int DV32>
 __global__ __launch_bounds__(256, 2) void palu_flash_prefill_kernel(const FlashPrefillArgs a) {
   constexpr bool TILED = SRC == PAGED_TILED;
   constexpr int DVP = DV32 == 3 && !TILED ? 128 : 32 * DV32;
-  constexpr int CPR = DVP / 8;            // 16-byte chunks of a V row
   constexpr int VI = DVP / 32;            // 1 KB copies of V per wave and tile
+  constexpr int VKB = TILED || DVP == 32 ? 1024 : 1088;   // a kilobyte of V and its padding
   // One array per stage: the compiler then knows that a copy into one stage is no store to the stage being read.
-  __shared__ __attribute__((aligned(1024))) __bf16 sk0[FP_KEYS * HD], sk1[FP_KEYS * HD], sv0[FP_KEYS * DVP], sv1[FP_KEYS * DVP];
+  __shared__ __attribute__((aligned(1024))) char sk0[FP_KEYS * HD * 2], sk1[FP_KEYS * HD * 2], sv0[4 * VI * VKB], sv1[4 * VI * VKB];
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, h = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   // A KV head's workgroups are n_kv ids apart, for 8 heads all on one XCD, whose L2 then holds that head's K and V.
@@ -145,116 +149,107 @@ __global__ __launch_bounds__(256, 2) void palu_flash_prefill_kernel(const FlashP
   sq.len = __builtin_amdgcn_readfirstlane(sq.len);
   sq.start = __builtin_amdgcn_readfirstlane(sq.start);
   const int rows = sq.len * a.rep, row0 = tile.j * FP_ROWS, last_row = min(row0 + FP_ROWS, rows) - 1;
-  auto key_pos = [&](int row) { return min(sq.start + row / a.rep, a.capacity - 1); };
+  auto key_pos = [&](int row) { return __builtin_amdgcn_readfirstlane(min(sq.start + row / a.rep, a.capacity - 1)); };
   const int kv_end = key_pos(last_row) + 1;               // keys of this workgroup
-  const int row = min(row0 + 32 * w + n, rows - 1);       // rows past the sequence repeat its last, unstored
-  const int ri = row / a.rep, pos = key_pos(row);
-  const long long head = (long long)kvh * a.rep + (row - ri * a.rep);
-  const int w_lo = __builtin_amdgcn_readfirstlane(key_pos(min(row0 + 32 * w, rows - 1)));
-  const int w_hi = row0 + 32 * w >= rows ? -1             // a wave without rows copies only
-                                         : __builtin_amdgcn_readfirstlane(key_pos(min(row0 + 32 * w + 31, rows - 1)));
   const int nt_all = kv_end > 0 ? (kv_end + FP_KEYS - 1) / FP_KEYS : 0;
   const int per_split = split_tiles(nt_all, a.nsplit);
   const int t_lo = split * per_split, nt = min(nt_all, t_lo + per_split);
   if (t_lo >= nt && split > 0) return;    // uniform
 
-  // ---- copies to LDS ------------------------------------------------------------------------
+  // ---- copies to LDS: wave w copies keys 16 w .. + 15 of a tile (half-block w % 2 of block w / 2 for K) ---------
+  const int last_blk = (kv_end - 1) >> 5, inpage = (1 << a.page_shift) - 1;
   const int32_t* pt = SRC == PACKED ? nullptr : a.page_table + (long long)tile.b * a.pt_stride;
-  auto page_of = [&](int t, int blk) {                    // page of block blk of tile t (past the end: the last block's)
+  auto page_of = [&](int t) {                             // the page of this wave's block of tile t (past the end: the last block's)
     if constexpr (SRC == PACKED) return 0;
-    const int p = load_uniform(pt, min(2 * t + blk, (kv_end - 1) >> 5) >> a.page_shift);
+    const int p = load_uniform(pt, min(2 * t + (w >> 1), last_blk) >> a.page_shift);
     return min(max(p, 0), a.n_pages - 1);
   };
-  const int last_blk = (kv_end - 1) >> 5;
   const __bf16* kh = a.k + (long long)kvh * a.k_sh + (SRC == PACKED ? (long long)sq.beg * a.k_st : 0);
   const __bf16* vh = a.v + (long long)kvh * a.v_sh + (SRC == PACKED ? (long long)sq.beg * a.v_st : 0);
-  auto copy_tile = [&](__bf16* sk, __bf16* sv, int t, int p0, int p1) __attribute__((always_inline)) {
-    if constexpr (TILED) {
-      const int inpage = (1 << a.page_shift) - 1;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {                       // kilobyte 4 w + i of the tile: block w / 2
-        const int blk = min(2 * t + (w >> 1), last_blk);
-        const __bf16* src = kh + (long long)(w >> 1 ? p1 : p0) * a.k_st + (long long)(blk & inpage) * (BLK * HD) +
-                            ((w & 1) * 4 + i) * 512 + lane * 8;
-        __builtin_amdgcn_global_load_lds((gvoid*)src, (lvoid*)(sk + (4 * w + i) * 512), 16, 0, 0);
-      }
-#pragma unroll
-      for (int i = 0; i < DV32; ++i) {
-        const int c = w * DV32 + i, b = c / (2 * DV32), mt = min(c - b * 2 * DV32, a.dv / 16 - 1);
-        const int blk = min(2 * t + b, last_blk);
-        const __bf16* src = vh + (long long)(b ? p1 : p0) * a.v_st + (long long)(blk & inpage) * (BLK * a.dv) + mt * 512 + lane * 8;
-        __builtin_amdgcn_global_load_lds((gvoid*)src, (lvoid*)(sv + c * 512), 16, 0, 0);
-      }
+  // a lane's K row in its block (K-tile order) and V row, chunk in the 16 of its wave
+  const int g4 = lane >> 4, n16 = lane & 15;
+  const int krow = 8 * (n16 >> 2) + 4 * (w & 1) + (n16 & 3);
+  constexpr int CPR = DVP / 8;            // 16-byte chunks of a V row in LDS
+  const int vline = lane / CPR, vchunk = min(lane % CPR, a.dv / 8 - 1);
+  // V row (of the tile's 64) that copy i of wave w brings to line vline of its kilobyte
+  auto vrow = [&](int i) {
+    if constexpr (DVP == 32) return 16 * w + vline;
+    else if constexpr (DVP == 64) return 32 * (w >> 1) + 4 * vline + 2 * (w & 1) + i;
+    else return 16 * w + 4 * vline + i;
+  };
+  auto vkb = [&](int i) { return DVP == 64 ? 4 * (w >> 1) + 2 * (w & 1) + i : VI * w + i; };
+  auto copy_k = [&](char* sk, int t, int pid) __attribute__((always_inline)) {
+    const __bf16* src;
+    if constexpr (SRC == PACKED) {
+      src = kh + (long long)min(t * FP_KEYS + 32 * (w >> 1) + krow, kv_end - 1) * a.k_st + 8 * g4;
     } else {
-      // Row r of the tile in memory: packed, clamped to the last key; in pages, a row of its block's page.
-      auto row_at = [&](const __bf16* base, long long st, long long pst, int width, int r) {
-        if constexpr (SRC == PACKED) return base + (long long)min(t * FP_KEYS + r, kv_end - 1) * st;
-        const int blk = min(2 * t + (r >> 5), last_blk);
-        const int in = ((blk & ((1 << a.page_shift) - 1)) << 5) + (r & 31);
-        return base + (long long)(r >> 5 ? p1 : p0) * pst + in * width;
-      };
-      // 16-byte chunks of a row are permuted by the row, so that the reads below meet all banks.
+      const int blk = min(2 * t + (w >> 1), last_blk);
+      const __bf16* page = kh + (long long)pid * a.k_st + (long long)(blk & inpage) * (BLK * HD);
+      src = TILED ? page + (w & 1) * 2048 + lane * 8 : page + krow * HD + 8 * g4;
+    }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {                       // rows 4 (4 w + i) .. + 3
-        const int r = 4 * (4 * w + i) + (lane >> 4);
-        const int c = (lane & 15) ^ (4 * ((r >> 3) & 3) + (r & 3));
-        __builtin_amdgcn_global_load_lds((gvoid*)(row_at(kh, a.k_st, a.k_st, HD, r) + 8 * c), (lvoid*)(sk + (4 * w + i) * 512), 16, 0, 0);
-      }
+    for (int kb = 0; kb < 4; ++kb)
+      __builtin_amdgcn_global_load_lds((gvoid*)(src + kb * (TILED ? 512 : 32)), (lvoid*)(sk + (4 * w + kb) * 1024), 16, 0, 0);
+  };
+  auto copy_v = [&](char* sv, int t, int pid) __attribute__((always_inline)) {
+    const int blk = min(2 * t + (w >> 1), last_blk);
+    const __bf16* page = SRC == PACKED ? nullptr : vh + (long long)pid * a.v_st + (long long)(blk & inpage) * (BLK * a.dv);
 #pragma unroll
-      for (int i = 0; i < VI; ++i) {
-        const int e = (VI * w + i) * 64 + lane, r = e / CPR;
-        const int g = CPR == 16 ? 2 * (r & 3) + ((r >> 2) & 1) : CPR == 8 ? 2 * ((r >> 1) & 1) : 0;
-        const int c = min((e % CPR) ^ (2 * g), a.dv / 8 - 1);
-        __builtin_amdgcn_global_load_lds((gvoid*)(row_at(vh, a.v_st, a.v_st, a.dv, r) + 8 * c), (lvoid*)(sv + (VI * w + i) * 512), 16, 0, 0);
+    for (int i = 0; i < VI; ++i) {
+      const __bf16* src;
+      int kb = vkb(i);
+      if constexpr (SRC == PACKED) {
+        src = vh + (long long)min(t * FP_KEYS + vrow(i), kv_end - 1) * a.v_st + 8 * vchunk;
+      } else if constexpr (TILED) {
+        kb = w * DV32 + i;
+        src = page + min(kb - (w >> 1) * 2 * DV32, a.dv / 16 - 1) * 512 + lane * 8;
+      } else {
+        src = page + (vrow(i) - 32 * (w >> 1)) * a.dv + 8 * vchunk;
       }
+      __builtin_amdgcn_global_load_lds((gvoid*)src, (lvoid*)(sv + kb * VKB), 16, 0, 0);
     }
   };
-
-  // ---- operands from LDS --------------------------------------------------------------------
-  const int c16 = n >> 4, nn = n & 15;
-  int kaddr[TILED ? 1 : 8];                               // byte offsets of a lane's K operand, dim block kk
-  if constexpr (TILED) {
-    kaddr[0] = c16 * 4096 + h * 256 + nn * 16;
-  } else {
-    const int p = 8 * (nn >> 2) + 4 * c16 + (nn & 3);
-#pragma unroll
-    for (int kk = 0; kk < 8; ++kk) kaddr[kk] = p * 256 + (((2 * kk + h) ^ nn) * 16);
-  }
-  auto read_k = [&](const __bf16* sk, int blk, int kk) {
-    const char* base = reinterpret_cast<const char*>(sk) + blk * 8192;
-    if constexpr (TILED) return *reinterpret_cast<const bf16x8*>(base + kaddr[0] + (kk >> 1) * 1024 + (kk & 1) * 512);
-    else return *reinterpret_cast<const bf16x8*>(base + kaddr[kk]);
+  // A tile's copies are asked for while the ones before it are computed; past the wait and the barrier they have arrived
+  // in every wave, and every wave is done with the stages that the next copies overwrite.
+  auto turn = [&]() __attribute__((always_inline)) {
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(0x0070);                   // vmcnt(0) lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
   };
-  // V^T operand of dims 32 md .. + 31 and keys 32 blk + 16 t .. + 15: lane (n, h) holds keys 8 (2 t + h) .. + 7 of a dim.
-  int vaddr[TILED ? 1 : 2 * DV32];
-  if constexpr (TILED) {
-    vaddr[0] = c16 * 1024 + h * 256 + nn * 16;
-  } else {
-    // a 16-lane group reads 4 keys of 16 dims and gets, per lane, the 4 keys of one dim
-    const int r = 8 * h + ((lane & 15) >> 2);
-#pragma unroll
-    for (int md = 0; md < DV32; ++md)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int rr = r + 4 * u, pr = 2 * md + ((lane >> 4) & 1);
-        const int g = CPR == 16 ? 2 * (rr & 3) + ((rr >> 2) & 1) : CPR == 8 ? 2 * ((rr >> 1) & 1) : 0;
-        vaddr[2 * md + u] = rr * (2 * DVP) + ((pr ^ g) * 32) + 8 * (lane & 3);
-      }
+  // Stage of iteration t: K of tile t + 2 over that of tile t, whose scores are there, and V of t + 1.
+  int page1 = 0, page2 = 0;               // pages of tiles t + 1 and t + 2
+  auto ahead = [&](char* sk, char* sv, int t) __attribute__((always_inline)) {
+    if (t + 1 < nt) copy_v(sv, t + 1, page1);
+    if (t + 2 < nt) copy_k(sk, t + 2, page2);
+    page1 = page2;
+    page2 = page_of(t + 3);
+  };
+  if (t_lo < nt) {
+    const int p = page_of(t_lo);
+    page1 = page_of(t_lo + 1);
+    page2 = page_of(t_lo + 2);
+    copy_k(sk0, t_lo, p);
+    copy_v(sv0, t_lo, p);
+    if (t_lo + 1 < nt) copy_k(sk1, t_lo + 1, page1);
   }
-  auto read_v = [&](const __bf16* sv, int blk, int t, int md) {
-    const char* base = reinterpret_cast<const char*>(sv);
-    if constexpr (TILED) {
-      return *reinterpret_cast<const bf16x8*>(base + vaddr[0] + blk * (DV32 * 2048) + md * 2048 + t * 512);
-    } else {
-      base += (32 * blk + 16 * t) * (2 * DVP);
-      typedef __attribute__((address_space(3))) s16x4 lds4;
-      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(base + vaddr[2 * md]));
-      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(base + vaddr[2 * md + 1]));
-      return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  if (row0 + 32 * w >= rows) {            // a wave without rows copies only
+    for (int t = t_lo; t < nt; t += 2) {
+      if (t == t_lo) turn();
+      turn();
+      ahead(sk0, sv1, t);
+      if (t + 1 >= nt) break;
+      turn();
+      ahead(sk1, sv0, t + 1);
     }
-  };
+    return;
+  }
 
-  // ---- state ----------------------------------------------------------------------------------
+  // ---- this wave's rows ---------------------------------------------------------------------------
+  const int row = min(row0 + 32 * w + n, rows - 1);       // rows past the sequence repeat its last, unstored
+  const int ri = row / a.rep, pos = min(sq.start + ri, a.capacity - 1);
+  const long long head = (long long)kvh * a.rep + (row - ri * a.rep);
+  const int w_hi = key_pos(min(row0 + 32 * w + 31, rows - 1));
   bf16x8 q[8];
   {
     const __bf16* qp = a.q + (sq.beg + ri) * a.q_st + head * a.q_sh + 8 * h;
@@ -265,27 +260,51 @@ __global__ __launch_bounds__(256, 2) void palu_flash_prefill_kernel(const FlashP
       if (a.sign == 0) q[kk] = bf16x8{};
     }
   }
+  const int c16 = n >> 4, nn = n & 15;
+  const int kaddr = c16 * 4096 + h * 256 + nn * 16;
+  auto read_k = [&](const char* sk, int blk, int kk) {
+    return *reinterpret_cast<const bf16x8*>(sk + kaddr + blk * 8192 + (kk >> 1) * 1024 + (kk & 1) * 512);
+  };
+  // V^T operand of dims 32 md .. + 31 and keys 32 blk + 16 t .. + 15: lane (n, h) holds keys 8 (2 t + h) .. + 7 of a dim.
+  // From rows, a 16-lane group reads 4 keys of 16 dims (lanes 4 x .. + 3 key x) and gets, per lane, the 4 keys of one dim.
+  const int x4 = n16 >> 2, vcol = ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
+  const int vaddr = TILED ? c16 * 1024 + h * 256 + nn * 16
+                  : DVP == 32 ? (8 * h + x4) * 64 + vcol
+                  : DVP == 64 ? x4 * VKB + h * 256 + vcol : x4 * VKB + h * 512 + vcol;
+  auto read_v = [&](const char* sv, int blk, int t, int md) {
+    if constexpr (TILED) {
+      return *reinterpret_cast<const bf16x8*>(sv + vaddr + blk * (DV32 * 2048) + md * 2048 + t * 512);
+    } else {
+      constexpr int U = DVP == 32 ? 256 : DVP == 64 ? 128 : 256;   // from keys 0 .. 3 to 4 .. 7 of a lane's eight
+      const int o = md * 64 + (DVP == 32 ? (32 * blk + 16 * t) * 64 : DVP == 64 ? blk * 4 * VKB + t * 512 : (2 * blk + t) * 4 * VKB);
+      typedef __attribute__((address_space(3))) s16x4 lds4;
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(sv + vaddr + o));
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(sv + vaddr + o + U));
+      return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+  };
   f32x16 O[DV32];
 #pragma unroll
   for (int md = 0; md < DV32; ++md)
 #pragma unroll
     for (int i = 0; i < 16; ++i) O[md][i] = 0.f;
   float m_run = NEG_INF, l_run = 0.f;
-
-  auto step = [&](const __bf16* sk, const __bf16* sv, int t) __attribute__((always_inline)) {
-    const int base = t * FP_KEYS;
-    if (base > w_hi) return;                              // uniform per wave: keys past all its rows
-    f32x16 s[2];
+  auto zero = [](f32x16 (&s)[2]) __attribute__((always_inline)) {
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[b][i] = 0.f;
-#pragma unroll
-    for (int kk = 0; kk < 8; ++kk)
-#pragma unroll
-      for (int b = 0; b < 2; ++b) s[b] = mfma32(read_k(sk, b, kk), q[kk], s[b]);
-    const bool masked = base + FP_KEYS - 1 > w_lo;
-    if (masked) {
+  };
+  auto fence = []() __attribute__((always_inline)) { __builtin_amdgcn_sched_barrier(0); };
+
+  // One tile: the scores of the next one (sn) beside the softmax of this one's (s), then its V. The products of
+  // the next tile's scores and this one's exponentials are independent and alternate, two products to an eighth of the tile.
+  auto step = [&](f32x16 (&s)[2], f32x16 (&sn)[2], const char* skn, const char* sv, int t, auto tail)
+      __attribute__((always_inline)) {
+    constexpr bool TAIL = decltype(tail)::value;          // some rows do not see some of the tile's keys
+    const int base = t * FP_KEYS;
+    if constexpr (TAIL) {
+      if (base > w_hi) return;                            // uniform per wave: keys past all its rows
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -313,19 +332,44 @@ __global__ __launch_bounds__(256, 2) void palu_flash_prefill_kernel(const FlashP
     }
     const float mref = m_run == NEG_INF ? 0.f : m_run;
     bf16x8 p[2][2];
+    zero(sn);
+    bf16x8 kq[2][2];
+    if constexpr (!TAIL) {
+      fence();
+      kq[0][0] = read_k(skn, 0, 0);
+      kq[0][1] = read_k(skn, 1, 0);
+      fence();
+    }
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int tt = 0; tt < 2; ++tt) {
-        float e[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          e[i] = __builtin_amdgcn_exp2f(fmaf(s[b][4 * tt + 8 * (i >> 2) + (i & 3)], a.qscale, -mref));
-          p[b][tt][i] = (__bf16)e[i];
+    for (int c = 0; c < 8; ++c) {
+      if constexpr (!TAIL) {                              // (behind the last tile the products are of what the stage holds, unused)
+        if (c < 7) {
+          kq[(c + 1) & 1][0] = read_k(skn, 0, c + 1);
+          kq[(c + 1) & 1][1] = read_k(skn, 1, c + 1);
         }
-        l_run += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+#pragma unroll
+        for (int b = 0; b < 2; ++b) sn[b] = mfma32(kq[c & 1][b], q[c], sn[b]);
       }
-    if (masked) {
+      // an eighth of the softmax: four scores of half tt of block b
+      const int b = c >> 2, tt = (c >> 1) & 1, lo = 4 * (c & 1);
+      float e[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        e[i] = __builtin_amdgcn_exp2f(fmaf(s[b][4 * tt + 2 * lo + i], a.qscale, -mref));
+        p[b][tt][lo + i] = (__bf16)e[i];
+      }
+      l_run += (e[0] + e[1]) + (e[2] + e[3]);
+      if constexpr (!TAIL) fence();
+    }
+    if constexpr (TAIL) {
+      if (base + FP_KEYS <= w_hi) {
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk)
+#pragma unroll
+          for (int b = 0; b < 2; ++b) sn[b] = mfma32(read_k(skn, b, kk), q[kk], sn[b]);
+      }
+    }
+    if constexpr (TAIL) {
       // A key that some rows do not see may hold an infinity or NaN in V, and 0 times that is NaN: such a tile (rare) is
       // added one key at a time, to the rows that see it.
       float bad = 0.f;
@@ -361,35 +405,46 @@ __global__ __launch_bounds__(256, 2) void palu_flash_prefill_kernel(const FlashP
         return;
       }
     }
+    bf16x8 vq[2];
+    vq[0] = read_v(sv, 0, 0, 0);
+    fence();
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-        for (int md = 0; md < DV32; ++md) O[md] = mfma32(read_v(sv, b, tt, md), p[b][tt], O[md]);
-  };
-  // A tile's copies are asked for while the one before it is computed; past the wait and the barrier they have arrived in
-  // every wave, and every wave is done with the stage that the next copies overwrite.
-  auto turn = [&]() __attribute__((always_inline)) {
-    __builtin_amdgcn_sched_barrier(0);
-    __builtin_amdgcn_s_waitcnt(0x0070);                   // vmcnt(0) lgkmcnt(0)
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_sched_barrier(0);
+    for (int c = 0; c < 4 * DV32; ++c) {                  // md innermost: consecutive products have different accumulators
+      if (c + 1 < 4 * DV32) vq[(c + 1) & 1] = read_v(sv, (c + 1) / (2 * DV32), (c + 1) / DV32 % 2, (c + 1) % DV32);
+      fence();
+      O[c % DV32] = mfma32(vq[c & 1], p[c / (2 * DV32)][c / DV32 % 2], O[c % DV32]);
+    }
+    fence();
   };
   if (t_lo < nt) {
-    int a0 = page_of(t_lo, 0), a1 = page_of(t_lo, 1);
-    copy_tile(sk0, sv0, t_lo, a0, a1);
-    a0 = page_of(t_lo + 1, 0), a1 = page_of(t_lo + 1, 1);
-    for (int t = t_lo; t < nt; t += 2) {
+    f32x16 s0[2], s1[2];
+    turn();
+    zero(s0);
+    if (t_lo * FP_KEYS <= w_hi) {
+#pragma unroll
+      for (int kk = 0; kk < 8; ++kk)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) s0[b] = mfma32(read_k(sk0, b, kk), q[kk], s0[b]);
+    }
+    int t = t_lo;
+    const int nfull = min(nt, (key_pos(row0) + 1) / FP_KEYS);   // tiles that all rows of the workgroup see whole
+    for (; t + 2 <= nfull; t += 2) {
       turn();
-      if (t + 1 < nt) copy_tile(sk1, sv1, t + 1, a0, a1);
-      a0 = page_of(t + 2, 0), a1 = page_of(t + 2, 1);
-      step(sk0, sv0, t);
+      ahead(sk0, sv1, t);
+      step(s0, s1, sk1, sv0, t, std::false_type{});
       turn();
-      if (t + 1 >= nt) break;
-      if (t + 2 < nt) copy_tile(sk0, sv0, t + 2, a0, a1);
-      a0 = page_of(t + 3, 0), a1 = page_of(t + 3, 1);
-      step(sk1, sv1, t + 1);
+      ahead(sk1, sv0, t + 1);
+      step(s1, s0, sk0, sv1, t + 1, std::false_type{});
+    }
+    while (t < nt) {
+      turn();
+      ahead(sk0, sv1, t);
+      step(s0, s1, sk1, sv0, t, std::true_type{});
+      if (++t >= nt) break;
+      turn();
+      ahead(sk1, sv0, t);
+      step(s1, s0, sk0, sv1, t, std::true_type{});
+      ++t;
     }
   }
 

@@ -72,57 +72,86 @@ __device__ __forceinline__ Seq lane_seq(const FlashPrefillArgs& a, int b) {
 
 // Work order: all tiles of the batch, those with the most keys first, so that the last ones to run are short. A tile's
 // level is its distance from position 0 in tiles, rounded down; item w of the descending order is found by halving over
-// levels, each lane counting the tiles of one sequence (all waves do it, without a barrier).
+// levels, the lanes counting the tiles of a sequence each (all waves do it, without a barrier; four sequences of a lane stay in
+// registers, further ones are read again for every level).
 struct Tile {
   int b, j;                               // j: tile of sequence b; b < 0: none
+  Seq seq;
 };
 __device__ __forceinline__ Tile find_tile(const FlashPrefillArgs& a, int w) {
+  constexpr int R = 4;
   const int lane = threadIdx.x & 63;
-  const int per = FP_ROWS / a.rep > 0 ? FP_ROWS / a.rep : 1;
-  auto seq_levels = [&](int b, int& base, int& n) {
-    const Seq s = lane_seq(a, min(b, a.B - 1));
-    n = b < a.B ? (int)(((long long)s.len * a.rep + FP_ROWS - 1) / FP_ROWS) : 0;
-    base = max(s.start, 0) / per;
+  const int per = max(1, FP_ROWS / a.rep);
+  struct Levels {
+    int base, n;
   };
-  int base0, n0;
-  seq_levels(lane, base0, n0);            // the first 64 sequences stay in registers
-  auto count = [&](int t, int& top) {     // tiles at level t or above; top: one past the highest level
-    int c = min(max(base0 + n0 - t, 0), n0), hi = n0 ? base0 + n0 : 0;
-    for (int b0 = 64; b0 < a.B; b0 += 64) {
-      int base, n;
-      seq_levels(b0 + lane, base, n);
-      c += min(max(base + n - t, 0), n);
-      hi = max(hi, n ? base + n : 0);
-    }
-    top = hi;
+  auto load = [&](int b) {
+    const Seq s = lane_seq(a, min(b, a.B - 1));
+    return b < a.B ? s : Seq{0, 0, 0};
+  };
+  auto levels = [&](const Seq& s) { return Levels{max(s.start, 0) / per, (int)(((long long)s.len * a.rep + FP_ROWS - 1) / FP_ROWS)}; };
+  Seq own[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) own[r] = load(64 * r + lane);
+  Levels lv[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) lv[r] = levels(own[r]);
+  auto above = [](Levels l, int t) { return min(max(l.base + l.n - t, 0), l.n); };
+  auto count = [&](int t) {               // tiles at level t or above
+    int c = 0;
+#pragma unroll
+    for (int r = 0; r < R; ++r) c += above(lv[r], t);
+    for (int b0 = 64 * R; b0 < a.B; b0 += 64) c += above(levels(load(b0 + lane)), t);
     return wave_sum_i(c);
   };
-  int top;
-  if (w >= count(0, top)) return Tile{-1, 0};
+  if (w >= count(0)) return Tile{-1, 0, {}};
+  int top = 0;                            // one past the highest level
+#pragma unroll
+  for (int r = 0; r < R; ++r) top = max(top, lv[r].n ? lv[r].base + lv[r].n : 0);
+  for (int b0 = 64 * R; b0 < a.B; b0 += 64) {
+    const Levels l = levels(load(b0 + lane));
+    top = max(top, l.n ? l.base + l.n : 0);
+  }
 #pragma unroll
   for (int o = 32; o; o >>= 1) top = max(top, __shfl_xor(top, o, 64));
-  int lo = 0, hi = __builtin_amdgcn_readfirstlane(top), unused;   // count(lo) > w, count(hi) = 0 <= w
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (count(mid, unused) > w) lo = mid;
-    else hi = mid;
-  }
-  int r = w - count(lo + 1, unused);      // which of the sequences that have level lo
-  for (int b0 = 0; b0 < a.B; b0 += 64) {
-    int base = base0, n = n0;
-    if (b0) seq_levels(b0 + lane, base, n);
-    const unsigned long long m = __ballot(n > 0 && base <= lo && lo < base + n);
+  int lo = 0, hi = __builtin_amdgcn_readfirstlane(top);   // count(lo) > w >= count(hi) = 0
+  if (a.B == 1) lo = hi - 1 - w;                          // one sequence has one tile at every level
+  else
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (count(mid) > w) lo = mid;
+      else hi = mid;
+    }
+  int r = a.B == 1 ? 0 : w - count(lo + 1);               // which of the sequences that have level lo
+  Tile found{-1, 0, {}};
+  auto pick = [&](int b0, const Seq& s) {
+    const Levels l = levels(s);
+    const unsigned long long m = __ballot(l.n > 0 && l.base <= lo && lo < l.base + l.n);
     const int c = __popcll(m);
-    if (r < c) {
-      const int before = __popcll(m & ((1ull << lane) - 1));
-      const unsigned long long me = __ballot(((m >> lane) & 1) && before == r);
-      const int l = __builtin_ctzll(me);
-      return Tile{b0 + l, lo - __builtin_amdgcn_readlane(base, l)};
+    if (r >= 0 && r < c) {
+      const unsigned long long me = __ballot(((m >> lane) & 1) && __popcll(m & ((1ull << lane) - 1)) == r);
+      const int x = __builtin_ctzll(me);
+      found = Tile{b0 + x, lo - __builtin_amdgcn_readlane(l.base, x), {__builtin_amdgcn_readlane(s.beg, x),
+                   __builtin_amdgcn_readlane(s.len, x), __builtin_amdgcn_readlane(s.start, x)}};
     }
     r -= c;
-  }
-  return Tile{-1, 0};
+  };
+#pragma unroll
+  for (int k = 0; k < R; ++k) pick(64 * k, own[k]);
+  for (int b0 = 64 * R; b0 < a.B && r >= 0; b0 += 64) pick(b0, load(b0 + lane));
+  return found;
 }
+
+// A tile's rows are rows row0 .. of the sequence, row = position * rep + head: position and head of row row0 + x.
+struct RowSplit {
+  int pos0, rem;
+  FDiv rep;
+};
+__device__ __forceinline__ RowSplit split_rows(int row0, int rep) {
+  const int p = (int)((unsigned)row0 / (unsigned)rep);
+  return RowSplit{p, row0 - p * rep, make_fdiv(rep)};
+}
+__device__ __forceinline__ int row_pos(const RowSplit& s, int x) { return s.pos0 + fdiv(s.rem + x, s.rep); }
 
 // dv = V width (a multiple of 16), DV32 its 32-wide tiles; row-major V rows stand DVP wide in LDS.
 //
@@ -144,13 +173,12 @@ __global__ __launch_bounds__(256, 2) void palu_flash_prefill_kernel(const FlashP
   const int item = blockIdx.x / a.n_kv / a.nsplit, split = blockIdx.x / a.n_kv - item * a.nsplit;
   const Tile tile = find_tile(a, item);
   if (tile.b < 0) return;                 // uniform, before any barrier
-  Seq sq = lane_seq(a, tile.b);
-  sq.beg = __builtin_amdgcn_readfirstlane(sq.beg);
-  sq.len = __builtin_amdgcn_readfirstlane(sq.len);
-  sq.start = __builtin_amdgcn_readfirstlane(sq.start);
-  const int rows = sq.len * a.rep, row0 = tile.j * FP_ROWS, last_row = min(row0 + FP_ROWS, rows) - 1;
-  auto key_pos = [&](int row) { return __builtin_amdgcn_readfirstlane(min(sq.start + row / a.rep, a.capacity - 1)); };
-  const int kv_end = key_pos(last_row) + 1;               // keys of this workgroup
+  const Seq sq = tile.seq;
+  const int row0 = tile.j * FP_ROWS, rows = min(sq.len * a.rep - row0, FP_ROWS);   // rows of this tile
+  const RowSplit rs = split_rows(row0, a.rep);
+  // the last key that a row sees, of row x of the tile, x uniform
+  auto key_pos = [&](int x) { return __builtin_amdgcn_readfirstlane(min(sq.start + row_pos(rs, x), a.capacity - 1)); };
+  const int kv_end = key_pos(rows - 1) + 1;               // keys of this workgroup
   const int nt_all = kv_end > 0 ? (kv_end + FP_KEYS - 1) / FP_KEYS : 0;
   const int per_split = split_tiles(nt_all, a.nsplit);
   const int t_lo = split * per_split, nt = min(nt_all, t_lo + per_split);
@@ -233,7 +261,7 @@ __global__ __launch_bounds__(256, 2) void palu_flash_prefill_kernel(const FlashP
     copy_v(sv0, t_lo, p);
     if (t_lo + 1 < nt) copy_k(sk1, t_lo + 1, page1);
   }
-  if (row0 + 32 * w >= rows) {            // a wave without rows copies only
+  if (32 * w >= rows) {                   // a wave without rows copies only
     for (int t = t_lo; t < nt; t += 2) {
       if (t == t_lo) turn();
       turn();
@@ -246,10 +274,10 @@ __global__ __launch_bounds__(256, 2) void palu_flash_prefill_kernel(const FlashP
   }
 
   // ---- this wave's rows ---------------------------------------------------------------------------
-  const int row = min(row0 + 32 * w + n, rows - 1);       // rows past the sequence repeat its last, unstored
-  const int ri = row / a.rep, pos = min(sq.start + ri, a.capacity - 1);
-  const long long head = (long long)kvh * a.rep + (row - ri * a.rep);
-  const int w_hi = key_pos(min(row0 + 32 * w + 31, rows - 1));
+  const int row = min(32 * w + n, rows - 1);              // rows past the sequence repeat its last, unstored
+  const int ri = row_pos(rs, row), pos = min(sq.start + ri, a.capacity - 1);
+  const long long head = (long long)kvh * a.rep + (rs.rem + row - (ri - rs.pos0) * a.rep);
+  const int w_hi = key_pos(min(32 * w + 31, rows - 1));
   bf16x8 q[8];
   {
     const __bf16* qp = a.q + (sq.beg + ri) * a.q_st + head * a.q_sh + 8 * h;
@@ -297,22 +325,9 @@ __global__ __launch_bounds__(256, 2) void palu_flash_prefill_kernel(const FlashP
   };
   auto fence = []() __attribute__((always_inline)) { __builtin_amdgcn_sched_barrier(0); };
 
-  // One tile: the scores of the next one (sn) beside the softmax of this one's (s), then its V. The products of
-  // the next tile's scores and this one's exponentials are independent and alternate, two products to an eighth of the tile.
-  auto step = [&](f32x16 (&s)[2], f32x16 (&sn)[2], const char* skn, const char* sv, int t, auto tail)
-      __attribute__((always_inline)) {
-    constexpr bool TAIL = decltype(tail)::value;          // some rows do not see some of the tile's keys
-    const int base = t * FP_KEYS;
-    if constexpr (TAIL) {
-      if (base > w_hi) return;                            // uniform per wave: keys past all its rows
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int j = i >> 2, key = base + 32 * b + 8 * (2 * (j & 1) + h) + 4 * (j >> 1) + (i & 3);
-          if (key > pos) s[b][i] = NEG_INF;
-        }
-    }
+  // The running maximum of every row after scores s; what was summed before is scaled to it. Refreshed by the row's own scores
+  // alone, so that a row's roundings do not depend on its neighbours'. Returns the reference of the exponents.
+  auto maximum = [&](const f32x16 (&s)[2]) __attribute__((always_inline)) {
     float mx = s[0][0];
 #pragma unroll
     for (int b = 0; b < 2; ++b)
@@ -320,7 +335,6 @@ __global__ __launch_bounds__(256, 2) void palu_flash_prefill_kernel(const FlashP
       for (int i = 0; i < 16; ++i) mx = __builtin_elementwise_maximum(mx, s[b][i]);
     mx *= a.qscale;
     if (__any(mx > m_run + LAZY_RESCALE_LOG2)) {
-      // Rows refresh by their own scores alone, so that a row's roundings do not depend on its neighbours'.
       const float top = fmaxf(mx, __shfl_xor(mx, 32, 64)), mn = top > m_run + LAZY_RESCALE_LOG2 ? top : m_run;
       const float alpha = m_run == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(m_run - mn);
 #pragma unroll
@@ -330,126 +344,166 @@ __global__ __launch_bounds__(256, 2) void palu_flash_prefill_kernel(const FlashP
       l_run *= alpha;
       m_run = mn;
     }
-    const float mref = m_run == NEG_INF ? 0.f : m_run;
-    bf16x8 p[2][2];
-    zero(sn);
-    bf16x8 kq[2][2];
-    if constexpr (!TAIL) {
-      fence();
-      kq[0][0] = read_k(skn, 0, 0);
-      kq[0][1] = read_k(skn, 1, 0);
-      fence();
+    return m_run == NEG_INF ? 0.f : m_run;
+  };
+  // An eighth of a tile's probabilities: four scores of half tt of block b.
+  auto eighth = [&](const f32x16 (&s)[2], bf16x8 (&p)[2][2], int c, float mref) __attribute__((always_inline)) {
+    const int b = c >> 2, tt = (c >> 1) & 1, lo = 4 * (c & 1);
+    float e[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      e[i] = __builtin_amdgcn_exp2f(fmaf(s[b][4 * tt + 2 * lo + i], a.qscale, -mref));
+      p[b][tt][lo + i] = (__bf16)e[i];
     }
+    l_run += (e[0] + e[1]) + (e[2] + e[3]);
+  };
+  // Operand c of a tile's products with V, md innermost: consecutive products have different accumulators. Operands are
+  // read ahead of their products, K two eighths and V three products: a read from LDS takes as long as some four products.
+  bf16x8 vq[4];
+  auto next_v = [&](const char* sv, int c) __attribute__((always_inline)) {
+    if (c < 4 * DV32) vq[c & 3] = read_v(sv, c / (2 * DV32), c / DV32 % 2, c % DV32);
+  };
+  // O += V^T P^T, the first `ready` operands read.
+  auto values = [&](const char* sv, const bf16x8 (&p)[2][2], int ready) __attribute__((always_inline)) {
 #pragma unroll
-    for (int c = 0; c < 8; ++c) {
-      if constexpr (!TAIL) {                              // (behind the last tile the products are of what the stage holds, unused)
-        if (c < 7) {
-          kq[(c + 1) & 1][0] = read_k(skn, 0, c + 1);
-          kq[(c + 1) & 1][1] = read_k(skn, 1, c + 1);
-        }
-#pragma unroll
-        for (int b = 0; b < 2; ++b) sn[b] = mfma32(kq[c & 1][b], q[c], sn[b]);
-      }
-      // an eighth of the softmax: four scores of half tt of block b
-      const int b = c >> 2, tt = (c >> 1) & 1, lo = 4 * (c & 1);
-      float e[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        e[i] = __builtin_amdgcn_exp2f(fmaf(s[b][4 * tt + 2 * lo + i], a.qscale, -mref));
-        p[b][tt][lo + i] = (__bf16)e[i];
-      }
-      l_run += (e[0] + e[1]) + (e[2] + e[3]);
-      if constexpr (!TAIL) fence();
-    }
-    if constexpr (TAIL) {
-      if (base + FP_KEYS <= w_hi) {
-#pragma unroll
-        for (int kk = 0; kk < 8; ++kk)
-#pragma unroll
-          for (int b = 0; b < 2; ++b) sn[b] = mfma32(read_k(skn, b, kk), q[kk], sn[b]);
-      }
-    }
-    if constexpr (TAIL) {
-      // A key that some rows do not see may hold an infinity or NaN in V, and 0 times that is NaN: such a tile (rare) is
-      // added one key at a time, to the rows that see it.
-      float bad = 0.f;
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-          for (int md = 0; md < DV32; ++md) {
-            const bf16x8 v = read_v(sv, b, tt, md);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              bad = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{v[2 * i], v[2 * i + 1]}, bf16x2{(__bf16)0.f, (__bf16)0.f}, bad, false);
-          }
-      if (__any(bad != bad)) {
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-          for (int tt = 0; tt < 2; ++tt)
-            for (int x = 0; x < 16; ++x) {
-              const int key = base + 32 * b + 16 * tt + x;
-              if (key > w_hi) break;
-#pragma unroll
-              for (int md = 0; md < DV32; ++md) {
-                bf16x8 v = read_v(sv, b, tt, md);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = 8 * h + i == x ? v[i] : (__bf16)0.f;
-                const f32x16 y = mfma32(v, p[b][tt], O[md]);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) O[md][i] = key <= pos ? y[i] : O[md][i];
-              }
-            }
-        return;
-      }
-    }
-    bf16x8 vq[2];
-    vq[0] = read_v(sv, 0, 0, 0);
+    for (int c = 0; c < 3; ++c)
+      if (c >= ready) next_v(sv, c);
     fence();
 #pragma unroll
-    for (int c = 0; c < 4 * DV32; ++c) {                  // md innermost: consecutive products have different accumulators
-      if (c + 1 < 4 * DV32) vq[(c + 1) & 1] = read_v(sv, (c + 1) / (2 * DV32), (c + 1) / DV32 % 2, (c + 1) % DV32);
+    for (int c = 0; c < 4 * DV32; ++c) {
+      next_v(sv, c + 3);
       fence();
-      O[c % DV32] = mfma32(vq[c & 1], p[c / (2 * DV32)][c / DV32 % 2], O[c % DV32]);
+      O[c % DV32] = mfma32(vq[c & 3], p[c / (2 * DV32)][c / DV32 % 2], O[c % DV32]);
     }
     fence();
   };
-  if (t_lo < nt) {
-    f32x16 s0[2], s1[2];
-    turn();
-    zero(s0);
-    if (t_lo * FP_KEYS <= w_hi) {
+  auto scores = [&](f32x16 (&s)[2], const char* sk) __attribute__((always_inline)) {
+    zero(s);
+    bf16x8 kq[2][2];
 #pragma unroll
-      for (int kk = 0; kk < 8; ++kk)
+    for (int b = 0; b < 2; ++b) kq[0][b] = read_k(sk, b, 0);
 #pragma unroll
-        for (int b = 0; b < 2; ++b) s0[b] = mfma32(read_k(sk0, b, kk), q[kk], s0[b]);
+    for (int c = 0; c < 8; ++c) {
+      if (c < 7)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) kq[(c + 1) & 1][b] = read_k(sk, b, c + 1);
+      fence();
+#pragma unroll
+      for (int b = 0; b < 2; ++b) s[b] = mfma32(kq[c & 1][b], q[c], s[b]);
     }
+  };
+
+  // A tile that all rows see whole: the scores of the next one (sn) beside the softmax of this one's (s), then its V. The
+  // products of the next tile's scores and this one's exponentials are independent and alternate. (Behind the last tile
+  // the products are of what the stage holds, and unused.)
+  auto step = [&](f32x16 (&s)[2], f32x16 (&sn)[2], const char* skn, const char* sv) __attribute__((always_inline)) {
+    const float mref = maximum(s);
+    bf16x8 p[2][2], kq[3][2];
+    auto next_k = [&](int c) __attribute__((always_inline)) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b) kq[c % 3][b] = read_k(skn, b, c);
+    };
+    zero(sn);
+    fence();
+    next_k(0);
+    next_k(1);
+    fence();
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      if (c < 6) next_k(c + 2);
+      else next_v(sv, c - 6);
+      fence();
+#pragma unroll
+      for (int b = 0; b < 2; ++b) sn[b] = mfma32(kq[c % 3][b], q[c], sn[b]);
+      eighth(s, p, c, mref);
+      fence();
+    }
+    values(sv, p, 2);
+  };
+  // A tile of which some rows do not see some keys; s becomes the next tile's scores.
+  auto tail = [&](f32x16 (&s)[2], const char* skn, const char* sv, int t) __attribute__((always_inline)) {
+    const int base = t * FP_KEYS;
+    if (base > w_hi) return;                              // uniform per wave: keys past all its rows
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int j = i >> 2, key = base + 32 * b + 8 * (2 * (j & 1) + h) + 4 * (j >> 1) + (i & 3);
+        if (key > pos) s[b][i] = NEG_INF;
+      }
+    const float mref = maximum(s);
+    bf16x8 p[2][2];
+#pragma unroll
+    for (int c = 0; c < 8; ++c) eighth(s, p, c, mref);
+    fence();
+    // A key that some rows do not see may hold an infinity or NaN in V, and 0 times that is NaN: such a tile (rare) is
+    // added one key at a time, to the rows that see it.
+    float bad[4] = {0.f, 0.f, 0.f, 0.f};
+    next_v(sv, 0);
+    next_v(sv, 1);
+    next_v(sv, 2);
+#pragma unroll
+    for (int c = 0; c < 4 * DV32; ++c) {
+      next_v(sv, c + 3);
+      fence();
+      const bf16x8 v = vq[c & 3];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        bad[i] = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{v[2 * i], v[2 * i + 1]}, bf16x2{(__bf16)0.f, (__bf16)0.f}, bad[i], false);
+    }
+    const float b4 = (bad[0] + bad[1]) + (bad[2] + bad[3]);
+    if (__any(b4 != b4)) {
+      for (int x = 0; x < FP_KEYS && base + x <= w_hi; ++x) {
+        const int bt = x >> 4;
+        bf16x8 px = p[0][0];
+#pragma unroll
+        for (int i = 1; i < 4; ++i)
+          if (bt == i) px = p[i >> 1][i & 1];
+#pragma unroll
+        for (int md = 0; md < DV32; ++md) {
+          bf16x8 v = read_v(sv, bt >> 1, bt & 1, md);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = 8 * h + i == (x & 15) ? v[i] : (__bf16)0.f;
+          const f32x16 y = mfma32(v, px, O[md]);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) O[md][i] = base + x <= pos ? y[i] : O[md][i];
+          fence();
+        }
+      }
+    } else {
+      values(sv, p, 0);
+    }
+    if (base + FP_KEYS <= w_hi) scores(s, skn);
+  };
+  if (t_lo < nt) {
+    f32x16 s0[2];
+    turn();
+    if (t_lo * FP_KEYS <= w_hi) scores(s0, sk0);
     int t = t_lo;
-    const int nfull = min(nt, (key_pos(row0) + 1) / FP_KEYS);   // tiles that all rows of the workgroup see whole
+    const int nfull = min(nt, (key_pos(0) + 1) / FP_KEYS);   // tiles that all rows of the workgroup see whole
     for (; t + 2 <= nfull; t += 2) {
+      f32x16 s1[2];
       turn();
       ahead(sk0, sv1, t);
-      step(s0, s1, sk1, sv0, t, std::false_type{});
+      step(s0, s1, sk1, sv0);
       turn();
       ahead(sk1, sv0, t + 1);
-      step(s1, s0, sk0, sv1, t + 1, std::false_type{});
+      step(s1, s0, sk0, sv1);
     }
     while (t < nt) {
       turn();
       ahead(sk0, sv1, t);
-      step(s0, s1, sk1, sv0, t, std::true_type{});
+      tail(s0, sk1, sv0, t);
       if (++t >= nt) break;
       turn();
       ahead(sk1, sv0, t);
-      step(s1, s0, sk0, sv1, t, std::true_type{});
+      tail(s0, sk0, sv1, t);
       ++t;
     }
   }
 
   const float l = l_run + __shfl_xor(l_run, 32, 64);
-  if (row0 + 32 * w + n >= rows) return;
+  if (32 * w + n >= rows) return;
   if (nt_all > per_split) {               // one of several splits
     const long long slot = ((long long)item * a.n_kv + kvh) * a.nsplit + split;
     float* po = a.part + slot * FP_ROWS * (a.dv + 2);
@@ -488,13 +542,14 @@ __global__ __launch_bounds__(256) void palu_flash_prefill_join_kernel(const Flas
   const int kvh = blockIdx.x % a.n_kv, rest = blockIdx.x / a.n_kv, item = rest >> 2;
   const Tile tile = find_tile(a, item);
   if (tile.b < 0) return;
-  const Seq sq = lane_seq(a, tile.b);
-  const int rows = sq.len * a.rep, row0 = tile.j * FP_ROWS;
-  const int last = min(sq.start + (min(row0 + FP_ROWS, rows) - 1) / a.rep, a.capacity - 1);
+  const Seq sq = tile.seq;
+  const int row0 = tile.j * FP_ROWS, rows = min(sq.len * a.rep - row0, FP_ROWS);
+  const RowSplit rs = split_rows(row0, a.rep);
+  const int last = min(sq.start + row_pos(rs, rows - 1), a.capacity - 1);
   const int nt = last >= 0 ? last / FP_KEYS + 1 : 0, per = split_tiles(nt, a.nsplit);
-  const int r = (rest & 3) * 32 + (threadIdx.x >> 3), row = row0 + r;
-  if (nt <= per || row >= rows) return;
-  const int ns = (nt + per - 1) / per, ri = row / a.rep;
+  const int r = (rest & 3) * 32 + (threadIdx.x >> 3);
+  if (nt <= per || r >= rows) return;
+  const int ns = (nt + per - 1) / per, ri = row_pos(rs, r);
   const long long stride = (long long)FP_ROWS * (a.dv + 2);
   const float* part = a.part + ((long long)item * a.n_kv + kvh) * a.nsplit * stride;
   const float* ml = part + FP_ROWS * a.dv + r;
@@ -503,7 +558,7 @@ __global__ __launch_bounds__(256) void palu_flash_prefill_join_kernel(const Flas
   const float ref = M == NEG_INF ? 0.f : M;
   for (int s = 0; s < ns; ++s) l += __builtin_amdgcn_exp2f(ml[s * stride] - ref) * ml[s * stride + FP_ROWS];
   const float inv = 1.f / l;
-  __bf16* o = a.out + ((long long)(sq.beg + ri) * a.n_q + (long long)kvh * a.rep + (row - ri * a.rep)) * a.dv;
+  __bf16* o = a.out + ((long long)(sq.beg + ri) * a.n_q + (long long)kvh * a.rep + (rs.rem + r - (ri - rs.pos0) * a.rep)) * a.dv;
   for (int d = 4 * (threadIdx.x & 7); d < a.dv; d += 32) {
     f32x4 y = {0.f, 0.f, 0.f, 0.f};
     for (int s = 0; s < ns; ++s)

@@ -81,7 +81,7 @@ struct Tile {
 __device__ __forceinline__ Tile find_tile(const FlashPrefillArgs& a, int w) {
   constexpr int R = 4;
   const int lane = threadIdx.x & 63;
-  const int per = max(1, FP_ROWS / a.rep);
+  const int shift = 31 - __builtin_clz(max(1, FP_ROWS / a.rep));   // positions of a tile, as a power of two: for the order only
   struct Levels {
     int base, n;
   };
@@ -89,13 +89,18 @@ __device__ __forceinline__ Tile find_tile(const FlashPrefillArgs& a, int w) {
     const Seq s = lane_seq(a, min(b, a.B - 1));
     return b < a.B ? s : Seq{0, 0, 0};
   };
-  auto levels = [&](const Seq& s) { return Levels{max(s.start, 0) / per, (int)(((long long)s.len * a.rep + FP_ROWS - 1) / FP_ROWS)}; };
+  auto levels = [&](const Seq& s) { return Levels{max(s.start, 0) >> shift, (s.len * a.rep + FP_ROWS - 1) / FP_ROWS}; };
   Seq own[R];
-#pragma unroll
-  for (int r = 0; r < R; ++r) own[r] = load(64 * r + lane);
   Levels lv[R];
 #pragma unroll
-  for (int r = 0; r < R; ++r) lv[r] = levels(own[r]);
+  for (int r = 0; r < R; ++r) {
+    own[r] = Seq{0, 0, 0};
+    lv[r] = Levels{0, 0};
+    if (64 * r < a.B) {
+      own[r] = load(64 * r + lane);
+      lv[r] = levels(own[r]);
+    }
+  }
   auto above = [](Levels l, int t) { return min(max(l.base + l.n - t, 0), l.n); };
   auto count = [&](int t) {               // tiles at level t or above
     int c = 0;
@@ -104,6 +109,12 @@ __device__ __forceinline__ Tile find_tile(const FlashPrefillArgs& a, int w) {
     for (int b0 = 64 * R; b0 < a.B; b0 += 64) c += above(levels(load(b0 + lane)), t);
     return wave_sum_i(c);
   };
+  if (a.B == 1) {                         // one sequence: its tiles from the last on
+    const Seq s{__builtin_amdgcn_readfirstlane(own[0].beg), __builtin_amdgcn_readfirstlane(own[0].len),
+                __builtin_amdgcn_readfirstlane(own[0].start)};
+    const int n = levels(s).n;
+    return Tile{w < n ? 0 : -1, n - 1 - w, s};
+  }
   if (w >= count(0)) return Tile{-1, 0, {}};
   int top = 0;                            // one past the highest level
 #pragma unroll
@@ -115,14 +126,12 @@ __device__ __forceinline__ Tile find_tile(const FlashPrefillArgs& a, int w) {
 #pragma unroll
   for (int o = 32; o; o >>= 1) top = max(top, __shfl_xor(top, o, 64));
   int lo = 0, hi = __builtin_amdgcn_readfirstlane(top);   // count(lo) > w >= count(hi) = 0
-  if (a.B == 1) lo = hi - 1 - w;                          // one sequence has one tile at every level
-  else
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (count(mid) > w) lo = mid;
-      else hi = mid;
-    }
-  int r = a.B == 1 ? 0 : w - count(lo + 1);               // which of the sequences that have level lo
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (count(mid) > w) lo = mid;
+    else hi = mid;
+  }
+  int r = w - count(lo + 1);              // which of the sequences that have level lo
   Tile found{-1, 0, {}};
   auto pick = [&](int b0, const Seq& s) {
     const Levels l = levels(s);
@@ -137,7 +146,8 @@ __device__ __forceinline__ Tile find_tile(const FlashPrefillArgs& a, int w) {
     r -= c;
   };
 #pragma unroll
-  for (int k = 0; k < R; ++k) pick(64 * k, own[k]);
+  for (int k = 0; k < R; ++k)
+    if (64 * k < a.B) pick(64 * k, own[k]);
   for (int b0 = 64 * R; b0 < a.B && r >= 0; b0 += 64) pick(b0, load(b0 + lane));
   return found;
 }
@@ -199,42 +209,43 @@ __global__ __launch_bounds__(256, 2) void palu_flash_prefill_kernel(const FlashP
   const int krow = 8 * (n16 >> 2) + 4 * (w & 1) + (n16 & 3);
   constexpr int CPR = DVP / 8;            // 16-byte chunks of a V row in LDS
   const int vline = lane / CPR, vchunk = min(lane % CPR, a.dv / 8 - 1);
-  // V row (of the tile's 64) that copy i of wave w brings to line vline of its kilobyte
+  // V row (of its block) that copy i of wave w brings to line vline of its kilobyte
   auto vrow = [&](int i) {
-    if constexpr (DVP == 32) return 16 * w + vline;
-    else if constexpr (DVP == 64) return 32 * (w >> 1) + 4 * vline + 2 * (w & 1) + i;
-    else return 16 * w + 4 * vline + i;
+    if constexpr (DVP == 32) return 16 * (w & 1) + vline;
+    else if constexpr (DVP == 64) return 4 * vline + 2 * (w & 1) + i;
+    else return 16 * (w & 1) + 4 * vline + i;
   };
   auto vkb = [&](int i) { return DVP == 64 ? 4 * (w >> 1) + 2 * (w & 1) + i : VI * w + i; };
+  // A row of the packed K or V: a uniform base and a lane's 32-bit offset (bytes), rows clamped to the last key.
+  const int rows16 = 32 * (w >> 1);
   auto copy_k = [&](char* sk, int t, int pid) __attribute__((always_inline)) {
-    const __bf16* src;
+    const char* src;
+    unsigned off;
     if constexpr (SRC == PACKED) {
-      src = kh + (long long)min(t * FP_KEYS + 32 * (w >> 1) + krow, kv_end - 1) * a.k_st + 8 * g4;
+      const int r0 = min(t * FP_KEYS + rows16, kv_end - 1);
+      src = reinterpret_cast<const char*>(kh + (long long)r0 * a.k_st);
+      off = __umul24(min(krow, kv_end - 1 - r0), (unsigned)a.k_st * 2) + 16 * g4;
     } else {
       const int blk = min(2 * t + (w >> 1), last_blk);
-      const __bf16* page = kh + (long long)pid * a.k_st + (long long)(blk & inpage) * (BLK * HD);
-      src = TILED ? page + (w & 1) * 2048 + lane * 8 : page + krow * HD + 8 * g4;
+      src = reinterpret_cast<const char*>(kh + (long long)pid * a.k_st + (long long)(blk & inpage) * (BLK * HD));
+      off = TILED ? (w & 1) * 4096 + lane * 16 : krow * (2 * HD) + 16 * g4;
     }
 #pragma unroll
     for (int kb = 0; kb < 4; ++kb)
-      __builtin_amdgcn_global_load_lds((gvoid*)(src + kb * (TILED ? 512 : 32)), (lvoid*)(sk + (4 * w + kb) * 1024), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((gvoid*)(src + off + kb * (TILED ? 1024 : 64)), (lvoid*)(sk + (4 * w + kb) * 1024), 16, 0, 0);
   };
   auto copy_v = [&](char* sv, int t, int pid) __attribute__((always_inline)) {
-    const int blk = min(2 * t + (w >> 1), last_blk);
-    const __bf16* page = SRC == PACKED ? nullptr : vh + (long long)pid * a.v_st + (long long)(blk & inpage) * (BLK * a.dv);
+    const int r0 = min(t * FP_KEYS + rows16, kv_end - 1), blk = min(2 * t + (w >> 1), last_blk);
+    const char* src = reinterpret_cast<const char*>(
+        SRC == PACKED ? vh + (long long)r0 * a.v_st : vh + (long long)pid * a.v_st + (long long)(blk & inpage) * (BLK * a.dv));
 #pragma unroll
     for (int i = 0; i < VI; ++i) {
-      const __bf16* src;
-      int kb = vkb(i);
-      if constexpr (SRC == PACKED) {
-        src = vh + (long long)min(t * FP_KEYS + vrow(i), kv_end - 1) * a.v_st + 8 * vchunk;
-      } else if constexpr (TILED) {
-        kb = w * DV32 + i;
-        src = page + min(kb - (w >> 1) * 2 * DV32, a.dv / 16 - 1) * 512 + lane * 8;
-      } else {
-        src = page + (vrow(i) - 32 * (w >> 1)) * a.dv + 8 * vchunk;
-      }
-      __builtin_amdgcn_global_load_lds((gvoid*)src, (lvoid*)(sv + kb * VKB), 16, 0, 0);
+      const int kb = TILED ? w * DV32 + i : vkb(i);
+      unsigned off;
+      if constexpr (SRC == PACKED) off = __umul24(min(vrow(i), kv_end - 1 - r0), (unsigned)a.v_st * 2) + 16 * vchunk;
+      else if constexpr (TILED) off = min(kb - (w >> 1) * 2 * DV32, a.dv / 16 - 1) * 1024 + lane * 16;
+      else off = vrow(i) * (2 * a.dv) + 16 * vchunk;
+      __builtin_amdgcn_global_load_lds((gvoid*)(src + off), (lvoid*)(sv + kb * VKB), 16, 0, 0);
     }
   };
   // A tile's copies are asked for while the ones before it are computed; past the wait and the barrier they have arrived
@@ -337,11 +348,13 @@ __global__ __launch_bounds__(256, 2) void palu_flash_prefill_kernel(const FlashP
     if (__any(mx > m_run + LAZY_RESCALE_LOG2)) {
       const float top = fmaxf(mx, __shfl_xor(mx, 32, 64)), mn = top > m_run + LAZY_RESCALE_LOG2 ? top : m_run;
       const float alpha = m_run == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(m_run - mn);
+      if (__any(m_run != NEG_INF)) {                      // (not at the first tile)
 #pragma unroll
-      for (int md = 0; md < DV32; ++md)
+        for (int md = 0; md < DV32; ++md)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) O[md][i] *= alpha;
-      l_run *= alpha;
+          for (int i = 0; i < 16; ++i) O[md][i] *= alpha;
+        l_run *= alpha;
+      }
       m_run = mn;
     }
     return m_run == NEG_INF ? 0.f : m_run;
@@ -356,6 +369,7 @@ __global__ __launch_bounds__(256, 2) void palu_flash_prefill_kernel(const FlashP
       p[b][tt][lo + i] = (__bf16)e[i];
     }
     l_run += (e[0] + e[1]) + (e[2] + e[3]);
+    asm volatile("" : "+v"(l_run));                       // now: put off, the sums would keep all their terms in registers
   };
   // Operand c of a tile's products with V, md innermost: consecutive products have different accumulators. Operands are
   // read ahead of their products, K two eighths and V three products: a read from LDS takes as long as some four products.
@@ -424,13 +438,12 @@ __global__ __launch_bounds__(256, 2) void palu_flash_prefill_kernel(const FlashP
   auto tail = [&](f32x16 (&s)[2], const char* skn, const char* sv, int t) __attribute__((always_inline)) {
     const int base = t * FP_KEYS;
     if (base > w_hi) return;                              // uniform per wave: keys past all its rows
-#pragma unroll
+    const int seen = pos - base - 8 * h;                  // register i of block b holds key 32 b + 16 (j % 2) + 4 (j / 2) + i % 4,
+#pragma unroll                                            // j = i / 4, from base + 8 h on
     for (int b = 0; b < 2; ++b)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int j = i >> 2, key = base + 32 * b + 8 * (2 * (j & 1) + h) + 4 * (j >> 1) + (i & 3);
-        if (key > pos) s[b][i] = NEG_INF;
-      }
+      for (int i = 0; i < 16; ++i)
+        if (32 * b + 16 * ((i >> 2) & 1) + 4 * (i >> 3) + (i & 3) > seen) s[b][i] = NEG_INF;
     const float mref = maximum(s);
     bf16x8 p[2][2];
 #pragma unroll
@@ -453,23 +466,21 @@ __global__ __launch_bounds__(256, 2) void palu_flash_prefill_kernel(const FlashP
     }
     const float b4 = (bad[0] + bad[1]) + (bad[2] + bad[3]);
     if (__any(b4 != b4)) {
-      for (int x = 0; x < FP_KEYS && base + x <= w_hi; ++x) {
-        const int bt = x >> 4;
-        bf16x8 px = p[0][0];
 #pragma unroll
-        for (int i = 1; i < 4; ++i)
-          if (bt == i) px = p[i >> 1][i & 1];
+      for (int md = 0; md < DV32; ++md)
+        for (int x = 0; x < FP_KEYS && base + x <= w_hi; ++x) {
+          const int bt = x >> 4;
+          bf16x8 px = p[0][0];
 #pragma unroll
-        for (int md = 0; md < DV32; ++md) {
+          for (int i = 1; i < 4; ++i)
+            if (bt == i) px = p[i >> 1][i & 1];
           bf16x8 v = read_v(sv, bt >> 1, bt & 1, md);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = 8 * h + i == (x & 15) ? v[i] : (__bf16)0.f;
+          for (int i = 0; i < 8; ++i) v[i] = i == (x & 15) - 8 * h ? v[i] : (__bf16)0.f;
           const f32x16 y = mfma32(v, px, O[md]);
 #pragma unroll
           for (int i = 0; i < 16; ++i) O[md][i] = base + x <= pos ? y[i] : O[md][i];
-          fence();
         }
-      }
     } else {
       values(sv, p, 0);
     }
@@ -622,7 +633,9 @@ int launch_prefill(FlashPrefillArgs& a, long long max_keys, void* workspace, siz
   return rc;
 }
 
-bool stride_ok(long long st, long long least) { return st >= least && st % 8 == 0; }
+// (a lane's offset in a block of 32 rows is a 24-bit product)
+bool stride_ok(long long st) { return st >= 0 && st % 8 == 0; }
+bool row_stride_ok(long long st) { return stride_ok(st) && st < (1 << 22); }
 
 }  // namespace
 
@@ -641,9 +654,9 @@ extern "C" int palu_flash_prefill(const void* q, long long q_row_stride, long lo
   const char* who = "palu_flash_prefill";
   if (!q || !k || !v || !cu_seqlens || !out) return fail(PALU_EINVAL, "%s: a required pointer is null", who);
   if (int rc = check_dims(rows, batch, n_q, n_kv, head_dim_v, who)) return rc;
-  if (!stride_ok(q_row_stride, 0) || !stride_ok(q_head_stride, 0) || !stride_ok(k_row_stride, 0) || !stride_ok(k_head_stride, 0) ||
-      !stride_ok(v_row_stride, 0) || !stride_ok(v_head_stride, 0))
-    return fail(PALU_EINVAL, "%s: strides must be non-negative multiples of 8", who);
+  if (!stride_ok(q_row_stride) || !stride_ok(q_head_stride) || !row_stride_ok(k_row_stride) || !stride_ok(k_head_stride) ||
+      !row_stride_ok(v_row_stride) || !stride_ok(v_head_stride))
+    return fail(PALU_EINVAL, "%s: strides must be non-negative multiples of 8, rows of k and v less than 2^22 apart", who);
   if (!al16(q) || !al16(k) || !al16(v) || !al16(out)) return fail(PALU_EINVAL, "%s: 16-byte alignment required", who);
   FlashPrefillArgs a{static_cast<const __bf16*>(q), q_row_stride, q_head_stride, static_cast<const __bf16*>(k),
                      static_cast<const __bf16*>(v), k_row_stride, k_head_stride, v_row_stride, v_head_stride, cu_seqlens, nullptr,
@@ -666,7 +679,7 @@ extern "C" int palu_flash_prefill_paged(const void* q, long long q_row_stride, l
   if (int rc = check_dims(rows, batch, n_q, n_kv, head_dim_v, who)) return rc;
   if (cache_layout != PALU_LAYOUT_ROWS && cache_layout != PALU_LAYOUT_TILED)
     return fail(PALU_EINVAL, "%s: cache layout must be PALU_LAYOUT_ROWS or PALU_LAYOUT_TILED, got %d", who, cache_layout);
-  if (!stride_ok(q_row_stride, 0) || !stride_ok(q_head_stride, 0))
+  if (!stride_ok(q_row_stride) || !stride_ok(q_head_stride))
     return fail(PALU_EINVAL, "%s: strides must be non-negative multiples of 8", who);
   if (!al16(q) || !al16(k_pages) || !al16(v_pages) || !al16(out)) return fail(PALU_EINVAL, "%s: 16-byte alignment required", who);
   const long long k_sh = (long long)page_size * HD, v_sh = (long long)page_size * head_dim_v;

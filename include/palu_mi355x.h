@@ -425,25 +425,26 @@ size_t palu_prefill_workspace_bytes(int users, int seq, int n_heads, int n_kv, i
  *   q [rows][n_q][128], k [rows][n_kv][128], v [rows][n_kv][head_dim_v] bf16, rows and heads at the element strides given
  *   (multiples of 8; head_dim_v a multiple of 16 up to 128); out [rows][n_q][head_dim_v] bf16, dense, not overlapping them.
  * Head h reads KV head h / (n_q / n_kv). fp32 scores, statistics and sums; probabilities rounded to bf16 for their
- * product with V. A NaN or infinity in K or V reaches the rows that see it and no others. workspace:
- * palu_flash_prefill_workspace_bytes with max_keys = rows; calls that share one must be ordered on one stream. */
+ * product with V. A NaN or infinity in K or V reaches the rows that see it and no others. */
 int palu_flash_prefill(const void* q, long long q_row_stride, long long q_head_stride, const void* k, long long k_row_stride,
                        long long k_head_stride, const void* v, long long v_row_stride, long long v_head_stride,
                        const int32_t* cu_seqlens, void* out, float scale, int rows, int batch, int n_q, int n_kv,
-                       int head_dim_v, void* workspace, size_t workspace_bytes, palu_stream_t stream);
+                       int head_dim_v, palu_stream_t stream);
 
 /* The same over page pools k_pages [num_pages][n_kv][page_size][128], v_pages [..][head_dim_v]: row i of sequence b stands
  * at position start_pos[b] + i (start_pos NULL: i) and sees positions 0 .. that of the sequence's pages, which hold the new
  * rows' keys and values already (palu_latent_fill_paged). A row at a negative position sees nothing and gets zeros; one past
- * the table's max_pages_per_seq * page_size positions sees those. Page ids are clamped into the pool. workspace as
- * above with max_keys = max_pages_per_seq * page_size: the keys of few rows are split among workgroups. */
+ * the table's max_pages_per_seq * page_size positions sees those. Page ids are clamped into the pool. Where few rows stand on
+ * long contexts, their keys are cut into pieces for several workgroups, which meet in the workspace
+ * (palu_flash_prefill_workspace_bytes; any contents; calls that share one must be ordered on one stream). */
 int palu_flash_prefill_paged(const void* q, long long q_row_stride, long long q_head_stride, const void* k_pages,
                              const void* v_pages, const int32_t* cu_seqlens, const int32_t* start_pos,
                              const int32_t* page_table, void* out, float scale, int rows, int batch, int n_q, int n_kv,
                              int num_pages, int page_size, int max_pages_per_seq, int head_dim_v, int cache_layout,
                              void* workspace, size_t workspace_bytes, palu_stream_t stream);
 
-/* Workspace bytes of palu_flash_prefill / _paged (0 when no keys are split, and for invalid shapes). */
+/* Workspace bytes of palu_flash_prefill_paged, max_keys = max_pages_per_seq * page_size (0 when no keys are cut, and for
+ * invalid shapes). */
 size_t palu_flash_prefill_workspace_bytes(int rows, int batch, int n_q, int n_kv, int max_keys, int head_dim_v);
 
 /* Packed rows into a page pool [num_pages][n_groups][page_size][width] (cache_layout PALU_LAYOUT_ROWS, _TILED or _TILED_V):

@@ -31,7 +31,7 @@ def _refused(lib, rc, code, what):
     (dict(k=P + 8), _native.PALU_EINVAL, "16-byte"), (dict(out=P + 2), _native.PALU_EINVAL, "16-byte")])
 def test_flash_prefill_refusals(lib, kw, code, what):
     a = dict(q=P, q_st=1024, q_sh=128, k=P, k_st=256, k_sh=128, v=P, v_st=128, v_sh=64, cu=P, out=P, scale=0.1, rows=5, batch=1, n_q=8,
-             n_kv=2, dv=64, ws=None, bytes=0, stream=None)
+             n_kv=2, dv=64, stream=None)
     a.update(kw)
     _refused(lib, lib.palu_flash_prefill(*a.values()), code, what)
 
@@ -52,11 +52,11 @@ def test_flash_prefill_paged_refusals(lib, kw, code, what):
 
 
 def test_flash_prefill_workspace(lib):
-    """None where the tiles fill the chip or the keys are few; a slot per tile, KV head and split else."""
+    """None for contexts that are not cut, slots of 128 rows for every KV head else."""
     f = lib.palu_flash_prefill_workspace_bytes
-    assert f(8192, 1, 32, 8, 8192, 128) == 0 and f(24, 1, 32, 8, 24, 128) == 0 and f(1, 1, 32, 8, 256, 128) == 0
+    assert f(1, 1, 32, 8, 256, 128) == 0 and f(1 << 24, 1, 32, 8, 65536, 128) == 0
     need = f(1, 1, 32, 8, 32768, 128)
-    assert need > 0 and need % (8 * 128 * 130 * 4) == 0
+    assert need > 0 and need % (8 * (128 * 130 * 4 + 32)) == 0
     assert f(0, 1, 32, 8, 100, 128) == 0 and f(5, 1, 7, 2, 100, 128) == 0 and f(5, 1, 8, 2, -1, 128) == 0
 
 

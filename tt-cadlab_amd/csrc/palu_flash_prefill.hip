@@ -24,8 +24,9 @@ namespace {
 
 constexpr int FP_ROWS = 128;              // rows of a tile: 4 waves of 32
 constexpr int FP_KEYS = 64;               // keys of a K / V tile: two 32-position blocks
-constexpr int FP_MIN_SPLIT = 4;           // key tiles of a split, at least
+constexpr int FP_MIN_KEYS = 256;          // keys of a piece of a split tile, about, at least
 constexpr int FP_WGS = 512;               // workgroups that the chip holds at once (two a CU)
+constexpr float FP_PIECE = 1.05f;         // a piece has at most about this share of a workgroup slot's part of the batch's keys
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -33,6 +34,11 @@ typedef __attribute__((address_space(1))) const void gvoid;
 typedef __attribute__((address_space(3))) void lvoid;
 
 enum Source { PACKED, PAGED_ROWS, PAGED_TILED };
+
+// What the join reads of an item: of a tile's first piece the number of pieces and its rows, else 0 pieces.
+struct Record {
+  int pieces, rows, beg, start, pos0, rem, unused[2];
+};
 
 struct FlashPrefillArgs {
   const __bf16* q;
@@ -48,12 +54,10 @@ struct FlashPrefillArgs {
   float qscale;                           // |scale| * log2 e (1 for a scale of 0: a masked score times 0 would be NaN)
   int sign;                               // of the scale: -1, 0, 1; Q is taken times that
   __bf16* out;                            // [T][n_q][dv]
-  int nsplit;                             // parts that the keys of a tile may be split into
-  float* part;                            // nsplit > 1: unnormalised O of every (item, split) [FP_ROWS][dv], then m and l [FP_ROWS] each
+  float* part;                            // where keys may be split: unnormalised O of a piece [FP_ROWS][dv], then m and l [FP_ROWS] each
+  Record* records;                        // of the items that may be pieces: `cut` per KV head
+  int cut;
 };
-
-// Key tiles first .. last of split s of an item of nt key tiles, and how many splits that item has.
-__device__ __forceinline__ int split_tiles(int nt, int nsplit) { return max(FP_MIN_SPLIT, (nt + nsplit - 1) / nsplit); }
 
 __device__ __forceinline__ f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
@@ -66,22 +70,26 @@ struct Seq {
 __device__ __forceinline__ Seq lane_seq(const FlashPrefillArgs& a, int b) {
   const int c0 = a.cu[b], c1 = a.cu[b + 1];
   const int beg = min(max(c0, 0), a.T), end = min(max(c1, beg), a.T);
-  const int s = a.start ? a.start[b] : 0;
-  return Seq{beg, end - beg, min(max(s, -(1 << 24)), 1 << 24)};
+  const int s = a.start ? a.start[b] : 0;                 // (rows past the capacity see all keys, before 0 none, however far)
+  return Seq{beg, end - beg, min(max(s, -(1 << 30)), a.capacity)};
 }
 
 // Work order: all tiles of the batch, those with the most keys first, so that the last ones to run are short. A tile's
-// level is its distance from position 0 in tiles, rounded down; item w of the descending order is found by halving over
-// levels, the lanes counting the tiles of a sequence each (all waves do it, without a barrier; four sequences of a lane stay in
-// registers, further ones are read again for every level).
+// level is its distance from position 0 in tiles (of a power of two positions), rounded down; item w of the descending order is
+// found by halving over levels, the lanes counting the tiles of a sequence each (all waves do it, without a barrier; four
+// sequences of a lane stay in registers, further ones are read again for every level).
+// Where a.part is given, a tile of level t is cut along its keys into t / len + 3 / 4 pieces (one below 1.25 len), items of
+// their own, next to each other: len levels are FP_PIECE times what a workgroup slot gets of the whole batch, so the batch is cut
+// only where single tiles are long for it (few new rows over long contexts).
 struct Tile {
   int b, j;                               // j: tile of sequence b; b < 0: none
+  int piece, pieces;
   Seq seq;
 };
 __device__ __forceinline__ Tile find_tile(const FlashPrefillArgs& a, int w) {
   constexpr int R = 4;
   const int lane = threadIdx.x & 63;
-  const int shift = 31 - __builtin_clz(max(1, FP_ROWS / a.rep));   // positions of a tile, as a power of two: for the order only
+  const int shift = 31 - __builtin_clz(max(1, FP_ROWS / a.rep));
   struct Levels {
     int base, n;
   };
@@ -101,21 +109,38 @@ __device__ __forceinline__ Tile find_tile(const FlashPrefillArgs& a, int w) {
       lv[r] = levels(own[r]);
     }
   }
-  auto above = [](Levels l, int t) { return min(max(l.base + l.n - t, 0), l.n); };
-  auto count = [&](int t) {               // tiles at level t or above
-    int c = 0;
-#pragma unroll
-    for (int r = 0; r < R; ++r) c += above(lv[r], t);
-    for (int b0 = 64 * R; b0 < a.B; b0 += 64) c += above(levels(load(b0 + lane)), t);
-    return wave_sum_i(c);
-  };
-  if (a.B == 1) {                         // one sequence: its tiles from the last on
+  if (a.B == 1 && !a.part) {              // one sequence: its tiles from the last on
     const Seq s{__builtin_amdgcn_readfirstlane(own[0].beg), __builtin_amdgcn_readfirstlane(own[0].len),
                 __builtin_amdgcn_readfirstlane(own[0].start)};
     const int n = levels(s).n;
-    return Tile{w < n ? 0 : -1, n - 1 - w, s};
+    return Tile{w < n ? 0 : -1, n - 1 - w, 0, 1, s};
   }
-  if (w >= count(0)) return Tile{-1, 0, {}};
+  // a sum over all sequences' levels
+  auto over_all = [&](auto f) {
+    auto x = f(lv[0]);
+#pragma unroll
+    for (int r = 1; r < R; ++r) x += f(lv[r]);
+    for (int b0 = 64 * R; b0 < a.B; b0 += 64) x += f(levels(load(b0 + lane)));
+    return x;
+  };
+  FDiv len = make_fdiv(1 << 30);          // levels of a piece
+  if (a.part) {
+    float keys = over_all([](Levels l) { return (float)l.n * ((float)l.base + 0.5f * (float)(l.n + 1)); });
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) keys += __shfl_xor(keys, o, 64);
+    const float most = fmaxf((float)(FP_MIN_KEYS >> shift), ceilf(keys * (float)a.n_kv * (FP_PIECE / FP_WGS)));
+    len = make_fdiv((int)fminf(fmaxf(most, 2.f), 1e9f));
+  }
+  const int round = len.d - (len.d >> 2) - 1;
+  auto pieces_below = [&](int t) {        // of one tile at each of levels 0 .. t - 1
+    if (!a.part) return t;
+    const int u = t + round, q = fdiv(u, len);            // the sum of u / len, and 1 in place of each 0
+    return q * (q - 1) / 2 * len.d + (u - q * len.d) * q + min(t, len.d - round);
+  };
+  auto count = [&](int t) {               // pieces at level t or above
+    return wave_sum_i(over_all([&](Levels l) { return l.base + l.n > t ? pieces_below(l.base + l.n) - pieces_below(max(l.base, t)) : 0; }));
+  };
+  if (w >= count(0)) return Tile{-1, 0, 0, 1, {}};
   int top = 0;                            // one past the highest level
 #pragma unroll
   for (int r = 0; r < R; ++r) top = max(top, lv[r].n ? lv[r].base + lv[r].n : 0);
@@ -131,8 +156,11 @@ __device__ __forceinline__ Tile find_tile(const FlashPrefillArgs& a, int w) {
     if (count(mid) > w) lo = mid;
     else hi = mid;
   }
-  int r = w - count(lo + 1);              // which of the sequences that have level lo
-  Tile found{-1, 0, {}};
+  const int pieces = a.part ? max(1, __builtin_amdgcn_readfirstlane(fdiv(lo + round, len))) : 1;
+  int r = w - count(lo + 1);              // which piece of the sequences that have level lo
+  const int piece = r % pieces;
+  r /= pieces;
+  Tile found{-1, 0, 0, 1, {}};
   auto pick = [&](int b0, const Seq& s) {
     const Levels l = levels(s);
     const unsigned long long m = __ballot(l.n > 0 && l.base <= lo && lo < l.base + l.n);
@@ -140,8 +168,8 @@ __device__ __forceinline__ Tile find_tile(const FlashPrefillArgs& a, int w) {
     if (r >= 0 && r < c) {
       const unsigned long long me = __ballot(((m >> lane) & 1) && __popcll(m & ((1ull << lane) - 1)) == r);
       const int x = __builtin_ctzll(me);
-      found = Tile{b0 + x, lo - __builtin_amdgcn_readlane(l.base, x), {__builtin_amdgcn_readlane(s.beg, x),
-                   __builtin_amdgcn_readlane(s.len, x), __builtin_amdgcn_readlane(s.start, x)}};
+      found = Tile{b0 + x, lo - __builtin_amdgcn_readlane(l.base, x), piece, pieces,
+                   {__builtin_amdgcn_readlane(s.beg, x), __builtin_amdgcn_readlane(s.len, x), __builtin_amdgcn_readlane(s.start, x)}};
     }
     r -= c;
   };
@@ -180,9 +208,15 @@ __global__ __launch_bounds__(256, 2) void palu_flash_prefill_kernel(const FlashP
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   // A KV head's workgroups are n_kv ids apart, for 8 heads all on one XCD, whose L2 then holds that head's K and V.
   const int kvh = blockIdx.x % a.n_kv;
-  const int item = blockIdx.x / a.n_kv / a.nsplit, split = blockIdx.x / a.n_kv - item * a.nsplit;
-  const Tile tile = find_tile(a, item);
-  if (tile.b < 0) return;                 // uniform, before any barrier
+  const Tile tile = find_tile(a, blockIdx.x / a.n_kv);
+  const bool recorded = blockIdx.x / a.n_kv < a.cut;
+  auto record = [&](const Record& r) {
+    if (recorded && threadIdx.x == 0) a.records[blockIdx.x] = r;
+  };
+  if (tile.b < 0) {                       // uniform, before any barrier
+    record(Record{});
+    return;
+  }
   const Seq sq = tile.seq;
   const int row0 = tile.j * FP_ROWS, rows = min(sq.len * a.rep - row0, FP_ROWS);   // rows of this tile
   const RowSplit rs = split_rows(row0, a.rep);
@@ -190,9 +224,11 @@ __global__ __launch_bounds__(256, 2) void palu_flash_prefill_kernel(const FlashP
   auto key_pos = [&](int x) { return __builtin_amdgcn_readfirstlane(min(sq.start + row_pos(rs, x), a.capacity - 1)); };
   const int kv_end = key_pos(rows - 1) + 1;               // keys of this workgroup
   const int nt_all = kv_end > 0 ? (kv_end + FP_KEYS - 1) / FP_KEYS : 0;
-  const int per_split = split_tiles(nt_all, a.nsplit);
-  const int t_lo = split * per_split, nt = min(nt_all, t_lo + per_split);
-  if (t_lo >= nt && split > 0) return;    // uniform
+  const int per_piece = (nt_all + tile.pieces - 1) / tile.pieces;
+  const int t_lo = tile.piece * per_piece, nt = min(nt_all, t_lo + per_piece);
+  const int n_pieces = nt_all > per_piece ? (nt_all + per_piece - 1) / per_piece : 1;
+  record(n_pieces > 1 && tile.piece == 0 ? Record{n_pieces, rows, sq.beg, sq.start, rs.pos0, rs.rem, {}} : Record{});
+  if (t_lo >= nt && tile.piece > 0) return;   // uniform
 
   // ---- copies to LDS: wave w copies keys 16 w .. + 15 of a tile (half-block w % 2 of block w / 2 for K) ---------
   const int last_blk = (kv_end - 1) >> 5, inpage = (1 << a.page_shift) - 1;
@@ -515,9 +551,8 @@ __global__ __launch_bounds__(256, 2) void palu_flash_prefill_kernel(const FlashP
 
   const float l = l_run + __shfl_xor(l_run, 32, 64);
   if (32 * w + n >= rows) return;
-  if (nt_all > per_split) {               // one of several splits
-    const long long slot = ((long long)item * a.n_kv + kvh) * a.nsplit + split;
-    float* po = a.part + slot * FP_ROWS * (a.dv + 2);
+  if (n_pieces > 1) {                     // one of several pieces (which are the first of all items)
+    float* po = a.part + (long long)blockIdx.x * FP_ROWS * (a.dv + 2);
     const int r = 32 * w + n;
     if (h == 0) {
       po[FP_ROWS * a.dv + r] = m_run;
@@ -547,54 +582,66 @@ __global__ __launch_bounds__(256, 2) void palu_flash_prefill_kernel(const FlashP
     }
 }
 
-// Joins the splits of an item: out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s. One workgroup per (item, KV head, 32 rows),
-// eight threads to a row.
+// Joins the pieces of a tile: out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s. One workgroup per (item, KV head, 32 rows), 32
+// threads to a row, those of a first piece work; what the item is stands in its record. Bound by latency: a row's threads
+// share the pieces' statistics, and the loads of eight pieces are in flight at once.
+constexpr int JOIN_ROWS = 32;
 __global__ __launch_bounds__(256) void palu_flash_prefill_join_kernel(const FlashPrefillArgs a) {
-  const int kvh = blockIdx.x % a.n_kv, rest = blockIdx.x / a.n_kv, item = rest >> 2;
-  const Tile tile = find_tile(a, item);
-  if (tile.b < 0) return;
-  const Seq sq = tile.seq;
-  const int row0 = tile.j * FP_ROWS, rows = min(sq.len * a.rep - row0, FP_ROWS);
-  const RowSplit rs = split_rows(row0, a.rep);
-  const int last = min(sq.start + row_pos(rs, rows - 1), a.capacity - 1);
-  const int nt = last >= 0 ? last / FP_KEYS + 1 : 0, per = split_tiles(nt, a.nsplit);
-  const int r = (rest & 3) * 32 + (threadIdx.x >> 3);
-  if (nt <= per || r >= rows) return;
-  const int ns = (nt + per - 1) / per, ri = row_pos(rs, r);
-  const long long stride = (long long)FP_ROWS * (a.dv + 2);
-  const float* part = a.part + ((long long)item * a.n_kv + kvh) * a.nsplit * stride;
-  const float* ml = part + FP_ROWS * a.dv + r;
-  float M = NEG_INF, l = 0.f;
-  for (int s = 0; s < ns; ++s) M = fmaxf(M, ml[s * stride]);
-  const float ref = M == NEG_INF ? 0.f : M;
-  for (int s = 0; s < ns; ++s) l += __builtin_amdgcn_exp2f(ml[s * stride] - ref) * ml[s * stride + FP_ROWS];
-  const float inv = 1.f / l;
-  __bf16* o = a.out + ((long long)(sq.beg + ri) * a.n_q + (long long)kvh * a.rep + (rs.rem + r - (ri - rs.pos0) * a.rep)) * a.dv;
-  for (int d = 4 * (threadIdx.x & 7); d < a.dv; d += 32) {
+  const int rest = blockIdx.x / a.n_kv, kvh = blockIdx.x - rest * a.n_kv, item = rest / (FP_ROWS / JOIN_ROWS);
+  const Record rec = a.records[item * a.n_kv + kvh];
+  const int r0 = rest % (FP_ROWS / JOIN_ROWS) * JOIN_ROWS, sub = threadIdx.x & 31, ns = rec.pieces;
+  if (ns == 0 || r0 >= rec.rows) return;
+  const RowSplit rs{rec.pos0, rec.rem, make_fdiv(a.rep)};
+  const long long stride = (long long)FP_ROWS * (a.dv + 2) * a.n_kv;   // pieces are n_kv workgroups apart
+  const float* part = a.part + ((long long)item * a.n_kv + kvh) * FP_ROWS * (a.dv + 2);
+  for (int r = r0 + (threadIdx.x >> 5); r < min(r0 + JOIN_ROWS, rec.rows); r += 8) {
+    const float* ml = part + FP_ROWS * a.dv + r;
+    float M = NEG_INF, l = 0.f;
+    for (int s = sub; s < ns; s += 32) M = fmaxf(M, ml[s * stride]);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) M = fmaxf(M, __shfl_xor(M, o, 32));
+    const float ref = M == NEG_INF ? 0.f : M;
+    for (int s = sub; s < ns; s += 32) l += __builtin_amdgcn_exp2f(ml[s * stride] - ref) * ml[s * stride + FP_ROWS];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) l += __shfl_xor(l, o, 32);
+    const int d = 4 * sub, pos = row_pos(rs, r);
+    if (d >= a.dv) continue;
     f32x4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
     for (int s = 0; s < ns; ++s)
       y += *reinterpret_cast<const f32x4*>(part + s * stride + r * a.dv + d) * __builtin_amdgcn_exp2f(ml[s * stride] - ref);
+    const float inv = 1.f / l;
     bf16x4 x;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = sq.start + ri < 0 ? (__bf16)0.f : (__bf16)(y[i] * inv);
-    *reinterpret_cast<bf16x4*>(o + d) = x;
+    for (int i = 0; i < 4; ++i) x[i] = rec.start + pos < 0 ? (__bf16)0.f : (__bf16)(y[i] * inv);
+    *reinterpret_cast<bf16x4*>(a.out + ((long long)(rec.beg + pos) * a.n_q + (long long)kvh * a.rep +
+                                        (rs.rem + r - (pos - rs.pos0) * a.rep)) * a.dv + d) = x;
   }
 }
 
 // Tiles of a batch, at most: a sequence's last tile may hold fewer rows.
 long long most_tiles(int T, int B, int rep) { return (long long)T * rep / FP_ROWS + std::min(T, B); }
 
-// Splits per tile: enough workgroups for the chip where the tiles are few, none of them under FP_MIN_SPLIT key tiles.
-int split_count(int T, int B, int n_q, int n_kv, long long max_keys) {
-  const long long items = most_tiles(T, B, n_q / n_kv) * n_kv;
-  return (int)std::max<long long>(1, std::min<long long>(FP_WGS / items, max_keys / (FP_MIN_SPLIT * FP_KEYS)));
+// Whether tiles may be cut along their keys: where contexts stand before the rows. (Packed prompts stand on their own keys; cutting
+// their longest tiles, one prompt of 1024 positions took 42 us instead of 27 and one of 2048 82 instead of 55.)
+bool may_split(int T, int n_q, bool paged, long long max_keys) {
+  return paged && max_keys > FP_MIN_KEYS && (long long)T * n_q <= (1ll << 28);   // (find_tile's levels stay below 2^22)
 }
+// Pieces of cut tiles per KV head, at most: with len levels to a piece, a tile of level t >= 1.25 len has at most t / len + 3 / 4
+// <= 2 t / len, and the levels' sum is at most FP_WGS / (FP_PIECE n_kv) times len.
+long long most_pieces(int n_kv) { return (long long)(2 * FP_WGS / FP_PIECE) / n_kv + 2; }
 
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-size_t part_bytes(int T, int B, int n_q, int n_kv, long long max_keys, int dv) {
-  const int ns = split_count(T, B, n_q, n_kv, max_keys);
-  return ns == 1 ? 0 : (size_t)most_tiles(T, B, n_q / n_kv) * n_kv * ns * FP_ROWS * (dv + 2) * sizeof(float);
+// Items of a KV head that may be pieces, where tiles may be cut.
+long long cut_items(int T, int B, int n_q, int n_kv) {
+  return std::min(most_tiles(T, B, n_q / n_kv) + most_pieces(n_kv), most_pieces(n_kv));
+}
+
+// Workspace: the pieces' partial results, then the items' records.
+size_t part_bytes(int n_q, int n_kv, int T, int B, bool paged, long long max_keys, int dv) {
+  if (!may_split(T, n_q, paged, max_keys)) return 0;
+  return (size_t)cut_items(T, B, n_q, n_kv) * n_kv * (FP_ROWS * (dv + 2) * sizeof(float) + sizeof(Record));
 }
 
 int check_dims(int T, int B, int n_q, int n_kv, int dv, const char* who) {
@@ -603,33 +650,35 @@ int check_dims(int T, int B, int n_q, int n_kv, int dv, const char* who) {
   if (n_q % n_kv) return fail(PALU_EINVAL, "%s: n_q = %d must be a multiple of the KV head count %d", who, n_q, n_kv);
   if (dv < 16 || dv > HD || dv % 16)
     return fail(PALU_EUNSUPPORTED, "%s: head_dim_v %d (multiples of 16 up to %d)", who, dv, HD);
-  if ((long long)T * n_q > (1ll << 30) || (long long)B > (1 << 24))
+  if ((long long)T * n_q > (1ll << 30) || n_q > 65535 || B > (1 << 24))
     return fail(PALU_EUNSUPPORTED, "%s: %d rows of %d heads in %d sequences exceed the grid", who, T, n_q, B);
   return PALU_OK;
 }
 
 template <Source SRC>
 int launch_prefill(FlashPrefillArgs& a, long long max_keys, void* workspace, size_t workspace_bytes, const char* who, hipStream_t s) {
-  a.nsplit = split_count(a.T, a.B, a.n_q, a.n_kv, max_keys);
-  const size_t need = part_bytes(a.T, a.B, a.n_q, a.n_kv, max_keys, a.dv);
+  const size_t need = part_bytes(a.n_q, a.n_kv, a.T, a.B, SRC != PACKED, max_keys, a.dv);
   if (need && (!workspace || workspace_bytes < need || !al16(workspace)))
     return fail(PALU_EINVAL, "%s: a 16-byte aligned workspace of %zu bytes needed (palu_flash_prefill_workspace_bytes), got %zu", who,
                 need, workspace ? workspace_bytes : 0);
-  a.part = static_cast<float*>(workspace);
-  const unsigned items = (unsigned)(most_tiles(a.T, a.B, a.rep) * a.n_kv);
-  auto go = [&](auto kern, unsigned grid) {
-    hipLaunchKernelGGL(kern, dim3(grid), dim3(256), 0, s, a);
+  a.cut = need ? (int)cut_items(a.T, a.B, a.n_q, a.n_kv) : 0;
+  a.part = need ? static_cast<float*>(workspace) : nullptr;
+  a.records = reinterpret_cast<Record*>(a.part + (size_t)a.cut * a.n_kv * FP_ROWS * (a.dv + 2));
+  const long long pieces = need ? most_pieces(a.n_kv) : 0;
+  const unsigned grid = (unsigned)((most_tiles(a.T, a.B, a.rep) + pieces) * a.n_kv);
+  auto go = [&](auto kern, unsigned wgs) {
+    hipLaunchKernelGGL(kern, dim3(wgs), dim3(256), 0, s, a);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? PALU_OK : fail(PALU_EHIP, "%s launch: %s", who, hipGetErrorString(e));
   };
   int rc = PALU_OK;
   switch ((a.dv + 31) / 32) {
-    case 1: rc = go(palu_flash_prefill_kernel<SRC, 1>, items * a.nsplit); break;
-    case 2: rc = go(palu_flash_prefill_kernel<SRC, 2>, items * a.nsplit); break;
-    case 3: rc = go(palu_flash_prefill_kernel<SRC, 3>, items * a.nsplit); break;
-    default: rc = go(palu_flash_prefill_kernel<SRC, 4>, items * a.nsplit); break;
+    case 1: rc = go(palu_flash_prefill_kernel<SRC, 1>, grid); break;
+    case 2: rc = go(palu_flash_prefill_kernel<SRC, 2>, grid); break;
+    case 3: rc = go(palu_flash_prefill_kernel<SRC, 3>, grid); break;
+    default: rc = go(palu_flash_prefill_kernel<SRC, 4>, grid); break;
   }
-  if (rc == PALU_OK && a.nsplit > 1) rc = go(palu_flash_prefill_join_kernel, items * 4);
+  if (rc == PALU_OK && need) rc = go(palu_flash_prefill_join_kernel, (unsigned)(a.cut * a.n_kv) * (FP_ROWS / JOIN_ROWS));
   return rc;
 }
 
@@ -642,14 +691,13 @@ bool row_stride_ok(long long st) { return stride_ok(st) && st < (1 << 22); }
 extern "C" size_t palu_flash_prefill_workspace_bytes(int rows, int batch, int n_q, int n_kv, int max_keys, int head_dim_v) {
   palu::g_err[0] = 0;
   if (max_keys <= 0 || check_dims(rows, batch, n_q, n_kv, head_dim_v, "palu_flash_prefill_workspace_bytes")) return 0;
-  return part_bytes(rows, batch, n_q, n_kv, max_keys, head_dim_v);
+  return part_bytes(n_q, n_kv, rows, batch, true, max_keys, head_dim_v);
 }
 
 extern "C" int palu_flash_prefill(const void* q, long long q_row_stride, long long q_head_stride, const void* k,
                                   long long k_row_stride, long long k_head_stride, const void* v, long long v_row_stride,
                                   long long v_head_stride, const int32_t* cu_seqlens, void* out, float scale, int rows,
-                                  int batch, int n_q, int n_kv, int head_dim_v, void* workspace, size_t workspace_bytes,
-                                  hipStream_t stream) {
+                                  int batch, int n_q, int n_kv, int head_dim_v, hipStream_t stream) {
   palu::g_err[0] = 0;
   const char* who = "palu_flash_prefill";
   if (!q || !k || !v || !cu_seqlens || !out) return fail(PALU_EINVAL, "%s: a required pointer is null", who);
@@ -662,8 +710,8 @@ extern "C" int palu_flash_prefill(const void* q, long long q_row_stride, long lo
                      static_cast<const __bf16*>(v), k_row_stride, k_head_stride, v_row_stride, v_head_stride, cu_seqlens, nullptr,
                      nullptr, 0, 0, 0, 0x7fffffff, rows, batch, n_q, n_kv, n_q / n_kv, head_dim_v,
                      scale == 0.f ? 1.f : fabsf(scale) * 1.44269504088896340736f, (scale > 0.f) - (scale < 0.f),
-                     static_cast<__bf16*>(out), 1, nullptr};
-  return launch_prefill<PACKED>(a, rows, workspace, workspace_bytes, who, stream);
+                     static_cast<__bf16*>(out), nullptr, nullptr, 0};
+  return launch_prefill<PACKED>(a, 0, nullptr, 0, who, stream);
 }
 
 extern "C" int palu_flash_prefill_paged(const void* q, long long q_row_stride, long long q_head_stride, const void* k_pages,
@@ -688,7 +736,7 @@ extern "C" int palu_flash_prefill_paged(const void* q, long long q_row_stride, l
                      static_cast<const __bf16*>(v_pages), k_sh * n_kv, k_sh, v_sh * n_kv, v_sh, cu_seqlens, start_pos, page_table,
                      max_pages_per_seq, num_pages, shift, capacity, rows, batch, n_q, n_kv, n_q / n_kv, head_dim_v,
                      scale == 0.f ? 1.f : fabsf(scale) * 1.44269504088896340736f, (scale > 0.f) - (scale < 0.f),
-                     static_cast<__bf16*>(out), 1, nullptr};
+                     static_cast<__bf16*>(out), nullptr, nullptr, 0};
   if (cache_layout == PALU_LAYOUT_TILED) return launch_prefill<PAGED_TILED>(a, capacity, workspace, workspace_bytes, who, stream);
   return launch_prefill<PAGED_ROWS>(a, capacity, workspace, workspace_bytes, who, stream);
 }

@@ -27,7 +27,7 @@ __device__ __forceinline__ void fill_seq(const FillArgs& a, int b, int& beg, int
   beg = min(max(c0, 0), a.T);
   len = min(max(c1, beg), a.T) - beg;
   start = a.start ? a.start[b] : 0;
-  start = min(max(start, -(1 << 24)), 1 << 24);
+  start = min(max(start, -(1 << 29)), 1 << 29);            // (farther is as far: at most 2^28 rows, 2^16 positions)
 }
 
 template <int LAYOUT>

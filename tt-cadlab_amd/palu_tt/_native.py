@@ -62,7 +62,7 @@ _SIGNATURES = {
     "palu_naive_decode": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _f, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _vp,
                                _sz, _vp]),
     "palu_naive_workspace_bytes": (_sz, [_i, _i, _i, _i]),
-    "palu_flash_prefill": (_i, [_vp, _ll, _ll, _vp, _ll, _ll, _vp, _ll, _ll, _vp, _vp, _f, _i, _i, _i, _i, _i, _vp, _sz, _vp]),
+    "palu_flash_prefill": (_i, [_vp, _ll, _ll, _vp, _ll, _ll, _vp, _ll, _ll, _vp, _vp, _f, _i, _i, _i, _i, _i, _vp]),
     "palu_flash_prefill_paged": (_i, [_vp, _ll, _ll, _vp, _vp, _vp, _vp, _vp, _vp, _f, _i, _i, _i, _i, _i, _i, _i, _i, _i,
                                       _vp, _sz, _vp]),
     "palu_flash_prefill_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i]),

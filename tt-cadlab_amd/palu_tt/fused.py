@@ -506,8 +506,9 @@ def flash_prefill(q, k, v, cu_seqlens, *, scale=None, head_dim_v=None, out=None,
     LatentCache) that hold the new rows already (paged_update_cache, paged_fill_cache), and row i of sequence b
     stands at position start_pos[b] + i (int32 [B]; None: i) behind the positions cached before. Query head h reads KV head
     h // (n_q // n_kv). head_dim_v: multiples of 16 up to 128. Returns [T, n_q, head_dim_v] bf16; rows past
-    cu_seqlens[B] are not written (``out``, which must not overlap the inputs, keeps what it held there). workspace: a uint8
-    device tensor of palu_flash_prefill_workspace_bytes(...) bytes, else one from torch's caching allocator where needed."""
+    cu_seqlens[B] are not written (``out``, which must not overlap the inputs, keeps what it held there). workspace (paged
+    calls): a uint8 device tensor of palu_flash_prefill_workspace_bytes(...) bytes, else one from torch's caching allocator where
+    few rows stand on long contexts."""
     q_st, q_sh = _strided_rows(q, "q", HEAD_DIM)
     dev = q.device
     T, n_q = q.shape[:2]
@@ -524,7 +525,6 @@ def flash_prefill(q, k, v, cu_seqlens, *, scale=None, head_dim_v=None, out=None,
         n_kv, dv = v.shape[1:]
         if k.shape[:2] != (T, n_kv) or v.shape[0] != T:
             raise RuntimeError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must have the {T} rows of q and the same heads")
-        max_keys = T
     else:
         k_store, k_shape, layout = _cache_arg(k, "k", dev, "k")
         v_store, v_shape, v_layout = _cache_arg(v, "v", dev, "v")
@@ -536,7 +536,6 @@ def flash_prefill(q, k, v, cu_seqlens, *, scale=None, head_dim_v=None, out=None,
         dv = v_shape[3]
         pt = _page_table(page_table_tensor, B, dev)
         start = None if start_pos is None else _seq_ints(start_pos, "start_pos", B, dev)
-        max_keys = pt.shape[1] * page_size
     if head_dim_v is not None and int(head_dim_v) != dv:
         raise RuntimeError(f"head_dim_v {head_dim_v} != V width {dv}")
     if out is None:
@@ -547,19 +546,19 @@ def flash_prefill(q, k, v, cu_seqlens, *, scale=None, head_dim_v=None, out=None,
             raise RuntimeError(f"out must be [{T}, {n_q}, {dv}]")
     if T == 0:
         return out
-    need = _native.load().palu_flash_prefill_workspace_bytes(T, B, n_q, n_kv, max_keys, dv)
+    sc = float(HEAD_DIM ** -0.5 if scale is None else scale)
+    if page_table_tensor is None:
+        _native.launch("flash_prefill", dev, q.data_ptr(), q_st, q_sh, k.data_ptr(), k_st, k_sh, v.data_ptr(), v_st, v_sh,
+                       cu.data_ptr(), out.data_ptr(), sc, T, B, n_q, n_kv, dv)
+        return out
+    need = _native.load().palu_flash_prefill_workspace_bytes(T, B, n_q, n_kv, pt.shape[1] * page_size, dv)
     if workspace is None:
         workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     elif not (workspace.device == dev and workspace.numel() * workspace.element_size() >= need):
         raise RuntimeError(f"workspace must hold {need} bytes on {dev}")
-    sc = float(HEAD_DIM ** -0.5 if scale is None else scale)
-    if page_table_tensor is None:
-        _native.launch("flash_prefill", dev, q.data_ptr(), q_st, q_sh, k.data_ptr(), k_st, k_sh, v.data_ptr(), v_st, v_sh,
-                       cu.data_ptr(), out.data_ptr(), sc, T, B, n_q, n_kv, dv, _native.ptr(workspace), need)
-    else:
-        _native.launch("flash_prefill_paged", dev, q.data_ptr(), q_st, q_sh, k_store.data_ptr(), v_store.data_ptr(),
-                       cu.data_ptr(), _native.ptr(start), pt.data_ptr(), out.data_ptr(), sc, T, B, n_q, n_kv, n_pages,
-                       page_size, pt.shape[1], dv, layout, _native.ptr(workspace), need)
+    _native.launch("flash_prefill_paged", dev, q.data_ptr(), q_st, q_sh, k_store.data_ptr(), v_store.data_ptr(),
+                   cu.data_ptr(), _native.ptr(start), pt.data_ptr(), out.data_ptr(), sc, T, B, n_q, n_kv, n_pages,
+                   page_size, pt.shape[1], dv, layout, _native.ptr(workspace), need)
     return out
 
 

@@ -485,10 +485,15 @@ size_t palu_pages_workspace_bytes(int batch, int num_pages);
 /* Log probabilities of row r's token tokens[r] under softmax(logits[r]), the entropy of that distribution in nats, and its
  * `top` largest entries (0 .. 64, at most n): log probabilities and ids, the lower id first among equal logits, NaN above
  * every number. logits [rows][n], rows ld elements apart, fp32 or bf16 (PALU_DTYPE_*). A negative token (padding) gets 0,
- * one past the row NaN; a row with a NaN or +infinity, or of -infinity alone, gives NaN. The reference's generation loop
+ * one past the row NaN; a row with a NaN or +infinity, or of -infinity alone, gives NaN. Few long rows are cut into parts that
+ * meet in the workspace (palu_token_logprobs_workspace_bytes, 16-byte aligned, any contents). The reference's generation loop
  * (generate.py:53-62) has the greedy pick only. */
 int palu_token_logprobs(const void* logits, long long ld, int dtype, const int64_t* tokens, int rows, int n, int top,
-                        float* logprob, float* entropy, float* top_logprobs, int64_t* top_ids, palu_stream_t stream);
+                        float* logprob, float* entropy, float* top_logprobs, int64_t* top_ids, void* workspace,
+                        size_t workspace_bytes, palu_stream_t stream);
+
+/* Workspace bytes of palu_token_logprobs (0 where rows are not cut, and for invalid shapes). */
+size_t palu_token_logprobs_workspace_bytes(int rows, int n, int top);
 
 #ifdef __cplusplus
 }

@@ -111,9 +111,10 @@ def test_compact_refusals(lib):
     (dict(x=None), _native.PALU_EINVAL, "null"), (dict(top_id=None), _native.PALU_EINVAL, "null"), (dict(rows=0), _native.PALU_EINVAL, "positive"),
     (dict(n=0), _native.PALU_EINVAL, "positive"), (dict(dtype=2), _native.PALU_EINVAL, "dtype"), (dict(top=65), _native.PALU_EINVAL, "top"),
     (dict(n=3, top=4), _native.PALU_EINVAL, "top"), (dict(top=-1), _native.PALU_EINVAL, "top"),
-    (dict(n=(1 << 30) + 1), _native.PALU_EUNSUPPORTED, "logits")])
+    (dict(n=(1 << 30) + 1), _native.PALU_EUNSUPPORTED, "logits"), (dict(n=128256, ws=None), _native.PALU_EINVAL, "workspace"),
+    (dict(n=128256, bytes=100), _native.PALU_EINVAL, "workspace"), (dict(n=128256, ws=P + 8), _native.PALU_EINVAL, "workspace")])
 def test_token_logprobs_refusals(lib, kw, code, what):
-    a = dict(x=P, ld=100, dtype=1, tokens=P, rows=2, n=100, top=5, lp=P, ent=P, top_lp=P, top_id=P, stream=None)
+    a = dict(x=P, ld=100, dtype=1, tokens=P, rows=2, n=100, top=5, lp=P, ent=P, top_lp=P, top_id=P, ws=P, bytes=1 << 30, stream=None)
     a.update(kw)
     _refused(lib, lib.palu_token_logprobs(*a.values()), code, what)
 

@@ -3,7 +3,8 @@
 // One pass: every lane keeps its own running maximum, sum and weighted sum, rescaled when the maximum rises, and
 // every wave the largest entries of what it has read, one per lane and sorted, which an entry joins only if it beats the
 // last of them. Among equal values the lower index comes first; NaN counts above every number (as in the greedy
-// pick), and makes the log probabilities and the entropy NaN. Bound by the logits' bytes.
+// pick), and makes the log probabilities and the entropy NaN. Bound by the logits' bytes; of few rows, which are cut
+// into parts for as many workgroups as the chip holds and joined by a second launch, by latency.
 #include "palu_kernel.h"
 
 #include <algorithm>
@@ -11,6 +12,10 @@
 namespace {
 
 constexpr int SCORE_TOP = 64;             // entries of a wave's list, one a lane
+constexpr int SCORE_WAVES = 4;            // of a workgroup
+constexpr int SCORE_WGS = 2048;           // workgroups that the chip holds at once
+constexpr int SCORE_PART = 8192;          // logits of a row's part, about, at least: 32 a lane
+constexpr int SCORE_PARTS = 32;          // of a row, at most
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 
 struct ScoreArgs {
@@ -22,27 +27,33 @@ struct ScoreArgs {
   float* ent;
   float* top_lp;                          // [rows][top]
   int64_t* top_id;
+  int parts;                              // of a row
+  char* ws;                               // parts > 1: per (row, part) its Stats (16 bytes) and `top` entries
 };
 
 // Entries compare as (value, lower index first): one 64-bit key, value made order-preserving above, complemented index below.
 // -0 counts as 0 and every NaN as one value.
-__device__ __forceinline__ unsigned order_key(float x) {
-  const unsigned b = __float_as_uint(x + 0.f);             // -0 + 0 = +0
-  const unsigned k = b & 0x80000000u ? ~b : b | 0x80000000u;
-  return x != x ? 0xffffffffu : k;
+__device__ __forceinline__ unsigned order_key(unsigned b) {   // of a float's bits (integers only: scalar where b is)
+  const unsigned k = b & 0x80000000u ? (b == 0x80000000u ? b : ~b) : b | 0x80000000u;
+  return (b & 0x7fffffffu) > 0x7f800000u ? 0xffffffffu : k;
 }
 __device__ __forceinline__ float key_value(unsigned k) {
   return __uint_as_float(k == 0xffffffffu ? 0x7fc00000u : k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 typedef unsigned long long u64;
-__device__ __forceinline__ u64 entry(float x, int i) { return (u64)order_key(x) << 32 | (unsigned)~i; }
+__device__ __forceinline__ u64 entry(unsigned bits, int i) { return (u64)order_key(bits) << 32 | (unsigned)~i; }
 
-__device__ __forceinline__ u64 shfl64(u64 v, int lane) {
-  const unsigned lo = __shfl((unsigned)v, lane, 64), hi = __shfl((unsigned)(v >> 32), lane, 64);
+__device__ __forceinline__ u64 lane_of(u64 v, int lane) {   // the entry of a uniform lane
+  const unsigned lo = __builtin_amdgcn_readlane((unsigned)v, lane), hi = __builtin_amdgcn_readlane((unsigned)(v >> 32), lane);
+  return (u64)hi << 32 | lo;
+}
+__device__ __forceinline__ u64 lane_before(u64 v) {       // the entry of the lane before (lane 0: none)
+  const unsigned lo = __builtin_amdgcn_update_dpp(0, (unsigned)v, 0x138, 0xf, 0xf, false);   // wave_shr 1
+  const unsigned hi = __builtin_amdgcn_update_dpp(0, (unsigned)(v >> 32), 0x138, 0xf, 0xf, false);
   return (u64)hi << 32 | lo;
 }
 
-struct Stats {
+struct __attribute__((aligned(16))) Stats {
   float m, z, e;                          // maximum, sum of p = exp(x - m), sum of p log2 p
 };
 // (log2 p is bounded below where it multiplies: p is 0 there, and -infinity times 0 is NaN.)
@@ -68,35 +79,126 @@ struct Vec<float> {
   typedef f32x4 V;
 };
 
-template <typename T, int NW>
-__global__ __launch_bounds__(NW * 64) void palu_score_kernel(const ScoreArgs a) {
+// The largest value bits t, to 16 bits, that at least `top` of the lanes' `n` keys (R of each, 0: none) reach.
+template <int R>
+__device__ __forceinline__ unsigned reached_by(const unsigned (&k)[R], int n, int top) {
+  unsigned t = 0;
+  for (int bit = 31; bit >= 16; --bit) {
+    const unsigned c = t | 1u << bit;
+    int m = 0;
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (64 * r < n) m += __popcll(__ballot(k[r] >= c));
+    if (m >= top) t = c;
+  }
+  return t;
+}
+
+// The largest `top` of `n` lists of `top` entries in LDS (0: none; no two others are equal), each with its place: use(place, entry).
+// What is left above reached_by is placed by the number of larger ones. At most 64 R entries; `left` and `count`: LDS for as
+// many and a counter. Returns how many are left.
+template <int R, typename F>
+__device__ __forceinline__ int merge_lists(const u64* lists, int n, int top, u64* left, int* count, F use) {
+  const int all = n * top, lane = threadIdx.x & 63;
+  if (threadIdx.x == 0) *count = 0;
+  unsigned t = 0;
+  if (all > 128) {                        // (of fewer the search costs more than the places of all)
+    unsigned k[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const unsigned x = (unsigned)(lists[min(64 * r + lane, all - 1)] >> 32);
+      k[r] = 64 * r + lane < all ? x : 0;
+    }
+    t = reached_by(k, all, top);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < all; i += SCORE_WAVES * 64) {
+    const u64 x = lists[i];
+    if (x != 0 && (unsigned)(x >> 32) >= t) left[atomicAdd(count, 1)] = x;   // in any order: places go by the entries
+  }
+  __syncthreads();
+  const int m = *count;
+  for (int i = threadIdx.x; i < m; i += SCORE_WAVES * 64) {
+    const u64 x = left[i];
+    int place = 0;
+#pragma unroll 8
+    for (int j = 0; j < m; ++j) place += left[j] > x;
+    if (place < top) use(place, x);
+  }
+  return m;
+}
+
+// The row's results from its whole statistics and the sorted lists of its parts.
+template <int R>
+__device__ __forceinline__ void finish_row(const ScoreArgs& a, long long row, const Stats& st, float token_logit, const u64* lists,
+                                           int n, u64* left, int* count) {
+  const float logz = __builtin_amdgcn_logf(st.z) * LN2;    // log2 Z, in natural units
+  if (threadIdx.x == 0) {
+    const long long t = a.tokens[row];
+    a.lp[row] = t < 0 ? 0.f : t >= a.n ? __builtin_nanf("") : (token_logit - st.m) - logz;
+    a.ent[row] = logz - st.e / st.z * LN2;
+  }
+  if (a.top)
+    merge_lists<R>(lists, n, a.top, left, count, [&](int place, u64 k) {
+      a.top_lp[row * a.top + place] = (key_value((unsigned)(k >> 32)) - st.m) - logz;
+      a.top_id[row * a.top + place] = (int64_t)(unsigned)~(unsigned)k;
+    });
+}
+
+template <typename T>
+__global__ __launch_bounds__(SCORE_WAVES * 64) void palu_score_kernel(const ScoreArgs a) {
   constexpr int N = Vec<T>::N, U = 32 / N;                 // a lane's vectors in flight: 32 entries
   typedef typename Vec<T>::V V;
-  __shared__ u64 lists[NW * SCORE_TOP];
-  __shared__ Stats stats[NW];
+  __shared__ u64 lists[SCORE_WAVES * SCORE_TOP], left[SCORE_WAVES * SCORE_TOP];
+  __shared__ Stats stats[SCORE_WAVES];
+  __shared__ unsigned maxima[2][SCORE_WAVES * 64];
+  __shared__ int count;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  const long long row = blockIdx.x;
+  const int part = blockIdx.x % a.parts;
+  const long long row = blockIdx.x / a.parts;
   const T* x = static_cast<const T*>(a.x) + row * a.ld;
   // Vector v holds entries N v - skew .. + N - 1, so that whole vectors are aligned; the row's ends are read one by one.
   const int skew = (int)(reinterpret_cast<uintptr_t>(x) / sizeof(T) % N);
-  const int nv = (a.n + skew + N - 1) / N;
+  const int nv = (a.n + skew + N - 1) / N, share = (nv + a.parts - 1) / a.parts;
+  const int v_lo = min(nv, part * share), v_hi = min(nv, v_lo + share);
+  float token_logit = 0.f;
+  if (tid == 0) {
+    const long long t = a.tokens[row];
+    if (t >= 0 && t < a.n) token_logit = (float)x[t];
+  }
   Stats st{NEG_INF, 0.f, 0.f};
-  u64 mine = 0;                           // entry `lane` of the wave's list (0: none), and its last entry
-  u64 least = 0;
-  for (int v0 = w * 64 * U; v0 < nv; v0 += NW * 64 * U) {
-    float f[U][N];
+  u64 mine = 0, least = 0;                // entry `lane` of the wave's list (0: none), and the last of its `top`
+  float bound = NEG_INF;                  // no entry below it can be among the top
+  int turn = 0;
+  for (int vc = v_lo; vc < v_hi; vc += SCORE_WAVES * 64 * U, ++turn) {   // uniform: all waves take every turn
+    const int v0 = vc + w * 64 * U;
+    // Whole vectors first, all loads at once; then the entries of the row's ends.
+    V q[U];
+    bool ends = false;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int e0 = (v0 + u * 64 + lane) * N - skew;
-      if (e0 >= 0 && e0 + N <= a.n) {
-        const V q = __builtin_nontemporal_load(reinterpret_cast<const V*>(x + e0));
+      const int v = v0 + u * 64 + lane, e0 = v * N - skew;
+      const bool whole = v < v_hi && e0 >= 0 && e0 + N <= a.n;
+      ends = ends || (v < v_hi && !whole);
 #pragma unroll
-        for (int i = 0; i < N; ++i) f[u][i] = (float)q[i];
-      } else {
+      for (int i = 0; i < N; ++i) q[u][i] = (T)NEG_INF;
+      if (whole) q[u] = __builtin_nontemporal_load(reinterpret_cast<const V*>(x + e0));
+    }
+    if (__any(ends)) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) f[u][i] = e0 + i >= 0 && e0 + i < a.n ? (float)x[e0 + i] : NEG_INF;
+      for (int u = 0; u < U; ++u) {
+        const int v = v0 + u * 64 + lane, e0 = v * N - skew;
+        if (v < v_hi && (e0 < 0 || e0 + N > a.n))
+#pragma unroll
+          for (int i = 0; i < N; ++i)
+            if (e0 + i >= 0 && e0 + i < a.n) q[u][i] = x[e0 + i];
       }
     }
+    float f[U][N];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < N; ++i) f[u][i] = (float)q[u][i];
     float mx = f[0][0];
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -115,27 +217,40 @@ __global__ __launch_bounds__(NW * 64) void palu_score_kernel(const ScoreArgs a) 
         st.z += p;
         st.e = fmaf(t, p, st.e);
       }
-    if (a.top && __any(order_key(mx) >= (unsigned)(least >> 32))) {
+    if (a.top == 0) continue;
+    if ((turn & (turn + 1)) == 0) {
+      // The top-th largest of all lanes' maxima so far bounds the top-th entry from below. Found bit by bit, to 16 bits, at turns
+      // 0, 1, 3, 7, .., it leaves about `top` entries a time for the workgroup's lists (each wave by its own entries: 5.6
+      // times as many, at 20 of 2048).
+      unsigned* const keys = maxima[(31 - __builtin_clz(turn + 1)) & 1];
+      keys[tid] = order_key(__float_as_uint(st.m));
+      __syncthreads();
+      unsigned k4[SCORE_WAVES];
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+      for (int r = 0; r < SCORE_WAVES; ++r) k4[r] = keys[64 * r + lane];
+      const unsigned t = reached_by(k4, SCORE_WAVES * 64, a.top);
+      if (t > order_key(0xff800000u)) bound = __builtin_elementwise_maximum(bound, key_value(t));
+    }
+    // Values compare as floats, NaN above all: !(x < bound).
+    if (!__any(!(mx < bound))) continue;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const int idx = (v0 + u * 64 + lane) * N - skew + i;
-          const u64 k = idx >= 0 && idx < a.n ? entry(f[u][i], idx) : 0;
-          u64 who = __ballot(k > least);
-          while (who) {
-            const int l = __builtin_ctzll(who);
-            const u64 c = shfl64(k, l);
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        u64 who = __ballot(!(f[u][i] < bound));
+        while (who) {                     // one lane's entry after the other, what can be in scalar registers
+          const int l = __builtin_ctzll(who), v = v0 + u * 64 + l, idx = v * N - skew + i;
+          who &= who - 1;
+          const u64 c = entry(__builtin_amdgcn_readlane(__float_as_uint(f[u][i]), l), idx);
+          if (c > least && v < v_hi && idx >= 0 && idx < a.n) {
             // the lanes that hold less move on by one, the first of them takes the entry
-            const u64 up = shfl64(mine, max(lane - 1, 0));
-            const u64 up_less = lane > 0 && up < c;
-            if (mine < c) mine = up_less ? up : c;
-            least = shfl64(mine, a.top - 1);
-            who &= who - 1;
-            who &= __ballot(k > least);
+            const u64 up = lane_before(mine);
+            if (mine < c) mine = lane > 0 && up < c ? up : c;
+            least = lane_of(mine, a.top - 1);
           }
         }
-    }
+      }
+    if (least) bound = __builtin_elementwise_maximum(bound, key_value((unsigned)(least >> 32)));
   }
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1)
@@ -144,31 +259,81 @@ __global__ __launch_bounds__(NW * 64) void palu_score_kernel(const ScoreArgs a) 
   if (lane < a.top) lists[w * a.top + lane] = mine;
   __syncthreads();
   st = stats[0];
-  for (int i = 1; i < NW; ++i) st = join(st, stats[i]);
-  const float logz = __builtin_amdgcn_logf(st.z) * LN2;    // log2 Z, in natural units
-  if (tid == 0) {
-    const long long t = a.tokens[row];
-    a.lp[row] = t < 0 ? 0.f : t >= a.n ? __builtin_nanf("") : ((float)x[t] - st.m) - logz;
-    a.ent[row] = logz - st.e / st.z * LN2;
+#pragma unroll
+  for (int i = 1; i < SCORE_WAVES; ++i) st = join(st, stats[i]);
+  if (a.parts == 1) {
+    finish_row<SCORE_WAVES>(a, row, st, token_logit, lists, SCORE_WAVES, left, &count);
+    return;
   }
-  // An entry's place among all lists is the number of larger ones (no two are equal).
-  const int all = NW * a.top;
-  for (int i = tid; i < all; i += NW * 64) {
-    const u64 k = lists[i];
-    if (k == 0) continue;
-    int place = 0;
-    for (int j = 0; j < all; ++j) place += lists[j] > k;
-    if (place < a.top) {
-      a.top_lp[row * a.top + place] = (key_value((unsigned)(k >> 32)) - st.m) - logz;
-      a.top_id[row * a.top + place] = (int64_t)(unsigned)~(unsigned)k;
-    }
+  char* ws = a.ws + (long long)blockIdx.x * (16 + 8 * a.top);
+  if (tid == 0) *reinterpret_cast<Stats*>(ws) = st;
+  if (a.top) {
+    u64* out = reinterpret_cast<u64*>(ws + 16);
+    const int m = merge_lists<SCORE_WAVES>(lists, SCORE_WAVES, a.top, left, &count, [&](int place, u64 k) { out[place] = k; });
+    if (m + tid < a.top) out[m + tid] = 0;
   }
 }
 
+// The parts of a row, a workgroup to a row.
+template <typename T>
+__global__ __launch_bounds__(SCORE_WAVES * 64) void palu_score_join_kernel(const ScoreArgs a) {
+  extern __shared__ u64 lists[];          // [parts][top], and as much for what is left of them
+  __shared__ int count;
+  const long long row = blockIdx.x;
+  const char* ws = a.ws + row * a.parts * (16 + 8 * a.top);
+  float token_logit = 0.f;
+  if (threadIdx.x == 0) {
+    const long long t = a.tokens[row];
+    if (t >= 0 && t < a.n) token_logit = (float)static_cast<const T*>(a.x)[row * a.ld + t];
+  }
+  const int lane = threadIdx.x & 63;
+  Stats st{NEG_INF, 0.f, 0.f};
+  if (lane < a.parts) st = *reinterpret_cast<const Stats*>(ws + lane * (16 + 8 * a.top));
+  u64 x[SCORE_PARTS / SCORE_WAVES];       // all loads at once: each comes from another XCD's writes, by way of memory
+#pragma unroll
+  for (int i = 0; i < SCORE_PARTS / SCORE_WAVES; ++i) {
+    const int p = i * SCORE_WAVES + (threadIdx.x >> 6);
+    x[i] = 0;
+    if (p < a.parts && lane < a.top) x[i] = reinterpret_cast<const u64*>(ws + p * (16 + 8 * a.top) + 16)[lane];
+  }
+#pragma unroll
+  for (int i = 0; i < SCORE_PARTS / SCORE_WAVES; ++i) {
+    const int p = i * SCORE_WAVES + (threadIdx.x >> 6);
+    if (p < a.parts && lane < a.top) lists[p * a.top + lane] = x[i];
+  }
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1)
+    st = join(st, Stats{__shfl_xor(st.m, o, 64), __shfl_xor(st.z, o, 64), __shfl_xor(st.e, o, 64)});
+  __syncthreads();
+  u64* left = lists + a.parts * a.top;
+  if (a.parts * a.top <= 64 * 8) finish_row<8>(a, row, st, token_logit, lists, a.parts, left, &count);
+  else finish_row<SCORE_PARTS>(a, row, st, token_logit, lists, a.parts, left, &count);
+}
+
+int score_parts(int rows, int n) { return std::max(1, std::min({SCORE_WGS / rows, (n + SCORE_PART - 1) / SCORE_PART, SCORE_PARTS})); }
+
+template <typename T>
+int launch_score(const ScoreArgs& a, const char* who, hipStream_t s) {
+  hipLaunchKernelGGL((palu_score_kernel<T>), dim3((unsigned)a.rows * a.parts), dim3(SCORE_WAVES * 64), 0, s, a);
+  if (a.parts > 1 && hipPeekAtLastError() == hipSuccess)
+    hipLaunchKernelGGL((palu_score_join_kernel<T>), dim3(a.rows), dim3(SCORE_WAVES * 64), 16 * a.parts * a.top, s, a);
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? PALU_OK : fail(PALU_EHIP, "%s launch: %s", who, hipGetErrorString(e));
+}
+
+bool score_dims_ok(int rows, int n, int top) { return rows > 0 && n > 0 && top >= 0 && top <= SCORE_TOP && top <= n; }
+
 }  // namespace
 
+extern "C" size_t palu_token_logprobs_workspace_bytes(int rows, int n, int top) {
+  if (!score_dims_ok(rows, n, top)) return 0;
+  const int parts = score_parts(rows, n);
+  return parts == 1 ? 0 : (size_t)rows * parts * (16 + 8 * top);
+}
+
 extern "C" int palu_token_logprobs(const void* logits, long long ld, int dtype, const int64_t* tokens, int rows, int n, int top,
-                                   float* logprob, float* entropy, float* top_logprobs, int64_t* top_ids, hipStream_t stream) {
+                                   float* logprob, float* entropy, float* top_logprobs, int64_t* top_ids, void* workspace,
+                                   size_t workspace_bytes, hipStream_t stream) {
   palu::g_err[0] = 0;
   const char* who = "palu_token_logprobs";
   if (!logits || !tokens || !logprob || !entropy || (top > 0 && (!top_logprobs || !top_ids)))
@@ -177,17 +342,12 @@ extern "C" int palu_token_logprobs(const void* logits, long long ld, int dtype, 
   if (n > (1 << 30)) return fail(PALU_EUNSUPPORTED, "%s: rows of %d logits", who, n);
   if (dtype != PALU_DTYPE_F32 && dtype != PALU_DTYPE_BF16)
     return fail(PALU_EINVAL, "%s: dtype must be PALU_DTYPE_F32 or PALU_DTYPE_BF16, got %d", who, dtype);
-  if (top < 0 || top > SCORE_TOP || top > n) return fail(PALU_EINVAL, "%s: top = %d (0 .. %d, at most n)", who, top, SCORE_TOP);
-  const ScoreArgs a{logits, ld, tokens, rows, n, top, logprob, entropy, top_logprobs, top_ids};
-  const bool few = rows < 512;            // a row to a CU: its waves share the row
-  if (dtype == PALU_DTYPE_BF16) {
-    if (few) hipLaunchKernelGGL((palu_score_kernel<__bf16, 16>), dim3(rows), dim3(1024), 0, stream, a);
-    else hipLaunchKernelGGL((palu_score_kernel<__bf16, 4>), dim3(rows), dim3(256), 0, stream, a);
-  } else {
-    if (few) hipLaunchKernelGGL((palu_score_kernel<float, 16>), dim3(rows), dim3(1024), 0, stream, a);
-    else hipLaunchKernelGGL((palu_score_kernel<float, 4>), dim3(rows), dim3(256), 0, stream, a);
-  }
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return fail(PALU_EHIP, "%s launch: %s", who, hipGetErrorString(e));
-  return PALU_OK;
+  if (!score_dims_ok(rows, n, top)) return fail(PALU_EINVAL, "%s: top = %d (0 .. %d, at most n)", who, top, SCORE_TOP);
+  const size_t need = palu_token_logprobs_workspace_bytes(rows, n, top);
+  if (need && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15)))
+    return fail(PALU_EINVAL, "%s: a 16-byte aligned workspace of %zu bytes needed (palu_token_logprobs_workspace_bytes), got %zu",
+                who, need, workspace ? workspace_bytes : 0);
+  const ScoreArgs a{logits, ld, tokens, rows, n, top, logprob, entropy, top_logprobs, top_ids, score_parts(rows, n),
+                    static_cast<char*>(workspace)};
+  return dtype == PALU_DTYPE_BF16 ? launch_score<__bf16>(a, who, stream) : launch_score<float>(a, who, stream);
 }

@@ -70,7 +70,8 @@ _SIGNATURES = {
     "palu_pages_update": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _sz, _vp]),
     "palu_pages_compact": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _sz, _vp]),
     "palu_pages_workspace_bytes": (_sz, [_i, _i]),
-    "palu_token_logprobs": (_i, [_vp, _ll, _i, _vp, _i, _i, _i, _vp, _vp, _vp, _vp, _vp]),
+    "palu_token_logprobs": (_i, [_vp, _ll, _i, _vp, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "palu_token_logprobs_workspace_bytes": (_sz, [_i, _i, _i]),
     "palu_prefill_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i]),
 }
 EXPORTED = tuple(_SIGNATURES)

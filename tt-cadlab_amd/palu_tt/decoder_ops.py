@@ -97,13 +97,15 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0):
         raise RuntimeError("token_logprobs has no backward pass: call it under torch.no_grad()")
     t = tokens if tokens.device == dev and tokens.dtype == torch.int64 else tokens.to(device=dev, dtype=torch.int64)
     t = t.contiguous()
-    lp, ent = torch.empty(2, rows, dtype=torch.float32, device=dev)
+    lp, ent = torch.empty(2, rows, dtype=torch.float32, device=dev).unbind(0)
     top_lp = torch.empty(rows, top, dtype=torch.float32, device=dev)
     ids = torch.empty(rows, top, dtype=torch.int64, device=dev)
     if rows:
+        need = _native.load().palu_token_logprobs_workspace_bytes(rows, n, top)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         _native.launch("token_logprobs", dev, logits.data_ptr(), logits.stride(0) if rows > 1 else n,
                        _native.DTYPE_BF16 if logits.dtype == torch.bfloat16 else _native.DTYPE_F32, t.data_ptr(), rows, n, top,
-                       lp.data_ptr(), ent.data_ptr(), top_lp.data_ptr(), ids.data_ptr())
+                       lp.data_ptr(), ent.data_ptr(), top_lp.data_ptr(), ids.data_ptr(), _native.ptr(ws), need)
     return lp, ent, top_lp, ids
 
 

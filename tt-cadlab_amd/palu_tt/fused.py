@@ -485,16 +485,11 @@ def _strided_rows(t, name: str, width: Optional[int], device=None):
         raise RuntimeError(f"{name} must be [rows, heads, {width or 'width'}], got {tuple(getattr(t, 'shape', ()))}")
     if not t.is_cuda or t.dtype != torch.bfloat16 or (device is not None and t.device != device):
         raise RuntimeError(f"{name} must be a torch.bfloat16 tensor on {device or 'the GPU'}, got {t.dtype} on {t.device}")
-    st = t.stride(0) if t.shape[0] > 1 else 0
-    sh = t.stride(1) if t.shape[1] > 1 else 0
-    if (t.stride(2) != 1 and t.shape[2] > 1) or st % 8 or sh % 8 or t.data_ptr() % 16:
+    (rows, heads, w), (st, sh, sw) = t.shape, t.stride()
+    st, sh = st if rows > 1 else 0, sh if heads > 1 else 0
+    if (sw != 1 and w > 1) or st % 8 or sh % 8 or t.data_ptr() % 16:
         raise RuntimeError(f"{name} must have contiguous heads, row and head strides in multiples of 8, and start 16-byte aligned")
     return st, sh
-
-
-def _no_grad_wanted(what: str, *tensors) -> None:
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad()")
 
 
 def flash_prefill(q, k, v, cu_seqlens, *, scale=None, head_dim_v=None, out=None, workspace=None, page_table_tensor=None,
@@ -516,7 +511,8 @@ def flash_prefill(q, k, v, cu_seqlens, *, scale=None, head_dim_v=None, out=None,
     B = cu.numel() - 1
     if B < 1:
         raise RuntimeError("cu_seqlens must hold at least one sequence")
-    _no_grad_wanted("flash_prefill", q, *(t for t in (k, v) if isinstance(t, torch.Tensor)))
+    if (q.requires_grad or getattr(k, "requires_grad", False) or getattr(v, "requires_grad", False)) and torch.is_grad_enabled():
+        raise RuntimeError("flash_prefill has no backward pass: call it under torch.no_grad()")
     if page_table_tensor is None:
         if start_pos is not None:
             raise RuntimeError("start_pos needs page_table_tensor: packed rows attend to themselves from position 0")

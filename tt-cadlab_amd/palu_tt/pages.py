@@ -87,11 +87,14 @@ class PagePools:
         new = None if new_lengths is None else _ints(new_lengths, "new_lengths", (B,), self.device)
         if out is None:
             out = torch.empty_like(pt), torch.empty_like(ln)
-        for t, like, name in zip(out, (pt, ln), ("page_table", "lengths")):
-            if t.shape != like.shape or t.dtype != torch.int32 or t.device != self.device or not t.is_contiguous():
-                raise RuntimeError(f"out: {name} must be a contiguous int32 {list(like.shape)} tensor on {self.device}")
-            if any(i is not None and _overlap(t, i) for i in (pt, ln, par, new)):
-                raise RuntimeError(f"out: {name} must be memory of its own")
+        else:
+            for t, like, name in zip(out, (pt, ln), ("page_table", "lengths")):
+                if t.shape != like.shape or t.dtype != torch.int32 or t.device != self.device or not t.is_contiguous():
+                    raise RuntimeError(f"out: {name} must be a contiguous int32 {list(like.shape)} tensor on {self.device}")
+                if any(i is not None and _overlap(t, i) for i in (pt, ln, par, new)):
+                    raise RuntimeError(f"out: {name} must be memory of its own")
+            if _overlap(*out):
+                raise RuntimeError("out: page_table and lengths must not overlap")
         if B:
             ws, need = self._workspace(B, workspace)
             _native.launch("pages_update", self.device, pt.data_ptr(), ln.data_ptr(), _native.ptr(par), _native.ptr(new),

@@ -458,6 +458,7 @@ __global__ __launch_bounds__(256, 2) void palu_flash_prefill_kernel(const FlashP
     next_k(0);
     next_k(1);
     fence();
+    __builtin_amdgcn_s_setprio(1);                        // ahead of the SIMD's other wave, whose products with V need few slots
 #pragma unroll
     for (int c = 0; c < 8; ++c) {
       if (c < 6) next_k(c + 2);
@@ -468,6 +469,7 @@ __global__ __launch_bounds__(256, 2) void palu_flash_prefill_kernel(const FlashP
       eighth(s, p, c, mref);
       fence();
     }
+    __builtin_amdgcn_s_setprio(0);
     values(sv, p, 2);
   };
   // A tile of which some rows do not see some keys; s becomes the next tile's scores.

@@ -125,11 +125,14 @@ struct PlanArgs {
   const int32_t* new_len;                 // [B] or null (as long as the parent)
   int32_t* table_out;
   int32_t* len_out;
-  int B, slots, n_pages, page;
+  int B, slots, n_pages, page, log2_page;
   int hash;                               // entries of the update's hash table, a power of two
   int32_t* ws;                            // [4]: number of copies; then src[n], dst[n]; then a list of n_pages
   int max_copies;
 };
+
+// Pages of n positions.
+__device__ __forceinline__ int pages_of(const PlanArgs& a, int n) { return (n + a.page - 1) >> a.log2_page; }
 
 // Exclusive prefix sum of x over the workgroup's threads, and its total. `part`: PLAN_THREADS / 64 + 1 ints.
 __device__ __forceinline__ int block_scan(int x, int* part, int& total) {
@@ -151,23 +154,39 @@ __device__ __forceinline__ bool in_pool(int p, int n) { return p >= 0 && p < n; 
 __device__ __forceinline__ void set_bit(unsigned* bits, int p) { atomicOr(&bits[p >> 5], 1u << (p & 31)); }
 __device__ __forceinline__ bool get_bit(const unsigned* bits, int p) { return bits[p >> 5] >> (p & 31) & 1; }
 
-// What becomes of row b: `keep` positions of its parent's, `want` in all.
-struct Row {
-  int parent, keep, want;
-};
-__device__ __forceinline__ Row plan_row(const PlanArgs& a, int b) {
-  const int most = a.slots * a.page;
-  int p = a.parents ? a.parents[b] : b;
-  if (!in_pool(p, a.B)) p = -1;
-  const int have = p < 0 ? 0 : min(max(a.len[p], 0), most);
-  const int want = a.new_len ? min(max(a.new_len[b], 0), most) : have;
-  return Row{p, min(have, want), want};
+// Rows of the table by waves, four at a time so that their loads are on their way together: use(b, j, entry) for the first
+// n(b) slots of every row's source row from(b).
+template <typename N, typename From, typename Use>
+__device__ __forceinline__ void each_entry(const PlanArgs& a, N n, From from, Use use) {
+  constexpr int R = 4, WAVES = PLAN_THREADS / 64;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  for (int b0 = w; b0 < a.B; b0 += R * WAVES) {
+    const int32_t* row[R];
+    int cnt[R], most = 0;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int b = b0 + r * WAVES;
+      cnt[r] = b < a.B ? n(b) : 0;
+      row[r] = a.table + (long long)(cnt[r] ? from(b) : 0) * a.slots;
+      most = max(most, cnt[r]);
+    }
+    for (int j = lane; j < most; j += 64) {
+      int x[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r) x[r] = row[r][min(j, max(cnt[r], 1) - 1)];
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        if (j < cnt[r]) use(b0 + r * WAVES, j, x[r]);
+    }
+  }
 }
 
 // A row's whole kept pages stay shared. The page that a row writes next, the one its kept positions end inside, has to be
 // its own: the first row in order that would write it keeps it, unless another row holds it as a whole page; the others get
 // copies. New pages are the lowest free ones, in the order of rows and slots; when they run out, a row's length is cut to
 // what it has. All choices go by row and page order, none by the order in which threads arrive.
+// Bound by latency, three loads deep (a row's parent, its length, its page) and a barrier for each step of the plan: 8 rows of 64
+// slots 5 us; rows one after the other, each with loads of its own at every step, took 14.8 us for 64 rows.
 __global__ __launch_bounds__(PLAN_THREADS) void palu_update_pages_kernel(const PlanArgs a) {
   extern __shared__ __attribute__((aligned(16))) unsigned lds[];
   __shared__ int part[PLAN_THREADS / 64 + 1], n_copies;
@@ -176,81 +195,77 @@ __global__ __launch_bounds__(PLAN_THREADS) void palu_update_pages_kernel(const P
   unsigned* bits = lds;
   int* key = reinterpret_cast<int*>(bits + words);        // page -> first row that would write it
   int* first = key + a.hash;
-  int* held = first + a.hash;                             // [B] pages a row has before new ones
-  int* off = held + a.B;                                  // [B] its first new page's place in the free list
+  int* parent = first + a.hash;                           // [B]; later the row's first new page's place in the free list
+  int* keep = parent + a.B;                               // [B] positions kept of the parent's; later the pages a row has
+  int* want = keep + a.B;                                 // [B] positions in all
+  int* last = want + a.B;                                 // [B] the page that the kept positions end inside, or -1
+  for (int b = tid; b < a.B; b += PLAN_THREADS) {
+    const int most = a.slots * a.page;
+    int p = a.parents ? a.parents[b] : b;
+    const int asked = a.new_len ? a.new_len[b] : 0;
+    if (!in_pool(p, a.B)) p = -1;
+    const int have = p < 0 ? 0 : min(max(a.len[p], 0), most);
+    const int all = a.new_len ? min(max(asked, 0), most) : have, kept = min(have, all);
+    int page = -1;
+    if (kept & (a.page - 1)) page = a.table[(long long)p * a.slots + (kept >> a.log2_page)];
+    parent[b] = p;
+    keep[b] = kept;
+    want[b] = all;
+    last[b] = in_pool(page, a.n_pages) ? page : -1;
+  }
   for (int i = tid; i < words; i += PLAN_THREADS) bits[i] = 0;
   for (int i = tid; i < a.hash; i += PLAN_THREADS) key[i] = -1, first[i] = 0x7fffffff;
   if (tid == 0) n_copies = 0;
   __syncthreads();
-  for (int b = w; b < a.B; b += PLAN_THREADS / 64) {      // a wave to a row
-    const Row r = plan_row(a, b);
-    const int full = r.keep / a.page, need = (r.want + a.page - 1) / a.page;
-    const int32_t* old = a.table + (long long)max(r.parent, 0) * a.slots;
-    int32_t* out = a.table_out + (long long)b * a.slots;
-    for (int j = lane; j < a.slots; j += 64) {
-      if (j < full) {
-        const int p = old[j];
-        out[j] = p;
-        if (in_pool(p, a.n_pages)) set_bit(bits, p);
-      } else if (j >= need) {
-        out[j] = -1;
-      }
-    }
-  }
+  each_entry(a, [&](int b) { return keep[b] >> a.log2_page; }, [&](int b) { return parent[b]; }, [&](int b, int j, int p) {
+    a.table_out[(long long)b * a.slots + j] = p;
+    if (in_pool(p, a.n_pages)) set_bit(bits, p);
+  });
+  for (int b = w; b < a.B; b += PLAN_THREADS / 64)
+    for (int j = pages_of(a, want[b]) + lane; j < a.slots; j += 64) a.table_out[(long long)b * a.slots + j] = -1;
   __syncthreads();
   const int per = (a.B + PLAN_THREADS - 1) / PLAN_THREADS;   // rows of a thread, next to each other
   const int b_lo = min(a.B, tid * per), b_hi = min(a.B, b_lo + per);
-  auto last_page = [&](const Row& r) {                    // the page that a row's kept positions end inside, or -1
-    if (r.keep % a.page == 0) return -1;
-    const int p = a.table[(long long)r.parent * a.slots + r.keep / a.page];
-    return in_pool(p, a.n_pages) ? p : -1;
-  };
-  auto slot_of = [&](int p) {
+  for (int b = b_lo; b < b_hi; ++b) {
+    const int p = last[b];
+    if (p < 0 || get_bit(bits, p)) continue;
     unsigned s = (unsigned)p * 2654435761u & (a.hash - 1);
     while (true) {
       const int k = atomicCAS(&key[s], -1, p);
-      if (k == -1 || k == p) return s;
+      if (k == -1 || k == p) break;
       s = (s + 1) & (a.hash - 1);                         // at most half the entries are taken
     }
-  };
-  for (int b = b_lo; b < b_hi; ++b) {
-    const int p = last_page(plan_row(a, b));
-    if (p >= 0 && !get_bit(bits, p)) atomicMin(&first[slot_of(p)], b);
+    atomicMin(&first[s], b);
   }
   __syncthreads();
   int demand = 0;
   for (int b = b_lo; b < b_hi; ++b) {
-    const Row r = plan_row(a, b);
-    const int p = last_page(r), full = r.keep / a.page;
-    // (a page that another row holds whole is in no entry: its bit was set before)
-    bool mine = false;
+    const int p = last[b], full = keep[b] >> a.log2_page;
+    bool mine = false;                                    // (a page that another row holds whole is in no entry)
     if (p >= 0) {
       unsigned s = (unsigned)p * 2654435761u & (a.hash - 1);
       while (key[s] != p && key[s] != -1) s = (s + 1) & (a.hash - 1);
       mine = key[s] == p && first[s] == b;
     }
-    held[b] = full + mine;
-    demand += (r.want + a.page - 1) / a.page - held[b];
+    if (mine) {
+      set_bit(bits, p);
+      a.table_out[(long long)b * a.slots + full] = p;
+      last[b] = -1;
+    }
+    keep[b] = full + mine;
+    demand += pages_of(a, want[b]) - keep[b];
   }
   int total;
   int at = block_scan(demand, part, total);
-  __syncthreads();                                        // every look at the bits is done
   for (int b = b_lo; b < b_hi; ++b) {
-    const Row r = plan_row(a, b);
-    const int full = r.keep / a.page;
-    if (held[b] > full) {
-      const int p = last_page(r);
-      set_bit(bits, p);
-      a.table_out[(long long)b * a.slots + full] = p;
-    }
-    off[b] = at;
-    at += (r.want + a.page - 1) / a.page - held[b];
+    parent[b] = at;
+    at += pages_of(a, want[b]) - keep[b];
   }
-  __syncthreads();
   // The lowest free pages in order, as many as are asked for.
-  int32_t* list = a.ws + 4 + 2 * a.max_copies;
+  int32_t* list = total <= 2 * a.hash ? key : a.ws + 4 + 2 * a.max_copies;   // (the hash table is done with)
   const int wper = (words + PLAN_THREADS - 1) / PLAN_THREADS, w_lo = min(words, tid * wper), w_hi = min(words, w_lo + wper);
   auto free_bits = [&](int i) { return ~bits[i] & (32 * i + 32 <= a.n_pages ? ~0u : (1u << (a.n_pages & 31)) - 1); };
+  __syncthreads();                                        // all bits are set
   int mine = 0;
   for (int i = w_lo; i < w_hi; ++i) mine += __popc(free_bits(i));
   int n_free;
@@ -260,20 +275,19 @@ __global__ __launch_bounds__(PLAN_THREADS) void palu_update_pages_kernel(const P
       if (rank < total) list[rank] = 32 * i + __builtin_ctz(f);
   __syncthreads();
   for (int b = w; b < a.B; b += PLAN_THREADS / 64) {
-    const Row r = plan_row(a, b);
-    const int have = held[b], need = (r.want + a.page - 1) / a.page, o = off[b];
+    const int have = keep[b], need = pages_of(a, want[b]), o = parent[b];
     const int got = min(need - have, max(n_free - o, 0));
     int32_t* out = a.table_out + (long long)b * a.slots;
-    for (int j = have + lane; j < need; j += 64) out[j] = j - have < got ? list[o + j - have] : -1;
-    if (lane == 0) {
-      a.len_out[b] = min(r.want, (have + got) * a.page);
-      const int p = last_page(r);
-      if (p >= 0 && have == r.keep / a.page && got > 0) {
+    for (int j = have + lane; j < need; j += 64) {
+      const int p = j - have < got ? list[o + j - have] : -1;
+      out[j] = p;
+      if (j == have && got > 0 && last[b] >= 0) {
         const int c = atomicAdd(&n_copies, 1);            // the copies do not touch each other: any order
-        a.ws[4 + c] = p;
-        a.ws[4 + a.max_copies + c] = list[o];
+        a.ws[4 + c] = last[b];
+        a.ws[4 + a.max_copies + c] = p;
       }
     }
+    if (lane == 0) a.len_out[b] = min(want[b], (have + got) * a.page);
   }
   __syncthreads();
   if (tid == 0) a.ws[0] = n_copies;
@@ -287,14 +301,11 @@ __global__ __launch_bounds__(PLAN_THREADS) void palu_compact_pages_kernel(const 
   const int words = (a.n_pages + 31) >> 5;
   for (int i = tid; i < words; i += PLAN_THREADS) bits[i] = 0;
   __syncthreads();
-  auto used = [&](int b) { return (int)(((long long)min(max(a.len[b], 0), a.slots * a.page) + a.page - 1) / a.page); };
-  for (int b = w; b < a.B; b += PLAN_THREADS / 64) {
-    const int n = used(b);
-    for (int j = lane; j < n; j += 64) {
-      const int p = a.table[(long long)b * a.slots + j];
-      if (in_pool(p, a.n_pages)) set_bit(bits, p);
-    }
-  }
+  auto used = [&](int b) { return pages_of(a, min(max(a.len[b], 0), a.slots * a.page)); };
+  auto itself = [](int b) { return b; };
+  each_entry(a, used, itself, [&](int, int, int p) {
+    if (in_pool(p, a.n_pages)) set_bit(bits, p);
+  });
   __syncthreads();
   const int wper = (words + PLAN_THREADS - 1) / PLAN_THREADS, w_lo = min(words, tid * wper), w_hi = min(words, w_lo + wper);
   int mine = 0;
@@ -325,14 +336,11 @@ __global__ __launch_bounds__(PLAN_THREADS) void palu_compact_pages_kernel(const 
   __syncthreads();
   for (int i = tid; i < low; i += PLAN_THREADS) to[src[i]] = dst[i];
   __syncthreads();
-  for (int b = w; b < a.B; b += PLAN_THREADS / 64) {
-    const int n = used(b);
-    for (int j = lane; j < a.slots; j += 64) {
-      const long long e = (long long)b * a.slots + j;
-      const int p = j < n ? a.table[e] : -1;
-      a.table_out[e] = in_pool(p, a.n_pages) && p >= n_live ? to[p] : p;
-    }
-  }
+  each_entry(a, used, itself, [&](int b, int j, int p) {
+    a.table_out[(long long)b * a.slots + j] = in_pool(p, a.n_pages) && p >= n_live ? to[p] : p;
+  });
+  for (int b = w; b < a.B; b += PLAN_THREADS / 64)
+    for (int j = used(b) + lane; j < a.slots; j += 64) a.table_out[(long long)b * a.slots + j] = -1;
   if (tid == 0) {
     a.ws[0] = low;
     n_live_out[0] = n_live;
@@ -373,13 +381,15 @@ __global__ __launch_bounds__(256) void palu_copy_pages_kernel(const CopyArgs a) 
 
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+int log2_of(int page_size) { return 31 - __builtin_clz(page_size); }
+
 int hash_entries(int B) {
   int h = 64;
   while (h < 2 * B) h *= 2;
   return h;
 }
 
-size_t update_lds(int B, int n_pages) { return 4 * ((size_t)(n_pages + 31) / 32 + 2 * (size_t)hash_entries(B) + 2 * (size_t)B); }
+size_t update_lds(int B, int n_pages) { return 4 * ((size_t)(n_pages + 31) / 32 + 2 * (size_t)hash_entries(B) + 4 * (size_t)B); }
 
 int check_table(const void* table, const void* len, const void* table_out, int B, int slots, int n_pages, int page, const void* ws,
                 size_t ws_bytes, size_t need, const char* who) {
@@ -480,7 +490,7 @@ extern "C" int palu_pages_update(const int32_t* page_table, const int32_t* lengt
   if (batch > 4096 || update_lds(batch, num_pages) > PLAN_LDS)
     return fail(PALU_EUNSUPPORTED, "%s: %d rows (at most 4096) over %d pages exceed the plan's LDS", who, batch, num_pages);
   const PlanArgs a{page_table, lengths, parents, new_lengths, page_table_out, lengths_out, batch, max_pages_per_seq, num_pages,
-                   page_size, hash_entries(batch), static_cast<int32_t*>(workspace), std::max(batch, num_pages / 2 + 1)};
+                   page_size, log2_of(page_size), hash_entries(batch), static_cast<int32_t*>(workspace), std::max(batch, num_pages / 2 + 1)};
   const size_t lds = update_lds(batch, num_pages);
   if (lds > (64 << 10)) {
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(palu_update_pages_kernel),
@@ -506,7 +516,7 @@ extern "C" int palu_pages_compact(const int32_t* page_table, const int32_t* leng
   const size_t lds = 4 * ((size_t)(num_pages + 31) / 32);
   if (lds > PLAN_LDS) return fail(PALU_EUNSUPPORTED, "%s: %d pages exceed the plan's LDS", who, num_pages);
   const PlanArgs a{page_table, lengths, nullptr, nullptr, page_table_out, nullptr, batch, max_pages_per_seq, num_pages,
-                   page_size, 0, static_cast<int32_t*>(workspace), std::max(batch, num_pages / 2 + 1)};
+                   page_size, log2_of(page_size), 0, static_cast<int32_t*>(workspace), std::max(batch, num_pages / 2 + 1)};
   if (lds > (64 << 10)) {
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(palu_compact_pages_kernel),
                                              hipFuncAttributeMaxDynamicSharedMemorySize, PLAN_LDS);

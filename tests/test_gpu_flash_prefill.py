@@ -117,11 +117,28 @@ def test_more_query_heads_than_rows_of_a_tile(gpu):
     _packed_check(*_packed(lens, 150, 1, 64, gpu), lens)
 
 
-def test_more_sequences_than_lanes(gpu):
-    g = torch.Generator().manual_seed(5)
-    lens = torch.randint(0, 40, (200,), generator=g).tolist()
-    lens[130] = 500
+@pytest.mark.parametrize("n", [64, 65, 200, 256, 257, 1000])
+def test_more_sequences_than_lanes(gpu, n):
+    g = torch.Generator().manual_seed(n)
+    lens = torch.randint(0, 20, (n,), generator=g).tolist()
+    lens[n // 2], lens[-1] = 500, 150
     _packed_check(*_packed(lens, 4, 2, 64, gpu), lens)
+
+
+def test_many_sequences_over_pages(gpu):
+    g = torch.Generator().manual_seed(9)
+    new, ctx = (torch.randint(lo, 30, (300,), generator=g).tolist() for lo in (0, 1))
+    ctx[250] = 700
+    _paged_check(new, ctx, 4, 2, 64, 32, "rows", gpu)
+
+
+def test_sequence_tables_that_make_no_sense_stay_inside_the_rows(gpu):
+    """Offsets that fall, or lie past the rows: what is computed is not defined, but nothing outside `out` is written."""
+    q, k, v = _packed([100], 4, 2, 64, gpu)
+    for cu in ([0, 50, 30, 200], [-5, 40, 100], [90, 10, 100], [200, 300, 400], [0] * 400 + [100, 0, 100, 7]):
+        guard = torch.full((300, 4, 64), 7.0, dtype=BF, device=gpu)
+        fused.flash_prefill(q, k, v, _ints(cu, gpu), out=guard[100:200])
+        assert (guard[:100] == 7).all() and (guard[200:] == 7).all() and torch.isfinite(guard).all()
 
 
 def test_strided_views_of_a_projection(gpu):

@@ -25,6 +25,7 @@ namespace {
 constexpr int FP_ROWS = 128;              // rows of a tile: 4 waves of 32
 constexpr int FP_KEYS = 64;               // keys of a K / V tile: two 32-position blocks
 constexpr int FP_MIN_KEYS = 256;          // keys of a piece of a split tile, about, at least
+constexpr int FP_SORTED = 256;            // sequences whose tiles are taken longest first
 constexpr int FP_WGS = 512;               // workgroups that the chip holds at once (two a CU)
 constexpr float FP_PIECE = 1.05f;         // a piece has at most about this share of a workgroup slot's part of the batch's keys
 
@@ -76,8 +77,8 @@ __device__ __forceinline__ Seq lane_seq(const FlashPrefillArgs& a, int b) {
 
 // Work order: all tiles of the batch, those with the most keys first, so that the last ones to run are short. A tile's
 // level is its distance from position 0 in tiles (of a power of two positions), rounded down; item w of the descending order is
-// found by halving over levels, the lanes counting the tiles of a sequence each (all waves do it, without a barrier; four
-// sequences of a lane stay in registers, further ones are read again for every level).
+// found by halving over levels, the lanes counting the tiles of up to four sequences each (all waves do it, without a barrier).
+// Batches of more than FP_SORTED sequences are taken sequence by sequence instead, in one pass over their lengths.
 // Where a.part is given, a tile of level t is cut along its keys into t / len + 3 / 4 pieces (one below 1.25 len), items of
 // their own, next to each other: len levels are FP_PIECE times what a workgroup slot gets of the whole batch, so the batch is cut
 // only where single tiles are long for it (few new rows over long contexts).
@@ -87,7 +88,7 @@ struct Tile {
   Seq seq;
 };
 __device__ __forceinline__ Tile find_tile(const FlashPrefillArgs& a, int w) {
-  constexpr int R = 4;
+  constexpr int R = FP_SORTED / 64;
   const int lane = threadIdx.x & 63;
   const int shift = 31 - __builtin_clz(max(1, FP_ROWS / a.rep));
   struct Levels {
@@ -98,6 +99,25 @@ __device__ __forceinline__ Tile find_tile(const FlashPrefillArgs& a, int w) {
     return b < a.B ? s : Seq{0, 0, 0};
   };
   auto levels = [&](const Seq& s) { return Levels{max(s.start, 0) >> shift, (s.len * a.rep + FP_ROWS - 1) / FP_ROWS}; };
+  auto the_seq = [](const Seq& s, int x) {                // lane x's
+    return Seq{__builtin_amdgcn_readlane(s.beg, x), __builtin_amdgcn_readlane(s.len, x), __builtin_amdgcn_readlane(s.start, x)};
+  };
+  if (a.B > FP_SORTED) {
+    int before = 0;
+    Seq next = load(lane);
+    for (int b0 = 0; b0 < a.B; b0 += 64) {
+      const Seq s = next;
+      next = load(b0 + 64 + lane);        // (past the batch: none)
+      const int n = levels(s).n, upto = before + wave_scan(n);
+      const unsigned long long m = __ballot(w < upto);
+      if (m) {
+        const int x = __builtin_ctzll(m);
+        return Tile{b0 + x, __builtin_amdgcn_readlane(upto, x) - 1 - w, 0, 1, the_seq(s, x)};   // its last tile first
+      }
+      before = __builtin_amdgcn_readlane(upto, 63);
+    }
+    return Tile{-1, 0, 0, 1, {}};
+  }
   Seq own[R];
   Levels lv[R];
 #pragma unroll
@@ -110,8 +130,7 @@ __device__ __forceinline__ Tile find_tile(const FlashPrefillArgs& a, int w) {
     }
   }
   if (a.B == 1 && !a.part) {              // one sequence: its tiles from the last on
-    const Seq s{__builtin_amdgcn_readfirstlane(own[0].beg), __builtin_amdgcn_readfirstlane(own[0].len),
-                __builtin_amdgcn_readfirstlane(own[0].start)};
+    const Seq s = the_seq(own[0], 0);
     const int n = levels(s).n;
     return Tile{w < n ? 0 : -1, n - 1 - w, 0, 1, s};
   }
@@ -120,7 +139,6 @@ __device__ __forceinline__ Tile find_tile(const FlashPrefillArgs& a, int w) {
     auto x = f(lv[0]);
 #pragma unroll
     for (int r = 1; r < R; ++r) x += f(lv[r]);
-    for (int b0 = 64 * R; b0 < a.B; b0 += 64) x += f(levels(load(b0 + lane)));
     return x;
   };
   FDiv len = make_fdiv(1 << 30);          // levels of a piece
@@ -144,10 +162,6 @@ __device__ __forceinline__ Tile find_tile(const FlashPrefillArgs& a, int w) {
   int top = 0;                            // one past the highest level
 #pragma unroll
   for (int r = 0; r < R; ++r) top = max(top, lv[r].n ? lv[r].base + lv[r].n : 0);
-  for (int b0 = 64 * R; b0 < a.B; b0 += 64) {
-    const Levels l = levels(load(b0 + lane));
-    top = max(top, l.n ? l.base + l.n : 0);
-  }
 #pragma unroll
   for (int o = 32; o; o >>= 1) top = max(top, __shfl_xor(top, o, 64));
   int lo = 0, hi = __builtin_amdgcn_readfirstlane(top);   // count(lo) > w >= count(hi) = 0
@@ -168,15 +182,13 @@ __device__ __forceinline__ Tile find_tile(const FlashPrefillArgs& a, int w) {
     if (r >= 0 && r < c) {
       const unsigned long long me = __ballot(((m >> lane) & 1) && __popcll(m & ((1ull << lane) - 1)) == r);
       const int x = __builtin_ctzll(me);
-      found = Tile{b0 + x, lo - __builtin_amdgcn_readlane(l.base, x), piece, pieces,
-                   {__builtin_amdgcn_readlane(s.beg, x), __builtin_amdgcn_readlane(s.len, x), __builtin_amdgcn_readlane(s.start, x)}};
+      found = Tile{b0 + x, lo - __builtin_amdgcn_readlane(l.base, x), piece, pieces, the_seq(s, x)};
     }
     r -= c;
   };
 #pragma unroll
   for (int k = 0; k < R; ++k)
     if (64 * k < a.B) pick(64 * k, own[k]);
-  for (int b0 = 64 * R; b0 < a.B && r >= 0; b0 += 64) pick(b0, load(b0 + lane));
   return found;
 }
 
@@ -626,8 +638,8 @@ long long most_tiles(int T, int B, int rep) { return (long long)T * rep / FP_ROW
 
 // Whether tiles may be cut along their keys: where contexts stand before the rows. (Packed prompts stand on their own keys; cutting
 // their longest tiles, one prompt of 1024 positions took 42 us instead of 27 and one of 2048 82 instead of 55.)
-bool may_split(int T, int n_q, bool paged, long long max_keys) {
-  return paged && max_keys > FP_MIN_KEYS && (long long)T * n_q <= (1ll << 28);   // (find_tile's levels stay below 2^22)
+bool may_split(int T, int B, int n_q, bool paged, long long max_keys) {
+  return paged && B <= FP_SORTED && max_keys > FP_MIN_KEYS && (long long)T * n_q <= (1ll << 28);   // (find_tile's levels stay below 2^22)
 }
 // Pieces of cut tiles per KV head, at most: with len levels to a piece, a tile of level t >= 1.25 len has at most t / len + 3 / 4
 // <= 2 t / len, and the levels' sum is at most FP_WGS / (FP_PIECE n_kv) times len.
@@ -642,7 +654,7 @@ long long cut_items(int T, int B, int n_q, int n_kv) {
 
 // Workspace: the pieces' partial results, then the items' records.
 size_t part_bytes(int n_q, int n_kv, int T, int B, bool paged, long long max_keys, int dv) {
-  if (!may_split(T, n_q, paged, max_keys)) return 0;
+  if (!may_split(T, B, n_q, paged, max_keys)) return 0;
   return (size_t)cut_items(T, B, n_q, n_kv) * n_kv * (FP_ROWS * (dv + 2) * sizeof(float) + sizeof(Record));
 }
 
@@ -652,7 +664,7 @@ int check_dims(int T, int B, int n_q, int n_kv, int dv, const char* who) {
   if (n_q % n_kv) return fail(PALU_EINVAL, "%s: n_q = %d must be a multiple of the KV head count %d", who, n_q, n_kv);
   if (dv < 16 || dv > HD || dv % 16)
     return fail(PALU_EUNSUPPORTED, "%s: head_dim_v %d (multiples of 16 up to %d)", who, dv, HD);
-  if ((long long)T * n_q > (1ll << 30) || n_q > 65535 || B > (1 << 24))
+  if ((long long)T * n_q > (1ll << 30) || n_q > 65535 || B > 65535 || most_tiles(T, B, n_q / n_kv) * n_kv > (1ll << 23))
     return fail(PALU_EUNSUPPORTED, "%s: %d rows of %d heads in %d sequences exceed the grid", who, T, n_q, B);
   return PALU_OK;
 }

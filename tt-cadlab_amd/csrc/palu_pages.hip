@@ -458,7 +458,7 @@ extern "C" int palu_latent_fill_paged(void* cache_pages, const void* rows, long 
   if (row_stride < 0 || row_stride % 8 || group_stride < 0 || group_stride % 8)
     return fail(PALU_EINVAL, "%s: source strides must be non-negative multiples of 8, got %lld and %lld", who, row_stride, group_stride);
   if (!al16(cache_pages) || !al16(rows)) return fail(PALU_EINVAL, "%s: 16-byte alignment required", who);
-  if (n_rows > (1 << 28) || batch > (1 << 24) || n_groups > 65535) return fail(PALU_EUNSUPPORTED, "%s: counts exceed the grid", who);
+  if (n_rows > (1 << 28) || batch > 65535 || n_groups > 65535) return fail(PALU_EUNSUPPORTED, "%s: counts exceed the grid", who);
   FillArgs a{static_cast<__bf16*>(cache_pages), static_cast<const __bf16*>(rows), row_stride, group_stride, cu_seqlens, start_pos,
              page_table, n_rows, batch, n_groups, width, num_pages, shift, max_pages_per_seq, 0};
   a.gpw = std::min(n_groups, std::max(1, 8192 / (32 * width)));   // 4 vectors of 8 a thread

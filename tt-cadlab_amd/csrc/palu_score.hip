@@ -339,7 +339,7 @@ extern "C" int palu_token_logprobs(const void* logits, long long ld, int dtype, 
   if (!logits || !tokens || !logprob || !entropy || (top > 0 && (!top_logprobs || !top_ids)))
     return fail(PALU_EINVAL, "%s: a required pointer is null", who);
   if (rows <= 0 || n <= 0 || ld < 0) return fail(PALU_EINVAL, "%s: rows and n must be positive, got %d and %d", who, rows, n);
-  if (n > (1 << 30)) return fail(PALU_EUNSUPPORTED, "%s: rows of %d logits", who, n);
+  if (n > (1 << 30) || rows > (1 << 23)) return fail(PALU_EUNSUPPORTED, "%s: %d rows of %d logits", who, rows, n);
   if (dtype != PALU_DTYPE_F32 && dtype != PALU_DTYPE_BF16)
     return fail(PALU_EINVAL, "%s: dtype must be PALU_DTYPE_F32 or PALU_DTYPE_BF16, got %d", who, dtype);
   if (!score_dims_ok(rows, n, top)) return fail(PALU_EINVAL, "%s: top = %d (0 .. %d, at most n)", who, top, SCORE_TOP);

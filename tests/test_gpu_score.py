@@ -76,6 +76,18 @@ def test_orders_of_the_logits(gpu, dtype):
         _check(x, t, top)
 
 
+@pytest.mark.parametrize("dtype", [BF, torch.float32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("rows,n", [(2, 50_000), (2100, 3001)])
+def test_rows_that_are_masked_but_for_a_few(gpu, dtype, rows, n):
+    """Fewer entries allowed than asked for, anywhere in the row: the others follow at -infinity, the lower id first."""
+    x, t = _case(rows, n, dtype, gpu)
+    keep = torch.randint(0, n, (rows, 6), generator=torch.Generator().manual_seed(2)).to(gpu)
+    x = torch.full_like(x, -math.inf).scatter(1, keep, x.gather(1, keep))
+    t = torch.where(t % 2 == 0, t, keep[:, 0])
+    for top in (1, 20, 64):
+        _check(x, t, top)
+
+
 def test_far_and_peaked_logits(gpu):
     """Large offsets (the statistics are differences from the maximum), one certain token, and -infinity in masked places."""
     x, t = _case(4, 3001, torch.float32, gpu)

@@ -15,7 +15,7 @@ constexpr int SCORE_TOP = 64;             // entries of a wave's list, one a lan
 constexpr int SCORE_WAVES = 4;            // of a workgroup
 constexpr int SCORE_WGS = 2048;           // workgroups that the chip holds at once
 constexpr int SCORE_PART = 8192;          // logits of a row's part, about, at least: 32 a lane
-constexpr int SCORE_PARTS = 32;          // of a row, at most
+constexpr int SCORE_PARTS = 32;           // of a row, at most
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 
 struct ScoreArgs {
@@ -33,7 +33,7 @@ struct ScoreArgs {
 
 // Entries compare as (value, lower index first): one 64-bit key, value made order-preserving above, complemented index below.
 // -0 counts as 0 and every NaN as one value.
-__device__ __forceinline__ unsigned order_key(unsigned b) {   // of a float's bits (integers only: scalar where b is)
+__device__ __forceinline__ unsigned order_key(unsigned b) {   // of a float's bits
   const unsigned k = b & 0x80000000u ? (b == 0x80000000u ? b : ~b) : b | 0x80000000u;
   return (b & 0x7fffffffu) > 0x7f800000u ? 0xffffffffu : k;
 }
@@ -238,16 +238,18 @@ __global__ __launch_bounds__(SCORE_WAVES * 64) void palu_score_kernel(const Scor
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         u64 who = __ballot(!(f[u][i] < bound));
-        while (who) {                     // one lane's entry after the other, what can be in scalar registers
-          const int l = __builtin_ctzll(who), v = v0 + u * 64 + l, idx = v * N - skew + i;
+        if (!who) continue;
+        // What beats the last of the list joins it, lane by lane; against the risen last the lanes compare again, so that a row
+        // of equal values (most of it masked) costs no more than what joins.
+        const int v = v0 + u * 64 + lane, idx = v * N - skew + i;
+        const u64 c = v < v_hi && idx >= 0 && idx < a.n ? entry(__float_as_uint(f[u][i]), idx) : 0;
+        while ((who &= __ballot(c > least))) {
+          const u64 x = lane_of(c, __builtin_ctzll(who));
           who &= who - 1;
-          const u64 c = entry(__builtin_amdgcn_readlane(__float_as_uint(f[u][i]), l), idx);
-          if (c > least && v < v_hi && idx >= 0 && idx < a.n) {
-            // the lanes that hold less move on by one, the first of them takes the entry
-            const u64 up = lane_before(mine);
-            if (mine < c) mine = lane > 0 && up < c ? up : c;
-            least = lane_of(mine, a.top - 1);
-          }
+          // the lanes that hold less move on by one, the first of them takes the entry
+          const u64 up = lane_before(mine);
+          if (mine < x) mine = lane > 0 && up < x ? up : x;
+          least = lane_of(mine, a.top - 1);
         }
       }
     if (least) bound = __builtin_elementwise_maximum(bound, key_value((unsigned)(least >> 32)));

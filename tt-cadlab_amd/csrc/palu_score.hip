@@ -8,6 +8,7 @@
 #include "palu_kernel.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace {
 
@@ -59,11 +60,26 @@ struct __attribute__((aligned(16))) Stats {
 // (log2 p is bounded below where it multiplies: p is 0 there, and -infinity times 0 is NaN.)
 __device__ __forceinline__ float log2p(float x, float m) { return __builtin_elementwise_maximum((x - m) * LOG2E, -1000.f); }
 
-__device__ __forceinline__ Stats join(Stats a, Stats b) {
-  const float m = __builtin_elementwise_maximum(a.m, b.m), ref = m == NEG_INF ? 0.f : m;
-  const float ta = log2p(a.m, ref), tb = log2p(b.m, ref);
-  const float ca = __builtin_amdgcn_exp2f(ta), cb = __builtin_amdgcn_exp2f(tb);
-  return Stats{m, ca * a.z + cb * b.z, ca * fmaf(ta, a.z, a.e) + cb * fmaf(tb, b.z, b.e)};
+// f over all lanes: within rows of 16 by DPP (a shuffle would go through LDS), then the four rows.
+template <typename F>
+__device__ __forceinline__ float over_lanes(float x, F f) {
+  auto dpp = [&](auto ctrl) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), decltype(ctrl)::value, 0xf, 0xf, false));
+  };
+  x = f(x, dpp(std::integral_constant<int, 0xb1>{}));     // lanes 1 apart, 2 apart,
+  x = f(x, dpp(std::integral_constant<int, 0x4e>{}));
+  x = f(x, dpp(std::integral_constant<int, 0x141>{}));    // the halves of 8, of 16, mirrored
+  x = f(x, dpp(std::integral_constant<int, 0x140>{}));
+  auto row = [&](int l) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), l)); };
+  return f(f(row(0), row(16)), f(row(32), row(48)));
+}
+
+// The lanes' statistics as one.
+__device__ __forceinline__ Stats join(const Stats& s) {
+  const float m = over_lanes(s.m, [](float a, float b) { return __builtin_elementwise_maximum(a, b); });
+  const float t = log2p(s.m, m == NEG_INF ? 0.f : m), c = __builtin_amdgcn_exp2f(t);
+  auto sum = [](float a, float b) { return a + b; };
+  return Stats{m, over_lanes(c * s.z, sum), over_lanes(c * fmaf(t, s.z, s.e), sum)};
 }
 
 template <typename T>
@@ -79,17 +95,23 @@ struct Vec<float> {
   typedef f32x4 V;
 };
 
-// The largest value bits t, to 16 bits, that at least `top` of the lanes' `n` keys (R of each, 0: none) reach.
-template <int R>
+// The largest value bits t, to 16 bits, that at least `top` of the lanes' `n` keys (R of each, 0: none) reach. BITS at a time:
+// two where a wave has its SIMD to itself (the counts of three candidates are independent; the join of 64 rows took 5.1 us in
+// place of 5.8), one where waves share it (three counts are more work; 300 rows took 31 us in place of 34).
+template <int R, int BITS>
 __device__ __forceinline__ unsigned reached_by(const unsigned (&k)[R], int n, int top) {
   unsigned t = 0;
-  for (int bit = 31; bit >= 16; --bit) {
-    const unsigned c = t | 1u << bit;
-    int m = 0;
+  for (int bit = 32 - BITS; bit >= 16; bit -= BITS) {
+    int m[1 << BITS] = {};
 #pragma unroll
     for (int r = 0; r < R; ++r)
-      if (64 * r < n) m += __popcll(__ballot(k[r] >= c));
-    if (m >= top) t = c;
+      if (64 * r < n)
+#pragma unroll
+        for (int d = 1; d < 1 << BITS; ++d) m[d] += __popcll(__ballot(k[r] >= (t | (unsigned)d << bit)));
+    unsigned most = 0;
+#pragma unroll
+    for (int d = 1; d < 1 << BITS; ++d) most = m[d] >= top ? d : most;
+    t |= most << bit;
   }
   return t;
 }
@@ -109,7 +131,7 @@ __device__ __forceinline__ int merge_lists(const u64* lists, int n, int top, u64
       const unsigned x = (unsigned)(lists[min(64 * r + lane, all - 1)] >> 32);
       k[r] = 64 * r + lane < all ? x : 0;
     }
-    t = reached_by(k, all, top);
+    t = reached_by<R, 2>(k, all, top);
   }
   __syncthreads();
   for (int i = threadIdx.x; i < all; i += SCORE_WAVES * 64) {
@@ -228,7 +250,7 @@ __global__ __launch_bounds__(SCORE_WAVES * 64) void palu_score_kernel(const Scor
       unsigned k4[SCORE_WAVES];
 #pragma unroll
       for (int r = 0; r < SCORE_WAVES; ++r) k4[r] = keys[64 * r + lane];
-      const unsigned t = reached_by(k4, SCORE_WAVES * 64, a.top);
+      const unsigned t = reached_by<SCORE_WAVES, 1>(k4, SCORE_WAVES * 64, a.top);
       if (t > order_key(0xff800000u)) bound = __builtin_elementwise_maximum(bound, key_value(t));
     }
     // Values compare as floats, NaN above all: !(x < bound).
@@ -254,15 +276,11 @@ __global__ __launch_bounds__(SCORE_WAVES * 64) void palu_score_kernel(const Scor
       }
     if (least) bound = __builtin_elementwise_maximum(bound, key_value((unsigned)(least >> 32)));
   }
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1)
-    st = join(st, Stats{__shfl_xor(st.m, o, 64), __shfl_xor(st.z, o, 64), __shfl_xor(st.e, o, 64)});
+  st = join(st);
   if (lane == 0) stats[w] = st;
   if (lane < a.top) lists[w * a.top + lane] = mine;
   __syncthreads();
-  st = stats[0];
-#pragma unroll
-  for (int i = 1; i < SCORE_WAVES; ++i) st = join(st, stats[i]);
+  st = join(lane < SCORE_WAVES ? stats[lane] : Stats{NEG_INF, 0.f, 0.f});
   if (a.parts == 1) {
     finish_row<SCORE_WAVES>(a, row, st, token_logit, lists, SCORE_WAVES, left, &count);
     return;
@@ -303,9 +321,7 @@ __global__ __launch_bounds__(SCORE_WAVES * 64) void palu_score_join_kernel(const
     const int p = i * SCORE_WAVES + (threadIdx.x >> 6);
     if (p < a.parts && lane < a.top) lists[p * a.top + lane] = x[i];
   }
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1)
-    st = join(st, Stats{__shfl_xor(st.m, o, 64), __shfl_xor(st.z, o, 64), __shfl_xor(st.e, o, 64)});
+  st = join(st);
   __syncthreads();
   u64* left = lists + a.parts * a.top;
   if (a.parts * a.top <= 64 * 8) finish_row<8>(a, row, st, token_logit, lists, a.parts, left, &count);

@@ -192,6 +192,13 @@ __device__ __forceinline__ Tile find_tile(const FlashPrefillArgs& a, int w) {
   return found;
 }
 
+// The item of workgroup w (of n per KV head). The first `half` go to a CU each, the next as many beside them: in reverse, so that the
+// longest items have the shortest of these for neighbours.
+__device__ __forceinline__ int place(int w, int n, int half) {
+  const int upto = min(2 * half, n);
+  return w >= half && w < upto ? half + upto - 1 - w : w;
+}
+
 // A tile's rows are rows row0 .. of the sequence, row = position * rep + head: position and head of row row0 + x.
 struct RowSplit {
   int pos0, rem;
@@ -220,10 +227,11 @@ __global__ __launch_bounds__(256, 2) void palu_flash_prefill_kernel(const FlashP
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   // A KV head's workgroups are n_kv ids apart, for 8 heads all on one XCD, whose L2 then holds that head's K and V.
   const int kvh = blockIdx.x % a.n_kv;
-  const Tile tile = find_tile(a, blockIdx.x / a.n_kv);
-  const bool recorded = blockIdx.x / a.n_kv < a.cut;
+  const int item = place(blockIdx.x / a.n_kv, gridDim.x / a.n_kv, FP_WGS / 2 / a.n_kv);
+  const Tile tile = find_tile(a, item);
+  const bool recorded = item < a.cut;
   auto record = [&](const Record& r) {
-    if (recorded && threadIdx.x == 0) a.records[blockIdx.x] = r;
+    if (recorded && threadIdx.x == 0) a.records[item * a.n_kv + kvh] = r;
   };
   if (tile.b < 0) {                       // uniform, before any barrier
     record(Record{});
@@ -566,7 +574,7 @@ __global__ __launch_bounds__(256, 2) void palu_flash_prefill_kernel(const FlashP
   const float l = l_run + __shfl_xor(l_run, 32, 64);
   if (32 * w + n >= rows) return;
   if (n_pieces > 1) {                     // one of several pieces (which are the first of all items)
-    float* po = a.part + (long long)blockIdx.x * FP_ROWS * (a.dv + 2);
+    float* po = a.part + ((long long)item * a.n_kv + kvh) * FP_ROWS * (a.dv + 2);
     const int r = 32 * w + n;
     if (h == 0) {
       po[FP_ROWS * a.dv + r] = m_run;

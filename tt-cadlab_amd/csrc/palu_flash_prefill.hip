@@ -137,8 +137,9 @@ __device__ __forceinline__ Tile find_tile(const FlashPrefillArgs& a, int w) {
   // a sum over all sequences' levels
   auto over_all = [&](auto f) {
     auto x = f(lv[0]);
+    if (a.B > 64)
 #pragma unroll
-    for (int r = 1; r < R; ++r) x += f(lv[r]);
+      for (int r = 1; r < R; ++r) x += f(lv[r]);
     return x;
   };
   FDiv len = make_fdiv(1 << 30);          // levels of a piece
@@ -158,20 +159,22 @@ __device__ __forceinline__ Tile find_tile(const FlashPrefillArgs& a, int w) {
   auto count = [&](int t) {               // pieces at level t or above
     return wave_sum_i(over_all([&](Levels l) { return l.base + l.n > t ? pieces_below(l.base + l.n) - pieces_below(max(l.base, t)) : 0; }));
   };
-  if (w >= count(0)) return Tile{-1, 0, 0, 1, {}};
-  int top = 0;                            // one past the highest level
+  int top = lv[0].n ? lv[0].base + lv[0].n : 0;            // one past the highest level
+  if (a.B > 64)
 #pragma unroll
-  for (int r = 0; r < R; ++r) top = max(top, lv[r].n ? lv[r].base + lv[r].n : 0);
-#pragma unroll
-  for (int o = 32; o; o >>= 1) top = max(top, __shfl_xor(top, o, 64));
-  int lo = 0, hi = __builtin_amdgcn_readfirstlane(top);   // count(lo) > w >= count(hi) = 0
+    for (int r = 1; r < R; ++r) top = max(top, lv[r].n ? lv[r].base + lv[r].n : 0);
+  int lo = 0, hi = wave_max_i(top), above = 0;            // the level lies in [lo, hi); above = count(hi) <= w
   while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (count(mid) > w) lo = mid;
-    else hi = mid;
+    const int mid = (lo + hi) >> 1, c = count(mid);
+    if (c > w) {
+      lo = mid;
+    } else {
+      hi = mid;
+      above = c;
+    }
   }
   const int pieces = a.part ? max(1, __builtin_amdgcn_readfirstlane(fdiv(lo + round, len))) : 1;
-  int r = w - count(lo + 1);              // which piece of the sequences that have level lo
+  int r = w - above;                      // which piece of the sequences that have level lo
   const int piece = r % pieces;
   r /= pieces;
   Tile found{-1, 0, 0, 1, {}};

@@ -409,6 +409,15 @@ __device__ __forceinline__ int wave_scan(int x) {
   return x;
 }
 __device__ __forceinline__ int wave_sum_i(int x) { return __builtin_amdgcn_readlane(wave_scan(x), 63); }
+// Maximum of non-negative values over the wave, uniform.
+__device__ __forceinline__ int wave_max_i(int x) {
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false));   // row_shr 1, 2, 4, 8
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false));
+  auto row = [&](int l) { return __builtin_amdgcn_readlane(x, l); };
+  return max(max(row(15), row(31)), max(row(47), row(63)));
+}
 
 // The row length of row r0 + lane (0 past the batch).
 __device__ __forceinline__ int lane_row_len(const DecodeArgs& a, int r0) {

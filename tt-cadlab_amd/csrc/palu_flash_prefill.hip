@@ -622,41 +622,72 @@ __global__ __launch_bounds__(256, 2) void palu_flash_prefill_kernel(const FlashP
     }
 }
 
-// Joins the pieces of a tile: out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s. One workgroup per (item, KV head, 32 rows), 32
-// threads to a row, those of a first piece work; what the item is stands in its record. Bound by latency: a row's threads
-// share the pieces' statistics, and the loads of eight pieces are in flight at once.
+// Joins the pieces of a tile: out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s. One workgroup per (item, KV head, 32 rows),
+// those of a first piece work; what the item is stands in its record. 32 threads to a row, N rows of a thread (8 apart).
+// Bound by latency (the record, the statistics, the results): the rows' and pieces' loads are on their way together.
 constexpr int JOIN_ROWS = 32;
-__global__ __launch_bounds__(256) void palu_flash_prefill_join_kernel(const FlashPrefillArgs a) {
-  const int rest = blockIdx.x / a.n_kv, kvh = blockIdx.x - rest * a.n_kv, item = rest / (FP_ROWS / JOIN_ROWS);
-  const Record rec = a.records[item * a.n_kv + kvh];
-  const int r0 = rest % (FP_ROWS / JOIN_ROWS) * JOIN_ROWS, sub = threadIdx.x & 31, ns = rec.pieces;
-  if (ns == 0 || r0 >= rec.rows) return;
+template <int N>
+__device__ __forceinline__ void join_rows(const FlashPrefillArgs& a, const Record& rec, const float* part, int kvh, int r0) {
+  const int sub = threadIdx.x & 31, ns = rec.pieces, rw = r0 + (threadIdx.x >> 5), d = 4 * sub;
   const RowSplit rs{rec.pos0, rec.rem, make_fdiv(a.rep)};
-  const long long stride = (long long)FP_ROWS * (a.dv + 2) * a.n_kv;   // pieces are n_kv workgroups apart
-  const float* part = a.part + ((long long)item * a.n_kv + kvh) * FP_ROWS * (a.dv + 2);
-  for (int r = r0 + (threadIdx.x >> 5); r < min(r0 + JOIN_ROWS, rec.rows); r += 8) {
-    const float* ml = part + FP_ROWS * a.dv + r;
-    float M = NEG_INF, l = 0.f;
-    for (int s = sub; s < ns; s += 32) M = fmaxf(M, ml[s * stride]);
+  const long long stride = (long long)FP_ROWS * (a.dv + 2) * a.n_kv;   // pieces are n_kv places apart
+  const float *ml[N], *o[N];
+  float M[N], l[N], w[N];
+  f32x4 y[N];
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) M = fmaxf(M, __shfl_xor(M, o, 32));
-    const float ref = M == NEG_INF ? 0.f : M;
-    for (int s = sub; s < ns; s += 32) l += __builtin_amdgcn_exp2f(ml[s * stride] - ref) * ml[s * stride + FP_ROWS];
+  for (int i = 0; i < N; ++i) {
+    const int r = min(rw + 8 * i, rec.rows - 1);
+    ml[i] = part + FP_ROWS * a.dv + r;
+    o[i] = part + r * a.dv + min(d, a.dv - 4);
+    M[i] = NEG_INF;
+    l[i] = 0.f;
+    y[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  for (int s = sub; s < ns; s += 32)
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) l += __shfl_xor(l, o, 32);
-    const int d = 4 * sub, pos = row_pos(rs, r);
-    if (d >= a.dv) continue;
-    f32x4 y = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-    for (int s = 0; s < ns; ++s)
-      y += *reinterpret_cast<const f32x4*>(part + s * stride + r * a.dv + d) * __builtin_amdgcn_exp2f(ml[s * stride] - ref);
-    const float inv = 1.f / l;
+    for (int i = 0; i < N; ++i) M[i] = fmaxf(M[i], ml[i][s * stride]);
+#pragma unroll
+  for (int x = 1; x < 32; x <<= 1)
+#pragma unroll
+    for (int i = 0; i < N; ++i) M[i] = fmaxf(M[i], __shfl_xor(M[i], x, 32));
+  for (int s0 = 0; s0 < ns; s0 += 32) {
+    const int s = s0 + sub;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {         // lane `sub` has the weight of piece s0 + sub
+      const float x = ml[i][min(s, ns - 1) * stride], z = ml[i][min(s, ns - 1) * stride + FP_ROWS];
+      w[i] = s < ns ? __builtin_amdgcn_exp2f(x - (M[i] == NEG_INF ? 0.f : M[i])) : 0.f;
+      l[i] += s < ns ? w[i] * z : 0.f;
+    }
+#pragma unroll 4
+    for (int c = 0; c < min(32, ns - s0); ++c)
+#pragma unroll
+      for (int i = 0; i < N; ++i) y[i] += *reinterpret_cast<const f32x4*>(o[i] + (s0 + c) * stride) * __shfl(w[i], c, 32);
+  }
+#pragma unroll
+  for (int x = 1; x < 32; x <<= 1)
+#pragma unroll
+    for (int i = 0; i < N; ++i) l[i] += __shfl_xor(l[i], x, 32);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int r = rw + 8 * i, pos = row_pos(rs, r);
+    if (d >= a.dv || r >= min(r0 + JOIN_ROWS, rec.rows)) continue;
+    const float inv = 1.f / l[i];
     bf16x4 x;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = rec.start + pos < 0 ? (__bf16)0.f : (__bf16)(y[i] * inv);
+    for (int k = 0; k < 4; ++k) x[k] = rec.start + pos < 0 ? (__bf16)0.f : (__bf16)(y[i][k] * inv);
     *reinterpret_cast<bf16x4*>(a.out + ((long long)(rec.beg + pos) * a.n_q + (long long)kvh * a.rep +
                                         (rs.rem + r - (pos - rs.pos0) * a.rep)) * a.dv + d) = x;
   }
+}
+
+__global__ __launch_bounds__(256) void palu_flash_prefill_join_kernel(const FlashPrefillArgs a) {
+  const int rest = blockIdx.x / a.n_kv, kvh = blockIdx.x - rest * a.n_kv, item = rest / (FP_ROWS / JOIN_ROWS);
+  const Record rec = a.records[item * a.n_kv + kvh];
+  const int r0 = rest % (FP_ROWS / JOIN_ROWS) * JOIN_ROWS;
+  if (rec.pieces == 0 || r0 >= rec.rows) return;
+  const float* part = a.part + ((long long)item * a.n_kv + kvh) * FP_ROWS * (a.dv + 2);
+  if (rec.rows - r0 <= 8) join_rows<1>(a, rec, part, kvh, r0);
+  else join_rows<JOIN_ROWS / 8>(a, rec, part, kvh, r0);
 }
 
 // Tiles of a batch, at most: a sequence's last tile may hold fewer rows.

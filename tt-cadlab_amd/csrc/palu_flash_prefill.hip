@@ -628,6 +628,7 @@ __global__ __launch_bounds__(256, 2) void palu_flash_prefill_kernel(const FlashP
 constexpr int JOIN_ROWS = 32;
 template <int N>
 __device__ __forceinline__ void join_rows(const FlashPrefillArgs& a, const Record& rec, const float* part, int kvh, int r0) {
+  constexpr int U = N == 1 ? 8 : 1;       // pieces at a time (4 for N = 4: 1 to 4 % more time for the whole call)
   const int sub = threadIdx.x & 31, ns = rec.pieces, rw = r0 + (threadIdx.x >> 5), d = 4 * sub;
   const RowSplit rs{rec.pos0, rec.rem, make_fdiv(a.rep)};
   const long long stride = (long long)FP_ROWS * (a.dv + 2) * a.n_kv;   // pieces are n_kv places apart
@@ -658,10 +659,20 @@ __device__ __forceinline__ void join_rows(const FlashPrefillArgs& a, const Recor
       w[i] = s < ns ? __builtin_amdgcn_exp2f(x - (M[i] == NEG_INF ? 0.f : M[i])) : 0.f;
       l[i] += s < ns ? w[i] * z : 0.f;
     }
-#pragma unroll 4
-    for (int c = 0; c < min(32, ns - s0); ++c)
+    for (int c = s0; c < min(s0 + 32, ns); c += U) {
+      f32x4 v[U][N];
 #pragma unroll
-      for (int i = 0; i < N; ++i) y[i] += *reinterpret_cast<const f32x4*>(o[i] + (s0 + c) * stride) * __shfl(w[i], c, 32);
+      for (int k = 0; k < U; ++k)
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[k][i] = *reinterpret_cast<const f32x4*>(o[i] + min(c + k, ns - 1) * stride);
+#pragma unroll
+      for (int k = 0; k < U; ++k)
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const f32x4 t = v[k][i] * __shfl(w[i], c + k - s0, 32);
+          if (c + k < ns) y[i] += t;
+        }
+    }
   }
 #pragma unroll
   for (int x = 1; x < 32; x <<= 1)

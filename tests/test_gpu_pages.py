@@ -353,3 +353,9 @@ def test_page_refusals(gpu):
     with pytest.raises(RuntimeError, match="at least one row"):
         h.compact(t[:0], ln[:0])
     assert h.update(t[:0], ln[:0])[0].shape == (0, 2)
+
+
+@pytest.mark.parametrize("shape", [(0, 2, 32, 16), (4, 0, 32, 16), (4, 2, 32, 0)])
+def test_empty_pools_are_refused(gpu, shape):
+    with pytest.raises(RuntimeError, match="not empty"):
+        PagePools([torch.zeros(*shape, dtype=BF, device=gpu)])

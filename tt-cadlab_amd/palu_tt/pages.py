@@ -43,11 +43,12 @@ class PagePools:
         stores = [p.data if isinstance(p, LatentCache) else p for p in self.pools]
         for p, s in zip(self.pools, stores):
             if not (isinstance(s, torch.Tensor) and len(p.shape) == 4 and s.is_cuda and s.dtype == torch.bfloat16 and
-                    s.is_contiguous() and s.data_ptr() % 16 == 0):
-                raise RuntimeError("a pool is a contiguous, 16-byte aligned bf16 [n_pages, n_groups, page_size, width] tensor on "
-                                   "the GPU or a LatentCache")
+                    s.is_contiguous() and s.data_ptr() % 16 == 0 and s.numel()):
+                raise RuntimeError("a pool is a contiguous, 16-byte aligned bf16 [n_pages, n_groups, page_size, width] tensor, "
+                                   "not empty, on the GPU or a LatentCache")
             if (p.shape[0], p.shape[2], s.device) != (self.pools[0].shape[0], self.pools[0].shape[2], stores[0].device):
-                raise RuntimeError(f"pools must agree in pages, page size and device: {tuple(p.shape)}, {tuple(self.pools[0].shape)}")
+                raise RuntimeError("pools must agree in pages, page size and device: "
+                                   f"{tuple(p.shape)}, {tuple(self.pools[0].shape)}")
         self.n_pages, self.page_size = int(self.pools[0].shape[0]), int(self.pools[0].shape[2])
         self.device = stores[0].device
         if any(_overlap(a, b) for i, a in enumerate(stores) for b in stores[:i]):

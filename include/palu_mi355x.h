@@ -418,8 +418,9 @@ size_t palu_prefill_workspace_bytes(int users, int seq, int n_heads, int n_kv, i
 /* ---- Packed batches over page pools -------------------------------------------------------------------
  * Sequences of different lengths in one call: the new rows of `batch` sequences lie one after another, sequence b's at
  * cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (int32 [batch + 1], device memory, not decreasing, from 0); rows past
- * cu_seqlens[batch] belong to no sequence: their outputs keep what they hold. At most 65535 sequences. Pages, tables and layouts as for
- * palu_flash_decode_paged. No counterparts in the reference (its caches are contiguous, its prefill one prompt). */
+ * cu_seqlens[batch] belong to no sequence: their outputs keep what they hold. At most 65535 sequences. Pages, tables and
+ * layouts as for palu_flash_decode_paged. No counterparts in the reference (its caches are contiguous, its prefill one
+ * prompt). */
 
 /* Causal attention of packed sequences over full K and V, each over its own rows: row i of a sequence sees its rows 0 .. i.
  *   q [rows][n_q][128], k [rows][n_kv][128], v [rows][n_kv][head_dim_v] bf16, rows and heads at the element strides given

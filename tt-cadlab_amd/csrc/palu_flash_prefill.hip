@@ -4,9 +4,9 @@
 // K and V either the packed rows themselves (start 0) or page pools, row-major or in the caches' tile order.
 //
 // One pass over the keys per tile of queries. The rows of a tile are (position, head of the KV group) pairs of one
-// sequence and one KV head, position-major: the heads of a group share every K and V tile, and a tile of 128 rows is 128 / rep
-// positions tall, so that little of its last key tiles lies past the diagonal. A workgroup's 4 waves take 32 rows
-// each and share 64-key tiles of K and V in LDS, copied straight there (global_load_lds) one tile ahead.
+// sequence and one KV head, position-major: the heads of a group share every K and V tile, and a tile of 128 rows is
+// 128 / rep positions tall, so that little of its last key tiles lies past the diagonal. A workgroup's 4 waves take 32 rows
+// each and share 64-key tiles of K and V in LDS, copied straight there (global_load_lds), K two tiles ahead and V one.
 //   S^T (keys x rows) = K Q^T, Q the B operand of v_mfma_f32_32x32x16_bf16, in registers for the whole pass;
 //   P^T = 2^(S^T - m), the running maximum m refreshed when a score exceeds it by more than 2^8;
 //   O^T (dims x rows) += V^T P^T.
@@ -14,8 +14,15 @@
 // keys 8 g .. + 7 in pairs of registers, which is the B operand of the second product, and no value changes lanes.
 // V^T comes from the caches' V tiles as it stands, from rows by transposing LDS reads (ds_read_b64_tr_b16).
 //
+// Bound by the matrix cores where sequences are long: they are busy 62 % of a CU's cycles over a prompt of 8192 positions,
+// at the 1.65 GHz that the card's power limit leaves; S of the next tile runs beside the exponentials of this one, and two
+// workgroups share a CU. 32 query heads over 8 KV heads, widths 128: a prompt of 8192 takes 506 us (1.09 PFLOP/s), of 16384
+// 1.97 ms (1.12); 2048 rows behind 30000 positions in pages 0.90 ms (1.16); 64 rows, one behind each of 8000 positions,
+// 365 us (5.7 TB/s). Short sequences pay for each tile's search, first loads and masked keys, some 20 thousand cycles beside
+// 2100 to 2900 per 64 keys: 8 prompts of 2 to 2048 79 us (0.74 PFLOP/s), 128 of 128 127 us.
+//
 // Rounding: scores, statistics and sums are fp32 (products of bf16 are exact in them); the probabilities are rounded to
-// bf16 for the second product, half a step of 2^-9 of each, less in their weighted sum than the output's own rounding.
+// bf16 for the second product, off by at most 2^-8 of each, less in their weighted sum than the output's own rounding.
 #include "palu_kernel.h"
 
 #include <algorithm>
@@ -27,7 +34,7 @@ constexpr int FP_KEYS = 64;               // keys of a K / V tile: two 32-positi
 constexpr int FP_MIN_KEYS = 256;          // keys of a piece of a split tile, about, at least
 constexpr int FP_SORTED = 256;            // sequences whose tiles are taken longest first
 constexpr int FP_WGS = 512;               // workgroups that the chip holds at once (two a CU)
-constexpr float FP_PIECE = 1.05f;         // a piece has at most about this share of a workgroup slot's part of the batch's keys
+constexpr float FP_PIECE = 1.05f;         // keys of a piece over a workgroup slot's part of the batch's, about, at most
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -55,7 +62,7 @@ struct FlashPrefillArgs {
   float qscale;                           // |scale| * log2 e (1 for a scale of 0: a masked score times 0 would be NaN)
   int sign;                               // of the scale: -1, 0, 1; Q is taken times that
   __bf16* out;                            // [T][n_q][dv]
-  float* part;                            // where keys may be split: unnormalised O of a piece [FP_ROWS][dv], then m and l [FP_ROWS] each
+  float* part;                            // where keys may be cut: a piece's unnormalised O [FP_ROWS][dv], m, l [FP_ROWS]
   Record* records;                        // of the items that may be pieces: `cut` per KV head
   int cut;
 };
@@ -76,12 +83,13 @@ __device__ __forceinline__ Seq lane_seq(const FlashPrefillArgs& a, int b) {
 }
 
 // Work order: all tiles of the batch, those with the most keys first, so that the last ones to run are short. A tile's
-// level is its distance from position 0 in tiles (of a power of two positions), rounded down; item w of the descending order is
-// found by halving over levels, the lanes counting the tiles of up to four sequences each (all waves do it, without a barrier).
-// Batches of more than FP_SORTED sequences are taken sequence by sequence instead, in one pass over their lengths.
+// level is its distance from position 0 in tiles (of a power of two positions), rounded down; item w of the descending
+// order is found by halving over levels, the lanes counting the tiles of up to four sequences each (all waves do it, without
+// a barrier; one sequence's is found directly). Batches of more than FP_SORTED sequences are taken sequence by sequence
+// instead, in one pass over their lengths.
 // Where a.part is given, a tile of level t is cut along its keys into t / len + 3 / 4 pieces (one below 1.25 len), items of
-// their own, next to each other: len levels are FP_PIECE times what a workgroup slot gets of the whole batch, so the batch is cut
-// only where single tiles are long for it (few new rows over long contexts).
+// their own, next to each other: len levels are FP_PIECE times what a workgroup slot gets of the whole batch, so the batch
+// is cut only where single tiles are long for it (few new rows over long contexts).
 struct Tile {
   int b, j;                               // j: tile of sequence b; b < 0: none
   int piece, pieces;
@@ -157,7 +165,10 @@ __device__ __forceinline__ Tile find_tile(const FlashPrefillArgs& a, int w) {
     return q * (q - 1) / 2 * len.d + (u - q * len.d) * q + min(t, len.d - round);
   };
   auto count = [&](int t) {               // pieces at level t or above
-    return wave_sum_i(over_all([&](Levels l) { return l.base + l.n > t ? pieces_below(l.base + l.n) - pieces_below(max(l.base, t)) : 0; }));
+    return wave_sum_i(over_all([&](Levels l) {
+      const int end = l.base + l.n;
+      return end > t ? pieces_below(end) - pieces_below(max(l.base, t)) : 0;
+    }));
   };
   int top = lv[0].n ? lv[0].base + lv[0].n : 0;            // one past the highest level
   if (a.B > 64)
@@ -195,8 +206,8 @@ __device__ __forceinline__ Tile find_tile(const FlashPrefillArgs& a, int w) {
   return found;
 }
 
-// The item of workgroup w (of n per KV head). The first `half` go to a CU each, the next as many beside them: in reverse, so that the
-// longest items have the shortest of these for neighbours.
+// The item of workgroup w (of n per KV head). The first `half` go to a CU each, the next as many beside them: in reverse, so
+// that the longest items have the shortest of these for neighbours (one prompt of 2048: 52 us instead of 56).
 __device__ __forceinline__ int place(int w, int n, int half) {
   const int upto = min(2 * half, n);
   return w >= half && w < upto ? half + upto - 1 - w : w;
@@ -553,8 +564,8 @@ __global__ __launch_bounds__(256, 2) void palu_flash_prefill_kernel(const FlashP
     if (t_lo * FP_KEYS <= w_hi) scores(s0, sk0);
     int t = t_lo;
     const int nfull = min(nt, (key_pos(0) + 1) / FP_KEYS);   // tiles that all rows of the workgroup see whole
-    // An odd last one of packed rows is a step, too (128 sequences of 128 rows: 123 us instead of 133). Over pages it is a tail: the
-    // exit in the loop's middle costs the loop 1.5 to 3 % there (2048 rows behind 30000 positions: 748 us instead of 726).
+    // An odd last one of packed rows is a step, too (128 sequences of 128 rows: 123 us instead of 133). Over pages it is a
+    // tail: the exit in the loop's middle costs the loop 1.5 to 3 % there (2048 rows behind 30000: 748 us instead of 726).
     const int whole = SRC == PACKED ? nfull : t_lo + ((nfull - t_lo) & ~1);
     bool odd = false;                     // which stages hold tile t
     while (t < whole) {
@@ -624,7 +635,9 @@ __global__ __launch_bounds__(256, 2) void palu_flash_prefill_kernel(const FlashP
 
 // Joins the pieces of a tile: out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s. One workgroup per (item, KV head, 32 rows),
 // those of a first piece work; what the item is stands in its record. 32 threads to a row, N rows of a thread (8 apart).
-// Bound by latency (the record, the statistics, the results): the rows' and pieces' loads are on their way together.
+// Bound by latency (the record, the statistics, the results): the rows' and pieces' loads are on their way together, which
+// took it from 15.4 to 8.4 us for 8 sequences of up to 300 rows over up to 32000 positions, and the whole call of one row
+// over 32000 from 41 to 31.
 constexpr int JOIN_ROWS = 32;
 template <int N>
 __device__ __forceinline__ void join_rows(const FlashPrefillArgs& a, const Record& rec, const float* part, int kvh, int r0) {
@@ -704,10 +717,11 @@ __global__ __launch_bounds__(256) void palu_flash_prefill_join_kernel(const Flas
 // Tiles of a batch, at most: a sequence's last tile may hold fewer rows.
 long long most_tiles(int T, int B, int rep) { return (long long)T * rep / FP_ROWS + std::min(T, B); }
 
-// Whether tiles may be cut along their keys: where contexts stand before the rows. (Packed prompts stand on their own keys; cutting
-// their longest tiles, one prompt of 1024 positions took 42 us instead of 27 and one of 2048 82 instead of 55.)
+// Whether tiles may be cut along their keys: where contexts stand before the rows. (Packed prompts stand on their own keys;
+// cutting their longest tiles, one prompt of 1024 positions took 42 us instead of 27 and one of 2048 82 instead of 55.)
+// Up to 2^28 rows of heads, which keeps find_tile's levels below 2^22.
 bool may_split(int T, int B, int n_q, bool paged, long long max_keys) {
-  return paged && B <= FP_SORTED && max_keys > FP_MIN_KEYS && (long long)T * n_q <= (1ll << 28);   // (find_tile's levels stay below 2^22)
+  return paged && B <= FP_SORTED && max_keys > FP_MIN_KEYS && (long long)T * n_q <= (1ll << 28);
 }
 // Pieces of cut tiles per KV head, at most: with len levels to a piece, a tile of level t >= 1.25 len has at most t / len + 3 / 4
 // <= 2 t / len, and the levels' sum is at most FP_WGS / (FP_PIECE n_kv) times len.
@@ -738,11 +752,12 @@ int check_dims(int T, int B, int n_q, int n_kv, int dv, const char* who) {
 }
 
 template <Source SRC>
-int launch_prefill(FlashPrefillArgs& a, long long max_keys, void* workspace, size_t workspace_bytes, const char* who, hipStream_t s) {
+int launch_prefill(FlashPrefillArgs& a, long long max_keys, void* workspace, size_t workspace_bytes, const char* who,
+                   hipStream_t s) {
   const size_t need = part_bytes(a.n_q, a.n_kv, a.T, a.B, SRC != PACKED, max_keys, a.dv);
   if (need && (!workspace || workspace_bytes < need || !al16(workspace)))
-    return fail(PALU_EINVAL, "%s: a 16-byte aligned workspace of %zu bytes needed (palu_flash_prefill_workspace_bytes), got %zu", who,
-                need, workspace ? workspace_bytes : 0);
+    return fail(PALU_EINVAL, "%s: a 16-byte aligned workspace of %zu bytes needed (palu_flash_prefill_workspace_bytes), got %zu",
+                who, need, workspace ? workspace_bytes : 0);
   a.cut = need ? (int)cut_items(a.T, a.B, a.n_q, a.n_kv) : 0;
   a.part = need ? static_cast<float*>(workspace) : nullptr;
   a.records = reinterpret_cast<Record*>(a.part + (size_t)a.cut * a.n_kv * FP_ROWS * (a.dv + 2));

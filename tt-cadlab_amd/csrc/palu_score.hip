@@ -3,8 +3,9 @@
 // One pass: every lane keeps its own running maximum, sum and weighted sum, rescaled when the maximum rises, and
 // every wave the largest entries of what it has read, one per lane and sorted, which an entry joins only if it beats the
 // last of them. Among equal values the lower index comes first; NaN counts above every number (as in the greedy
-// pick), and makes the log probabilities and the entropy NaN. Bound by the logits' bytes; of few rows, which are cut
-// into parts for as many workgroups as the chip holds and joined by a second launch, by latency.
+// pick), and makes the log probabilities and the entropy NaN. Bound by the logits' bytes (4096 rows of 128256 bf16, top 1:
+// 171 us, 6.1 TB/s); of few rows, which are cut into parts for as many workgroups as the chip holds and joined by a second
+// launch, by latency (64 rows fp32, top 20: 13.7 + 5.3 us, 7.2 + 1.7 without a top; one row, top 5: 6.2 + 3.4).
 #include "palu_kernel.h"
 
 #include <algorithm>
@@ -116,9 +117,9 @@ __device__ __forceinline__ unsigned reached_by(const unsigned (&k)[R], int n, in
   return t;
 }
 
-// The largest `top` of `n` lists of `top` entries in LDS (0: none; no two others are equal), each with its place: use(place, entry).
-// What is left above reached_by is placed by the number of larger ones. At most 64 R entries; `left` and `count`: LDS for as
-// many and a counter. Returns how many are left.
+// The largest `top` of `n` lists of `top` entries in LDS (0: none; no two others are equal), each with its place:
+// use(place, entry). What is left above reached_by is placed by the number of larger ones. At most 64 R entries; `left` and
+// `count`: LDS for as many and a counter. Returns how many are left.
 template <int R, typename F>
 __device__ __forceinline__ int merge_lists(const u64* lists, int n, int top, u64* left, int* count, F use) {
   const int all = n * top, lane = threadIdx.x & 63;
@@ -328,7 +329,9 @@ __global__ __launch_bounds__(SCORE_WAVES * 64) void palu_score_join_kernel(const
   else finish_row<SCORE_PARTS>(a, row, st, token_logit, lists, a.parts, left, &count);
 }
 
-int score_parts(int rows, int n) { return std::max(1, std::min({SCORE_WGS / rows, (n + SCORE_PART - 1) / SCORE_PART, SCORE_PARTS})); }
+int score_parts(int rows, int n) {
+  return std::max(1, std::min({SCORE_WGS / rows, (n + SCORE_PART - 1) / SCORE_PART, SCORE_PARTS}));
+}
 
 template <typename T>
 int launch_score(const ScoreArgs& a, const char* who, hipStream_t s) {

@@ -268,6 +268,39 @@ def test_few_rows_over_long_contexts_are_split_and_joined(gpu, layout, new, ctx)
     _paged_check(new, ctx, 8, 2, 64, 64, layout, gpu, seed=ctx[0])
 
 
+@pytest.mark.parametrize("layout", ["rows", "tiled"])
+@pytest.mark.parametrize("rows", [1, 3, 6])
+def test_more_pieces_than_the_chip_holds_at_once(gpu, layout, rows):
+    """Some hundred tiles per KV head, some of them cut: all of the work order, and joins of 1, 8 and more rows."""
+    g = torch.Generator().manual_seed(rows)
+    ctx = torch.randint(1, 900, (100,), generator=g).tolist()
+    ctx[3], ctx[40], ctx[99] = 9000, 12_000, 7000
+    _paged_check([rows] * 100, ctx, 32, 8, 48, 32, layout, gpu, seed=rows)
+
+
+def test_non_finite_values_of_cut_contexts(gpu):
+    """A NaN or infinity in one piece reaches the rows of its sequence and KV head, through the join."""
+    new, ctx = [3, 1], [6000, 700]
+    g = torch.Generator().manual_seed(6)
+    q = torch.randn(4, 4, HD, generator=g).to(gpu, BF)
+    k, v = (torch.randn(6704, 2, w, generator=g).to(gpu, BF) for w in (HD, 64))
+    run = lambda k, v: _paged_run(q, k, v, new, ctx, 64, "rows")[0]
+    clean = run(k, v)
+    for bad in (math.nan, math.inf):
+        v2 = v.clone()
+        v2[4321, 1, 5] = bad
+        got = run(k, v2)
+        hit = torch.zeros_like(clean, dtype=torch.bool)
+        hit[:3, 2:, 5] = True
+        assert torch.equal(got[~hit], clean[~hit]) and (got[hit].isnan() | (got[hit] == bad)).all()
+    k2 = k.clone()
+    k2[70, 0, 9] = math.nan
+    got = run(k2, v)
+    hit = torch.zeros_like(clean, dtype=torch.bool)
+    hit[:3, :2] = True
+    assert torch.equal(got[~hit], clean[~hit]) and got[hit].isnan().all()
+
+
 def test_single_tokens_agree_with_the_flash_decode(gpu):
     """One new row per sequence is a decode step: the stock flash-decode over the same pages, both against 64 bits elsewhere;
     here to each other within the roundings of both (the bound above, twice, for values of spread 1)."""

@@ -34,7 +34,9 @@ constexpr int FP_KEYS = 64;               // keys of a K / V tile: two 32-positi
 constexpr int FP_MIN_KEYS = 256;          // keys of a piece of a split tile, about, at least
 constexpr int FP_SORTED = 256;            // sequences whose tiles are taken longest first
 constexpr int FP_WGS = 512;               // workgroups that the chip holds at once (two a CU)
-constexpr float FP_PIECE = 1.05f;         // keys of a piece over a workgroup slot's part of the batch's, about, at most
+// Keys of a piece over a workgroup slot's part of the batch's, about, at most. (8 sequences of up to 300 rows over up to 32000
+// positions: 136 us, with 0.8 175, with 0.55 151; one row over 32000: 32, 39 and 43.)
+constexpr float FP_PIECE = 1.05f;
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));

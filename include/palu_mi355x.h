@@ -424,7 +424,8 @@ size_t palu_prefill_workspace_bytes(int users, int seq, int n_heads, int n_kv, i
 
 /* Causal attention of packed sequences over full K and V, each over its own rows: row i of a sequence sees its rows 0 .. i.
  *   q [rows][n_q][128], k [rows][n_kv][128], v [rows][n_kv][head_dim_v] bf16, rows and heads at the element strides given
- *   (multiples of 8; head_dim_v a multiple of 16 up to 128); out [rows][n_q][head_dim_v] bf16, dense, not overlapping them.
+ *   (multiples of 8, rows of k and v less than 2^22 apart; head_dim_v a multiple of 16 up to 128); out
+ *   [rows][n_q][head_dim_v] bf16, dense, not overlapping them.
  * Head h reads KV head h / (n_q / n_kv). fp32 scores, statistics and sums; probabilities rounded to bf16 for their
  * product with V. A NaN or infinity in K or V reaches the rows that see it and no others. */
 int palu_flash_prefill(const void* q, long long q_row_stride, long long q_head_stride, const void* k, long long k_row_stride,

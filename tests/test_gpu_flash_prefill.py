@@ -278,6 +278,10 @@ def test_more_pieces_than_the_chip_holds_at_once(gpu, layout, rows):
     _paged_check([rows] * 100, ctx, 32, 8, 48, 32, layout, gpu, seed=rows)
 
 
+def test_cut_contexts_of_more_query_heads_than_rows_of_a_tile(gpu):
+    _paged_check([2, 1], [5000, 30], 256, 1, 16, 64, "rows", gpu, seed=3)
+
+
 def test_non_finite_values_of_cut_contexts(gpu):
     """A NaN or infinity in one piece reaches the rows of its sequence and KV head, through the join."""
     new, ctx = [3, 1], [6000, 700]

@@ -18,7 +18,7 @@
 // at the 1.65 GHz that the card's power limit leaves; S of the next tile runs beside the exponentials of this one, and two
 // workgroups share a CU. 32 query heads over 8 KV heads, widths 128: a prompt of 8192 takes 506 us (1.09 PFLOP/s), of 16384
 // 1.97 ms (1.12); 2048 rows behind 30000 positions in pages 0.90 ms (1.16); 64 rows, one behind each of 8000 positions,
-// 365 us (5.7 TB/s). Short sequences pay for each tile's search, first loads and masked keys, some 20 thousand cycles beside
+// 365 us (5.7 TB/s). Short sequences pay for each tile's search, first loads and masked keys, some 17 thousand cycles beside
 // 2100 to 2900 per 64 keys: 8 prompts of 2 to 2048 79 us (0.74 PFLOP/s), 128 of 128 127 us.
 //
 // Rounding: scores, statistics and sums are fp32 (products of bf16 are exact in them); the probabilities are rounded to

@@ -359,3 +359,32 @@ def test_page_refusals(gpu):
 def test_empty_pools_are_refused(gpu, shape):
     with pytest.raises(RuntimeError, match="not empty"):
         PagePools([torch.zeros(*shape, dtype=BF, device=gpu)])
+
+
+@pytest.mark.parametrize("role", ["rows", "k"])
+def test_caches_whose_storage_was_replaced(gpu, role):
+    """Between two calls a cache gets another storage: the copies go there, and the old one keeps what it holds."""
+    g = torch.Generator().manual_seed(4)
+    rand = lambda: torch.randn(6, 2, 32, 32, generator=g).to(gpu, BF)
+    cache = rand() if role == "rows" else LatentCache.from_rows(rand(), role)
+    other = rand()
+    h = PagePools([cache, other])
+    t, ln = _ints([[4], [-1]], gpu), _ints([5, 0], gpu)
+    fork = lambda: h.update(t, ln, parents=_ints([0, 0], gpu), new_lengths=_ints([6, 6], gpu))
+    fork()
+    store = cache if role == "rows" else cache.data
+    old = store.detach()
+    was = old.clone()
+    new = rand() if role == "rows" else LatentCache.from_rows(rand(), role).data
+    if role == "rows":
+        cache.data = new
+    else:
+        cache.data = new.clone()
+    store = cache if role == "rows" else cache.data
+    table, lengths = fork()
+    assert table.tolist() == [[4], [0]] and lengths.tolist() == [6, 6]
+    assert torch.equal(store[0], store[4]) and torch.equal(store[1:], new[1:]) and torch.equal(old, was)
+    assert torch.equal(other[0], other[4])
+    store[3] = 7
+    table, n = h.compact(_ints([[3]], gpu), _ints([2], gpu))
+    assert table.tolist() == [[0]] and (store[0] == 7).all() and torch.equal(old, was)

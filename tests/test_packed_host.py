@@ -130,3 +130,58 @@ def test_cpu_tensors_are_refused():
         PagePools([t(3, 2, 32, 64)])
     with pytest.raises(RuntimeError, match="GPU"):
         decoder_ops.token_logprobs(t(4, 10), ints([0, 1, 2, 3]))
+
+
+# ---- calls of the Python layer with the launch taken down: tensors that say they are on the GPU ---------------------
+
+class _OnGpu(torch.Tensor):
+    is_cuda = property(lambda self: True)
+
+
+def _gpu_like(*shape, dtype=torch.bfloat16):
+    return torch.zeros(*shape, dtype=dtype).as_subclass(_OnGpu)
+
+
+@pytest.fixture
+def launches(lib, monkeypatch):
+    """The launches' arguments in place of the launches."""
+    calls = []
+    monkeypatch.setattr(_native, "launch", lambda name, device, *args: calls.append((name, args)))
+    return calls
+
+
+def _ints(x):
+    return torch.tensor(x, dtype=torch.int32)
+
+
+def _pool_addresses(args, at):
+    """The pools' addresses and page bytes that a page-table call was given."""
+    ptrs, sizes, n = args[at:at + 3]
+    return list(zip(list(ptrs), list(sizes)))[:n]
+
+
+def test_page_pools_follow_their_caches(launches):
+    """A cache whose storage was replaced, and a tensor that was, are read where they are now."""
+    from palu_tt.cache import LatentCache
+    cache, rows = LatentCache(_gpu_like(5, 2, 1, 2, 64, 8), "k"), _gpu_like(5, 2, 32, 32)
+    h = PagePools([cache, rows])
+    call = lambda: h.update(_ints([[0, 1]]), _ints([3]))
+    call()
+    cache.data = _gpu_like(5, 2, 1, 4, 64, 8)                          # wider, elsewhere
+    rows.set_(_gpu_like(5, 3, 32, 32))
+    call()
+    h.compact(_ints([[0, 1]]), _ints([3]))
+    now = [(cache.data.data_ptr(), 2 * 32 * 64 * 2), (rows.data_ptr(), 3 * 32 * 32 * 2)]
+    assert _pool_addresses(launches[0][1], 6) != now
+    assert _pool_addresses(launches[1][1], 6) == now and _pool_addresses(launches[2][1], 4) == now
+    cache.data, rows.data = _gpu_like(7, 2, 1, 2, 64, 8), _gpu_like(7, 2, 32, 32)   # larger pools: their page count counts
+    call()
+    assert launches[3][1][10] == h.n_pages == 7
+    for bad in (_gpu_like(6, 2, 1, 2, 64, 8), _gpu_like(7, 2, 2, 2, 64, 8), _gpu_like(7, 2, 1, 2, 64, 16)[..., ::2], rows,
+                _gpu_like(7, 2, 1, 2, 64, 8, dtype=torch.float16)):
+        cache.data = bad
+        with pytest.raises(RuntimeError):
+            call()
+        with pytest.raises(RuntimeError):
+            h.compact(_ints([[0, 1]]), _ints([3]))
+    assert len(launches) == 4

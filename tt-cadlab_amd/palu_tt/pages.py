@@ -10,6 +10,7 @@ reference counts and no free list, so a row is freed by giving it the length 0. 
 (a common prefix, the siblings of a beam); ``update`` gives every row its own copy of the page that it writes next.
 """
 import ctypes
+from operator import is_
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -32,6 +33,10 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     return a0 < b1 and b0 < a1
 
 
+def _places(stores):
+    return list(map(torch.Tensor.data_ptr, stores)), list(map(torch.Tensor.numel, stores))
+
+
 class PagePools:
     """The page pools that share a page table: row-major [n_pages, n_groups, page_size, width] bf16 tensors or LatentCache
     pools (of any group counts and widths)."""
@@ -39,8 +44,16 @@ class PagePools:
     def __init__(self, pools: Sequence):
         if not pools:
             raise RuntimeError("PagePools needs at least one pool")
-        self.pools = list(pools)                                  # kept alive: the kernels see their addresses
+        self.pools = list(pools)
+        self._stores, self._places = [], None
+        self._look()
+
+    def _look(self) -> None:
+        """Takes the pools' storage as it is now: a LatentCache's ``data`` may be another tensor than at the last call, and a
+        tensor may have been given other memory or another size. Pools where nothing changed are not checked again."""
         stores = [p.data if isinstance(p, LatentCache) else p for p in self.pools]
+        if len(stores) == len(self._stores) and all(map(is_, stores, self._stores)) and _places(stores) == self._places:
+            return
         for p, s in zip(self.pools, stores):
             if not (isinstance(s, torch.Tensor) and len(p.shape) == 4 and s.is_cuda and s.dtype == torch.bfloat16 and
                     s.is_contiguous() and s.data_ptr() % 16 == 0 and s.numel()):
@@ -49,15 +62,17 @@ class PagePools:
             if (p.shape[0], p.shape[2], s.device) != (self.pools[0].shape[0], self.pools[0].shape[2], stores[0].device):
                 raise RuntimeError("pools must agree in pages, page size and device: "
                                    f"{tuple(p.shape)}, {tuple(self.pools[0].shape)}")
-        self.n_pages, self.page_size = int(self.pools[0].shape[0]), int(self.pools[0].shape[2])
-        self.device = stores[0].device
         if any(_overlap(a, b) for i, a in enumerate(stores) for b in stores[:i]):
             raise RuntimeError("pools must not overlap")
+        self.n_pages, self.page_size = int(self.pools[0].shape[0]), int(self.pools[0].shape[2])
+        self.device = stores[0].device
         n = len(stores)
         self._ptrs = (ctypes.c_void_p * n)(*[s.data_ptr() for s in stores])
         self._bytes = (ctypes.c_longlong * n)(*[s.numel() * 2 // self.n_pages for s in stores])
+        self._stores, self._places = stores, _places(stores)
 
     def _args(self, page_table, lengths):
+        self._look()
         if not (isinstance(page_table, torch.Tensor) and page_table.dim() == 2):
             raise RuntimeError("page_table must be [B, max_pages] int32")
         B, slots = page_table.shape

@@ -185,3 +185,33 @@ def test_page_pools_follow_their_caches(launches):
         with pytest.raises(RuntimeError):
             h.compact(_ints([[0, 1]]), _ints([3]))
     assert len(launches) == 4
+
+
+def test_workspaces_in_one_piece(lib, launches):
+    """A workspace of as many elements as asked for that do not lie next to each other, or lie elsewhere, is refused: by every
+    call that takes one, before anything is launched."""
+    t = lambda *s: _gpu_like(*s)
+    pool = t(4, 2, 32, 128)
+    table, ints = _ints([[0] * 16]), _ints([0, 1])
+    need = lib.palu_flash_prefill_workspace_bytes(1, 1, 4, 2, 512, 128)
+    assert need > 0
+    h = PagePools([t(4, 1, 32, 8)])
+    cur = _ints([5])
+    run = {
+        "flash_prefill": lambda ws: fused.flash_prefill(t(1, 4, 128), pool, pool, ints, page_table_tensor=table, workspace=ws),
+        "update": lambda ws: h.update(_ints([[0]]), cur, workspace=ws),
+        "compact": lambda ws: h.compact(_ints([[0]]), cur, workspace=ws),
+        "flash_decode": lambda ws: fused.flash_decode(t(1, 1, 4, 128), t(1, 2, 16384, 128), t(1, 2, 16384, 128), cur, workspace=ws),
+        "linear_argmax": lambda ws: decoder_ops.linear_argmax(t(8, 64), t(32, 64), 1, workspace=ws),
+        "linear_tiled": lambda ws: decoder_ops.linear_tiled(t(4, 512), t(32, 512), 2, 4, out=t(4, 32), workspace=ws)}
+    size = 1 << 24
+    bad = {"expanded": torch.zeros(1, dtype=torch.uint8).expand(size), "strided": torch.zeros(2 * size, dtype=torch.uint8)[::2],
+           "elsewhere": torch.zeros(size, dtype=torch.uint8, device="meta")}
+    for call in run.values():
+        for ws in bad.values():
+            with pytest.raises(RuntimeError, match="workspace must be a contiguous tensor"):
+                call(ws)
+    assert not launches
+    for name in ("flash_prefill", "update", "compact"):
+        run[name](torch.zeros(size, dtype=torch.uint8))
+    assert [name for name, _ in launches] == ["flash_prefill_paged", "pages_update", "pages_compact"]

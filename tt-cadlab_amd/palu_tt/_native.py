@@ -114,6 +114,16 @@ def ptr(t) -> int:
     return 0 if t is None else t.data_ptr()
 
 
+def workspace_bytes(workspace, need: int, device, what: str = "workspace") -> int:
+    """The size of a caller's workspace, refused unless its `need` bytes lie in one piece on the device: the kernels write
+    them from its start on."""
+    if isinstance(workspace, torch.Tensor) and workspace.device == device and workspace.is_contiguous():
+        size = workspace.numel() * workspace.element_size()
+        if size >= need:
+            return size
+    raise RuntimeError(f"{what} must be a contiguous tensor of {need} bytes on {device}")
+
+
 def launch(name: str, device, *args) -> None:
     """check(palu_<name>(*args, the current stream of `device`)) with that device current."""
     fn = getattr(load(), "palu_" + name)

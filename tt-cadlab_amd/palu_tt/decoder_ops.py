@@ -374,6 +374,8 @@ def linear_tiled(x: torch.Tensor, w_tiled: torch.Tensor, rtw: int, ks: int, out:
     need = lib.palu_linear_workspace_bytes(rows, n, k, ks) if mode == "bf16" else 0
     if need and (workspace is None or workspace.numel() < need):
         workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
+    elif need:
+        _native.workspace_bytes(workspace, need, x.device)
     _native.check(lib.palu_linear_tiled(
         _native.ptr(x), x.stride(0), int(x_tiled), rows, _native.ptr(w_tiled), n, k, _native.ptr(out),
         out.stride(0) if mode == "bf16" else n, _LINEAR_MODES[mode], rtw, ks,
@@ -558,13 +560,14 @@ def linear_argmax(x: torch.Tensor, w_tiled: torch.Tensor, rtw: int, workspace: O
     need = lib.palu_linear_argmax_workspace_bytes(rows, n)
     if workspace is None:
         workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=x.device)
+    size = _native.workspace_bytes(workspace, need, x.device)
     if out is None:
         out = torch.empty(rows, dtype=torch.int64, device=x.device)
     if out.dtype != torch.int64 or out.shape != (rows,) or not out.is_contiguous() or out.device != x.device:
         raise RuntimeError(f"out must be a contiguous int64 [{rows}] tensor on {x.device}")
     _native.check(lib.palu_linear_argmax(_native.ptr(x), 64 if x_tiled else x.stride(0), int(x_tiled), rows,
                                          _native.ptr(w_tiled), n, k, rtw, _native.ptr(out), _native.ptr(workspace),
-                                         workspace.numel(), _native.stream_handle(x.device)))
+                                         size, _native.stream_handle(x.device)))
     return out
 
 

@@ -191,9 +191,7 @@ def _workspace(batch: int, n_kv: int, seq_len: int, width: int, device, workspac
     if need == 0:
         return None, 0
     if workspace is not None:
-        if not (workspace.is_cuda and workspace.numel() * workspace.element_size() >= need):
-            raise RuntimeError(f"workspace must hold {need} bytes on the GPU")
-        return workspace, workspace.numel() * workspace.element_size()
+        return workspace, _native.workspace_bytes(workspace, need, device)
     return torch.empty(need, dtype=torch.uint8, device=device), need
 
 
@@ -201,9 +199,7 @@ def _glrd_workspace(batch: int, n_q: int, n_kv: int, n_groups: int, seq_len: int
     """Workspace of the grouped-latent path: partial scores and latent PV partials between its passes."""
     need = _native.load().palu_glrd_workspace_bytes(batch, n_q, n_kv, n_groups, seq_len, r_v)
     if workspace is not None:
-        if not (workspace.is_cuda and workspace.numel() * workspace.element_size() >= need):
-            raise RuntimeError(f"workspace must hold {need} bytes on the GPU (palu_glrd_workspace_bytes)")
-        return workspace, workspace.numel() * workspace.element_size()
+        return workspace, _native.workspace_bytes(workspace, need, device, "workspace (palu_glrd_workspace_bytes)")
     return torch.empty(max(need, 1), dtype=torch.uint8, device=device), need
 
 
@@ -550,8 +546,8 @@ def flash_prefill(q, k, v, cu_seqlens, *, scale=None, head_dim_v=None, out=None,
     need = _native.load().palu_flash_prefill_workspace_bytes(T, B, n_q, n_kv, pt.shape[1] * page_size, dv)
     if workspace is None:
         workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    elif not (workspace.device == dev and workspace.numel() * workspace.element_size() >= need):
-        raise RuntimeError(f"workspace must hold {need} bytes on {dev}")
+    else:
+        _native.workspace_bytes(workspace, need, dev)
     _native.launch("flash_prefill_paged", dev, q.data_ptr(), q_st, q_sh, k_store.data_ptr(), v_store.data_ptr(),
                    cu.data_ptr(), _native.ptr(start), pt.data_ptr(), out.data_ptr(), sc, T, B, n_q, n_kv, n_pages,
                    page_size, pt.shape[1], dv, layout, _native.ptr(workspace), need)

@@ -82,8 +82,7 @@ class PagePools:
         need = _native.load().palu_pages_workspace_bytes(B, self.n_pages)
         if workspace is None:
             return torch.empty(need, dtype=torch.uint8, device=self.device), need
-        if not (workspace.device == self.device and workspace.numel() * workspace.element_size() >= need):
-            raise RuntimeError(f"workspace must hold {need} bytes on {self.device}")
+        _native.workspace_bytes(workspace, need, self.device)
         return workspace, need
 
     def update(self, page_table, lengths, *, parents=None, new_lengths=None, out=None,

@@ -204,7 +204,7 @@ def test_workspaces_in_one_piece(lib, launches):
         "flash_decode": lambda ws: fused.flash_decode(t(1, 1, 4, 128), t(1, 2, 16384, 128), t(1, 2, 16384, 128), cur, workspace=ws),
         "linear_argmax": lambda ws: decoder_ops.linear_argmax(t(8, 64), t(32, 64), 1, workspace=ws),
         "linear_tiled": lambda ws: decoder_ops.linear_tiled(t(4, 512), t(32, 512), 2, 4, out=t(4, 32), workspace=ws)}
-    size = 1 << 24
+    size = 1 << 27
     bad = {"expanded": torch.zeros(1, dtype=torch.uint8).expand(size), "strided": torch.zeros(2 * size, dtype=torch.uint8)[::2],
            "elsewhere": torch.zeros(size, dtype=torch.uint8, device="meta")}
     for call in run.values():

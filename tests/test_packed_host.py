@@ -215,3 +215,38 @@ def test_workspaces_in_one_piece(lib, launches):
     for name in ("flash_prefill", "update", "compact"):
         run[name](torch.zeros(size, dtype=torch.uint8))
     assert [name for name, _ in launches] == ["flash_prefill_paged", "pages_update", "pages_compact"]
+
+
+def test_out_of_the_packed_attention_is_memory_of_its_own(launches):
+    """An `out` over an input is refused; one that lies in the same allocation, behind or between the rows read, is not."""
+    ints = _ints([0, 6])
+    buf = _gpu_like(6 * 3 * 4 * 128)
+    q = buf[:6 * 4 * 128].view(6, 4, 128)
+    k, v = _gpu_like(6, 2, 128), _gpu_like(6, 2, 64)
+    pool, vpool, table = _gpu_like(4, 2, 32, 128), _gpu_like(4, 2, 32, 64), _ints([[0, 1]])
+    own, shared = _gpu_like(6, 4, 64), lambda t: t.view(-1)[:6 * 4 * 64].view(6, 4, 64)
+    packed = lambda out, **kw: fused.flash_prefill(kw.get("q", q), kw.get("k", k), kw.get("v", v), ints, out=out)
+    paged = lambda out, **kw: fused.flash_prefill(q, pool, vpool, ints, page_table_tensor=kw.get("table", table), out=out,
+                                                  start_pos=kw.get("start"), workspace=kw.get("workspace"))
+    wide = _gpu_like(6, 6, 128)                                             # k and v as columns of wider rows
+    calls = [lambda: packed(shared(q)), lambda: packed(buf[6 * 4 * 128 - 8:][:6 * 4 * 64].view(6, 4, 64)),
+             lambda: packed(shared(wide), k=wide[:, 2:4]), lambda: packed(shared(wide), v=wide[:, 4:, :64]),
+             lambda: packed(shared(wide), k=wide.view(6, 768)[:, 512:].unflatten(1, (2, 128))),
+             lambda: paged(shared(pool)), lambda: paged(shared(vpool)),
+             lambda: paged(own, workspace=own.view(-1).view(torch.uint8)),
+             lambda: paged(own, table=own.view(-1).view(torch.int32)[8:10].view(1, 2)),
+             lambda: paged(own, start=own.view(-1).view(torch.int32)[:1])]
+    for call in calls:
+        with pytest.raises(RuntimeError, match="memory of its own"):
+            call()
+    assert not launches
+    packed(own)
+    paged(own)
+    packed(buf[6 * 4 * 128:][:6 * 4 * 64].view(6, 4, 64))                 # right behind q
+    apart = _gpu_like(6, 6 * 4 * 64 + 512)                                # rows so far apart that `out` fits between two
+    packed(apart[2, 512:].view(6, 4, 64), q=apart[:, :512].unflatten(1, (4, 128)))
+    one = _gpu_like(7, 4, 128)
+    packed(one[3:].view(-1)[512:512 + 1536].view(6, 4, 64), q=torch.as_strided(one, (6, 4, 128), (0, 128, 1)).as_subclass(_OnGpu))
+    assert len(launches) == 5
+    with pytest.raises(RuntimeError, match="memory of its own"):
+        packed(apart[2, 504:504 + 1536].view(6, 4, 64), q=apart[:, :512].unflatten(1, (4, 128)))

@@ -488,6 +488,23 @@ def _strided_rows(t, name: str, width: Optional[int], device=None):
     return st, sh
 
 
+def _overlap(out: torch.Tensor, t: torch.Tensor) -> bool:
+    """Whether the contiguous `out` shares memory with t: contiguous, or a [rows, heads, width] view of contiguous heads (`out`
+    may lie between its rows)."""
+    size = t.element_size()
+    lo, hi = (out.data_ptr() - t.data_ptr()) // size, -((t.data_ptr() - out.data_ptr() - out.numel() * out.element_size()) // size)
+    if not (t.numel() and out.numel()) or hi <= 0 or lo > sum((n - 1) * st for n, st in zip(t.shape, t.stride())):
+        return False
+    if t.is_contiguous():
+        return True
+    (rows, heads, w), (st, sh, _) = t.shape, t.stride()
+    for at in range(0, heads * sh if sh else 1, sh or 1):                # a head's rows at..: is one of them below hi and above lo?
+        first = max(0, -((at + w - 1 - lo) // st)) if st else 0
+        if first < rows and first * st + at < hi and first * st + at + w > lo:
+            return True
+    return False
+
+
 def flash_prefill(q, k, v, cu_seqlens, *, scale=None, head_dim_v=None, out=None, workspace=None, page_table_tensor=None,
                   start_pos=None) -> torch.Tensor:
     """Causal attention of packed sequences of different lengths over full rotated K and V, the prompts' counterpart of
@@ -536,6 +553,9 @@ def flash_prefill(q, k, v, cu_seqlens, *, scale=None, head_dim_v=None, out=None,
         _as_dev(out, "out", torch.bfloat16, dev)
         if tuple(out.shape) != (T, n_q, dv):
             raise RuntimeError(f"out must be [{T}, {n_q}, {dv}]")
+        reads = (q, k, v, cu) if page_table_tensor is None else (q, k_store, v_store, cu, pt, start, workspace)
+        if any(t is not None and _overlap(out, t) for t in reads):
+            raise RuntimeError("out must be memory of its own: it overlaps an input or the workspace")
     if T == 0:
         return out
     sc = float(HEAD_DIM ** -0.5 if scale is None else scale)

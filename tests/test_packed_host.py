@@ -250,3 +250,54 @@ def test_out_of_the_packed_attention_is_memory_of_its_own(launches):
     assert len(launches) == 5
     with pytest.raises(RuntimeError, match="memory of its own"):
         packed(apart[2, 504:504 + 1536].view(6, 4, 64), q=apart[:, :512].unflatten(1, (4, 128)))
+
+
+def _packed_inputs():
+    from palu_tt.cache import LatentCache
+    t = _gpu_like
+    return dict(q=t(6, 4, 128), k=t(6, 2, 128), v=t(6, 2, 64), kp=t(4, 2, 32, 128), vp=t(4, 2, 32, 64),
+                kc=LatentCache(t(4, 2, 1, 8, 64, 8), "k"), vc=LatentCache(t(4, 2, 1, 4, 64, 8), "v"), logits=t(3, 50))
+
+
+def _forward_only_calls(a):
+    """The forward-only calls, each with the names of the inputs that a derivative could come by."""
+    cu, table = _ints([0, 6]), _ints([[0, 1]])
+    return [(("q", "k", "v"), lambda: fused.flash_prefill(a["q"], a["k"], a["v"], cu)),
+            (("q", "kp", "vp"), lambda: fused.flash_prefill(a["q"], a["kp"], a["vp"], cu, page_table_tensor=table)),
+            (("q", "kc", "vc"), lambda: fused.flash_prefill(a["q"], a["kc"], a["vc"], cu, page_table_tensor=table)),
+            (("logits",), lambda: decoder_ops.token_logprobs(a["logits"], _ints([1, 2, 3])))]
+
+
+def _with(t, change):
+    from palu_tt.cache import LatentCache
+    return LatentCache(change(t.data), t.role) if isinstance(t, LatentCache) else change(t)
+
+
+@pytest.mark.parametrize("grad", [True, False], ids=["grad", "no_grad"])
+def test_tangents_are_refused(launches, grad):
+    """A forward-mode tangent would be dropped without a word, with gradients enabled or not."""
+    import torch.autograd.forward_ad as fw
+    with torch.set_grad_enabled(grad):
+        for i, (names, _) in enumerate(_forward_only_calls(_packed_inputs())):
+            for name in names:
+                a = _packed_inputs()
+                with fw.dual_level():
+                    a[name] = _with(a[name], lambda t: fw.make_dual(t, torch.ones_like(t)))
+                    with pytest.raises(RuntimeError, match="tangent"):
+                        _forward_only_calls(a)[i][1]()
+            with fw.dual_level():
+                _forward_only_calls(_packed_inputs())[i][1]()               # without tangents all is well
+    assert len(launches) == 4
+
+
+def test_gradients_are_refused(launches):
+    """So would a backward pass, through a cache object's storage, too."""
+    for i, (names, _) in enumerate(_forward_only_calls(_packed_inputs())):
+        for name in names:
+            a = _packed_inputs()
+            a[name] = _with(a[name], lambda t: t.requires_grad_())
+            with pytest.raises(RuntimeError, match="backward"):
+                _forward_only_calls(a)[i][1]()
+            with torch.no_grad():
+                _forward_only_calls(a)[i][1]()
+    assert len(launches) == 10

@@ -124,6 +124,16 @@ def workspace_bytes(workspace, need: int, device, what: str = "workspace") -> in
     raise RuntimeError(f"{what} must be a contiguous tensor of {need} bytes on {device}")
 
 
+def refuse_derivatives(what: str, *tensors) -> None:
+    """Raises where a derivative would go through these tensors: the kernels see their values only, and it would come out as
+    none without a word."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad()")
+    if torch.autograd.forward_ad._current_level >= 0 and any(
+            torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{what} has no forward-mode derivative: an input has a tangent")
+
+
 def launch(name: str, device, *args) -> None:
     """check(palu_<name>(*args, the current stream of `device`)) with that device current."""
     fn = getattr(load(), "palu_" + name)

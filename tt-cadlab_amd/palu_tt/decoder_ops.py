@@ -93,8 +93,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0):
         raise RuntimeError(f"tokens must be an integer tensor [{rows}]")
     if n < 1 or not 0 <= top <= min(64, n):
         raise RuntimeError(f"top must be in 0 .. {min(64, n)}, got {top}")
-    if torch.is_grad_enabled() and logits.requires_grad:
-        raise RuntimeError("token_logprobs has no backward pass: call it under torch.no_grad()")
+    _native.refuse_derivatives("token_logprobs", logits)
     t = tokens if tokens.device == dev and tokens.dtype == torch.int64 else tokens.to(device=dev, dtype=torch.int64)
     t = t.contiguous()
     lp, ent = torch.empty(2, rows, dtype=torch.float32, device=dev).unbind(0)

@@ -524,19 +524,19 @@ def flash_prefill(q, k, v, cu_seqlens, *, scale=None, head_dim_v=None, out=None,
     B = cu.numel() - 1
     if B < 1:
         raise RuntimeError("cu_seqlens must hold at least one sequence")
-    if (q.requires_grad or getattr(k, "requires_grad", False) or getattr(v, "requires_grad", False)) and torch.is_grad_enabled():
-        raise RuntimeError("flash_prefill has no backward pass: call it under torch.no_grad()")
     if page_table_tensor is None:
         if start_pos is not None:
             raise RuntimeError("start_pos needs page_table_tensor: packed rows attend to themselves from position 0")
         k_st, k_sh = _strided_rows(k, "k", HEAD_DIM, dev)
         v_st, v_sh = _strided_rows(v, "v", None, dev)
+        _native.refuse_derivatives("flash_prefill", q, k, v)
         n_kv, dv = v.shape[1:]
         if k.shape[:2] != (T, n_kv) or v.shape[0] != T:
             raise RuntimeError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must have the {T} rows of q and the same heads")
     else:
         k_store, k_shape, layout = _cache_arg(k, "k", dev, "k")
         v_store, v_shape, v_layout = _cache_arg(v, "v", dev, "v")
+        _native.refuse_derivatives("flash_prefill", q, k_store, v_store)
         if layout != v_layout or layout == _native.LAYOUT_TILED_GROUPED:
             raise RuntimeError("k and v must use the same cache layout (row-major or LatentCache pools)")
         n_pages, n_kv, page_size, hd = k_shape

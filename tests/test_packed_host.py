@@ -301,3 +301,27 @@ def test_gradients_are_refused(launches):
             with torch.no_grad():
                 _forward_only_calls(a)[i][1]()
     assert len(launches) == 10
+
+
+@pytest.mark.parametrize("which", ["rows", "cache", "tiled cache"])
+def test_fill_refuses_derivatives(launches, which):
+    """Rows or a cache with a gradient or a tangent: the attention over the pages would see neither."""
+    import torch.autograd.forward_ad as fw
+    from palu_tt.cache import LatentCache
+    cu, table = _ints([0, 6]), _ints([[0, 1]])
+
+    def call(change):
+        rows, pool = _gpu_like(6, 2, 64), _gpu_like(4, 2, 1, 4, 64, 8) if which == "tiled cache" else _gpu_like(4, 2, 32, 64)
+        rows, pool = (change(rows), pool) if which == "rows" else (rows, change(pool))
+        fused.paged_fill_cache(LatentCache(pool, "v") if which == "tiled cache" else pool, rows, cu, table)
+
+    with pytest.raises(RuntimeError, match="backward"):
+        call(lambda t: t.requires_grad_())
+    with fw.dual_level():
+        with pytest.raises(RuntimeError, match="tangent"):
+            call(lambda t: fw.make_dual(t, torch.ones_like(t)))
+    assert not launches
+    call(lambda t: t)
+    with torch.no_grad():
+        call(lambda t: t.requires_grad_())
+    assert len(launches) == 2

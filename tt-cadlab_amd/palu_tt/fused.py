@@ -579,12 +579,14 @@ def paged_fill_cache(cache, rows: torch.Tensor, cu_seqlens, page_table, start_po
     [T, n_groups, width] bf16 (a strided view such as columns of a projection), goes to position start_pos[b] + i (int32 [B];
     None: i) of its pages, page_table[b, position // page_size]. ``cache`` is a [n_pages, n_groups, page_size, width] tensor or a
     LatentCache pool. Positions outside the table and page ids outside the pool are skipped; the rest of the pool
-    keeps what it holds. Sequences of one call must not share the pages that they write."""
+    keeps what it holds. Sequences of one call must not share the pages that they write. Forward only: rows or a cache that a
+    derivative would go through are refused."""
     if isinstance(cache, GroupedLatentCache):
         raise RuntimeError("a GroupedLatentCache is contiguous")
     st, sg = _strided_rows(rows, "rows", None)
     dev = rows.device
     store, (n_pages, G, page_size, width), layout = _cache_arg(cache, "cache", dev)
+    _native.refuse_derivatives("paged_fill_cache", rows, store)
     if tuple(rows.shape[1:]) != (G, width):
         raise RuntimeError(f"rows must be [T, {G}, {width}] for this cache, got {tuple(rows.shape)}")
     cu = _seq_ints(cu_seqlens, "cu_seqlens", None, dev)

@@ -325,3 +325,12 @@ def test_fill_refuses_derivatives(launches, which):
     with torch.no_grad():
         call(lambda t: t.requires_grad_())
     assert len(launches) == 2
+
+
+def test_token_logprobs_workspace(lib):
+    """Whole 16 bytes for every part of a row, whatever the number of entries: each starts with 16-byte aligned statistics."""
+    f = lib.palu_token_logprobs_workspace_bytes
+    parts = f(1, 128256, 0) // 16
+    assert parts > 1 and f(3000, 128256, 5) == 0
+    for top in range(1, 65):
+        assert f(1, 128256, top) == parts * (16 + 8 * (top + top % 2)) and f(7, 128256, top) % 16 == 0

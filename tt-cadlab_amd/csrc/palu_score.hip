@@ -30,8 +30,10 @@ struct ScoreArgs {
   float* top_lp;                          // [rows][top]
   int64_t* top_id;
   int parts;                              // of a row
-  char* ws;                               // parts > 1: per (row, part) its Stats (16 bytes) and `top` entries
+  char* ws;                               // parts > 1: a record per (row, part), its Stats (16 bytes) and `top` entries
 };
+// Bytes of a record: whole 16s, so that every Stats lies as its type says.
+__host__ __device__ constexpr int record_bytes(int top) { return 16 + 8 * (top + (top & 1)); }
 
 // Entries compare as (value, lower index first): one 64-bit key, value made order-preserving above, complemented index below.
 // -0 counts as 0 and every NaN as one value.
@@ -286,7 +288,7 @@ __global__ __launch_bounds__(SCORE_WAVES * 64) void palu_score_kernel(const Scor
     finish_row<SCORE_WAVES>(a, row, st, token_logit, lists, SCORE_WAVES, left, &count);
     return;
   }
-  char* ws = a.ws + (long long)blockIdx.x * (16 + 8 * a.top);
+  char* ws = a.ws + (long long)blockIdx.x * record_bytes(a.top);
   if (tid == 0) *reinterpret_cast<Stats*>(ws) = st;
   if (a.top) {
     u64* out = reinterpret_cast<u64*>(ws + 16);
@@ -301,7 +303,8 @@ __global__ __launch_bounds__(SCORE_WAVES * 64) void palu_score_join_kernel(const
   extern __shared__ u64 lists[];          // [parts][top], and as much for what is left of them
   __shared__ int count;
   const long long row = blockIdx.x;
-  const char* ws = a.ws + row * a.parts * (16 + 8 * a.top);
+  const int record = record_bytes(a.top);
+  const char* ws = a.ws + row * a.parts * record;
   float token_logit = 0.f;
   if (threadIdx.x == 0) {
     const long long t = a.tokens[row];
@@ -309,13 +312,13 @@ __global__ __launch_bounds__(SCORE_WAVES * 64) void palu_score_join_kernel(const
   }
   const int lane = threadIdx.x & 63;
   Stats st{NEG_INF, 0.f, 0.f};
-  if (lane < a.parts) st = *reinterpret_cast<const Stats*>(ws + lane * (16 + 8 * a.top));
+  if (lane < a.parts) st = *reinterpret_cast<const Stats*>(ws + lane * record);
   u64 x[SCORE_PARTS / SCORE_WAVES];       // all loads at once: each comes from another XCD's writes, by way of memory
 #pragma unroll
   for (int i = 0; i < SCORE_PARTS / SCORE_WAVES; ++i) {
     const int p = i * SCORE_WAVES + (threadIdx.x >> 6);
     x[i] = 0;
-    if (p < a.parts && lane < a.top) x[i] = reinterpret_cast<const u64*>(ws + p * (16 + 8 * a.top) + 16)[lane];
+    if (p < a.parts && lane < a.top) x[i] = reinterpret_cast<const u64*>(ws + p * record + 16)[lane];
   }
 #pragma unroll
   for (int i = 0; i < SCORE_PARTS / SCORE_WAVES; ++i) {
@@ -349,7 +352,7 @@ bool score_dims_ok(int rows, int n, int top) { return rows > 0 && n > 0 && top >
 extern "C" size_t palu_token_logprobs_workspace_bytes(int rows, int n, int top) {
   if (!score_dims_ok(rows, n, top)) return 0;
   const int parts = score_parts(rows, n);
-  return parts == 1 ? 0 : (size_t)rows * parts * (16 + 8 * top);
+  return parts == 1 ? 0 : (size_t)rows * parts * record_bytes(top);
 }
 
 extern "C" int palu_token_logprobs(const void* logits, long long ld, int dtype, const int64_t* tokens, int rows, int n, int top,

@@ -434,3 +434,48 @@ def test_empty_batches_and_refusals(gpu):
         fused.flash_prefill(q, pool, pool, cu, page_table_tensor=_ints([[0], [1]], gpu))
     with pytest.raises(RuntimeError, match="tile order"):
         fused.flash_prefill(q, LatentCache.from_rows(pool, "v"), LatentCache.from_rows(pool, "v"), cu, page_table_tensor=_ints([[0]], gpu))
+
+
+# A mean of equal values is that value: the sum of the weights that divides has to be that of the rounded weights that multiplied. A
+# dominating key's probability is rounded by up to 2^-8 where it is not the running maximum's own (which lags behind by up to 2^8);
+# divided by the sum of unrounded ones that is up to 2^-8 of the result, half a bf16 step near the lower end of a binade and a
+# whole one near the upper. The fp32 sums of n keys are off by (n + 64) 2^-23 together, 2^-12 for n = 2000: less than half the
+# 2^-9 between a bf16 value and the nearest rounding border (just below a power of two), so the result is the value itself.
+_CONSTANTS = [1.9921875, 1.0, 1.9921875 * 2.0 ** 20, -1.5, -1.9921875, 2.0 ** -30]
+
+
+def _constant_values(rows, nkv, w, dev):
+    c = torch.tensor(_CONSTANTS, dtype=BF, device=dev).repeat(-(-w // len(_CONSTANTS)))[:w]
+    v = torch.stack([c.roll(j) for j in range(nkv)])
+    return v.expand(rows, nkv, w).contiguous(), v
+
+
+@pytest.mark.parametrize("std", [0.5, 3.0, 20.0])
+def test_equal_values_come_back_exactly(gpu, std):
+    lens = [1, 70, 300, 1000, 129]
+    q, k, _ = _packed(lens, 8, 2, 64, gpu, seed=int(std * 2), std=std)
+    vals, c = _constant_values(sum(lens), 2, 64, gpu)
+    got = fused.flash_prefill(q, k, vals, _cu(lens, gpu))
+    assert torch.equal(got, c.repeat_interleave(4, 0).expand_as(got))
+
+
+@pytest.mark.parametrize("layout", ["rows", "tiled"])
+@pytest.mark.parametrize("new,ctx", [([40, 7], [100, 500]), ([1, 3], [2000, 9])], ids=str)
+def test_equal_values_in_pages_come_back_exactly(gpu, layout, new, ctx):
+    g = torch.Generator().manual_seed(12)
+    q = (torch.randn(sum(new), 8, HD, generator=g) * 4).to(gpu, BF)
+    k = torch.randn(sum(new) + sum(ctx), 2, HD, generator=g).to(gpu, BF)
+    vals, c = _constant_values(sum(new) + sum(ctx), 2, 64, gpu)
+    got = _paged_run(q, k, vals, new, ctx, 64, layout)[0]
+    assert torch.equal(got, c.repeat_interleave(4, 0).expand_as(got))
+
+
+def test_values_that_cancel(gpu):
+    """Neighbouring keys of almost equal scores and opposite values: the result is small beside sum p |v|, of which the rounding
+    of the probabilities is up to 2^-8. (The bound of every test here; where the result is small it is the larger part.)"""
+    lens = [400, 33]
+    q, k, v = _packed(lens, 8, 2, 64, gpu, seed=13)
+    k[1::2], v[1::2] = k[:-1:2][:k[1::2].shape[0]], -v[:-1:2][:v[1::2].shape[0]]
+    got = _packed_check(q, k, v, lens)
+    k[1::2, :, 0] += 2.0 ** -5                                          # no longer equal: what is left is a difference of weights
+    assert got[1::2][:200].abs().max() < 0.05 and _packed_check(q, k, v, lens).isfinite().all()

@@ -21,8 +21,12 @@
 // 365 us (5.7 TB/s). Short sequences pay for each tile's search, first loads and masked keys, some 17 thousand cycles beside
 // 2100 to 2900 per 64 keys: 8 prompts of 2 to 2048 79 us (0.74 PFLOP/s), 128 of 128 127 us.
 //
-// Rounding: scores, statistics and sums are fp32 (products of bf16 are exact in them); the probabilities are rounded to
-// bf16 for the second product, off by at most 2^-8 of each, less in their weighted sum than the output's own rounding.
+// Rounding: scores, statistics and sums are fp32 (products of bf16 are exact in them); the probabilities are rounded to bf16
+// for the second product, by up to 2^-8 of each, and it is the rounded ones that are summed to divide by. So a result is a mean of V
+// with weights off by that much: by at most 2^-8 sum_t p_t |v_t - out| before its own rounding to bf16, which is more than the latter
+// where values cancel, and nothing where they are equal. (Divided by the sum of the unrounded ones, one dominating key alone
+// was off by up to 2^-8; a prompt of 8192 took 524 us, with the rounded ones' 537. A second bf16 plane for what the rounding
+// drops, which would leave 2^-16: 733 us.)
 #include "palu_kernel.h"
 
 #include <algorithm>
@@ -431,17 +435,17 @@ __global__ __launch_bounds__(256, 2) void palu_flash_prefill_kernel(const FlashP
     }
     return m_run == NEG_INF ? 0.f : m_run;
   };
-  // An eighth of a tile's probabilities: four scores of half tt of block b.
+  // An eighth of a tile's probabilities, four scores of half tt of block b: rounded, and their sum. (Two accumulators, the sums an
+  // eighth later, or beside the products with V: within 1 % of this, the last 4 % slower.)
   auto eighth = [&](const f32x16 (&s)[2], bf16x8 (&p)[2][2], int c, float mref) __attribute__((always_inline)) {
     const int b = c >> 2, tt = (c >> 1) & 1, lo = 4 * (c & 1);
-    float e[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      e[i] = __builtin_amdgcn_exp2f(fmaf(s[b][4 * tt + 2 * lo + i], a.qscale, -mref));
-      p[b][tt][lo + i] = (__bf16)e[i];
-    }
-    l_run += (e[0] + e[1]) + (e[2] + e[3]);
-    asm volatile("" : "+v"(l_run));                       // now: put off, the sums would keep all their terms in registers
+    for (int i = 0; i < 4; ++i)
+      p[b][tt][lo + i] = (__bf16)__builtin_amdgcn_exp2f(fmaf(s[b][4 * tt + 2 * lo + i], a.qscale, -mref));
+#pragma unroll
+    for (int i = lo; i < lo + 4; i += 2)
+      l_run = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{p[b][tt][i], p[b][tt][i + 1]}, bf16x2{(__bf16)1.f, (__bf16)1.f}, l_run, false);
+    asm volatile("" : "+v"(l_run));                       // now: put off, the sums would keep more registers live
   };
   // Operand c of a tile's products with V, md innermost: consecutive products have different accumulators. Operands are
   // read ahead of their products, K two eighths and V three products: a read from LDS takes as long as some four products.

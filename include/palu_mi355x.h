@@ -438,15 +438,17 @@ int palu_flash_prefill(const void* q, long long q_row_stride, long long q_head_s
  * rows' keys and values already (palu_latent_fill_paged). A row at a negative position sees nothing and gets zeros; one past
  * the table's max_pages_per_seq * page_size positions sees those. Page ids are clamped into the pool. Where few rows stand on
  * long contexts, their keys are cut into pieces for several workgroups, which meet in the workspace
- * (palu_flash_prefill_workspace_bytes; any contents; calls that share one must be ordered on one stream). */
+ * (palu_flash_prefill_workspace_bytes; any contents; calls that share one must be ordered on one stream). Batches of more than
+ * 256 sequences are not cut: there a tile of 128 (row, head)s passes over all of its keys in one workgroup per KV head. */
 int palu_flash_prefill_paged(const void* q, long long q_row_stride, long long q_head_stride, const void* k_pages,
                              const void* v_pages, const int32_t* cu_seqlens, const int32_t* start_pos,
                              const int32_t* page_table, void* out, float scale, int rows, int batch, int n_q, int n_kv,
                              int num_pages, int page_size, int max_pages_per_seq, int head_dim_v, int cache_layout,
                              void* workspace, size_t workspace_bytes, palu_stream_t stream);
 
-/* Workspace bytes of palu_flash_prefill_paged, max_keys = max_pages_per_seq * page_size (0 when no keys are cut, and for
- * invalid shapes). */
+/* Workspace bytes of palu_flash_prefill_paged, max_keys = max_pages_per_seq * page_size: what the batch may be cut into, which
+ * lengths and positions on the device decide (32 heads over 8: 1 MB for one row over 512 positions, at most 66 MB). 0 for up
+ * to 256 positions, for more than 256 sequences or 2^28 rows of heads, and for invalid shapes. */
 size_t palu_flash_prefill_workspace_bytes(int rows, int batch, int n_q, int n_kv, int max_keys, int head_dim_v);
 
 /* Packed rows into a page pool [num_pages][n_groups][page_size][width] (cache_layout PALU_LAYOUT_ROWS, _TILED or _TILED_V):

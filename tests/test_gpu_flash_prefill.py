@@ -479,3 +479,27 @@ def test_values_that_cancel(gpu):
     got = _packed_check(q, k, v, lens)
     k[1::2, :, 0] += 2.0 ** -5                                          # no longer equal: what is left is a difference of weights
     assert got[1::2][:200].abs().max() < 0.05 and _packed_check(q, k, v, lens).isfinite().all()
+
+
+@pytest.mark.parametrize("nq,nkv", [(6, 2), (7, 1), (18, 3), (40, 8)])
+@pytest.mark.parametrize("new,ctx", [([1, 5], [5000, 30]), ([40, 3, 1], [3000, 7000, 300]), ([1], [290])], ids=str)
+def test_cut_contexts_of_head_groups_that_do_not_divide_a_tile(gpu, nq, nkv, new, ctx):
+    _paged_check(new, ctx, nq, nkv, 48, 32, "rows", gpu, seed=nq)
+
+
+@pytest.mark.parametrize("rows,B,nq,nkv", [(1, 200, 4, 1), (3, 60, 8, 2), (1, 256, 3, 1), (2, 31, 32, 8)])
+def test_overlapping_sequences_stay_inside_the_workspace(gpu, rows, B, nq, nkv):
+    """Offsets that fall back to the first row again and again, all over long contexts: more pieces than the workspace holds. What
+    comes out is not defined, what lies around the output and the workspace keeps what it holds."""
+    from palu_tt import _native
+    g = torch.Generator().manual_seed(rows)
+    q = torch.randn(rows, nq, HD, generator=g).to(gpu, BF)
+    kp, vp = (torch.randn(5, nkv, 64, w, generator=g).to(gpu, BF) for w in (HD, 64))
+    table = torch.randint(0, 5, (2 * B, 500), generator=g).to(gpu, torch.int32)[:min(256, 2 * B)]
+    B = table.shape[0]
+    cu = _ints([0, rows] * (B // 2) + [0], gpu)[:B + 1]
+    need = _native.load().palu_flash_prefill_workspace_bytes(rows, B, nq, nkv, 500 * 64, 64)
+    ws, out = torch.full((need + 8192,), 77, dtype=torch.uint8, device=gpu), torch.full((rows + 2, nq, 64), 7.0, dtype=BF, device=gpu)
+    fused.flash_prefill(q, kp, vp, cu, page_table_tensor=table, start_pos=torch.full((B,), 31_000, dtype=torch.int32, device=gpu),
+                        out=out[1:-1], workspace=ws[4096:4096 + need])
+    assert need and (ws[:4096] == 77).all() and (ws[4096 + need:] == 77).all() and (out[0] == 7).all() and (out[-1] == 7).all()

@@ -334,3 +334,18 @@ def test_token_logprobs_workspace(lib):
     assert parts > 1 and f(3000, 128256, 5) == 0
     for top in range(1, 65):
         assert f(1, 128256, top) == parts * (16 + 8 * (top + top % 2)) and f(7, 128256, top) % 16 == 0
+
+
+def test_flash_prefill_workspace_goes_by_the_batch(lib):
+    """No more pieces than the batch's tiles can be cut into: a tile of 128 rows stands at most max_keys / 32 levels from the start
+    (4 heads to a KV head) and is cut into pieces of 8 levels or more."""
+    f = lib.palu_flash_prefill_workspace_bytes
+    piece = 8 * (128 * 130 * 4 + 32)                                    # of every KV head
+    assert f(1, 1, 32, 8, 256, 128) == 0
+    assert f(1, 1, 32, 8, 288, 128) <= 2 * piece and f(1, 1, 32, 8, 512, 128) <= 3 * piece and f(4, 4, 32, 8, 512, 128) <= 12 * piece
+    assert f(1, 1, 32, 8, 2048, 128) <= 9 * piece
+    # long contexts: a piece to each of the 512 places' parts, and one more for every tile
+    assert f(1, 1, 32, 8, 65536, 128) <= (512 // 8 + 1) * piece
+    sizes = [f(rows, rows, 32, 8, 65536, 128) for rows in (1, 8, 64, 256)]
+    assert sizes == sorted(sizes) and sizes[-1] <= 2 * (512 // 8 + 1) * piece
+    assert f(257, 257, 32, 8, 65536, 128) == 0                          # more than 256 sequences are not cut

@@ -267,8 +267,10 @@ __global__ __launch_bounds__(256, 2) void palu_flash_prefill_kernel(const FlashP
   const int per_piece = (nt_all + tile.pieces - 1) / tile.pieces;
   const int t_lo = tile.piece * per_piece, nt = min(nt_all, t_lo + per_piece);
   const int n_pieces = nt_all > per_piece ? (nt_all + per_piece - 1) / per_piece : 1;
-  record(n_pieces > 1 && tile.piece == 0 ? Record{n_pieces, rows, sq.beg, sq.start, rs.pos0, rs.rem, {}} : Record{});
-  if (t_lo >= nt && tile.piece > 0) return;   // uniform
+  // (Sequences that overlap, where the offsets make no sense, can be more tiles than the workspace was sized for.)
+  const bool fits = SRC == PACKED || item - tile.piece + n_pieces <= a.cut;
+  record(n_pieces > 1 && fits && tile.piece == 0 ? Record{n_pieces, rows, sq.beg, sq.start, rs.pos0, rs.rem, {}} : Record{});
+  if ((t_lo >= nt && tile.piece > 0) || (n_pieces > 1 && !fits)) return;   // uniform
 
   // ---- copies to LDS: wave w copies keys 16 w .. + 15 of a tile (half-block w % 2 of block w / 2 for K) ---------
   const int last_blk = (kv_end - 1) >> 5, inpage = (1 << a.page_shift) - 1;
@@ -725,25 +727,27 @@ long long most_tiles(int T, int B, int rep) { return (long long)T * rep / FP_ROW
 
 // Whether tiles may be cut along their keys: where contexts stand before the rows. (Packed prompts stand on their own keys;
 // cutting their longest tiles, one prompt of 1024 positions took 42 us instead of 27 and one of 2048 82 instead of 55.)
-// Up to 2^28 rows of heads, which keeps find_tile's levels below 2^22.
+// Up to 2^28 rows of heads, which keeps find_tile's levels below 2^22, and up to FP_SORTED sequences.
 bool may_split(int T, int B, int n_q, bool paged, long long max_keys) {
   return paged && B <= FP_SORTED && max_keys > FP_MIN_KEYS && (long long)T * n_q <= (1ll << 28);
 }
-// Pieces of cut tiles per KV head, at most: with len levels to a piece, a tile of level t >= 1.25 len has at most t / len + 3 / 4
-// <= 2 t / len, and the levels' sum is at most FP_WGS / (FP_PIECE n_kv) times len.
-long long most_pieces(int n_kv) { return (long long)(2 * FP_WGS / FP_PIECE) / n_kv + 2; }
+
+// Items of a KV head that may be pieces of cut tiles (they are the first of all items), at most; 0: no tile is cut. With len levels to a
+// piece (find_tile), a tile of level t is cut into t / len + 3 / 4 pieces where t >= 1.25 len, so into fewer than 2 t / len; all
+// tiles' levels together are at most FP_WGS / (FP_PIECE n_kv) times len; len is not below `least`, no level above `top`.
+long long cut_items(int T, int B, int n_q, int n_kv, long long max_keys) {
+  const int rep = n_q / n_kv, shift = 31 - __builtin_clz(std::max(1, FP_ROWS / rep)), least = std::max(2, FP_MIN_KEYS >> shift);
+  const long long tiles = most_tiles(T, B, rep), top = (max_keys >> shift) + ((long long)T * rep + FP_ROWS - 1) / FP_ROWS - 1;
+  const long long of_tile = (top + least - least / 4 - 1) / least, share = (long long)(FP_WGS / FP_PIECE) / n_kv + 1;
+  return of_tile < 2 ? 0 : std::min({tiles * of_tile, share + tiles, 2 * share});
+}
 
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-
-// Items of a KV head that may be pieces, where tiles may be cut.
-long long cut_items(int T, int B, int n_q, int n_kv) {
-  return std::min(most_tiles(T, B, n_q / n_kv) + most_pieces(n_kv), most_pieces(n_kv));
-}
 
 // Workspace: the pieces' partial results, then the items' records.
 size_t part_bytes(int n_q, int n_kv, int T, int B, bool paged, long long max_keys, int dv) {
   if (!may_split(T, B, n_q, paged, max_keys)) return 0;
-  return (size_t)cut_items(T, B, n_q, n_kv) * n_kv * (FP_ROWS * (dv + 2) * sizeof(float) + sizeof(Record));
+  return (size_t)cut_items(T, B, n_q, n_kv, max_keys) * n_kv * (FP_ROWS * (dv + 2) * sizeof(float) + sizeof(Record));
 }
 
 int check_dims(int T, int B, int n_q, int n_kv, int dv, const char* who) {
@@ -764,11 +768,10 @@ int launch_prefill(FlashPrefillArgs& a, long long max_keys, void* workspace, siz
   if (need && (!workspace || workspace_bytes < need || !al16(workspace)))
     return fail(PALU_EINVAL, "%s: a 16-byte aligned workspace of %zu bytes needed (palu_flash_prefill_workspace_bytes), got %zu",
                 who, need, workspace ? workspace_bytes : 0);
-  a.cut = need ? (int)cut_items(a.T, a.B, a.n_q, a.n_kv) : 0;
+  a.cut = need ? (int)cut_items(a.T, a.B, a.n_q, a.n_kv, max_keys) : 0;
   a.part = need ? static_cast<float*>(workspace) : nullptr;
   a.records = reinterpret_cast<Record*>(a.part + (size_t)a.cut * a.n_kv * FP_ROWS * (a.dv + 2));
-  const long long pieces = need ? most_pieces(a.n_kv) : 0;
-  const unsigned grid = (unsigned)((most_tiles(a.T, a.B, a.rep) + pieces) * a.n_kv);
+  const unsigned grid = (unsigned)((most_tiles(a.T, a.B, a.rep) + a.cut) * a.n_kv);
   auto go = [&](auto kern, unsigned wgs) {
     hipLaunchKernelGGL(kern, dim3(wgs), dim3(256), 0, s, a);
     const hipError_t e = hipGetLastError();

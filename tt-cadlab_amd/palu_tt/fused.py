@@ -515,8 +515,8 @@ def flash_prefill(q, k, v, cu_seqlens, *, scale=None, head_dim_v=None, out=None,
     stands at position start_pos[b] + i (int32 [B]; None: i) behind the positions cached before. Query head h reads KV head
     h // (n_q // n_kv). head_dim_v: multiples of 16 up to 128. Returns [T, n_q, head_dim_v] bf16; rows past
     cu_seqlens[B] are not written (``out``, which must not overlap the inputs, keeps what it held there). workspace (paged
-    calls): a uint8 device tensor of palu_flash_prefill_workspace_bytes(...) bytes, else one from torch's caching allocator where
-    few rows stand on long contexts."""
+    calls): a uint8 device tensor of palu_flash_prefill_workspace_bytes(...) bytes, else one from torch's caching allocator (tables of
+    more than 256 positions, up to 256 sequences; larger batches are not cut along their keys)."""
     q_st, q_sh = _strided_rows(q, "q", HEAD_DIM)
     dev = q.device
     T, n_q = q.shape[:2]

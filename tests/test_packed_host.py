@@ -349,3 +349,17 @@ def test_flash_prefill_workspace_goes_by_the_batch(lib):
     sizes = [f(rows, rows, 32, 8, 65536, 128) for rows in (1, 8, 64, 256)]
     assert sizes == sorted(sizes) and sizes[-1] <= 2 * (512 // 8 + 1) * piece
     assert f(257, 257, 32, 8, 65536, 128) == 0                          # more than 256 sequences are not cut
+
+
+def test_out_of_an_update_is_memory_of_its_own(launches):
+    """Neither a pool nor the workspace may be what the new table or the new lengths are written to."""
+    pool = _gpu_like(4, 1, 32, 8)
+    h = PagePools([pool])
+    t, ln, ws = _ints([[0, 1]]), _ints([3]), torch.zeros(1024, dtype=torch.int32)
+    over = lambda x: x.view(-1).as_subclass(torch.Tensor).view(torch.int32)
+    for out in ((over(pool)[:2].view(1, 2), ln.clone()), (t.clone(), over(pool)[5:6]), (ws[8:10].view(1, 2), ln.clone()), (t.clone(), ws[1023:])):
+        with pytest.raises(RuntimeError, match="memory of its own"):
+            h.update(t, ln, out=out, workspace=ws)
+    assert not launches
+    h.update(t, ln, out=(t.clone(), ln.clone()), workspace=ws)
+    assert len(launches) == 1

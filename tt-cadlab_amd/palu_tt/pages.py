@@ -98,6 +98,7 @@ class PagePools:
         int32 [B] and [B, max_pages] on the device; entries past a row's pages are -1. out: (page_table, lengths) to
         write, memory of their own. Do not share a workspace (uint8, palu_pages_workspace_bytes) between calls that may overlap."""
         pt, ln, B, slots = self._args(page_table, lengths)
+        ws, need = self._workspace(B, workspace) if B else (None, 0)
         par = None if parents is None else _ints(parents, "parents", (B,), self.device)
         new = None if new_lengths is None else _ints(new_lengths, "new_lengths", (B,), self.device)
         if out is None:
@@ -106,12 +107,11 @@ class PagePools:
             for t, like, name in zip(out, (pt, ln), ("page_table", "lengths")):
                 if t.shape != like.shape or t.dtype != torch.int32 or t.device != self.device or not t.is_contiguous():
                     raise RuntimeError(f"out: {name} must be a contiguous int32 {list(like.shape)} tensor on {self.device}")
-                if any(i is not None and _overlap(t, i) for i in (pt, ln, par, new)):
+                if any(i is not None and _overlap(t, i) for i in (pt, ln, par, new, workspace, *self._stores)):
                     raise RuntimeError(f"out: {name} must be memory of its own")
             if _overlap(*out):
                 raise RuntimeError("out: page_table and lengths must not overlap")
         if B:
-            ws, need = self._workspace(B, workspace)
             _native.launch("pages_update", self.device, pt.data_ptr(), ln.data_ptr(), _native.ptr(par), _native.ptr(new),
                            out[0].data_ptr(), out[1].data_ptr(), self._ptrs, self._bytes, len(self.pools), B, self.n_pages,
                            self.page_size, slots, ws.data_ptr(), need)

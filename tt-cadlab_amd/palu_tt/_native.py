@@ -9,6 +9,7 @@ import ctypes
 import threading
 
 import torch  # noqa: F401  (loads the HIP runtime the library binds to)
+from torch.autograd import forward_ad
 
 from palu_tt._build import library_path
 
@@ -127,10 +128,10 @@ def workspace_bytes(workspace, need: int, device, what: str = "workspace") -> in
 def refuse_derivatives(what: str, *tensors) -> None:
     """Raises where a derivative would go through these tensors: the kernels see their values only, and it would come out as
     none without a word."""
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad()")
-    if torch.autograd.forward_ad._current_level >= 0 and any(
-            torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+    for t in tensors:
+        if t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad()")
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise RuntimeError(f"{what} has no forward-mode derivative: an input has a tangent")
 
 

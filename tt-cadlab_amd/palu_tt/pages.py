@@ -10,7 +10,6 @@ reference counts and no free list, so a row is freed by giving it the length 0. 
 (a common prefix, the siblings of a beam); ``update`` gives every row its own copy of the page that it writes next.
 """
 import ctypes
-from operator import is_
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -33,10 +32,6 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     return a0 < b1 and b0 < a1
 
 
-def _places(stores):
-    return list(map(torch.Tensor.data_ptr, stores)), list(map(torch.Tensor.numel, stores))
-
-
 class PagePools:
     """The page pools that share a page table: row-major [n_pages, n_groups, page_size, width] bf16 tensors or LatentCache
     pools (of any group counts and widths)."""
@@ -45,15 +40,19 @@ class PagePools:
         if not pools:
             raise RuntimeError("PagePools needs at least one pool")
         self.pools = list(pools)
-        self._stores, self._places = [], None
-        self._look()
+        self._take()
 
     def _look(self) -> None:
-        """Takes the pools' storage as it is now: a LatentCache's ``data`` may be another tensor than at the last call, and a
-        tensor may have been given other memory or another size. Pools where nothing changed are not checked again."""
+        """Takes the pools anew if one is not what it was: a LatentCache's ``data`` may be another tensor than at the last
+        call, and a tensor may have been given other memory or another size."""
+        for cache, store, place, size in self._seen:
+            if (cache is not None and cache.data is not store) or store.data_ptr() != place or store.numel() != size:
+                self._take()
+                return
+
+    def _take(self) -> None:
+        """Checks the pools as they are now and takes their storage, which is held for as long as its address is."""
         stores = [p.data if isinstance(p, LatentCache) else p for p in self.pools]
-        if len(stores) == len(self._stores) and all(map(is_, stores, self._stores)) and _places(stores) == self._places:
-            return
         for p, s in zip(self.pools, stores):
             if not (isinstance(s, torch.Tensor) and len(p.shape) == 4 and s.is_cuda and s.dtype == torch.bfloat16 and
                     s.is_contiguous() and s.data_ptr() % 16 == 0 and s.numel()):
@@ -69,7 +68,8 @@ class PagePools:
         n = len(stores)
         self._ptrs = (ctypes.c_void_p * n)(*[s.data_ptr() for s in stores])
         self._bytes = (ctypes.c_longlong * n)(*[s.numel() * 2 // self.n_pages for s in stores])
-        self._stores, self._places = stores, _places(stores)
+        self._seen = [(p if isinstance(p, LatentCache) else None, s, s.data_ptr(), s.numel()) for p, s in zip(self.pools, stores)]
+        self._stores = stores
 
     def _args(self, page_table, lengths):
         self._look()

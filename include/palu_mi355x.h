@@ -467,7 +467,8 @@ int palu_latent_fill_paged(void* cache_pages, const void* rows, long long row_st
  * page that a row writes next, which its kept positions end inside, becomes its own: of the rows that would write a page the
  * first keeps it, unless another row holds it whole; the others get a copy of it in every pool. New pages are the
  * lowest free ones in the order of rows and slots; where they run out, lengths_out[b] is what the row's pages hold.
- * Entries past a row's pages become -1. Ids outside the pool are kept as entries and name no page.
+ * Entries past a row's pages become -1. Ids outside the pool are kept as entries and name no page. The copies may overwrite
+ * pages that no row of the new table names: the old table is not to be used again, not even where lengths come out shorter.
  *   page_table, page_table_out [batch][max_pages_per_seq], lengths, lengths_out [batch] int32: separate memory
  *   pools: n_pools device pointers (host array) to pools of num_pages pages of page_bytes[i] bytes (a multiple of 16)
  * At most 4096 rows; the bits of num_pages pages and the rows' data fit 156 KB of LDS (a million pages for small batches).

@@ -14,19 +14,20 @@
 // keys 8 g .. + 7 in pairs of registers, which is the B operand of the second product, and no value changes lanes.
 // V^T comes from the caches' V tiles as it stands, from rows by transposing LDS reads (ds_read_b64_tr_b16).
 //
-// Bound by the matrix cores where sequences are long: they are busy 62 % of a CU's cycles over a prompt of 8192 positions,
+// Bound by the matrix cores where sequences are long: they are busy 57 % of a CU's cycles over a prompt of 8192 positions,
 // at the 1.65 GHz that the card's power limit leaves; S of the next tile runs beside the exponentials of this one, and two
-// workgroups share a CU. 32 query heads over 8 KV heads, widths 128: a prompt of 8192 takes 506 us (1.09 PFLOP/s), of 16384
-// 1.97 ms (1.12); 2048 rows behind 30000 positions in pages 0.90 ms (1.16); 64 rows, one behind each of 8000 positions,
-// 365 us (5.7 TB/s). Short sequences pay for each tile's search, first loads and masked keys, some 17 thousand cycles beside
-// 2100 to 2900 per 64 keys: 8 prompts of 2 to 2048 79 us (0.74 PFLOP/s), 128 of 128 127 us.
+// workgroups share a CU. 32 query heads over 8 KV heads, widths 128: a prompt of 8192 takes 526 us (1.05 PFLOP/s), of 16384
+// 2.02 ms (1.09); 2048 rows behind 30000 positions in pages 0.95 ms (1.09); 64 rows, one behind each of 8000 positions,
+// 365 us (5.7 TB/s). Short sequences pay for each tile's search, first loads and masked keys, some 17 thousand cycles together (not
+// measured apart) beside 2100 to 2900 per 64 keys: 8 prompts of 2 to 2048 82 us (0.71 PFLOP/s), 128 of 128 127 us. At width
+// 128 four to seven registers spill, 20 to 32 bytes a thread.
 //
 // Rounding: scores, statistics and sums are fp32 (products of bf16 are exact in them); the probabilities are rounded to bf16
 // for the second product, by up to 2^-8 of each, and it is the rounded ones that are summed to divide by. So a result is a mean of V
 // with weights off by that much: by at most 2^-8 sum_t p_t |v_t - out| before its own rounding to bf16, which is more than the latter
 // where values cancel, and nothing where they are equal. (Divided by the sum of the unrounded ones, one dominating key alone
-// was off by up to 2^-8; a prompt of 8192 took 524 us, with the rounded ones' 537. A second bf16 plane for what the rounding
-// drops, which would leave 2^-16: 733 us.)
+// was off by up to 2^-8; a prompt of 8192 takes 3 % longer for it. A second bf16 plane for what the rounding drops, which
+// would leave 2^-16, takes another 37 %.)
 #include "palu_kernel.h"
 
 #include <algorithm>
@@ -38,8 +39,9 @@ constexpr int FP_KEYS = 64;               // keys of a K / V tile: two 32-positi
 constexpr int FP_MIN_KEYS = 256;          // keys of a piece of a split tile, about, at least
 constexpr int FP_SORTED = 256;            // sequences whose tiles are taken longest first
 constexpr int FP_WGS = 512;               // workgroups that the chip holds at once (two a CU)
-// Keys of a piece over a workgroup slot's part of the batch's, about, at most. (8 sequences of up to 300 rows over up to 32000
-// positions: 136 us, with 0.8 175, with 0.55 151; one row over 32000: 32, 39 and 43.)
+// Keys of a piece over a workgroup slot's part of the batch's, about, at most. Measured on two batches only: 8 sequences of up to 300
+// rows over up to 32000 positions 136 us, with 0.8 175, with 0.55 151; one row over 32000 32, 39 and 43. What counts is how a
+// batch's pieces fall on the slots, so no rule follows for others, but that a little over one part each leaves no second turn.
 constexpr float FP_PIECE = 1.05f;
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -727,7 +729,8 @@ long long most_tiles(int T, int B, int rep) { return (long long)T * rep / FP_ROW
 
 // Whether tiles may be cut along their keys: where contexts stand before the rows. (Packed prompts stand on their own keys;
 // cutting their longest tiles, one prompt of 1024 positions took 42 us instead of 27 and one of 2048 82 instead of 55.)
-// Up to 2^28 rows of heads, which keeps find_tile's levels below 2^22, and up to FP_SORTED sequences.
+// Up to 2^28 rows of heads, which keeps find_tile's levels below 2^22, and up to FP_SORTED sequences, whose lengths a wave holds
+// in registers. (Single rows, one behind 60000 positions and the others behind 500, 8 KV heads: 256 take 180 us, 300 1039.)
 bool may_split(int T, int B, int n_q, bool paged, long long max_keys) {
   return paged && B <= FP_SORTED && max_keys > FP_MIN_KEYS && (long long)T * n_q <= (1ll << 28);
 }

@@ -94,7 +94,8 @@ class PagePools:
 
         Whole pages are shared; the page that a row writes next is its own: the first row that would write it keeps it, unless
         another holds it whole, the others get a copy in every pool. New pages are the lowest free ones. Where the pool has
-        no more, the returned length of a row is what its pages hold: compare with what was asked for. All integers are
+        no more, the returned length of a row is what its pages hold: compare with what was asked for, and go on from the new table
+        (pages that it does not name may hold other rows' copies already, so the old one is done with). All integers are
         int32 [B] and [B, max_pages] on the device; entries past a row's pages are -1. out: (page_table, lengths) to
         write, memory of their own. Do not share a workspace (uint8, palu_pages_workspace_bytes) between calls that may overlap."""
         pt, ln, B, slots = self._args(page_table, lengths)

@@ -250,6 +250,8 @@ def test_out_of_the_packed_attention_is_memory_of_its_own(launches):
     assert len(launches) == 5
     with pytest.raises(RuntimeError, match="memory of its own"):
         packed(apart[2, 504:504 + 1536].view(6, 4, 64), q=apart[:, :512].unflatten(1, (4, 128)))
+    with pytest.raises(RuntimeError, match="workspace must be"):          # (one in pieces over the output, too)
+        paged(own, workspace=own.view(-1)[::2], table=_ints([list(range(4)) * 4]))
 
 
 def _packed_inputs():

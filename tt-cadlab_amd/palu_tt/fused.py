@@ -491,9 +491,11 @@ def _strided_rows(t, name: str, width: Optional[int], device=None):
 def _overlap(out: torch.Tensor, t: torch.Tensor) -> bool:
     """Whether the contiguous `out` shares memory with t: contiguous, or a [rows, heads, width] view of contiguous heads (`out`
     may lie between its rows)."""
-    size = t.element_size()
-    lo, hi = (out.data_ptr() - t.data_ptr()) // size, -((t.data_ptr() - out.data_ptr() - out.numel() * out.element_size()) // size)
-    if not (t.numel() and out.numel()) or hi <= 0 or lo > sum((n - 1) * st for n, st in zip(t.shape, t.stride())):
+    ahead, size = out.data_ptr() - t.data_ptr(), t.element_size()         # in elements of t, `out` lies in lo .. hi - 1
+    if ahead >= 0 and t.is_contiguous():
+        return ahead < t.numel() * size and out.numel() > 0
+    lo, hi = ahead // size, -((-ahead - out.numel() * out.element_size()) // size)
+    if hi <= 0 or not (t.numel() and out.numel()) or lo > sum((n - 1) * st for n, st in zip(t.shape, t.stride())):
         return False
     if t.is_contiguous():
         return True
@@ -553,9 +555,9 @@ def flash_prefill(q, k, v, cu_seqlens, *, scale=None, head_dim_v=None, out=None,
         _as_dev(out, "out", torch.bfloat16, dev)
         if tuple(out.shape) != (T, n_q, dv):
             raise RuntimeError(f"out must be [{T}, {n_q}, {dv}]")
-        reads = (q, k, v, cu) if page_table_tensor is None else (q, k_store, v_store, cu, pt, start, workspace)
-        if any(t is not None and _overlap(out, t) for t in reads):
-            raise RuntimeError("out must be memory of its own: it overlaps an input or the workspace")
+        for t in (q, k, v, cu) if page_table_tensor is None else (q, k_store, v_store, cu, pt, start):
+            if t is not None and _overlap(out, t):
+                raise RuntimeError("out must be memory of its own: it overlaps an input")
     if T == 0:
         return out
     sc = float(HEAD_DIM ** -0.5 if scale is None else scale)
@@ -568,6 +570,8 @@ def flash_prefill(q, k, v, cu_seqlens, *, scale=None, head_dim_v=None, out=None,
         workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     else:
         _native.workspace_bytes(workspace, need, dev)
+        if _overlap(out, workspace):
+            raise RuntimeError("out must be memory of its own: it overlaps the workspace")
     _native.launch("flash_prefill_paged", dev, q.data_ptr(), q_st, q_sh, k_store.data_ptr(), v_store.data_ptr(),
                    cu.data_ptr(), _native.ptr(start), pt.data_ptr(), out.data_ptr(), sc, T, B, n_q, n_kv, n_pages,
                    page_size, pt.shape[1], dv, layout, _native.ptr(workspace), need)

@@ -21,7 +21,7 @@
 extern "C" {
 #endif
 
-#define PALU_ABI_VERSION 17
+#define PALU_ABI_VERSION 18
 
 #define PALU_OK 0
 #define PALU_EINVAL 1       /* arguments outside the op's envelope */
@@ -54,6 +54,24 @@ extern "C" {
  * element b * S * sum(ranks) + S * (sum of the ranks of groups 0 .. g-1). No counterpart in the
  * reference, which pads every group to the layer's widest (convert.py:178). */
 #define PALU_LAYOUT_TILED_GROUPED 3
+
+/* Quantised caches, of appends, packed fills and reads, palu_flash_decode and its paged and shared forms: bytes, 32
+ * neighbouring channels of a position with one scale, a power of two kept as its exponent in a byte (2^(byte - 127); 255: all
+ * 32 are NaN), as fp8 (e4m3: up to 448) or fp4 (e2m1: 0, 0.5, 1, 1.5, 2, 3, 4, 6). Widths are multiples of 32. A 32-position
+ * block of a cache `width` wide takes 33 * width bytes (MX4: 17 * width), blocks lie as those of the tiled layouts do: a page
+ * is [n_groups][page_size / 32] of them. In a block, position 8 t + 4 c + i (t < 4, c < 2, i < 4) with n = 4 t + i:
+ *   K order: MX8 [c][h < 2][g < width / 32][n] pieces of 16 bytes, channels 32 g + 16 h + 0 .. 15;
+ *            MX4 [c][g][n] pieces of 16 bytes, channels 32 g + 0 .. 31, the lower of two in a byte's low half;
+ *            then the scales [g][n][c], a byte each;
+ *   V order, position 8 o + j: MX8 [b < width / 32][o < 4][m < 16][j < 8] pairs of bytes, channels 32 b + 2 m, 32 b + 2 m + 1;
+ *            MX4 bytes in the same order, of the same two channels; then the scales [b][position].
+ * A write takes as a block's scale the smallest power of two, from 2^-117 on, over which its largest magnitude is at most 464
+ * (MX4: 7), and rounds each value over the scale to the nearest element, ties to the even code; magnitudes past 1.75 * 2^127
+ * are taken as that, a block with an infinity or NaN becomes NaN. What is read back is exact in bf16. */
+#define PALU_LAYOUT_MX8 4   /* fp8: decode K in K order, V in V order; others: K order */
+#define PALU_LAYOUT_MX8_V 5 /* fp8, V order */
+#define PALU_LAYOUT_MX4 6   /* fp4, as PALU_LAYOUT_MX8 */
+#define PALU_LAYOUT_MX4_V 7 /* fp4, V order */
 
 #define PALU_ROT_LEGACY 0
 #define PALU_ROT_PACK 1
@@ -459,6 +477,35 @@ int palu_latent_fill_paged(void* cache_pages, const void* rows, long long row_st
                            const int32_t* cu_seqlens, const int32_t* start_pos, const int32_t* page_table, int n_rows,
                            int batch, int n_groups, int num_pages, int page_size, int max_pages_per_seq, int width,
                            int cache_layout, palu_stream_t stream);
+
+/* The rows back out of a page pool in any of those layouts: out [n_rows][n_groups][width] bf16, row i of sequence b from position
+ * start_pos[b] + i (start_pos NULL: i). Positions outside the table and page ids outside the pool give zeros; rows past
+ * cu_seqlens[batch] keep what they hold. */
+int palu_latent_read_paged(const void* cache_pages, void* out, const int32_t* cu_seqlens, const int32_t* start_pos,
+                           const int32_t* page_table, int n_rows, int batch, int n_groups, int num_pages, int page_size,
+                           int max_pages_per_seq, int width, int cache_layout, palu_stream_t stream);
+
+/* Workspace bytes of palu_flash_decode and palu_flash_decode_paged in the layouts PALU_LAYOUT_MX8 and _MX4 (any contents, 16-byte
+ * aligned; calls that share one must be ordered on one stream); 0 for invalid shapes. There head_dim_v is a multiple of 32 up to
+ * 128, a row has at most 65536 positions (contiguous: a multiple of 32), and calls are bit-reproducible whatever `deterministic`. */
+size_t palu_mx_decode_workspace_bytes(int batch, int n_q, int n_kv, int head_dim_v);
+
+/* palu_flash_decode_paged of a batch in groups of neighbouring rows that share a prefix: rows cu_groups[i] .. cu_groups[i + 1] - 1
+ * (int32 [n_groups + 1], device memory, not decreasing; NULL: n_groups is 1 and all rows are one group) share their first
+ * shared_len[i] positions (int32 [n_groups], device memory). Whole 32-position blocks of them are read through the page table of
+ * the group's first row, once for all rows of the group that see them all; the rest of a row is read through its own table
+ * (whose entries before that are not looked at). Rows of no group stand alone. Layouts PALU_LAYOUT_ROWS, _TILED (head_dim_v
+ * multiples of 16 up to 128), _MX8 and _MX4 (of 32). A row at a negative position sees nothing and gets zeros, one past the
+ * table sees all of it; page ids are clamped into the pool. At most 4096 rows. Bit-reproducible. workspace:
+ * palu_flash_decode_shared_workspace_bytes, any contents, 16-byte aligned; calls that share one must be ordered on one stream. */
+int palu_flash_decode_shared(const void* q, const void* k_pages, const void* v_pages, const int32_t* cur_pos,
+                             const int32_t* page_table, const int32_t* cu_groups, const int32_t* shared_len, void* out,
+                             float scale, int batch, int n_groups, int n_q, int n_kv, int num_pages, int page_size,
+                             int max_pages_per_seq, int head_dim_v, int out_dtype, int cache_layout, void* workspace,
+                             size_t workspace_bytes, palu_stream_t stream);
+
+/* Workspace bytes of palu_flash_decode_shared (0 for invalid shapes). */
+size_t palu_flash_decode_shared_workspace_bytes(int batch, int n_groups, int n_q, int n_kv, int head_dim_v);
 
 /* Forks, ends, cuts and grows the rows of a page table in one step. Row b becomes a copy of row parents[b] as it was
  * (parents NULL: of itself; an index outside the batch: of an empty row), cut or grown to new_lengths[b] positions (NULL: as

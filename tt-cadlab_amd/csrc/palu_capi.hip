@@ -2,6 +2,7 @@
 // validation with the reference op's messages, the latent-append kernel, and dispatch to the decode
 // translation units.
 #include "palu_kernel.h"
+#include "palu_mx.h"
 
 #include <atomic>
 #include <mutex>
@@ -575,6 +576,9 @@ int palu_flash_decode(const void* q, const void* k, const void* v, const int32_t
                       int batch, int n_q, int n_kv, int seq_len, int head_dim_v, int out_dtype, int cache_layout,
                       int deterministic, void* workspace, size_t workspace_bytes, hipStream_t stream) {
   palu::g_err[0] = 0;
+  if (is_mx(cache_layout))
+    return mx_flash_decode(q, k, v, cur_pos, out, scale, batch, n_q, n_kv, seq_len, nullptr, 0, 0, 0, head_dim_v, out_dtype,
+                           cache_layout, workspace, workspace_bytes, "palu_flash_decode", stream);
   DecodeArgs a;
   if (int rc = flash_setup(a, q, k, v, cur_pos, out, scale, batch, n_q, n_kv, seq_len, head_dim_v, out_dtype,
                            cache_layout, deterministic, workspace, workspace_bytes, "palu_flash_decode"))
@@ -595,6 +599,10 @@ int palu_flash_decode_paged(const void* q, const void* k_pages, const void* v_pa
   int shift = 0;
   if (int rc = check_pages(page_table, num_pages, page_size, max_pages_per_seq, &shift, "palu_flash_decode_paged"))
     return rc;
+  if (is_mx(cache_layout))
+    return mx_flash_decode(q, k_pages, v_pages, cur_pos, out, scale, batch, n_q, n_kv, page_size, page_table, max_pages_per_seq,
+                           num_pages, shift, head_dim_v, out_dtype, cache_layout, workspace, workspace_bytes,
+                           "palu_flash_decode_paged", stream);
   const int seq_len = max_pages_per_seq * page_size;
   DecodeArgs a;
   if (int rc = flash_setup(a, q, k_pages, v_pages, cur_pos, out, scale, batch, n_q, n_kv, seq_len, head_dim_v,
@@ -614,6 +622,9 @@ int palu_flash_decode_paged(const void* q, const void* k_pages, const void* v_pa
 int palu_latent_append(void* cache, const void* new_rows, const int32_t* update_idxs, int batch, int n_groups,
                        int seq_len, int width, int cache_layout, hipStream_t stream) {
   palu::g_err[0] = 0;
+  if (is_mx(cache_layout))
+    return mx_append(cache, new_rows, (long long)n_groups * width, width, update_idxs, nullptr, 0, 0, batch, n_groups, seq_len,
+                     width, cache_layout, "palu_latent_append", stream);
   if (int rc = check_append(cache, new_rows, update_idxs, batch, n_groups, seq_len, width, cache_layout,
                             "palu_latent_append"))
     return rc;
@@ -706,6 +717,9 @@ int palu_latent_append_paged(void* cache_pages, const void* new_rows, const int3
   int shift = 0;
   if (int rc = check_pages(page_table, num_pages, page_size, max_pages_per_seq, &shift, "palu_latent_append_paged"))
     return rc;
+  if (is_mx(cache_layout))
+    return mx_append(cache_pages, new_rows, (long long)n_groups * width, width, update_idxs, page_table, max_pages_per_seq,
+                     num_pages, batch, n_groups, page_size, width, cache_layout, "palu_latent_append_paged", stream);
   if (int rc = check_append(cache_pages, new_rows, update_idxs, batch, n_groups, page_size, width, cache_layout,
                             "palu_latent_append_paged"))
     return rc;

@@ -1,7 +1,8 @@
 // Page pools of several sequences: rows of a packed batch into their pages, and the bookkeeping of a page table with the
 // copies of pages that it asks for. The pools of all layers share one page table; a page is free when no row's
 // used entries name it, so nothing but the table and the lengths has to be kept.
-#include "palu_kernel.h"
+#include "palu_mx.h"
+#include "palu_packed.h"
 
 #include <algorithm>
 
@@ -14,57 +15,23 @@ namespace {
 // rows of 16 sequences into K tiles take 13.1 us (5.2 TB/s read and written), into V tiles, whose regrouping goes through registers, 20.2
 // (3.4), 57 rows 3.7 us.
 struct FillArgs {
+  PackedSeqs seqs;
   __bf16* cache;                          // [n_pages][G][page][width]
   const __bf16* rows;
   long long st, sg;                       // source strides: row, group
-  const int32_t* cu;
-  const int32_t* start;                   // or null
-  const int32_t* table;
-  int T, B, G, width, n_pages, page_shift, pt_stride, gpw;   // gpw: groups per workgroup
+  int G, width, gpw;                      // gpw: groups per workgroup
 };
-
-// Sequence b's packed rows inside [0, T) and the position of its first.
-__device__ __forceinline__ void fill_seq(const FillArgs& a, int b, int& beg, int& len, int& start) {
-  const int c0 = a.cu[b], c1 = a.cu[b + 1];
-  beg = min(max(c0, 0), a.T);
-  len = min(max(c1, beg), a.T) - beg;
-  start = a.start ? a.start[b] : 0;
-  start = min(max(start, -(1 << 29)), 1 << 29);            // (farther is as far: at most 2^28 rows, 2^16 positions)
-}
 
 template <int LAYOUT>
 __global__ __launch_bounds__(256) void palu_fill_pages_kernel(const FillArgs a) {
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int cap_blocks = a.pt_stride << a.page_shift;
-  // this workgroup's block: number blockIdx.x of the batch
-  int beg = 0, len = 0, start = 0, blk = -1, b = 0;
-  int before = 0;
-  for (int b0 = 0; b0 < a.B; b0 += 64) {
-    int lb, ll, ls;
-    fill_seq(a, min(b0 + lane, a.B - 1), lb, ll, ls);
-    const int first = max(ls, 0) >> 5, end = min((ls + ll + 31) >> 5, cap_blocks);   // blocks first .. end - 1
-    const int n = b0 + lane < a.B && ll > 0 && end > first ? end - first : 0;
-    const int upto = before + wave_scan(n), want = (int)blockIdx.x;
-    const unsigned long long m = __ballot(want < upto);
-    if (m) {
-      const int l = __builtin_ctzll(m);
-      beg = __builtin_amdgcn_readlane(lb, l);
-      len = __builtin_amdgcn_readlane(ll, l);
-      start = __builtin_amdgcn_readlane(ls, l);
-      blk = __builtin_amdgcn_readlane(first, l) + want - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(n, l));
-      b = b0 + l;
-      break;
-    }
-    before = __builtin_amdgcn_readlane(upto, 63);
-  }
-  if (blk < 0) return;
-  const int pid = a.table[(long long)b * a.pt_stride + (blk >> a.page_shift)];
-  if (pid < 0 || pid >= a.n_pages) return;                // as the append: ids outside the pool are skipped
-  const int lo = max(start, 32 * blk), hi = min(start + len, 32 * blk + 32);   // the block's positions lo .. hi - 1
-  const int vec = a.width / 8, page = 32 << a.page_shift, g0 = blockIdx.y * a.gpw, g1 = min(a.G, g0 + a.gpw);
-  const int inpage = (blk & ((1 << a.page_shift) - 1)) * 32;
-  const __bf16* src = a.rows + (long long)(beg - start) * a.st;
-  __bf16* dst = a.cache + (long long)pid * a.G * page * a.width;
+  const int tid = threadIdx.x;
+  const PackedBlock p = packed_block(a.seqs, (int)blockIdx.x);   // this workgroup's block
+  if (p.b < 0 || p.pid < 0 || p.pid >= a.seqs.n_pages) return;   // as the append: ids outside the pool are skipped
+  const int blk = p.blk, lo = p.lo, hi = p.hi;
+  const int vec = a.width / 8, page = 32 << a.seqs.page_shift, g0 = blockIdx.y * a.gpw, g1 = min(a.G, g0 + a.gpw);
+  const int inpage = (blk & ((1 << a.seqs.page_shift) - 1)) * 32;
+  const __bf16* src = a.rows + (long long)p.row0 * a.st;
+  __bf16* dst = a.cache + (long long)p.pid * a.G * page * a.width;
   if constexpr (LAYOUT == PALU_LAYOUT_TILED_V) {
     // 8 positions x 8 columns a thread: eight 16-byte loads, regrouped, eight 16-byte slots
     for (int e = tid; e < (g1 - g0) * 4 * vec; e += 256) {
@@ -103,9 +70,9 @@ __global__ __launch_bounds__(256) void palu_fill_pages_kernel(const FillArgs a) 
         t = x / vec;
         v = x - t * vec;
       }
-      const int p = 32 * blk + t;
-      if (p < lo || p >= hi) continue;
-      const bf16x8 y = *reinterpret_cast<const bf16x8*>(src + (long long)p * a.st + g * a.sg + 8 * v);
+      const int pos = 32 * blk + t;
+      if (pos < lo || pos >= hi) continue;
+      const bf16x8 y = *reinterpret_cast<const bf16x8*>(src + (long long)pos * a.st + g * a.sg + 8 * v);
       __bf16* out = dst + (long long)g * page * a.width;
       if constexpr (LAYOUT == PALU_LAYOUT_TILED) store_k8(out, inpage + t, 8 * v, a.width, y);
       else *reinterpret_cast<bf16x8*>(out + (long long)(inpage + t) * a.width + 8 * v) = y;
@@ -455,9 +422,11 @@ extern "C" int palu_latent_fill_paged(void* cache_pages, const void* rows, long 
   if (int rc = palu::check_pages(page_table, num_pages, page_size, max_pages_per_seq, &shift, who)) return rc;
   if (n_rows <= 0 || batch <= 0 || n_groups <= 0)
     return fail(PALU_EINVAL, "%s: row, sequence and group counts must be positive, got %d, %d, %d", who, n_rows, batch, n_groups);
-  if (cache_layout != PALU_LAYOUT_ROWS && cache_layout != PALU_LAYOUT_TILED && cache_layout != PALU_LAYOUT_TILED_V)
-    return fail(PALU_EINVAL, "%s: cache layout must be PALU_LAYOUT_ROWS, _TILED or _TILED_V, got %d", who, cache_layout);
-  const int step = cache_layout == PALU_LAYOUT_ROWS ? 8 : 16;
+  const bool mx = is_mx(cache_layout);
+  if (!mx && cache_layout != PALU_LAYOUT_ROWS && cache_layout != PALU_LAYOUT_TILED && cache_layout != PALU_LAYOUT_TILED_V)
+    return fail(PALU_EINVAL, "%s: cache layout must be PALU_LAYOUT_ROWS, _TILED, _TILED_V or one of the MX layouts, got %d", who,
+                cache_layout);
+  const int step = mx ? 32 : cache_layout == PALU_LAYOUT_ROWS ? 8 : 16;
   if (width <= 0 || width % step || width > 512)
     return fail(PALU_EINVAL, "%s: width must be a multiple of %d up to 512, got %d", who, step, width);
   if (row_stride < 0 || row_stride % 8 || group_stride < 0 || group_stride % 8)
@@ -465,11 +434,13 @@ extern "C" int palu_latent_fill_paged(void* cache_pages, const void* rows, long 
                 group_stride);
   if (!al16(cache_pages) || !al16(rows)) return fail(PALU_EINVAL, "%s: 16-byte alignment required", who);
   if (n_rows > (1 << 28) || batch > 65535 || n_groups > 65535) return fail(PALU_EUNSUPPORTED, "%s: counts exceed the grid", who);
-  FillArgs a{static_cast<__bf16*>(cache_pages), static_cast<const __bf16*>(rows), row_stride, group_stride, cu_seqlens, start_pos,
-             page_table, n_rows, batch, n_groups, width, num_pages, shift, max_pages_per_seq, 0};
+  if (mx)
+    return mx_fill(cache_pages, rows, row_stride, group_stride, cu_seqlens, start_pos, page_table, n_rows, batch, n_groups,
+                   num_pages, shift, max_pages_per_seq, width, cache_layout, who, stream);
+  FillArgs a{{cu_seqlens, start_pos, page_table, n_rows, batch, num_pages, shift, max_pages_per_seq},
+             static_cast<__bf16*>(cache_pages), static_cast<const __bf16*>(rows), row_stride, group_stride, n_groups, width, 0};
   a.gpw = std::min(n_groups, std::max(1, 8192 / (32 * width)));   // 4 vectors of 8 a thread
-  // A sequence of n rows touches at most n / 32 + 2 blocks, and at most n.
-  const dim3 grid((unsigned)std::min<long long>(n_rows, n_rows / 32 + 2LL * batch), (unsigned)((n_groups + a.gpw - 1) / a.gpw));
+  const dim3 grid(packed_blocks(n_rows, batch), (unsigned)((n_groups + a.gpw - 1) / a.gpw));
   auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, stream, a); };
   if (cache_layout == PALU_LAYOUT_TILED) go(palu_fill_pages_kernel<PALU_LAYOUT_TILED>);
   else if (cache_layout == PALU_LAYOUT_TILED_V) go(palu_fill_pages_kernel<PALU_LAYOUT_TILED_V>);

@@ -22,8 +22,9 @@ SOURCES = ["palu_capi.hip", "palu_decode_rows.hip", "palu_decode_tiled.hip", "pa
            "palu_decode_tiled_paged.hip", "palu_decode_tiled_k16.hip", "palu_decode_tiled_paged_k16.hip",
            "palu_decode_full.hip", "palu_glrd.hip", "palu_glrd_narrow.hip", "palu_decoder.hip", "palu_linear.hip",
            "palu_linear_m16.hip", "palu_linear_m32.hip", "palu_prefill.hip", "palu_rows.hip", "palu_naive.hip",
-           "palu_flash_prefill.hip", "palu_pages.hip", "palu_score.hip"]
-HEADERS = ["palu_kernel.h", "palu_glrd_scores.h", "palu_linear_kernel.h"]
+           "palu_flash_prefill.hip", "palu_pages.hip", "palu_score.hip", "palu_mx_cache.hip",
+           "palu_step_mx.hip", "palu_step_bf16.hip"]
+HEADERS = ["palu_kernel.h", "palu_glrd_scores.h", "palu_linear_kernel.h", "palu_packed.h", "palu_mx.h", "palu_step.h"]
 # Per-file flags: the narrow-rank grouped-latent scores kernels keep their MFMA results in VGPRs.
 SOURCE_FLAGS = {"palu_glrd_narrow.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 

@@ -16,8 +16,9 @@ from palu_tt._build import library_path
 PALU_OK, PALU_EINVAL, PALU_EUNSUPPORTED, PALU_EHIP = 0, 1, 2, 3
 DTYPE_F32, DTYPE_BF16 = 0, 1
 OUT_TILED_ROWS = 0x100      # PALU_OUT_TILED_ROWS, OR'ed into palu_sdpa_decode's out_dtype
-ABI_VERSION = 17
+ABI_VERSION = 18
 LAYOUT_ROWS, LAYOUT_TILED, LAYOUT_TILED_V, LAYOUT_TILED_GROUPED = 0, 1, 2, 3
+LAYOUT_MX8, LAYOUT_MX8_V, LAYOUT_MX4, LAYOUT_MX4_V = 4, 5, 6, 7
 
 _vp, _i, _f, _sz, _ll = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_size_t, ctypes.c_longlong
 
@@ -68,6 +69,11 @@ _SIGNATURES = {
                                       _vp, _sz, _vp]),
     "palu_flash_prefill_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i]),
     "palu_latent_fill_paged": (_i, [_vp, _vp, _ll, _ll, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _vp]),
+    "palu_latent_read_paged": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _vp]),
+    "palu_mx_decode_workspace_bytes": (_sz, [_i, _i, _i, _i]),
+    "palu_flash_decode_shared": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _f, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _vp,
+                                      _sz, _vp]),
+    "palu_flash_decode_shared_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
     "palu_pages_update": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _sz, _vp]),
     "palu_pages_compact": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _sz, _vp]),
     "palu_pages_workspace_bytes": (_sz, [_i, _i]),

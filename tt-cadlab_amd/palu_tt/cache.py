@@ -197,3 +197,139 @@ class GroupedLatentCache:
 
     def nbytes(self) -> int:
         return self.data.numel() * self.data.element_size()
+
+
+MX_FORMATS = ("fp8", "fp4")
+# per format: the largest element, the largest value that is held as it, the mantissa's bits, the lowest exponent
+_MX = {"fp8": (448.0, 464.0, 3, -6), "fp4": (6.0, 7.0, 1, 0)}
+_MX_LEAST, _MX_LARGEST = -117, 1.75 * 2.0 ** 127
+
+
+def _pow2(e: torch.Tensor) -> torch.Tensor:
+    """2^e, exact, of integers in -126 .. 127."""
+    return ((e.int() + 127) << 23).view(torch.float32)
+
+
+def mx_values(fmt: str, device=None) -> torch.Tensor:
+    """The value of every code of a format (fp8: 256, fp4: 16), fp32."""
+    bits, low = _MX[fmt][2:]
+    code = torch.arange(256 if fmt == "fp8" else 16, device=device)
+    mag = code % (128 if fmt == "fp8" else 8)
+    e, m = mag >> bits, mag % (1 << bits)
+    v = torch.where(e > 0, (1 + m * 2.0 ** -bits) * 2.0 ** (e + low - 1), m * 2.0 ** (low - bits))
+    if fmt == "fp8":
+        v = torch.where(mag == 127, float("nan"), v)
+    return torch.where(code != mag, -v, v).float()
+
+
+def mx_quantize(rows: torch.Tensor, fmt: str) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(codes [.., w], scale bytes [.., w / 32]) of rows [.., w], uint8: what the ops that write an MXCache hold them as."""
+    most, held, bits, low = _MX[fmt]
+    x = rows.float().unflatten(-1, (-1, 32))
+    top = x.abs().amax(-1, keepdim=True)
+    good = torch.isfinite(top)
+    x, top = x.clamp(-_MX_LARGEST, _MX_LARGEST), torch.where(good, top, 0).clamp(max=_MX_LARGEST)
+    m, e = torch.frexp(top / held)                     # the smallest power of two that is not below top / held
+    e = torch.where(top == 0, _MX_LEAST, torch.where(m == 0.5, e - 1, e)).clamp(min=_MX_LEAST)
+    y = torch.where(good, x * _pow2(-e), 0.0)
+    step = _pow2((torch.frexp(y)[1] - 1).clamp(min=low) - bits)
+    v = (torch.round(y / step) * step).clamp(-most, most)
+    grid = mx_values(fmt, rows.device)[:127 if fmt == "fp8" else 8].contiguous()
+    codes = torch.searchsorted(grid, v.abs().contiguous()) + (128 if fmt == "fp8" else 8) * torch.signbit(v)
+    codes = torch.where(good, codes, 0)
+    return codes.flatten(-2).to(torch.uint8), torch.where(good, e + 127, 255)[..., 0].to(torch.uint8)
+
+
+def mx_dequantize(codes: torch.Tensor, scales: torch.Tensor, fmt: str) -> torch.Tensor:
+    """The values of codes [.., w] under their scale bytes [.., w / 32], bf16 (exact)."""
+    s = torch.where(scales == 255, float("nan"), _pow2(scales.int().clamp(1, 254) - 127))
+    v = mx_values(fmt, codes.device)[codes.int()].unflatten(-1, (-1, 32)) * s[..., None]
+    return v.flatten(-2).to(torch.bfloat16)
+
+
+@dataclass
+class MXCache:
+    """A K ("k") or V ("v") cache of logical shape [B, n_groups, max_seq, width], held in 8 or 4 bits: 32 neighbouring channels of
+    a position share a power of two as their scale (one byte, 2^(byte - 127); 255: NaN) and are fp8 (e4m3) or fp4 (e2m1)
+    elements. As a page pool its first two dimensions are [n_pages, n_groups] and max_seq is the page size. The reference
+    keeps its latents in bf16 or a shared-exponent type of its device.
+
+    The scale is the smallest power of two (from 2^-117 on) over which the 32 values are at most 464 (fp8; fp4: 7) and each is
+    rounded to the nearest element, ties to the even code: off by up to 2^-4 of itself in fp8 (2^-10 of the scale where that is
+    more), by up to a quarter of itself in fp4 (a quarter of the scale). Read back they are exact in bf16. A block with
+    an infinity or NaN reads back as NaN.
+
+    ``data`` is uint8 [B, n_groups, max_seq / 32, bytes of a block]: a 32-position block's elements in the operand order of the
+    attention's products, then its scales (33 * width bytes in fp8, 17 * width in fp4; the order stands at PALU_LAYOUT_MX8
+    in include/palu_mi355x.h, and ``from_rows`` / ``to_rows`` follow it). Zeroed memory is a cache of zeros. Written by
+    fused.paged_fill_cache and paged_update_cache, read by flash_decode, flash_decode_shared and paged_read_cache."""
+    data: torch.Tensor
+    role: str
+    fmt: str
+    width: int
+
+    def __post_init__(self):
+        assert self.role in ROLES, f"role must be 'k' or 'v', got {self.role!r}"
+        assert self.fmt in MX_FORMATS, f"fmt must be one of {MX_FORMATS}, got {self.fmt!r}"
+        assert self.width > 0 and self.width % 32 == 0, f"the width must be a multiple of 32, got {self.width}"
+        size = self.block_bytes(self.fmt, self.width)
+        assert self.data.dim() == 4 and self.data.dtype == torch.uint8 and self.data.shape[3] == size, \
+            f"data must be uint8 [B, n_groups, max_seq / 32, {size}], got {self.data.dtype} {tuple(self.data.shape)}"
+
+    @staticmethod
+    def block_bytes(fmt: str, width: int) -> int:
+        return (33 if fmt == "fp8" else 17) * width
+
+    @staticmethod
+    def zeros(batch: int, n_groups: int, max_seq: int, width: int, device, role: str = "k", fmt: str = "fp8") -> "MXCache":
+        assert max_seq % BLOCK == 0, f"max_seq must be a multiple of {BLOCK}, got {max_seq}"
+        return MXCache(torch.zeros(batch, n_groups, max_seq // BLOCK, MXCache.block_bytes(fmt, width), dtype=torch.uint8,
+                                   device=device), role, fmt, width)
+
+    @staticmethod
+    def from_rows(rows: torch.Tensor, role: str = "k", fmt: str = "fp8") -> "MXCache":
+        """Quantises rows [B, n_groups, max_seq, width]."""
+        B, G, S, w = rows.shape
+        assert S % BLOCK == 0, f"max_seq must be a multiple of {BLOCK}, got {S}"
+        codes, scales = mx_quantize(rows, fmt)
+        if fmt == "fp4":
+            codes = codes[..., 0::2] | (codes[..., 1::2] << 4)
+        nblk, nb = S // BLOCK, w // 32
+        if role == "k":
+            x = codes.reshape(B, G, nblk, 4, 2, 4, nb, -1, 16).permute(0, 1, 2, 4, 7, 6, 3, 5, 8)
+            s = scales.reshape(B, G, nblk, 4, 2, 4, nb).permute(0, 1, 2, 6, 3, 5, 4)
+        else:
+            x = codes.reshape(B, G, nblk, 4, 8, nb, 16, -1).permute(0, 1, 2, 5, 3, 6, 4, 7)
+            s = scales.reshape(B, G, nblk, BLOCK, nb).transpose(3, 4)
+        return MXCache(torch.cat([x.reshape(B, G, nblk, -1), s.reshape(B, G, nblk, -1)], -1).contiguous(), role, fmt, w)
+
+    def parts(self) -> Tuple[torch.Tensor, torch.Tensor]:
+        """(codes [B, n_groups, max_seq, width], scale bytes [B, n_groups, max_seq, width / 32]), uint8."""
+        B, G, S, w = self.shape
+        nblk, nb, size = S // BLOCK, w // 32, (32 if self.fmt == "fp8" else 16) * w
+        x, s = self.data[..., :size], self.data[..., size:]
+        if self.role == "k":
+            x = x.reshape(B, G, nblk, 2, -1, nb, 4, 4, 16).permute(0, 1, 2, 6, 3, 7, 5, 4, 8)
+            s = s.reshape(B, G, nblk, nb, 4, 4, 2).permute(0, 1, 2, 4, 6, 5, 3)
+        else:
+            x = x.reshape(B, G, nblk, nb, 4, 16, 8, -1).permute(0, 1, 2, 4, 6, 3, 5, 7)
+            s = s.reshape(B, G, nblk, nb, BLOCK).transpose(3, 4)
+        x = x.reshape(B, G, S, -1)
+        if self.fmt == "fp4":
+            x = torch.stack([x & 15, x >> 4], -1).flatten(-2)
+        return x, s.reshape(B, G, S, nb)
+
+    def to_rows(self) -> torch.Tensor:
+        return mx_dequantize(*self.parts(), self.fmt)
+
+    @property
+    def shape(self) -> Tuple[int, int, int, int]:
+        B, G, nblk = self.data.shape[:3]
+        return (B, G, nblk * BLOCK, self.width)
+
+    @property
+    def device(self):
+        return self.data.device
+
+    def nbytes(self) -> int:
+        return self.data.numel()

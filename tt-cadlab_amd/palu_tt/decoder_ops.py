@@ -12,7 +12,7 @@ from typing import Optional
 import torch
 
 from palu_tt import _native
-from palu_tt.cache import GroupedLatentCache, LatentCache
+from palu_tt.cache import GroupedLatentCache, LatentCache, MXCache
 
 
 def _check(t: torch.Tensor, name: str, dtype=torch.bfloat16) -> None:
@@ -25,6 +25,12 @@ def aligned(t: torch.Tensor) -> torch.Tensor:
     (a view into another tensor)."""
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _refuse_mx(*caches) -> None:
+    """The fused decoder-step ops write bf16 caches."""
+    if any(isinstance(c, MXCache) for c in caches):
+        raise RuntimeError("an MXCache is written by fused.paged_fill_cache and paged_update_cache")
 
 
 def rmsnorm(x: torch.Tensor, weight: torch.Tensor, eps: float, res: Optional[torch.Tensor] = None,
@@ -150,6 +156,7 @@ def append_from(cache, src: torch.Tensor, group_stride: int, width: int, pos: to
     """cache[b, g, pos[b], :] = src[b, g * group_stride : g * group_stride + width] for a row-strided
     src [B, >= ...] (the latent columns of the QKV output). cache: LatentCache (tiled), a row-major
     [B, G, S, width] bf16 tensor, or a GroupedLatentCache (each group takes its first ranks[g] columns)."""
+    _refuse_mx(cache)
     _check(src, "src")
     if src.dim() != 2 or src.stride(1) != 1:
         raise RuntimeError("src must be a row-strided [rows, width] view")
@@ -186,6 +193,7 @@ def fill_from(cache, user: int, src: torch.Tensor, users: int, n_pos: int, col: 
     row-strided src [users * n_pos, ...] (the QKV projection's rows), positions past n_pos untouched. cache: LatentCache,
     a row-major [B, G, S, width] bf16 tensor or a GroupedLatentCache (each group its first ranks[g] columns). With cos /
     sin (fp32 [>= n_pos, 128]) the 128-wide rows are rotated at their positions first."""
+    _refuse_mx(cache)
     _check(src, "src")
     if src.dim() != 2 or src.stride(1) != 1 or src.shape[0] != users * n_pos:
         raise RuntimeError(f"src must be a row-strided [{users * n_pos}, columns] view")
@@ -439,6 +447,7 @@ def linear_residual(x: torch.Tensor, w_tiled: torch.Tensor, rtw: int, h: torch.T
 
 def _cache_args(cache):
     """(storage, layout, [B, G, S, width]) of a latent cache: LatentCache (tiled) or a row-major tensor."""
+    _refuse_mx(cache)
     if isinstance(cache, LatentCache):
         layout = _native.LAYOUT_TILED if cache.role == "k" else _native.LAYOUT_TILED_V
         return cache.data, layout, cache.shape

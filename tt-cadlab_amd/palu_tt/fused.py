@@ -29,7 +29,7 @@ from typing import Optional, Tuple
 import torch
 
 from palu_tt import _native, decoder_ops
-from palu_tt.cache import GroupedLatentCache, LatentCache
+from palu_tt.cache import GroupedLatentCache, LatentCache, MXCache
 
 MAX_CHUNK = 512          # the reference's cap on the static K chunk (ttnn sdpa_decode)
 HEAD_DIM = 128
@@ -166,9 +166,18 @@ def _as_dev(t: torch.Tensor, name: str, dtype=None, device=None) -> torch.Tensor
     return t
 
 
-def _cache_arg(t, name: str, device, role: Optional[str] = None):
-    """(storage tensor, logical shape, layout id) of a row-major tensor or a LatentCache; a tiled cache
-    passed where the op reads K (role "k") or V (role "v") must be stored in that role's tile order."""
+def _cache_arg(t, name: str, device, role: Optional[str] = None, mx: bool = False):
+    """(storage tensor, logical shape, layout id) of a row-major tensor, a LatentCache or, with mx, an MXCache; a tiled or
+    quantised cache passed where the op reads K (role "k") or V (role "v") must be stored in that role's order."""
+    if isinstance(t, MXCache):
+        if not mx:
+            raise RuntimeError(f"{name} is an MXCache, which this op does not read or write (flash_decode, flash_decode_shared, "
+                               "paged_fill_cache, paged_update_cache and paged_read_cache do)")
+        _as_dev(t.data, name, torch.uint8, device)
+        if not (role is None or t.role == role):
+            raise RuntimeError(f"{name} is an MXCache in {t.role!r} order; this argument reads a {role!r} cache")
+        layout = _native.LAYOUT_MX8 if t.fmt == "fp8" else _native.LAYOUT_MX4
+        return t.data, tuple(t.shape), layout + (1 if role is None and t.role == "v" else 0)
     if isinstance(t, GroupedLatentCache):
         _as_dev(t.data, name, torch.bfloat16, device)
         if not (role is not None and t.role == role):
@@ -385,13 +394,14 @@ def flash_decode(q, k, v, cur_pos_tensor, *, scale=None, head_dim_v=None, out_dt
     MI355X counterpart of ttnn.transformer.scaled_dot_product_attention_decode (head_dim_v 128) and
     flash_multi_latent_attention_decode (head_dim_v = V width). Returns [1, B, n_q, head_dim_v].
     With page_table_tensor, k and v are page pools [n_pages, n_kv, page_size, width] (ttnn's
-    paged_scaled_dot_product_attention_decode)."""
+    paged_scaled_dot_product_attention_decode). k and v may both be MXCache of one format (head_dim_v multiples of 32; calls are
+    then bit-identical with or without deterministic, and a workspace is of palu_mx_decode_workspace_bytes bytes)."""
     if not (isinstance(q, torch.Tensor) and q.dim() == 4 and q.shape[0] == 1 and q.shape[3] == HEAD_DIM):
         raise RuntimeError(f"q must be [1, B, n_q, {HEAD_DIM}]")
     dev = q.device
     _as_dev(q, "q", torch.bfloat16)
-    k_store, k_shape, layout = _cache_arg(k, "k", dev, "k")
-    v_store, v_shape, v_layout = _cache_arg(v, "v", dev, "v")
+    k_store, k_shape, layout = _cache_arg(k, "k", dev, "k", mx=True)
+    v_store, v_shape, v_layout = _cache_arg(v, "v", dev, "v", mx=True)
     if layout != v_layout:
         raise RuntimeError("k and v must use the same cache layout")
     B, n_kv, S, hd, v_width, pt, page_size, n_pages = _pool_dims(k_shape, v_shape, q, page_table_tensor, dev, "n_kv")
@@ -406,6 +416,9 @@ def flash_decode(q, k, v, cur_pos_tensor, *, scale=None, head_dim_v=None, out_dt
     if out_dtype not in _DTYPES:
         raise RuntimeError(f"out_dtype must be torch.float32 or torch.bfloat16, got {out_dtype}")
     cp = _cur_pos(cur_pos_tensor, B, dev)
+    if layout in (_native.LAYOUT_MX8, _native.LAYOUT_MX4):
+        return _mx_decode(q, k_store, v_store, cp, pt, out, workspace, scale, n_kv, S if pt is None else page_size, n_pages, width,
+                          out_dtype, layout)
     if out is None:
         out = torch.empty(1, B, n_q, width, dtype=out_dtype, device=dev)
     ws, ws_bytes = _workspace(B, n_kv, S, width, dev, workspace)
@@ -421,6 +434,87 @@ def flash_decode(q, k, v, cur_pos_tensor, *, scale=None, head_dim_v=None, out_dt
             _native.ptr(q), _native.ptr(k_store), _native.ptr(v_store), _native.ptr(cp), _native.ptr(pt),
             _native.ptr(out), sc, B, n_q, n_kv, n_pages, page_size, pt.shape[1], width, _DTYPES[out_dtype], layout,
             int(bool(deterministic)), _native.ptr(ws), ws_bytes, _native.stream_handle(dev)))
+    return out
+
+
+def _step_out(q, n_kv: int, width: int, out_dtype, out, workspace, need: int, inputs):
+    """(out, workspace) of a decode over packed or quantised pools: out checked or made, the workspace checked or made."""
+    _, B, n_q, _ = q.shape
+    dev = q.device
+    _native.refuse_derivatives("flash_decode over these caches", q, *(t for t in inputs if t.is_floating_point()))
+    if out_dtype not in _DTYPES:
+        raise RuntimeError(f"out_dtype must be torch.float32 or torch.bfloat16, got {out_dtype}")
+    made = workspace is None
+    if made:
+        workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
+    else:
+        _native.workspace_bytes(workspace, need, dev)
+    if out is None:
+        return torch.empty(1, B, n_q, width, dtype=out_dtype, device=dev), workspace
+    _as_dev(out, "out", out_dtype, dev)
+    if tuple(out.shape) != (1, B, n_q, width):
+        raise RuntimeError(f"out must be [1, {B}, {n_q}, {width}]")
+    if any(_overlap(out, t) for t in (q, *inputs) + (() if made else (workspace,))):
+        raise RuntimeError("out must be memory of its own: it overlaps an input or the workspace")
+    return out, workspace
+
+
+def _mx_decode(q, k, v, cp, pt, out, workspace, scale, n_kv, positions, n_pages, width, out_dtype, layout):
+    """flash_decode over the storages k, v of an MXCache pair."""
+    _, B, n_q, _ = q.shape
+    need = _native.load().palu_mx_decode_workspace_bytes(B, n_q, n_kv, width)
+    out, ws = _step_out(q, n_kv, width, out_dtype, out, workspace, need, [t for t in (k, v, cp, pt) if t is not None])
+    sc = float(HEAD_DIM ** -0.5 if scale is None else scale)
+    if pt is None:
+        _native.launch("flash_decode", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), cp.data_ptr(), out.data_ptr(), sc, B, n_q,
+                       n_kv, positions, width, _DTYPES[out_dtype], layout, 1, ws.data_ptr(), need)
+    else:
+        _native.launch("flash_decode_paged", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), cp.data_ptr(), pt.data_ptr(),
+                       out.data_ptr(), sc, B, n_q, n_kv, n_pages, positions, pt.shape[1], width, _DTYPES[out_dtype], layout, 1,
+                       ws.data_ptr(), need)
+    return out
+
+
+def flash_decode_shared(q, k, v, cur_pos_tensor, page_table_tensor, shared_len, cu_groups=None, *, scale=None, head_dim_v=None,
+                        out_dtype=torch.bfloat16, out=None, workspace=None) -> torch.Tensor:
+    """flash_decode over page pools for a batch in which neighbouring rows share a prefix (samples of one prompt, beams, one
+    system prompt in front of all): rows cu_groups[i] .. cu_groups[i + 1] - 1 (int32 [n + 1] on the device; None: all rows are
+    one group) share their first shared_len[i] positions (int32 [n] on the device). The prefix's whole 32-position blocks are read
+    through the page table of the group's first row, once for all rows of the group that see them all; what is behind them
+    through each row's own, whose entries before that are not looked at. Rows of no group stand alone. q, cur_pos_tensor,
+    the pools (row-major tensors, LatentCache or MXCache pairs) and the result as for flash_decode; head_dim_v multiples of 16 (of
+    32 for MXCache). At most 4096 rows. Repeated calls are bit-identical. out must not overlap the inputs; workspace: uint8, of
+    palu_flash_decode_shared_workspace_bytes bytes, not shared between calls that may overlap. Forward only."""
+    if not (isinstance(q, torch.Tensor) and q.dim() == 4 and q.shape[0] == 1 and q.shape[3] == HEAD_DIM):
+        raise RuntimeError(f"q must be [1, B, n_q, {HEAD_DIM}]")
+    dev = q.device
+    _as_dev(q, "q", torch.bfloat16)
+    k_store, k_shape, layout = _cache_arg(k, "k", dev, "k", mx=True)
+    v_store, v_shape, v_layout = _cache_arg(v, "v", dev, "v", mx=True)
+    if layout != v_layout or layout == _native.LAYOUT_TILED_GROUPED:
+        raise RuntimeError("k and v must use the same cache layout (row-major, LatentCache or MXCache pools)")
+    if page_table_tensor is None:
+        raise RuntimeError("page_table_tensor must be [B, max_pages_per_seq] int32")
+    B, n_kv, _, hd, width, pt, page_size, n_pages = _pool_dims(k_shape, v_shape, q, page_table_tensor, dev, "n_kv")
+    if hd != HEAD_DIM:
+        raise RuntimeError(f"k must be [n_pages, n_kv, page_size, {HEAD_DIM}], got {k_shape}")
+    if head_dim_v is not None and int(head_dim_v) != width:
+        raise RuntimeError(f"head_dim_v {head_dim_v} != V width {width}")
+    cp = _cur_pos(cur_pos_tensor, B, dev)
+    cu = None if cu_groups is None else _seq_ints(cu_groups, "cu_groups", None, dev)
+    n = 1 if cu is None else cu.numel() - 1
+    if n < 1:
+        raise RuntimeError("cu_groups must hold at least one group")
+    shared = _seq_ints(shared_len, "shared_len", n, dev)
+    n_q = q.shape[2]
+    need = _native.load().palu_flash_decode_shared_workspace_bytes(B, n, n_q, n_kv, width)
+    out, ws = _step_out(q, n_kv, width, out_dtype, out, workspace, need,
+                        [t for t in (k_store, v_store, cp, pt, cu, shared) if t is not None])
+    if B == 0:
+        return out
+    _native.launch("flash_decode_shared", dev, q.data_ptr(), k_store.data_ptr(), v_store.data_ptr(), cp.data_ptr(), pt.data_ptr(),
+                   _native.ptr(cu), shared.data_ptr(), out.data_ptr(), float(HEAD_DIM ** -0.5 if scale is None else scale), B, n,
+                   n_q, n_kv, n_pages, page_size, pt.shape[1], width, _DTYPES[out_dtype], layout, ws.data_ptr(), need)
     return out
 
 
@@ -581,15 +675,15 @@ def flash_prefill(q, k, v, cu_seqlens, *, scale=None, head_dim_v=None, out=None,
 def paged_fill_cache(cache, rows: torch.Tensor, cu_seqlens, page_table, start_pos=None) -> None:
     """The rows of packed sequences into a page pool (paged_update_cache for whole prompts): row i of sequence b, rows
     [T, n_groups, width] bf16 (a strided view such as columns of a projection), goes to position start_pos[b] + i (int32 [B];
-    None: i) of its pages, page_table[b, position // page_size]. ``cache`` is a [n_pages, n_groups, page_size, width] tensor or a
-    LatentCache pool. Positions outside the table and page ids outside the pool are skipped; the rest of the pool
+    None: i) of its pages, page_table[b, position // page_size]. ``cache`` is a [n_pages, n_groups, page_size, width] tensor, a
+    LatentCache or an MXCache pool (rows are quantised as they are written). Positions outside the table and page ids outside the pool are skipped; the rest of the pool
     keeps what it holds. Sequences of one call must not share the pages that they write. Forward only: rows or a cache that a
     derivative would go through are refused."""
     if isinstance(cache, GroupedLatentCache):
         raise RuntimeError("a GroupedLatentCache is contiguous")
     st, sg = _strided_rows(rows, "rows", None)
     dev = rows.device
-    store, (n_pages, G, page_size, width), layout = _cache_arg(cache, "cache", dev)
+    store, (n_pages, G, page_size, width), layout = _cache_arg(cache, "cache", dev, mx=True)
     _native.refuse_derivatives("paged_fill_cache", rows, store)
     if tuple(rows.shape[1:]) != (G, width):
         raise RuntimeError(f"rows must be [T, {G}, {width}] for this cache, got {tuple(rows.shape)}")
@@ -603,6 +697,41 @@ def paged_fill_cache(cache, rows: torch.Tensor, cu_seqlens, page_table, start_po
         return
     _native.launch("latent_fill_paged", dev, store.data_ptr(), rows.data_ptr(), st, sg, cu.data_ptr(), _native.ptr(start),
                    pt.data_ptr(), rows.shape[0], B, G, n_pages, page_size, pt.shape[1], width, layout)
+
+
+def paged_read_cache(cache, n_rows: int, cu_seqlens, page_table, start_pos=None, *, out=None) -> torch.Tensor:
+    """The rows of packed sequences out of a page pool, paged_fill_cache the other way: [n_rows, n_groups, width] bf16, row i of
+    sequence b from position start_pos[b] + i of its pages (cu_seqlens int32 [B + 1] on the device, start_pos int32 [B]; None:
+    i). ``cache`` is a [n_pages, n_groups, page_size, width] tensor, a LatentCache or an MXCache pool (whose values are exact in
+    bf16). Positions outside the table and page ids outside the pool give zeros; rows past cu_seqlens[B] are not written
+    (``out``, contiguous and not overlapping the inputs, keeps what it held there). Forward only."""
+    if isinstance(cache, GroupedLatentCache):
+        raise RuntimeError("a GroupedLatentCache is contiguous")
+    dev = getattr(cache, "device", None)
+    store, (n_pages, G, page_size, width), layout = _cache_arg(cache, "cache", dev, mx=True)
+    if store.is_floating_point():
+        _native.refuse_derivatives("paged_read_cache", store)
+    cu = _seq_ints(cu_seqlens, "cu_seqlens", None, dev)
+    B = cu.numel() - 1
+    if B < 1:
+        raise RuntimeError("cu_seqlens must hold at least one sequence")
+    pt = _page_table(page_table, B, dev)
+    start = None if start_pos is None else _seq_ints(start_pos, "start_pos", B, dev)
+    n_rows = int(n_rows)
+    if n_rows < 0:
+        raise RuntimeError(f"n_rows must not be negative, got {n_rows}")
+    if out is None:
+        out = torch.empty(n_rows, G, width, dtype=torch.bfloat16, device=dev)
+    else:
+        _as_dev(out, "out", torch.bfloat16, dev)
+        if tuple(out.shape) != (n_rows, G, width):
+            raise RuntimeError(f"out must be [{n_rows}, {G}, {width}]")
+        if any(t is not None and _overlap(out, t) for t in (store, cu, pt, start)):
+            raise RuntimeError("out must be memory of its own: it overlaps an input")
+    if n_rows:
+        _native.launch("latent_read_paged", dev, store.data_ptr(), out.data_ptr(), cu.data_ptr(), _native.ptr(start), pt.data_ptr(),
+                       n_rows, B, G, n_pages, page_size, pt.shape[1], width, layout)
+    return out
 
 
 def scaled_dot_product_attention_decode(q, k, v, cur_pos_tensor, scale=None, **_):
@@ -623,7 +752,7 @@ def paged_scaled_dot_product_attention_decode(q, k, v, cur_pos_tensor, page_tabl
 def paged_update_cache(cache, new_rows: torch.Tensor, update_idxs_tensor: torch.Tensor, page_table=None) -> None:
     """Latent append (ttnn.experimental.paged_update_cache on a latent cache, attention.py:622-623):
     cache[b, g, update_idxs[b], :] = new_rows[..., b, g, :] for every b with 0 <= idx < S. ``cache`` is a
-    [B, G, S, width] bf16 tensor or a LatentCache. With ``page_table`` [B, max_pages] int32 the cache is a
+    [B, G, S, width] bf16 tensor, a LatentCache or an MXCache (the rows are quantised as they are written). With ``page_table`` [B, max_pages] int32 the cache is a
     page pool [n_pages, G, page_size, width] and row b goes to page page_table[b, idx // page_size]."""
     dev = cache.device
     if isinstance(cache, GroupedLatentCache):
@@ -632,20 +761,20 @@ def paged_update_cache(cache, new_rows: torch.Tensor, update_idxs_tensor: torch.
         B, G, S, width = cache.shape
         decoder_ops.append_from(cache, new_rows.reshape(B, G * width), width, width, update_idxs_tensor)
         return
-    store, (N, G, S, width), layout = _cache_arg(cache, "cache", dev)
-    lib = _native.load()
+    store, (N, G, S, width), layout = _cache_arg(cache, "cache", dev, mx=True)
+    if isinstance(cache, MXCache):
+        _native.refuse_derivatives("paged_update_cache of an MXCache", new_rows)
     if page_table is None:
         B = N
         rows = new_rows.reshape(B, G, width)
         _as_dev(rows, "new_rows", torch.bfloat16, dev)
         cp = _cur_pos(update_idxs_tensor, B, dev)
-        _native.check(lib.palu_latent_append(_native.ptr(store), _native.ptr(rows), _native.ptr(cp), B, G, S, width,
-                                             layout, _native.stream_handle(dev)))
+        _native.launch("latent_append", dev, _native.ptr(store), _native.ptr(rows), _native.ptr(cp), B, G, S, width, layout)
         return
     B = update_idxs_tensor.numel()
     rows = new_rows.reshape(B, G, width)
     _as_dev(rows, "new_rows", torch.bfloat16, dev)
     cp = _cur_pos(update_idxs_tensor, B, dev)
     pt = _page_table(page_table, B, dev)
-    _native.check(lib.palu_latent_append_paged(_native.ptr(store), _native.ptr(rows), _native.ptr(cp), _native.ptr(pt),
-                                               B, G, N, S, pt.shape[1], width, layout, _native.stream_handle(dev)))
+    _native.launch("latent_append_paged", dev, _native.ptr(store), _native.ptr(rows), _native.ptr(cp), _native.ptr(pt), B, G, N, S,
+                   pt.shape[1], width, layout)

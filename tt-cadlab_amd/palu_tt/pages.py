@@ -1,6 +1,7 @@
 """The page table of a server over paged caches: rows forked, ended, cut and grown, pools compacted.
 
-The paged ops (fused.palu_sdpa_decode, flash_decode, flash_prefill, paged_update_cache, paged_fill_cache) read a page table
+The paged ops (fused.palu_sdpa_decode, flash_decode, flash_decode_shared, flash_prefill, paged_update_cache,
+paged_fill_cache, paged_read_cache) read a page table
 [B, max_pages] int32 and page pools [n_pages, n_groups, page_size, width], one table for the K and V pools of all layers.
 ``PagePools`` holds the pools of a server and changes the table, with the copies of pages in all pools that this asks for, on
 the device and without a synchronisation. The reference has no counterpart (its caches are contiguous).
@@ -15,7 +16,7 @@ from typing import Optional, Sequence, Tuple
 import torch
 
 from palu_tt import _native
-from palu_tt.cache import LatentCache
+from palu_tt.cache import LatentCache, MXCache
 
 
 def _ints(t, name: str, shape, device) -> torch.Tensor:
@@ -33,8 +34,8 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
 
 
 class PagePools:
-    """The page pools that share a page table: row-major [n_pages, n_groups, page_size, width] bf16 tensors or LatentCache
-    pools (of any group counts and widths)."""
+    """The page pools that share a page table: row-major [n_pages, n_groups, page_size, width] bf16 tensors, LatentCache
+    or MXCache pools (of any group counts and widths)."""
 
     def __init__(self, pools: Sequence):
         if not pools:
@@ -52,12 +53,13 @@ class PagePools:
 
     def _take(self) -> None:
         """Checks the pools as they are now and takes their storage, which is held for as long as its address is."""
-        stores = [p.data if isinstance(p, LatentCache) else p for p in self.pools]
+        stores = [p.data if isinstance(p, (LatentCache, MXCache)) else p for p in self.pools]
         for p, s in zip(self.pools, stores):
-            if not (isinstance(s, torch.Tensor) and len(p.shape) == 4 and s.is_cuda and s.dtype == torch.bfloat16 and
-                    s.is_contiguous() and s.data_ptr() % 16 == 0 and s.numel()):
+            dtype = torch.uint8 if isinstance(p, MXCache) else torch.bfloat16
+            if not (isinstance(s, torch.Tensor) and len(p.shape) == 4 and s.is_cuda and s.dtype == dtype and s.is_contiguous() and
+                    s.data_ptr() % 16 == 0 and s.numel()):
                 raise RuntimeError("a pool is a contiguous, 16-byte aligned bf16 [n_pages, n_groups, page_size, width] tensor, "
-                                   "not empty, on the GPU or a LatentCache")
+                                   "not empty, on the GPU, a LatentCache or an MXCache")
             if (p.shape[0], p.shape[2], s.device) != (self.pools[0].shape[0], self.pools[0].shape[2], stores[0].device):
                 raise RuntimeError("pools must agree in pages, page size and device: "
                                    f"{tuple(p.shape)}, {tuple(self.pools[0].shape)}")
@@ -67,8 +69,8 @@ class PagePools:
         self.device = stores[0].device
         n = len(stores)
         self._ptrs = (ctypes.c_void_p * n)(*[s.data_ptr() for s in stores])
-        self._bytes = (ctypes.c_longlong * n)(*[s.numel() * 2 // self.n_pages for s in stores])
-        self._seen = [(p if isinstance(p, LatentCache) else None, s, s.data_ptr(), s.numel()) for p, s in zip(self.pools, stores)]
+        self._bytes = (ctypes.c_longlong * n)(*[s.numel() * s.element_size() // self.n_pages for s in stores])
+        self._seen = [(p if isinstance(p, (LatentCache, MXCache)) else None, s, s.data_ptr(), s.numel()) for p, s in zip(self.pools, stores)]
         self._stores = stores
 
     def _args(self, page_table, lengths):

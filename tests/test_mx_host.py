@@ -215,7 +215,7 @@ def test_workspaces(lib):
     """Per part of a split item its query heads' results and statistics and a flag; the prefixes' pieces behind them."""
     f, s = lib.palu_mx_decode_workspace_bytes, lib.palu_flash_decode_shared_workspace_bytes
     assert f(0, 8, 2, 64) == f(1, 7, 2, 64) == f(1, 34, 2, 64) == f(1, 8, 2, 40) == f(40000, 8, 2, 64) == 0
-    assert f(1, 8, 2, 64) == 1024 * (4 * 66 * 4 + 8) and f(1000, 8, 2, 128) == 2512 * (4 * 130 * 4 + 8)
+    assert f(1, 8, 2, 64) == 514 * (4 * 66 * 4 + 8) and f(1000, 8, 2, 128) == 2512 * (4 * 130 * 4 + 8)
     assert s(4, 0, 8, 2, 64) == 0 and s(4, 1, 8, 2, 64) > f(4, 8, 2, 64)
     assert all(s(b, g, 32, 8, 128) > 0 for b in (1, 64, 4096) for g in (1, 7, 4096))
 

@@ -62,52 +62,109 @@ int step_bf16(const StepArgs& a, int layout, const char* who, hipStream_t s);   
 namespace {
 
 // ---- blocks --------------------------------------------------------------------------------------
-// The registers of a block as it is loaded: K, V of NB blocks of 32 channels.
+// A block on its way: copied to LDS as it lies (row-major K in the order of its operands), a wave's own place, then read into
+// registers at once, so that the next copy can go to the same place while this block is computed.
+typedef __attribute__((address_space(1))) const void gvoid;
+typedef __attribute__((address_space(3))) void lvoid;
+
+// The registers of a block: K, V of NB blocks of 32 channels.
 template <int L, int NB>
 struct Raw {
   static constexpr bool MX = is_mx(L), FP8 = mx_fp8(L);
-  u32x4 k[MX ? (FP8 ? 4 : 2) : 8];
+  static constexpr int KI = MX ? (FP8 ? 4 : 2) : 8, VI = MX ? (FP8 ? NB : (NB + 1) / 2) : 2 * NB;   // copies of a kilobyte
+  static constexpr int COPIES = KI + VI + (MX ? 1 : 0);                                           // and one of the scales
+  static constexpr int BYTES = (KI + VI) * 1024 + (MX ? 256 : 0);
+  u32x4 k[KI];
   unsigned ks;                            // scales of half-blocks 0 and 1
-  u32x4 v[MX ? (FP8 ? NB : (NB + 1) / 2) : 2 * NB];
+  u32x4 v[VI];
   u32x2 vs[MX ? NB : 1];
 };
 
-// lane = 16 g + n
-template <int L, int NB>
-__device__ __forceinline__ void load_block(Raw<L, NB>& r, const char* k, const char* v, int dv) {
+// lane = 16 g + n. NT: the data is read once, by this workgroup.
+template <bool NT, int L, int NB>
+__device__ __forceinline__ void copy_block(char* to, const char* k, const char* v, int dv) {
+  using R = Raw<L, NB>;
   const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-  if constexpr (Raw<L, NB>::MX) {
-    constexpr bool FP8 = Raw<L, NB>::FP8;
+
+  // Copy i of a run that lies the same way in memory and in LDS: the instruction's offset counts for both (up to 4 KB).
+  auto run = [&](const char* from, char* at, auto count) __attribute__((always_inline)) {
+    constexpr int N = decltype(count)::value;
+    if constexpr (N > 0) __builtin_amdgcn_global_load_lds((gvoid*)from, (lvoid*)at, 16, 0, NT ? 2 : 0);
+    if constexpr (N > 1) __builtin_amdgcn_global_load_lds((gvoid*)from, (lvoid*)at, 16, 1024, NT ? 2 : 0);
+    if constexpr (N > 2) __builtin_amdgcn_global_load_lds((gvoid*)from, (lvoid*)at, 16, 2048, NT ? 2 : 0);
+    if constexpr (N > 3) __builtin_amdgcn_global_load_lds((gvoid*)from, (lvoid*)at, 16, 3072, NT ? 2 : 0);
+  };
+  auto one = [&](const char* from, int i) __attribute__((always_inline)) {
+    __builtin_amdgcn_global_load_lds((gvoid*)from, (lvoid*)(to + i * 1024), 16, 0, NT ? 2 : 0);
+  };
+  const unsigned l16 = lane * 16;
+  if constexpr (L == PALU_LAYOUT_ROWS) {  // key (c, n), channels 32 s + 8 g .. + 7
 #pragma unroll
-    for (int i = 0; i < (FP8 ? 4 : 2); ++i) r.k[i] = *reinterpret_cast<const u32x4*>(k + i * 1024 + lane * 16);
-    r.ks = *reinterpret_cast<const unsigned short*>(k + mx_codes(FP8, HD) + 2 * lane);
+    for (int i = 0; i < R::KI; ++i) one(k + (unsigned)((8 * (n >> 2) + 4 * (i >> 2) + (n & 3)) * (2 * HD) + (i & 3) * 64 + g * 16), i);
+  } else {
+#pragma unroll
+    for (int i = 0; i < R::KI; i += 4) run(k + i * 1024 + l16, to + i * 1024, std::integral_constant<int, (R::KI > 4 ? 4 : R::KI)>());
+  }
+  char* tv = to + R::KI * 1024;
+  if constexpr (L == PALU_LAYOUT_TILED || L == PALU_LAYOUT_ROWS) {
+#pragma unroll
+    for (int i = 0; i < R::VI; ++i)       // (of an odd multiple of 16 the last tile, or kilobyte, again)
+      one(v + (L == PALU_LAYOUT_TILED ? min(i, dv / 16 - 1) * 1024 + l16 : min(i * 1024 + l16, 64u * dv - 16)), R::KI + i);
+  } else {                                // (past the end, of half a kilobyte, the last piece again)
+    constexpr int FULL = mx_codes(R::FP8, 32 * NB) / 1024;
+    run(v + l16, tv, std::integral_constant<int, FULL>());
+    if constexpr (FULL < R::VI) one(v + FULL * 1024 + min(l16, 512u - 16), R::KI + FULL);
+    // 128 bytes of K's scales, then those of V
+    const char* from = lane < 32 ? k + mx_codes(R::FP8, HD) + 4 * lane : v + mx_codes(R::FP8, 32 * NB) + min(4 * (lane - 32), 32 * NB - 4);
+    __builtin_amdgcn_global_load_lds((gvoid*)from, (lvoid*)(to + (R::KI + R::VI) * 1024), 4, 0, NT ? 2 : 0);
+  }
+}
+template <int L, int NB>
+__device__ __forceinline__ void read_block(Raw<L, NB>& r, const char* s, int dv) {
+  using R = Raw<L, NB>;
+  const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+#pragma unroll
+  for (int i = 0; i < R::KI; ++i) r.k[i] = *reinterpret_cast<const u32x4*>(s + i * 1024 + lane * 16);
+  const char* v = s + R::KI * 1024;
+  if constexpr (R::MX) {
+    const char* sc = s + (R::KI + R::VI) * 1024;
+    r.ks = *reinterpret_cast<const unsigned short*>(sc + 2 * lane);
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      if constexpr (FP8) {
+      if constexpr (R::FP8) {
         r.v[b] = *reinterpret_cast<const u32x4*>(v + b * 1024 + lane * 16);
       } else {
         const u32x2 x = *reinterpret_cast<const u32x2*>(v + b * 512 + lane * 8);
         r.v[b / 2][2 * (b & 1)] = x[0];
         r.v[b / 2][2 * (b & 1) + 1] = x[1];
       }
-      r.vs[b] = *reinterpret_cast<const u32x2*>(v + mx_codes(FP8, 32 * NB) + b * 32 + 8 * g);
+      r.vs[b] = *reinterpret_cast<const u32x2*>(sc + 128 + b * 32 + 8 * g);
     }
   } else if constexpr (L == PALU_LAYOUT_TILED) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) r.k[i] = *reinterpret_cast<const u32x4*>(k + i * 1024 + lane * 16);
-#pragma unroll
-    for (int i = 0; i < 2 * NB; ++i)      // (of a width that is an odd multiple of 16 the last tile twice)
-      r.v[i] = *reinterpret_cast<const u32x4*>(v + min(i, dv / 16 - 1) * 1024 + lane * 16);
+    for (int i = 0; i < R::VI; ++i) r.v[i] = *reinterpret_cast<const u32x4*>(v + i * 1024 + lane * 16);
   } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)           // key (c, n), channels 32 s + 8 g .. + 7
-      r.k[i] = *reinterpret_cast<const u32x4*>(k + (8 * (n >> 2) + 4 * (i >> 2) + (n & 3)) * (2 * HD) + (i & 3) * 64 + g * 16);
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
       for (int j = 0; j < 8; ++j)         // position 8 g + j, channels 32 b + 2 n and 2 n + 1
         r.v[2 * b + j / 4][j & 3] = *reinterpret_cast<const unsigned*>(v + (8 * g + j) * (2 * dv) + min(64 * b + 4 * n, 2 * dv - 4));
   }
+}
+
+// Neighbouring blocks that a wave takes together: some 8 KB or more on their way to it.
+constexpr int step_group(int layout) { return layout == PALU_LAYOUT_MX4 ? 2 : 1; }
+
+// This wave's copies have arrived, its reads from LDS are done.
+__device__ __forceinline__ void wait_copies() {
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_waitcnt(0x0f70);     // vmcnt(0)
+  __builtin_amdgcn_sched_barrier(0);
+}
+__device__ __forceinline__ void wait_reads() {
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_waitcnt(0xc07f);     // lgkmcnt(0)
+  __builtin_amdgcn_sched_barrier(0);
 }
 
 // Channel of element j of product step s in lane group g's Q and K operands.
@@ -234,65 +291,98 @@ struct Wave {
     }
   }
 
-  // Blocks first, first + step, .. below end of a sequence that is seen up to position seen - 1; where(blk, k, v) gives a
-  // block's places.
-  template <typename F>
-  __device__ __forceinline__ void pass(int first, int end, int step, int seen, float qscale, int dv, F&& where) {
+  // This wave's blocks of first .. end - 1, of a sequence that is seen up to position seen - 1 (ALL: whole blocks only): every
+  // fourth group of them. page_at(blk) gives a block's page, where(page, blk, k, v) its places; s: the wave's place in LDS. While
+  // a group is computed the next one is on its way; its pages are asked for a turn earlier.
+  template <bool ALL, typename P, typename F>
+  __device__ __forceinline__ void pass(int first, int end, int seen, float qscale, int dv, char* s, P&& page_at, F&& where) {
+    using R = Raw<L, NB>;
+    constexpr int G = step_group(L);
+    first += (int)(threadIdx.x >> 6) * G;
+    first = __builtin_amdgcn_readfirstlane(first);
     if (first >= end) return;
-    const int last = first + (end - 1 - first) / step * step;
-    Raw<L, NB> a, b;
-    const char *k, *v;
-    auto load = [&](Raw<L, NB>& r, int blk) __attribute__((always_inline)) {
-      where(min(blk, last), k, v);
-      load_block<L, NB>(r, k, v, dv);
+    int page[G];
+    auto pages = [&](int blk) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < G; ++i) page[i] = page_at(min(blk + i, end - 1));
     };
-    auto use = [&](const Raw<L, NB>& r, int blk) __attribute__((always_inline)) {
-      if (32 * blk + 32 <= seen) add<false>(r, qscale, 32);
-      else if (32 * blk < seen) add<true>(r, qscale, seen - 32 * blk);
+    auto fetch = [&](int blk) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < G; ++i) {
+        const char *k, *v;
+        where(page[i], min(blk + i, end - 1), k, v);
+        copy_block<!ALL, L, NB>(s + i * R::BYTES, k, v, dv);
+      }
     };
-    load(a, first);
-    for (int blk = first;; blk += 2 * step) {
-      load(b, blk + step);
-      use(a, blk);
-      if (blk + step > last) break;
-      load(a, blk + 2 * step);
-      use(b, blk + step);
-      if (blk + 2 * step > last) break;
+    pages(first);
+    wait_copies();                        // the queries are here (the pages took as long)
+    fetch(first);
+    for (int blk = first; blk < end;) {
+      const int next = blk + 4 * G;
+      pages(min(next, end - 1));
+      wait_copies();
+      R r[G];
+#pragma unroll
+      for (int i = 0; i < G; ++i) read_block<L, NB>(r[i], s + i * R::BYTES, dv);
+      wait_reads();
+      if (next < end) fetch(next);
+#pragma unroll
+      for (int i = 0; i < G; ++i) {
+        if (ALL ? blk + i < end : 32 * (blk + i) + 32 <= seen && blk + i < end) add<false>(r[i], qscale, 32);
+        else if (!ALL && blk + i < end) add<true>(r[i], qscale, seen - 32 * (blk + i));
+      }
+      blk = next;
     }
   }
 };
 
-// Column tile x of every wave's state to LDS, [wave][16][OS] O and [wave][16] m, l; barriers around it are the caller's.
+// Column tile x of every wave's state in LDS: O [wave][cols][OS], then m and l [wave][cols]; only the first `cols` columns.
+// Barriers around it are the caller's.
 template <int NB>
 struct WaveLds {
   static constexpr int OS = 32 * NB + 4;
-  float o[4][16][OS], m[4][16], l[4][16];
+  float* o;
+  int cols;
+  __host__ __device__ static constexpr int bytes(int cols) { return 4 * cols * (OS + 2) * (int)sizeof(float); }
+  __device__ __forceinline__ float* row(int w, int n) const { return o + (w * cols + n) * OS; }
+  __device__ __forceinline__ float& m(int w, int n) const { return o[4 * cols * OS + w * cols + n]; }
+  __device__ __forceinline__ float& l(int w, int n) const { return o[4 * cols * (OS + 1) + w * cols + n]; }
 };
+// LDS of a workgroup: the waves' places for blocks on their way, afterwards their results.
+template <int L, int NB>
+constexpr int place_bytes() { return step_group(L) * Raw<L, NB>::BYTES; }
+template <int L, int NB>
+constexpr int step_lds() {
+  return 4 * place_bytes<L, NB>() > WaveLds<NB>::bytes(16) ? 4 * place_bytes<L, NB>() : WaveLds<NB>::bytes(16);
+}
+
 template <int L, int NB, int C>
-__device__ __forceinline__ void to_lds(WaveLds<NB>& s, const Wave<L, NB, C>& st, int x) {
+__device__ __forceinline__ void to_lds(const WaveLds<NB>& s, const Wave<L, NB, C>& st, int x) {
   const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4, w = threadIdx.x >> 6;
   const float l = wave_sum_xor48(st.l[x]);
+  if (n >= s.cols) return;
   if (g == 0) {
-    s.m[w][n] = st.m[x];
-    s.l[w][n] = l;
+    s.m(w, n) = st.m[x];
+    s.l(w, n) = l;
   }
+  float* row = s.row(w, n);
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
     const f32x4 y = st.o[x][2 * b], z = st.o[x][2 * b + 1];    // rows 4 g .. + 3 of tiles 0 and 1
     if constexpr (L == PALU_LAYOUT_TILED) {
-      *reinterpret_cast<f32x4*>(&s.o[w][n][32 * b + 4 * g]) = y;
-      *reinterpret_cast<f32x4*>(&s.o[w][n][32 * b + 16 + 4 * g]) = z;
+      *reinterpret_cast<f32x4*>(row + 32 * b + 4 * g) = y;
+      *reinterpret_cast<f32x4*>(row + 32 * b + 16 + 4 * g) = z;
     } else {
-      *reinterpret_cast<f32x4*>(&s.o[w][n][32 * b + 8 * g]) = f32x4{y[0], z[0], y[1], z[1]};
-      *reinterpret_cast<f32x4*>(&s.o[w][n][32 * b + 8 * g + 4]) = f32x4{y[2], z[2], y[3], z[3]};
+      *reinterpret_cast<f32x4*>(row + 32 * b + 8 * g) = f32x4{y[0], z[0], y[1], z[1]};
+      *reinterpret_cast<f32x4*>(row + 32 * b + 8 * g + 4) = f32x4{y[2], z[2], y[3], z[3]};
     }
   }
 }
 
 // Four channels of a column, summed from parts: y and l stand over 2^m.
 struct Joined {
-  f32x4 y{0.f, 0.f, 0.f, 0.f};
-  float m = NEG_INF, l = 0.f;
+  f32x4 y;
+  float m, l;
   __device__ __forceinline__ void add(f32x4 py, float pm, float pl) {
     const float mn = fmaxf(m, pm);
     const float ref = mn == NEG_INF ? 0.f : mn;               // (then both have nothing, or NaN)
@@ -302,11 +392,12 @@ struct Joined {
     m = mn;
   }
 };
+__device__ __forceinline__ Joined no_parts() { return Joined{{0.f, 0.f, 0.f, 0.f}, NEG_INF, 0.f}; }
 template <int NB>
 __device__ __forceinline__ Joined join_waves(const WaveLds<NB>& s, int n, int d) {
-  Joined j;
+  Joined j = no_parts();
 #pragma unroll
-  for (int w = 0; w < 4; ++w) j.add(*reinterpret_cast<const f32x4*>(&s.o[w][n][d]), s.m[w][n], s.l[w][n]);
+  for (int w = 0; w < 4; ++w) j.add(*reinterpret_cast<const f32x4*>(s.row(w, n) + d), s.m(w, n), s.l(w, n));
   return j;
 }
 
@@ -323,32 +414,64 @@ __device__ __forceinline__ int wg_scan(int x, int* part, int& total) {
     before += i < w ? part[i] : 0;
     total += part[i];
   }
+  total = __builtin_amdgcn_readfirstlane(total);            // what follows from it is uniform, and the page reads scalar
   return before + s - x;
+}
+
+// How items are cut into pieces of up to len blocks, a workgroup each: the first of a few lengths, from an even share of all blocks
+// on, of which the chip holds all pieces (`slots`) at once, and at least `least`. of(i) gives n items of some blocks each; a thread has
+// i0 .. i1 - 1. Its pieces are number before .. before + mine - 1 of all; where that never fits, at most slots + all items.
+struct Cut {
+  int len, before, mine, all;
+  __device__ __forceinline__ int pieces(int blocks) const { return (blocks + len - 1) / len; }
+};
+struct Items {
+  int n, blocks;
+};
+template <typename F>
+__device__ __forceinline__ Cut cut_items(int i0, int i1, int slots, int least, int* scan, F&& of) {
+  int mine = 0, total;
+  for (int i = i0; i < i1; ++i) {
+    const Items x = of(i);
+    mine += x.n * x.blocks;
+  }
+  wg_scan(mine, scan, total);
+  const int share = (total + slots - 1) / slots;
+  Cut c;
+  for (int t = 0; t < 4; ++t) {           // uniform
+    c.len = max(least, share + share * t / 8);
+    c.mine = 0;
+    for (int i = i0; i < i1; ++i) {
+      const Items x = of(i);
+      c.mine += x.n * c.pieces(x.blocks);
+    }
+    c.before = wg_scan(c.mine, scan, c.all);
+    if (c.all <= slots) break;
+  }
+  return c;
 }
 
 __device__ __forceinline__ int seen_of(const StepArgs& a, int pos) { return min(max(pos, -1), a.capacity - 1) + 1; }
 
-// Places of block blk of a row's KV head.
-__device__ __forceinline__ void place_of(const StepArgs& a, int row, int kvh, int blk, const char*& k, const char*& v) {
-  long long page = row;
-  if (a.table) page = min(max(load_uniform(a.table, (long long)row * a.pt_stride + (blk >> a.page_shift)), 0), a.n_pages - 1);
+// The page of block blk of a row, and the places of a KV head's block on it.
+__device__ __forceinline__ int page_of(const StepArgs& a, int row, int blk) {
+  if (!a.table) return row;
+  return min(max(load_uniform(a.table, (long long)row * a.pt_stride + (blk >> a.page_shift)), 0), a.n_pages - 1);
+}
+__device__ __forceinline__ void place_of(const StepArgs& a, int page, int kvh, int blk, const char*& k, const char*& v) {
   const int at = a.table ? blk & ((1 << a.page_shift) - 1) : blk;
   k = a.k + page * a.k_page + kvh * a.k_head + (long long)at * a.k_blk;
   v = a.v + page * a.v_page + kvh * a.v_head + (long long)at * a.v_blk;
 }
 
 // ---- the rows' own blocks -----------------------------------------------------------------------
-// An item is a row's KV head: its blocks, but for those that have been read with the group's prefix. All items' blocks lie one
-// after another, row by row, KV head by KV head. Where a workgroup's share of them (of STEP_WGS) is at least STEP_LEAST blocks
-// each takes such a share, from wherever it begins to wherever it ends; below that an item is cut into even pieces of up
-// to STEP_LEAST blocks, a workgroup each. An item in several workgroups is joined by the one that finds all parts done.
-constexpr int STEP_WGS = 512;             // workgroups that the chip holds at once (two a CU)
-constexpr int STEP_LEAST = 16;            // blocks
-
-inline int step_grid(int B, int n_kv) { return STEP_WGS + B * n_kv; }          // pieces of STEP_LEAST, at most
-inline int step_slots(int B, int n_kv) { return std::max(2 * STEP_WGS, step_grid(B, n_kv)); }
+// An item is a row's KV head: its blocks, but for those that have been read with the group's prefix, cut into even pieces. The
+// pieces of an item are joined by the workgroup that finds all of them done.
+constexpr int STEP_LEAST = 16;            // blocks of a piece, at least
+constexpr int STEP_WGS = 512;             // workgroups that the chip holds at once, by the kernel's LDS and registers
+inline int step_grid(int B, int n_kv) { return STEP_WGS + B * n_kv; }
 inline size_t step_bytes(int B, int n_kv, int rep, int dv) {
-  return (size_t)step_slots(B, n_kv) * ((size_t)rep * (dv + 2) * sizeof(float) + sizeof(unsigned long long));
+  return (size_t)step_grid(B, n_kv) * ((size_t)rep * (dv + 2) * sizeof(float) + sizeof(unsigned long long));
 }
 
 struct RowWork {
@@ -373,6 +496,12 @@ __device__ __forceinline__ RowWork row_work(const StepArgs& a, int b) {
   return r;
 }
 
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ RowWork uniform(const RowWork& r) {
+  return RowWork{uniform(r.lead), uniform(r.first), uniform(r.end),  uniform(r.seen),
+                 uniform(r.pieces), uniform(r.base), uniform(r.local), uniform(r.pblocks)};
+}
+
 __device__ __forceinline__ void store4(const StepArgs& a, long long at, f32x4 y) {
   if (a.f32_out) {
     *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + at) = y;
@@ -384,149 +513,181 @@ __device__ __forceinline__ void store4(const StepArgs& a, long long at, f32x4 y)
   }
 }
 
+// Parts go to memory and come from there, past the XCD's L2, whichever XCD wrote them.
+__device__ __forceinline__ void store_part(float* p, float x) { __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM); }
+__device__ __forceinline__ float load_part(const float* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM); }
+// Four of them, 8-byte aligned.
+__device__ __forceinline__ void store_part4(float* p, f32x4 x) {
+  typedef unsigned long long u64;
+  const u32x4 u = __builtin_bit_cast(u32x4, x);
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    __hip_atomic_store(reinterpret_cast<u64*>(p) + i, u[2 * i] | (u64)u[2 * i + 1] << 32, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+}
+__device__ __forceinline__ f32x4 load_part4(const float* p) {
+  typedef unsigned long long u64;
+  u32x4 u;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const u64 x = __hip_atomic_load(reinterpret_cast<const u64*>(p) + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+    u[2 * i] = (unsigned)x;
+    u[2 * i + 1] = (unsigned)(x >> 32);
+  }
+  return __builtin_bit_cast(f32x4, u);
+}
+
 template <int L, int NB>
 __global__ __launch_bounds__(256, 2) void palu_step_kernel(const StepArgs a) {
-  __shared__ WaveLds<NB> lds;
-  __shared__ int scan[4], found[4];
-  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), wg = blockIdx.x;
+  __shared__ __attribute__((aligned(1024))) char smem[step_lds<L, NB>()];
+  const WaveLds<NB> lds{reinterpret_cast<float*>(smem), a.rep};
+  __shared__ int scan[4], found[2];
+  __shared__ RowWork found_row;
+  __shared__ float top[16][16];
+  __shared__ Joined sums[256];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int per = (a.B + 255) / 256, r0 = min(tid * per, a.B), r1 = min(r0 + per, a.B);
-  // this workgroup's part of the batch
-  int mine = 0, total, pieces;
-  for (int b = r0; b < r1; ++b) {
-    const RowWork r = row_work(a, b);
-    mine += r.end - r.first;
-  }
-  int before = wg_scan(mine, scan, total);
-  total *= a.n_kv;
-  const int share = (total + STEP_WGS - 1) / STEP_WGS;
-  const bool cut = share < STEP_LEAST;    // items in pieces, not shares
-  auto pieces_of = [](const RowWork& r) { return (r.end - r.first + STEP_LEAST - 1) / STEP_LEAST; };
-  if (cut) {
-    mine = 0;
-    for (int b = r0; b < r1; ++b) mine += pieces_of(row_work(a, b));
-    before = wg_scan(mine, scan, pieces);
-  }
-  if (!cut && wg >= STEP_WGS) return;     // uniform
-  const int want = cut ? wg : wg * share;
-  if (want >= (cut ? pieces * a.n_kv : total)) return;
-  if (want >= before * a.n_kv && want < (before + mine) * a.n_kv) {
-    int at = before * a.n_kv, b = r0;
-    for (; b < r1; ++b) {
-      const RowWork r = row_work(a, b);
-      const int n = (cut ? pieces_of(r) : r.end - r.first) * a.n_kv;
-      if (want < at + n) break;
+  // this workgroup's piece
+  RowWork own;                            // of a thread's only row
+  if (r0 < r1) own = row_work(a, r0);
+  auto row = [&](int b) { return per == 1 ? own : row_work(a, b); };
+  const Cut cut = cut_items(r0, r1, STEP_WGS, STEP_LEAST, scan, [&](int b) {
+    const RowWork r = row(b);
+    return Items{a.n_kv, r.end - r.first};
+  });
+  const int want = blockIdx.x;
+  if (want >= cut.all) return;            // uniform
+  if (want >= cut.before && want < cut.before + cut.mine) {
+    int at = cut.before, b = r0;
+    RowWork r = row(b);
+    for (;;) {
+      const int n = cut.pieces(r.end - r.first) * a.n_kv;
+      if (want < at + n || b + 1 >= r1) break;
       at += n;
+      r = row(++b);
     }
     found[0] = b;
-    found[1] = at;
+    found[1] = want - at;
+    found_row = r;
   }
   __syncthreads();
-  int b = __builtin_amdgcn_readfirstlane(found[0]), at = __builtin_amdgcn_readfirstlane(found[1]);
-  const int stop = cut ? want + 1 : min(total, want + share);
+  const int b = __builtin_amdgcn_readfirstlane(found[0]), in = __builtin_amdgcn_readfirstlane(found[1]);
+  const RowWork r = uniform(found_row);
+  const int chunks = uniform(cut.pieces(r.end - r.first)), kvh = uniform(in / chunks), chunk = in - kvh * chunks, wg0 = want - chunk;
+  const int len = uniform((r.end - r.first + chunks - 1) / chunks), lo = r.first + chunk * len, hi = min(r.end, lo + len);
   const int n16 = lane & 15, g = lane >> 4;
 
-  for (int here = want; here < stop;) {   // uniform
-    RowWork r = row_work(a, b);
-    const int unit = cut ? pieces_of(r) : r.end - r.first;  // of an item, in what `here` counts
-    const int kvh = (here - at) / unit, in = here - at - kvh * unit;
-    const int item = at + kvh * unit;                       // its first
-    int lo, hi, chunk, chunks, wg0;
-    if (cut) {
-      const int len = (r.end - r.first + unit - 1) / unit;
-      lo = r.first + in * len;
-      hi = min(r.end, lo + len);
-      chunk = in;
-      chunks = unit;
-      wg0 = item;
-      here += 1;
+  Wave<L, NB, 1> st;
+  st.clear();
+  {
+    const __bf16* q = a.q + ((long long)b * a.n_q + kvh * a.rep + min(n16, a.rep - 1)) * HD;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) st.q[0][s] = *reinterpret_cast<const bf16x8*>(q + q_chan<L>(s, g));
+  }
+  st.template pass<false>(
+      lo, min(hi, (r.seen + 31) >> 5), r.seen, a.qscale, a.dv, smem + w * place_bytes<L, NB>(),
+      [&](int blk) __attribute__((always_inline)) { return page_of(a, blk < r.pblocks ? r.lead : b, blk); },
+      [&](int page, int blk, const char*& k, const char*& v) __attribute__((always_inline)) { place_of(a, page, kvh, blk, k, v); });
+  __syncthreads();                        // every wave is done with its places
+  to_lds(lds, st, 0);
+  __syncthreads();
+  const int vecs = a.dv / 4, units = a.rep * vecs;
+  const long long part_size = (long long)a.rep * (a.dv + 2);
+  if (chunks > 1) {
+    float* po = a.part + want * part_size;
+    for (int e = tid; e < units; e += 256) {
+      const int h = e / vecs, d = 4 * (e - h * vecs);
+      const Joined j = join_waves(lds, h, d);
+      store_part4(po + h * a.dv + d, j.y);
+      if (d == 0) {
+        store_part(po + a.rep * a.dv + h, j.m);
+        store_part(po + a.rep * a.dv + a.rep + h, j.l);
+      }
+    }
+    if (!chunks_all_done(a.flags + wg0, a.epoch, chunks, chunk, found)) return;   // uniform
+  }
+  auto finish = [&](int h, int d, const Joined& j) __attribute__((always_inline)) {
+    const float inv = 1.f / j.l;
+    const f32x4 y = r.seen == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : j.y * inv;       // a row that sees nothing: zeros
+    store4(a, ((long long)b * a.n_q + kvh * a.rep + h) * a.dv + d, y);
+  };
+  // The parts: this workgroup's own (in LDS), or all workgroups' (one of which is its own), and the prefix's pieces. First
+  // every column's largest m, then sums over parts, 256 / units threads to a part of 4 channels each.
+  const int n_chunks = chunks == 1 ? 0 : chunks, n_parts = n_chunks + r.pieces;
+  const long long size = (long long)a.pre_cols * (a.dv + 2);
+  auto part = [&](int c, int h, const float*& o, const float*& m, const float*& l) __attribute__((always_inline)) {
+    if (c < n_chunks) {
+      const float* po = a.part + (wg0 + c) * part_size;
+      o = po + h * a.dv;
+      m = po + a.rep * a.dv + h;
+      l = m + a.rep;
     } else {
-      const int n = min(unit - in, stop - here);
-      lo = r.first + in;
-      hi = lo + n;
-      wg0 = item / share;
-      chunk = wg - wg0;
-      chunks = (item + unit - 1) / share - wg0 + 1;
-      here += n;
+      const int col = r.local * a.rep + h, tile = col / a.pre_cols, x = col - tile * a.pre_cols;
+      const float* po = a.pre + (r.base + (long long)(tile * a.n_kv + kvh) * r.pieces + (c - n_chunks)) * size;
+      o = po + x * a.dv;
+      m = po + a.pre_cols * a.dv + x;
+      l = m + a.pre_cols;
     }
-    const bool next_row = here - at >= unit * a.n_kv;
-
-    Wave<L, NB, 1> st;
-    st.clear();
-    {
-      const __bf16* q = a.q + ((long long)b * a.n_q + kvh * a.rep + min(n16, a.rep - 1)) * HD;
+  };
+  if (n_parts) {
+    const int h = tid & 15;
+    float m = NEG_INF;
+    if (h < a.rep)
+      for (int c = tid >> 4; c < n_parts; c += 16) {
+        const float *po, *pm, *pl;
+        part(c, h, po, pm, pl);
+        m = fmaxf(m, load_part(pm));
+      }
+    top[tid >> 4][h] = m;
+  }
+  __syncthreads();
+  const int groups = max(1, 256 / units), grp = min(tid / units, groups);   // (threads past the groups: none)
+  for (int e = groups > 1 ? tid - grp * units : tid; e < units && grp < groups; e += 256) {
+    const int h = e / vecs, d = 4 * (e - h * vecs);
+    Joined j = no_parts();
+    if (n_parts) {
+      float mx = NEG_INF;
 #pragma unroll
-      for (int s = 0; s < 4; ++s) st.q[0][s] = *reinterpret_cast<const bf16x8*>(q + q_chan<L>(s, g));
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, top[i][h]);
+      j.m = mx;
+      const float ref = mx == NEG_INF ? 0.f : mx;
+      constexpr int U = 8;                // parts whose loads are under way together
+      for (int c0 = grp; c0 < n_parts; c0 += U * groups) {
+        f32x4 y[U];
+        float m[U], l[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const float *po, *pm, *pl;
+          part(min(c0 + u * groups, n_parts - 1), h, po, pm, pl);
+          m[u] = load_part(pm);
+          l[u] = load_part(pl);
+          y[u] = load_part4(po + d);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (c0 + u * groups >= n_parts) continue;
+          const float f = __builtin_amdgcn_exp2f(m[u] - ref);
+          j.l += f * l[u];
+          j.y += f * y[u];
+        }
+      }
     }
-    st.pass(lo + w, min(hi, (r.seen + 31) >> 5), 4, r.seen, a.qscale, a.dv, [&](int blk, const char*& k, const char*& v) __attribute__((always_inline)) {
-      place_of(a, blk < r.pblocks ? r.lead : b, kvh, blk, k, v);
-    });
-    __syncthreads();                      // lds may still be read for the item before
-    to_lds(lds, st, 0);
+    if (chunks == 1 && grp == 0) {
+      const Joined own_part = join_waves(lds, h, d);
+      j.add(own_part.y, own_part.m, own_part.l);
+    }
+    if (groups == 1) {
+      finish(h, d, j);
+    } else {
+      sums[tid] = j;
+    }
+  }
+  if (groups > 1) {
     __syncthreads();
-    const int vecs = a.dv / 4;
-    auto slot = [&](int c) { return cut ? wg0 + c : 2 * (wg0 + c) + (c < chunks - 1 ? 1 : 0); };
-    const long long part_size = (long long)a.rep * (a.dv + 2);
-    bool join = true;
-    if (chunks > 1) {
-      float* po = a.part + slot(chunk) * part_size;
-      for (int e = tid; e < a.rep * vecs; e += 256) {
-        const int h = e / vecs, d = 4 * (e - h * vecs);
-        const Joined j = join_waves(lds, h, d);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) __hip_atomic_store(po + h * a.dv + d + i, j.y[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-        if (d == 0) {
-          __hip_atomic_store(po + a.rep * a.dv + h, j.m, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-          __hip_atomic_store(po + a.rep * a.dv + a.rep + h, j.l, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-        }
-      }
-      // The parts' done flags, as the split items of the decode have them (chunks_all_done), but not next to each other.
-      __builtin_amdgcn_s_waitcnt(0);      // this thread's part has been written
-      __syncthreads();
-      if (tid < 64) {
-        if (tid == 0) __hip_atomic_store(a.flags + slot(chunk), a.epoch, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the flag is in memory before the others are read
-        bool set = true;
-        for (int c = tid; c < chunks; c += 64)
-          set = set && __hip_atomic_load(a.flags + slot(c), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM) == a.epoch;
-        const bool all = __all(set);
-        if (all)
-          for (int c = tid; c < chunks; c += 64) __hip_atomic_store(a.flags + slot(c), 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-        if (tid == 0) found[2] = all ? 1 : 0;
-      }
-      __syncthreads();
-      join = found[2] != 0;
-    }
-    if (join) {
-      for (int e = tid; e < a.rep * vecs; e += 256) {
-        const int h = e / vecs, d = 4 * (e - h * vecs);
-        Joined j;
-        if (chunks == 1) {
-          j = join_waves(lds, h, d);
-        } else {
-          for (int c = 0; c < chunks; ++c) {
-            const float* po = a.part + slot(c) * part_size;
-            f32x4 y;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) y[i] = __hip_atomic_load(po + h * a.dv + d + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-            j.add(y, __hip_atomic_load(po + a.rep * a.dv + h, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM),
-                  __hip_atomic_load(po + a.rep * a.dv + a.rep + h, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM));
-          }
-        }
-        if (r.pieces) {
-          const int col = r.local * a.rep + h, tile = col / a.pre_cols, x = col - tile * a.pre_cols;
-          const long long size = (long long)a.pre_cols * (a.dv + 2);
-          const float* po = a.pre + (r.base + (long long)(tile * a.n_kv + kvh) * r.pieces) * size;
-          for (int c = 0; c < r.pieces; ++c, po += size)
-            j.add(*reinterpret_cast<const f32x4*>(po + x * a.dv + d), po[a.pre_cols * a.dv + x], po[a.pre_cols * (a.dv + 1) + x]);
-        }
-        const float inv = 1.f / j.l;
-        const f32x4 y = r.seen == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : j.y * inv;   // a row that sees nothing: zeros
-        store4(a, ((long long)b * a.n_q + kvh * a.rep + h) * a.dv + d, y);
-      }
-    }
-    if (next_row) {
-      at += unit * a.n_kv;
-      ++b;
+    if (tid < units) {
+      Joined j = sums[tid];
+      for (int i = 1; i < groups; ++i) j.add(sums[tid + i * units].y, sums[tid + i * units].m, sums[tid + i * units].l);
+      const int h = tid / vecs;
+      finish(h, 4 * (tid - h * vecs), j);
     }
   }
 }
@@ -536,15 +697,16 @@ __global__ __launch_bounds__(256, 2) void palu_step_kernel(const StepArgs a) {
 // of pieces, a workgroup each, so that all pieces fit the chip at once where they can. The first workgroups write what the
 // second launch has to know of every row.
 
-inline int pre_wgs(int C) { return C == 4 ? 256 : 512; }    // that the chip holds at once
+constexpr int PRE_WGS = 512;              // workgroups that the chip holds at once
+constexpr int PRE_LEAST = 8;              // blocks of a piece, at least
 inline int pre_tile(int B, int n_groups, int rep) {         // C by the average group
   const int cols = (B + n_groups - 1) / n_groups * rep;
-  return cols <= 16 ? 1 : cols <= 32 ? 2 : 4;
+  return cols <= 16 ? 1 : 2;
 }
 // Column tiles of all groups, at most, and pieces: tiles of n blocks are cut into at most n / len + 1 pieces, len at least the
 // workgroups' even share of all blocks.
 inline long long pre_tiles(int B, int n_groups, int rep, int C) { return (long long)B * rep / (16 * C) + std::min(B, n_groups); }
-inline long long pre_slots(int B, int n_groups, int rep, int n_kv, int C) { return pre_wgs(C) + pre_tiles(B, n_groups, rep, C) * n_kv; }
+inline long long pre_slots(int B, int n_groups, int rep, int n_kv, int C) { return PRE_WGS + pre_tiles(B, n_groups, rep, C) * n_kv; }
 inline size_t pre_bytes(int B, int n_groups, int rep, int n_kv, int dv) {
   const int C = pre_tile(B, n_groups, rep);
   return (size_t)pre_slots(B, n_groups, rep, n_kv, C) * 16 * C * (dv + 2) * sizeof(float) + (size_t)B * sizeof(RowPrefix);
@@ -563,35 +725,24 @@ __device__ __forceinline__ Group group_of(const StepArgs& a, int gi) {
 }
 
 template <int L, int NB, int C>
-__global__ __launch_bounds__(256, C == 4 ? 1 : 2) void palu_prefix_kernel(const StepArgs a) {
-  __shared__ WaveLds<NB> lds;
-  __shared__ int scan[4], found[2], bases[256];
+__global__ __launch_bounds__(256, 2) void palu_prefix_kernel(const StepArgs a) {
+  __shared__ __attribute__((aligned(1024))) char smem[step_lds<L, NB>()];
+  const WaveLds<NB> lds{reinterpret_cast<float*>(smem), 16};
+  __shared__ int scan[4], found[4], bases[256];
   constexpr int COLS = 16 * C;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int per = (a.n_groups + 255) / 256, g0 = min(tid * per, a.n_groups), g1 = min(g0 + per, a.n_groups);
-  constexpr int WGS = C == 4 ? 256 : 512;
   auto tiles_of = [&](const Group& g) { return g.blocks ? (g.rows * a.rep + COLS - 1) / COLS * a.n_kv : 0; };   // of all KV heads
-  // blocks of a piece: the first of a few lengths whose pieces the chip holds at once
-  int mine = 0, total, len = 8;
-  for (int i = g0; i < g1; ++i) {
-    const Group g = group_of(a, i);
-    mine += tiles_of(g) * g.blocks;
-  }
-  wg_scan(mine, scan, total);
-  int before, all;
-  for (int t = 0; t < 4; ++t) {           // uniform
-    len = max(8, (int)(((long long)(total + WGS - 1) / WGS) * (8 + t) / 8));
-    mine = 0;
-    for (int i = g0; i < g1; ++i) {
-      const Group g = group_of(a, i);
-      mine += tiles_of(g) * ((g.blocks + len - 1) / len);
-    }
-    before = wg_scan(mine, scan, all);
-    if (all <= WGS) break;
-  }
+  Group own;                              // a thread's only group
+  if (g0 < g1) own = group_of(a, g0);
+  auto group = [&](int i) { return per == 1 ? own : group_of(a, i); };
+  const Cut cut = cut_items(g0, g1, PRE_WGS, PRE_LEAST, scan, [&](int i) {
+    const Group g = group(i);
+    return Items{tiles_of(g), g.blocks};
+  });
   const int row_wgs = (a.B + 255) / 256;
   if ((int)blockIdx.x < row_wgs) {        // the rows' records, a thread each
-    bases[tid] = before;
+    bases[tid] = cut.before;
     __syncthreads();
     const int b = (int)blockIdx.x * 256 + tid;
     if (b >= a.B) return;
@@ -607,9 +758,9 @@ __global__ __launch_bounds__(256, C == 4 ? 1 : 2) void palu_prefix_kernel(const 
       int base = bases[gi / per];
       for (int i = gi / per * per; i < gi; ++i) {
         const Group x = group_of(a, i);
-        base += tiles_of(x) * ((x.blocks + len - 1) / len);
+        base += tiles_of(x) * cut.pieces(x.blocks);
       }
-      const int pieces = (g.blocks + len - 1) / len;
+      const int pieces = cut.pieces(g.blocks);
       // (Groups that overlap, where the offsets make no sense, can be more pieces than the workspace was sized for.)
       r = RowPrefix{g.row, g.blocks, base >= 0 && base + tiles_of(g) * pieces <= a.pre_slots ? pieces : 0, base, b - g.row, {}};
     }
@@ -619,26 +770,28 @@ __global__ __launch_bounds__(256, C == 4 ? 1 : 2) void palu_prefix_kernel(const 
   const int want = (int)blockIdx.x - row_wgs;
   if (tid == 0) found[0] = -1;
   __syncthreads();
-  if (want >= before && want < before + mine) {
-    int at = before;
+  if (want >= cut.before && want < cut.before + cut.mine) {
+    int at = cut.before;
     for (int i = g0; i < g1; ++i) {
-      const Group g = group_of(a, i);
-      const int pieces = (g.blocks + len - 1) / len, n = tiles_of(g) * pieces;
+      const Group g = group(i);
+      const int n = tiles_of(g) * cut.pieces(g.blocks);
       if (want >= at && want < at + n) {
-        found[0] = i;
-        found[1] = want - at;
+        found[0] = want - at;
+        found[1] = g.row;
+        found[2] = g.rows;
+        found[3] = g.blocks;
         break;
       }
       at += n;
     }
   }
   __syncthreads();
-  const int gi = __builtin_amdgcn_readfirstlane(found[0]);
-  if (gi < 0) return;                     // uniform: past the last piece
-  const Group g = group_of(a, gi);
-  const int in = __builtin_amdgcn_readfirstlane(found[1]), pieces = (g.blocks + len - 1) / len;
-  const int tile = in / pieces, piece = in - tile * pieces, kvh = tile % a.n_kv, ct = tile / a.n_kv;
-  const int each = (g.blocks + pieces - 1) / pieces, lo = piece * each, hi = min(g.blocks, lo + each);
+  const int in = __builtin_amdgcn_readfirstlane(found[0]);
+  if (in < 0) return;                     // uniform: past the last piece
+  const Group g{__builtin_amdgcn_readfirstlane(found[1]), __builtin_amdgcn_readfirstlane(found[2]), __builtin_amdgcn_readfirstlane(found[3])};
+  const int pieces = uniform(cut.pieces(g.blocks)), tile = uniform(in / pieces), piece = in - tile * pieces;
+  const int ct = uniform(tile / a.n_kv), kvh = tile - ct * a.n_kv;
+  const int each = uniform((g.blocks + pieces - 1) / pieces), lo = piece * each, hi = min(g.blocks, lo + each);
   const int n16 = lane & 15, gl = lane >> 4;
   Wave<L, NB, C> st;
   st.clear();
@@ -649,14 +802,14 @@ __global__ __launch_bounds__(256, C == 4 ? 1 : 2) void palu_prefix_kernel(const 
 #pragma unroll
     for (int s = 0; s < 4; ++s) st.q[x][s] = *reinterpret_cast<const bf16x8*>(q + q_chan<L>(s, gl));
   }
-  st.pass(lo + w, hi, 4, 32 * g.blocks, a.qscale, a.dv, [&](int blk, const char*& k, const char*& v) __attribute__((always_inline)) {
-    place_of(a, g.row, kvh, blk, k, v);
-  });
+  st.template pass<true>(
+      lo, hi, 32 * g.blocks, a.qscale, a.dv, smem + w * place_bytes<L, NB>(), [&](int blk) __attribute__((always_inline)) { return page_of(a, g.row, blk); },
+      [&](int page, int blk, const char*& k, const char*& v) __attribute__((always_inline)) { place_of(a, page, kvh, blk, k, v); });
   float* po = a.pre + (long long)want * COLS * (a.dv + 2);
   const int vecs = a.dv / 4;
 #pragma unroll
   for (int x = 0; x < C; ++x) {
-    if (x) __syncthreads();
+    __syncthreads();                      // every wave is done with its places, or with the results before
     to_lds(lds, st, x);
     __syncthreads();
     for (int e = tid; e < 16 * vecs; e += 256) {
@@ -673,8 +826,8 @@ __global__ __launch_bounds__(256, C == 4 ? 1 : 2) void palu_prefix_kernel(const 
 
 // ---- launches -----------------------------------------------------------------------------------
 template <typename K>
-int step_launch(K kern, unsigned grid, const StepArgs& a, const char* who, hipStream_t s) {
-  hipLaunchKernelGGL(kern, dim3(grid), dim3(256), 0, s, a);
+int step_launch(K kern, unsigned grid, int lds, const StepArgs& a, const char* who, hipStream_t s) {
+  hipLaunchKernelGGL(kern, dim3(grid), dim3(256), lds, s, a);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? PALU_OK : fail(PALU_EHIP, "%s launch: %s", who, hipGetErrorString(e));
 }
@@ -683,12 +836,11 @@ template <int L, int NB>
 int step_run_nb(const StepArgs& a, const char* who, hipStream_t s) {
   if (a.rows) {
     const unsigned grid = (unsigned)((a.B + 255) / 256 + a.pre_slots);
-    const int rc = a.pre_cols == 16   ? step_launch(palu_prefix_kernel<L, NB, 1>, grid, a, who, s)
-                   : a.pre_cols == 32 ? step_launch(palu_prefix_kernel<L, NB, 2>, grid, a, who, s)
-                                      : step_launch(palu_prefix_kernel<L, NB, 4>, grid, a, who, s);
+    const int rc = a.pre_cols == 16   ? step_launch(palu_prefix_kernel<L, NB, 1>, grid, 0, a, who, s)
+                                      : step_launch(palu_prefix_kernel<L, NB, 2>, grid, 0, a, who, s);
     if (rc) return rc;
   }
-  return step_launch(palu_step_kernel<L, NB>, (unsigned)step_grid(a.B, a.n_kv), a, who, s);
+  return step_launch(palu_step_kernel<L, NB>, (unsigned)step_grid(a.B, a.n_kv), 0, a, who, s);
 }
 
 template <int L>

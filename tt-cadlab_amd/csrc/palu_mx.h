@@ -49,8 +49,11 @@ typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 // The scale as the conversions take it. (byte 0, memory never written: 2^-127; 255: NaN)
 __device__ __forceinline__ float mx_scale(unsigned byte) { return __builtin_bit_cast(float, byte << 23); }
-// Of byte j of a word.
-__device__ __forceinline__ float mx_scale(unsigned word, int j) { return mx_scale((word >> (8 * j)) & 255u); }
+// Of byte j of a word (j a constant after unrolling): the conversions look at the exponent alone, so that the other bytes may be
+// where sign and mantissa are.
+__device__ __forceinline__ float mx_scale(unsigned word, int j) {
+  return __builtin_bit_cast(float, j < 3 ? word << (23 - 8 * j) : word >> 1);
+}
 
 // Elements 2 p and 2 p + 1 of a word of codes as a pair of bf16 (p < 2 in fp8, < 4 in fp4; a constant after unrolling).
 template <bool FP8>

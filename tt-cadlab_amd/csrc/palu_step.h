@@ -234,6 +234,17 @@ struct Wave {
     }
   }
 
+  // One row's query, 16 bytes a piece. Its signs are turned for a negative scale, so that qscale is not, and the largest score
+  // is that of the largest product.
+  __device__ __forceinline__ void query(int x, const __bf16* from, bool neg) {
+    const unsigned sign = neg ? 0x80008000u : 0u;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const u32x4 u = *reinterpret_cast<const u32x4*>(from + q_chan<L>(s, (threadIdx.x & 63) >> 4)) ^ sign;
+      q[x][s] = __builtin_bit_cast(bf16x8, u);
+    }
+  }
+
   // The block's positions 0 .. seen - 1 (MASK: the rest may hold anything).
   template <bool MASK>
   __device__ __forceinline__ void add(const Raw<L, NB>& r, float qscale, int seen) {
@@ -253,11 +264,9 @@ struct Wave {
 #pragma unroll
       for (int c = 0; c < 2; ++c)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          s[x][c][i] *= qscale;
+        for (int i = 0; i < 4; ++i)
           if (MASK && 8 * g + 4 * c + i >= seen) s[x][c][i] = NEG_INF;
-        }
-      const float top = max8(s[x][0], s[x][1]);
+      const float top = max8(s[x][0], s[x][1]) * qscale;
       if (__any(top > m[x] + LAZY_RESCALE_LOG2)) {
         const float all = wave_max_xor48(top), mn = all > m[x] + LAZY_RESCALE_LOG2 ? all : m[x];
         const float alpha = m[x] == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(m[x] - mn);
@@ -270,7 +279,10 @@ struct Wave {
       }
       const float ref = m[x] == NEG_INF ? 0.f : m[x];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) p[x][j] = (__bf16)__builtin_amdgcn_exp2f(s[x][j >> 2][j & 3] - ref);
+      for (int j = 0; j < 8; ++j) {
+        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][j >> 2][j & 3], qscale, -ref));
+        p[x][j] = (__bf16)(MASK && 8 * g + j >= seen ? 0.f : e);               // (-inf times a scale of 0 would be NaN)
+      }
 #pragma unroll
       for (int j = 0; j < 8; j += 2)
         l[x] = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{p[x][j], p[x][j + 1]}, bf16x2{(__bf16)1.f, (__bf16)1.f}, l[x], false);
@@ -418,8 +430,31 @@ __device__ __forceinline__ int wg_scan(int x, int* part, int& total) {
   return before + s - x;
 }
 
-// How items are cut into pieces of up to len blocks, a workgroup each: the first of a few lengths, from an even share of all blocks
-// on, of which the chip holds all pieces (`slots`) at once, and at least `least`. of(i) gives n items of some blocks each; a thread has
+// Sums of x and y over the workgroup's 256 threads, in every thread and uniform: of counts, exact up to 2^24. `part`: 8 floats.
+__device__ __forceinline__ void wg_sum2(float& x, float& y, float* part) {
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    x += __shfl_xor(x, d);
+    y += __shfl_xor(y, d);
+  }
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) {
+    part[threadIdx.x >> 6] = x;
+    part[4 + (threadIdx.x >> 6)] = y;
+  }
+  __syncthreads();
+  auto all = [&](const float* p) { return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, p[0] + p[1] + p[2] + p[3]))); };
+  x = all(part);
+  y = all(part + 4);
+}
+__device__ __forceinline__ float wg_sum(float x, float* part) {
+  float none = 0.f;
+  wg_sum2(x, none, part);
+  return x;
+}
+
+// How items are cut into pieces of up to len blocks, a workgroup each: the first of a few lengths, from an even share of all
+// blocks (total: in a float, since rows that share their pages can be more blocks than an int holds) on, of which the chip holds all pieces (`slots`) at once, and at least `least`. of(i) gives n items of some blocks each; a thread has
 // i0 .. i1 - 1. Its pieces are number before .. before + mine - 1 of all; where that never fits, at most slots + all items.
 struct Cut {
   int len, before, mine, all;
@@ -429,17 +464,11 @@ struct Items {
   int n, blocks;
 };
 template <typename F>
-__device__ __forceinline__ Cut cut_items(int i0, int i1, int slots, int least, int* scan, F&& of) {
-  int mine = 0, total;
-  for (int i = i0; i < i1; ++i) {
-    const Items x = of(i);
-    mine += x.n * x.blocks;
-  }
-  wg_scan(mine, scan, total);
-  const int share = (total + slots - 1) / slots;
+__device__ __forceinline__ Cut cut_items(float total, int i0, int i1, int slots, int least, int* scan, F&& of) {
+  const int share = (int)ceilf(total / (float)slots * (total < 0x1p24f ? 1.f : 1.f + 0x1p-14f));   // (a little more where it is rounded)
   Cut c;
   for (int t = 0; t < 4; ++t) {           // uniform
-    c.len = max(least, share + share * t / 8);
+    c.len = max(least, share + share / 8 * t + share % 8 * t / 8);
     c.mine = 0;
     for (int i = i0; i < i1; ++i) {
       const Items x = of(i);
@@ -513,45 +542,45 @@ __device__ __forceinline__ void store4(const StepArgs& a, long long at, f32x4 y)
   }
 }
 
-// Parts go to memory and come from there, past the XCD's L2, whichever XCD wrote them.
+// Parts of this launch go to memory and come from there, past the caches, whichever XCD wrote them: system-scope accesses of 4 and
+// of 16 bytes (a piece of 16 is not written or read as one, nor has it to be: a flag says that all of a part is there).
+constexpr int SYSTEM_SCOPE = 1 | 16;      // sc0, sc1
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t parts_at(float* base) {
+  return __builtin_amdgcn_make_buffer_rsrc(base, 0, 0x7fffffff, 0x00027000);   // plain bytes
+}
 __device__ __forceinline__ void store_part(float* p, float x) { __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM); }
 __device__ __forceinline__ float load_part(const float* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM); }
-// Four of them, 8-byte aligned.
-__device__ __forceinline__ void store_part4(float* p, f32x4 x) {
-  typedef unsigned long long u64;
-  const u32x4 u = __builtin_bit_cast(u32x4, x);
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-    __hip_atomic_store(reinterpret_cast<u64*>(p) + i, u[2 * i] | (u64)u[2 * i + 1] << 32, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+__device__ __forceinline__ void store_part4(__amdgpu_buffer_rsrc_t p, int at, f32x4 x) {
+  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), p, at * 4, 0, SYSTEM_SCOPE);
 }
-__device__ __forceinline__ f32x4 load_part4(const float* p) {
-  typedef unsigned long long u64;
-  u32x4 u;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const u64 x = __hip_atomic_load(reinterpret_cast<const u64*>(p) + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-    u[2 * i] = (unsigned)x;
-    u[2 * i + 1] = (unsigned)(x >> 32);
-  }
-  return __builtin_bit_cast(f32x4, u);
+__device__ __forceinline__ f32x4 load_part4(__amdgpu_buffer_rsrc_t p, int at) {
+  return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(p, at * 4, 0, SYSTEM_SCOPE));
 }
 
 template <int L, int NB>
 __global__ __launch_bounds__(256, 2) void palu_step_kernel(const StepArgs a) {
   __shared__ __attribute__((aligned(1024))) char smem[step_lds<L, NB>()];
   const WaveLds<NB> lds{reinterpret_cast<float*>(smem), a.rep};
-  __shared__ int scan[4], found[2];
+  __shared__ int scan[8], found[2];
   __shared__ RowWork found_row;
-  __shared__ float top[16][16];
-  __shared__ Joined sums[256];
+  constexpr int U = 8, MAX_GROUPS = 4;   // parts that a thread has under way, and threads to a column's four channels, at most
+  __shared__ union {
+    float stats[2][U * MAX_GROUPS][16];   // m and l of parts
+    Joined sums[256];
+  } joining;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int per = (a.B + 255) / 256, r0 = min(tid * per, a.B), r1 = min(r0 + per, a.B);
   // this workgroup's piece
   RowWork own;                            // of a thread's only row
   if (r0 < r1) own = row_work(a, r0);
   auto row = [&](int b) { return per == 1 ? own : row_work(a, b); };
-  const Cut cut = cut_items(r0, r1, STEP_WGS, STEP_LEAST, scan, [&](int b) {
-    const RowWork r = row(b);
+  float mine = 0.f;
+  for (int i = r0; i < r1; ++i) {
+    const RowWork r = row(i);
+    mine += (float)a.n_kv * (float)(r.end - r.first);
+  }
+  const Cut cut = cut_items(wg_sum(mine, reinterpret_cast<float*>(scan)), r0, r1, STEP_WGS, STEP_LEAST, scan, [&](int i) {
+    const RowWork r = row(i);
     return Items{a.n_kv, r.end - r.first};
   });
   const int want = blockIdx.x;
@@ -574,17 +603,11 @@ __global__ __launch_bounds__(256, 2) void palu_step_kernel(const StepArgs a) {
   const RowWork r = uniform(found_row);
   const int chunks = uniform(cut.pieces(r.end - r.first)), kvh = uniform(in / chunks), chunk = in - kvh * chunks, wg0 = want - chunk;
   const int len = uniform((r.end - r.first + chunks - 1) / chunks), lo = r.first + chunk * len, hi = min(r.end, lo + len);
-  const int n16 = lane & 15, g = lane >> 4;
-
   Wave<L, NB, 1> st;
   st.clear();
-  {
-    const __bf16* q = a.q + ((long long)b * a.n_q + kvh * a.rep + min(n16, a.rep - 1)) * HD;
-#pragma unroll
-    for (int s = 0; s < 4; ++s) st.q[0][s] = *reinterpret_cast<const bf16x8*>(q + q_chan<L>(s, g));
-  }
+  st.query(0, a.q + ((long long)b * a.n_q + kvh * a.rep + min(lane & 15, a.rep - 1)) * HD, a.qscale < 0.f);
   st.template pass<false>(
-      lo, min(hi, (r.seen + 31) >> 5), r.seen, a.qscale, a.dv, smem + w * place_bytes<L, NB>(),
+      lo, min(hi, (r.seen + 31) >> 5), r.seen, fabsf(a.qscale), a.dv, smem + w * place_bytes<L, NB>(),
       [&](int blk) __attribute__((always_inline)) { return page_of(a, blk < r.pblocks ? r.lead : b, blk); },
       [&](int page, int blk, const char*& k, const char*& v) __attribute__((always_inline)) { place_of(a, page, kvh, blk, k, v); });
   __syncthreads();                        // every wave is done with its places
@@ -594,10 +617,11 @@ __global__ __launch_bounds__(256, 2) void palu_step_kernel(const StepArgs a) {
   const long long part_size = (long long)a.rep * (a.dv + 2);
   if (chunks > 1) {
     float* po = a.part + want * part_size;
+    const __amdgpu_buffer_rsrc_t p4 = parts_at(po);
     for (int e = tid; e < units; e += 256) {
       const int h = e / vecs, d = 4 * (e - h * vecs);
       const Joined j = join_waves(lds, h, d);
-      store_part4(po + h * a.dv + d, j.y);
+      store_part4(p4, h * a.dv + d, j.y);
       if (d == 0) {
         store_part(po + a.rep * a.dv + h, j.m);
         store_part(po + a.rep * a.dv + a.rep + h, j.l);
@@ -610,84 +634,95 @@ __global__ __launch_bounds__(256, 2) void palu_step_kernel(const StepArgs a) {
     const f32x4 y = r.seen == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : j.y * inv;       // a row that sees nothing: zeros
     store4(a, ((long long)b * a.n_q + kvh * a.rep + h) * a.dv + d, y);
   };
-  // The parts: this workgroup's own (in LDS), or all workgroups' (one of which is its own), and the prefix's pieces. First
-  // every column's largest m, then sums over parts, 256 / units threads to a part of 4 channels each.
-  const int n_chunks = chunks == 1 ? 0 : chunks, n_parts = n_chunks + r.pieces;
-  const long long size = (long long)a.pre_cols * (a.dv + 2);
-  auto part = [&](int c, int h, const float*& o, const float*& m, const float*& l) __attribute__((always_inline)) {
-    if (c < n_chunks) {
-      const float* po = a.part + (wg0 + c) * part_size;
-      o = po + h * a.dv;
-      m = po + a.rep * a.dv + h;
-      l = m + a.rep;
-    } else {
-      const int col = r.local * a.rep + h, tile = col / a.pre_cols, x = col - tile * a.pre_cols;
-      const float* po = a.pre + (r.base + (long long)(tile * a.n_kv + kvh) * r.pieces + (c - n_chunks)) * size;
-      o = po + x * a.dv;
-      m = po + a.pre_cols * a.dv + x;
-      l = m + a.pre_cols;
-    }
+  // The parts: this workgroup's own (in LDS), or all workgroups' (one of which is its own), and the prefix's pieces, which the launch
+  // before wrote.
+  const __amdgpu_buffer_rsrc_t parts = parts_at(a.part + wg0 * part_size);
+  const int pre_size = a.pre_cols * (a.dv + 2);
+  auto pieces_of = [&](int h, int& x) {   // the pieces of a head, in column x of theirs
+    const int col = r.local * a.rep + h, tile = r.pieces ? col / a.pre_cols : 0;
+    x = col - tile * a.pre_cols;
+    return a.pre + (r.base + (long long)(tile * a.n_kv + kvh) * r.pieces) * pre_size;
   };
-  if (n_parts) {
-    const int h = tid & 15;
-    float m = NEG_INF;
-    if (h < a.rep)
-      for (int c = tid >> 4; c < n_parts; c += 16) {
-        const float *po, *pm, *pl;
-        part(c, h, po, pm, pl);
-        m = fmaxf(m, load_part(pm));
-      }
-    top[tid >> 4][h] = m;
-  }
-  __syncthreads();
-  const int groups = max(1, 256 / units), grp = min(tid / units, groups);   // (threads past the groups: none)
-  for (int e = groups > 1 ? tid - grp * units : tid; e < units && grp < groups; e += 256) {
-    const int h = e / vecs, d = 4 * (e - h * vecs);
+  const int groups = min(max(1, 256 / units), MAX_GROUPS), grp = groups > 1 ? tid / units : 0, batch = U * groups;
+  for (int e0 = 0; e0 < units; e0 += 256) {                   // (uniform)
+    const int e = groups > 1 ? tid - grp * units : e0 + tid;
+    const bool on = e < units && grp < groups;
+    const int h = on ? e / vecs : 0, d = on ? 4 * (e - h * vecs) : 0;
     Joined j = no_parts();
-    if (n_parts) {
-      float mx = NEG_INF;
+    // n parts, U to each of 256 / units threads at a time, whose loads are all under way together: stat(c, x, m, l) loads the
+    // statistics of part c's column x, four(c) this thread's four channels.
+    auto gather = [&](int n, auto&& stat, auto&& four) __attribute__((always_inline)) {
+      for (int c0 = 0; c0 < n; c0 += batch) {                 // (uniform)
+        float m[MAX_GROUPS], l[MAX_GROUPS];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, top[i][h]);
-      j.m = mx;
-      const float ref = mx == NEG_INF ? 0.f : mx;
-      constexpr int U = 8;                // parts whose loads are under way together
-      for (int c0 = grp; c0 < n_parts; c0 += U * groups) {
+        for (int i = 0; i < MAX_GROUPS; ++i) {
+          if (16 * i >= batch || c0 + 16 * i >= n) break;     // (uniform)
+          stat(min(c0 + 16 * i + (tid >> 4), n - 1), min(tid & 15, a.rep - 1), m[i], l[i]);
+        }
         f32x4 y[U];
-        float m[U], l[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const float *po, *pm, *pl;
-          part(min(c0 + u * groups, n_parts - 1), h, po, pm, pl);
-          m[u] = load_part(pm);
-          l[u] = load_part(pl);
-          y[u] = load_part4(po + d);
+          if (c0 + u * groups >= n) break;                    // (uniform)
+          y[u] = four(min(c0 + u * groups + min(grp, groups - 1), n - 1));
         }
+        __syncthreads();                  // the batch before has been read
+#pragma unroll
+        for (int i = 0; i < MAX_GROUPS; ++i) {
+          const int c = 16 * i + (tid >> 4);
+          if (16 * i >= batch || c0 + 16 * i >= n) break;
+          joining.stats[0][c][tid & 15] = m[i];
+          joining.stats[1][c][tid & 15] = l[i];
+        }
+        __syncthreads();
+        if (!on) continue;
+        Joined b = no_parts();
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          if (c0 + u * groups >= n_parts) continue;
-          const float f = __builtin_amdgcn_exp2f(m[u] - ref);
-          j.l += f * l[u];
-          j.y += f * y[u];
+          if (c0 + u * groups + grp >= n) break;
+          b.m = fmaxf(b.m, joining.stats[0][u * groups + grp][h]);
         }
+        const float ref = b.m == NEG_INF ? 0.f : b.m;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (c0 + u * groups + grp >= n) break;
+          const float f = __builtin_amdgcn_exp2f(joining.stats[0][u * groups + grp][h] - ref);
+          b.l += f * joining.stats[1][u * groups + grp][h];
+          b.y += f * y[u];
+        }
+        j.add(b.y, b.m, b.l);
       }
-    }
-    if (chunks == 1 && grp == 0) {
-      const Joined own_part = join_waves(lds, h, d);
-      j.add(own_part.y, own_part.m, own_part.l);
+    };
+    gather(chunks == 1 ? 0 : chunks, [&](int c, int x, float& m, float& l) __attribute__((always_inline)) {
+             const float* p = a.part + (wg0 + c) * part_size + a.rep * a.dv + x;
+             m = load_part(p);
+             l = load_part(p + a.rep);
+           }, [&](int c) __attribute__((always_inline)) { return load_part4(parts, c * (int)part_size + h * a.dv + d); });
+    int col, stat_col;
+    const float *pre = pieces_of(h, col), *stats = pieces_of(min(tid & 15, a.rep - 1), stat_col);
+    gather(r.pieces, [&](int c, int x, float& m, float& l) __attribute__((always_inline)) {
+             const float* p = stats + (long long)c * pre_size + a.pre_cols * a.dv + stat_col;
+             m = p[0];
+             l = p[a.pre_cols];
+           }, [&](int c) __attribute__((always_inline)) {
+             return *reinterpret_cast<const f32x4*>(pre + (long long)c * pre_size + col * a.dv + d);
+           });
+    if (on && chunks == 1 && grp == 0) {
+      const Joined mine = join_waves(lds, h, d);
+      j.add(mine.y, mine.m, mine.l);
     }
     if (groups == 1) {
-      finish(h, d, j);
-    } else {
-      sums[tid] = j;
+      if (on) finish(h, d, j);
+      continue;
     }
-  }
-  if (groups > 1) {
+    __syncthreads();                      // the last batch has been read
+    if (on) joining.sums[tid] = j;
     __syncthreads();
     if (tid < units) {
-      Joined j = sums[tid];
-      for (int i = 1; i < groups; ++i) j.add(sums[tid + i * units].y, sums[tid + i * units].m, sums[tid + i * units].l);
-      const int h = tid / vecs;
-      finish(h, 4 * (tid - h * vecs), j);
+      for (int i = 1; i < groups; ++i) {
+        const Joined x = joining.sums[tid + i * units];
+        j.add(x.y, x.m, x.l);
+      }
+      finish(h, d, j);
     }
   }
 }
@@ -715,12 +750,12 @@ inline size_t pre_bytes(int B, int n_groups, int rep, int n_kv, int dv) {
 struct Group {
   int row, rows, blocks;                  // blocks: of the prefix, 0 where nothing is shared
 };
-__device__ __forceinline__ Group group_of(const StepArgs& a, int gi) {
+__device__ __forceinline__ Group group_of(const StepArgs& a, int gi, bool lone) {
   const int c0 = a.cu ? a.cu[gi] : 0, c1 = a.cu ? a.cu[gi + 1] : a.B;
   Group g;
   g.row = min(max(c0, 0), a.B);
   g.rows = min(max(c1, g.row), a.B) - g.row;
-  g.blocks = g.rows > 1 ? min(max(a.shared[gi], 0), a.capacity) >> 5 : 0;      // (a lone row has its blocks to itself)
+  g.blocks = g.rows > (lone ? 0 : 1) ? min(max(a.shared[gi], 0), a.capacity) >> 5 : 0;
   return g;
 }
 
@@ -728,15 +763,25 @@ template <int L, int NB, int C>
 __global__ __launch_bounds__(256, 2) void palu_prefix_kernel(const StepArgs a) {
   __shared__ __attribute__((aligned(1024))) char smem[step_lds<L, NB>()];
   const WaveLds<NB> lds{reinterpret_cast<float*>(smem), 16};
-  __shared__ int scan[4], found[4], bases[256];
+  __shared__ int scan[8], found[4], bases[256];
   constexpr int COLS = 16 * C;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int per = (a.n_groups + 255) / 256, g0 = min(tid * per, a.n_groups), g1 = min(g0 + per, a.n_groups);
   auto tiles_of = [&](const Group& g) { return g.blocks ? (g.rows * a.rep + COLS - 1) / COLS * a.n_kv : 0; };   // of all KV heads
-  Group own;                              // a thread's only group
-  if (g0 < g1) own = group_of(a, g0);
-  auto group = [&](int i) { return per == 1 ? own : group_of(a, i); };
-  const Cut cut = cut_items(g0, g1, PRE_WGS, PRE_LEAST, scan, [&](int i) {
+  // Lone rows' blocks that groups "share" are read here too if there are no more of them than of larger groups: then they do not keep a few
+  // workgroups of the second launch busy when all others are done (16 groups of 64 rows over 2048 positions, one of them of a single row:
+  // 39 -> 28 us). Else the second launch is the better place, which reads them past the L2.
+  Group own{0, 0, 0};                     // a thread's only group
+  float of_lone = 0.f, of_larger = 0.f;
+  for (int i = g0; i < g1; ++i) {
+    own = group_of(a, i, true);
+    (own.rows > 1 ? of_larger : of_lone) += (float)tiles_of(own) * (float)own.blocks;
+  }
+  wg_sum2(of_lone, of_larger, reinterpret_cast<float*>(scan));
+  const bool lone = of_lone <= of_larger;
+  if (!lone && own.rows == 1) own.blocks = 0;
+  auto group = [&](int i) { return per == 1 ? own : group_of(a, i, lone); };
+  const Cut cut = cut_items(of_larger + (lone ? of_lone : 0.f), g0, g1, PRE_WGS, PRE_LEAST, scan, [&](int i) {
     const Group g = group(i);
     return Items{tiles_of(g), g.blocks};
   });
@@ -753,11 +798,11 @@ __global__ __launch_bounds__(256, 2) void palu_prefix_kernel(const StepArgs a) {
       else end = mid;
     }
     RowPrefix r{b, 0, 0, 0, 0, {}};
-    const Group g = group_of(a, gi);
+    const Group g = group_of(a, gi, lone);
     if (g.blocks && b >= g.row && b < g.row + g.rows) {
       int base = bases[gi / per];
       for (int i = gi / per * per; i < gi; ++i) {
-        const Group x = group_of(a, i);
+        const Group x = group_of(a, i, lone);
         base += tiles_of(x) * cut.pieces(x.blocks);
       }
       const int pieces = cut.pieces(g.blocks);
@@ -792,18 +837,15 @@ __global__ __launch_bounds__(256, 2) void palu_prefix_kernel(const StepArgs a) {
   const int pieces = uniform(cut.pieces(g.blocks)), tile = uniform(in / pieces), piece = in - tile * pieces;
   const int ct = uniform(tile / a.n_kv), kvh = tile - ct * a.n_kv;
   const int each = uniform((g.blocks + pieces - 1) / pieces), lo = piece * each, hi = min(g.blocks, lo + each);
-  const int n16 = lane & 15, gl = lane >> 4;
   Wave<L, NB, C> st;
   st.clear();
 #pragma unroll
   for (int x = 0; x < C; ++x) {
-    const int col = min(ct * COLS + 16 * x + n16, g.rows * a.rep - 1), row = col / a.rep;   // columns past the group repeat its last
-    const __bf16* q = a.q + ((long long)(g.row + row) * a.n_q + kvh * a.rep + (col - row * a.rep)) * HD;
-#pragma unroll
-    for (int s = 0; s < 4; ++s) st.q[x][s] = *reinterpret_cast<const bf16x8*>(q + q_chan<L>(s, gl));
+    const int col = min(ct * COLS + 16 * x + (lane & 15), g.rows * a.rep - 1), row = col / a.rep;   // columns past the group repeat its last
+    st.query(x, a.q + ((long long)(g.row + row) * a.n_q + kvh * a.rep + (col - row * a.rep)) * HD, a.qscale < 0.f);
   }
   st.template pass<true>(
-      lo, hi, 32 * g.blocks, a.qscale, a.dv, smem + w * place_bytes<L, NB>(), [&](int blk) __attribute__((always_inline)) { return page_of(a, g.row, blk); },
+      lo, hi, 32 * g.blocks, fabsf(a.qscale), a.dv, smem + w * place_bytes<L, NB>(), [&](int blk) __attribute__((always_inline)) { return page_of(a, g.row, blk); },
       [&](int page, int blk, const char*& k, const char*& v) __attribute__((always_inline)) { place_of(a, page, kvh, blk, k, v); });
   float* po = a.pre + (long long)want * COLS * (a.dv + 2);
   const int vecs = a.dv / 4;

@@ -324,7 +324,7 @@ class MXCache:
 
     @property
     def shape(self) -> Tuple[int, int, int, int]:
-        B, G, nblk = self.data.shape[:3]
+        B, G, nblk, _ = self.data.shape
         return (B, G, nblk * BLOCK, self.width)
 
     @property

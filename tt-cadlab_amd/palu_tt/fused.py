@@ -177,7 +177,7 @@ def _cache_arg(t, name: str, device, role: Optional[str] = None, mx: bool = Fals
         if not (role is None or t.role == role):
             raise RuntimeError(f"{name} is an MXCache in {t.role!r} order; this argument reads a {role!r} cache")
         layout = _native.LAYOUT_MX8 if t.fmt == "fp8" else _native.LAYOUT_MX4
-        return t.data, tuple(t.shape), layout + (1 if role is None and t.role == "v" else 0)
+        return t.data, t.shape, layout + (1 if role is None and t.role == "v" else 0)
     if isinstance(t, GroupedLatentCache):
         _as_dev(t.data, name, torch.bfloat16, device)
         if not (role is not None and t.role == role):
@@ -215,12 +215,12 @@ def _glrd_workspace(batch: int, n_q: int, n_kv: int, n_groups: int, seq_len: int
 def _cur_pos(cur_pos_tensor: torch.Tensor, batch: int, device) -> torch.Tensor:
     if not isinstance(cur_pos_tensor, torch.Tensor):
         raise RuntimeError("cur_pos_tensor must be a torch.Tensor")
-    cp = cur_pos_tensor.reshape(-1)
+    cp = cur_pos_tensor if cur_pos_tensor.dim() == 1 else cur_pos_tensor.reshape(-1)
     if cp.numel() != batch:
         raise RuntimeError(f"cur_pos_tensor has {cp.numel()} entries for batch {batch}")
     if cp.device != device or cp.dtype != torch.int32:
         cp = cp.to(device=device, dtype=torch.int32)
-    return cp.contiguous()
+    return cp if cp.is_contiguous() else cp.contiguous()
 
 
 def _page_table(page_table_tensor, batch: int, device) -> torch.Tensor:
@@ -231,7 +231,7 @@ def _page_table(page_table_tensor, batch: int, device) -> torch.Tensor:
     pt = page_table_tensor
     if pt.device != device or pt.dtype != torch.int32:
         pt = pt.to(device=device, dtype=torch.int32)
-    return pt.contiguous()
+    return pt if pt.is_contiguous() else pt.contiguous()
 
 
 def _pool_dims(k_shape, v_shape, q, page_table_tensor, dev, what):
@@ -441,7 +441,7 @@ def _step_out(q, n_kv: int, width: int, out_dtype, out, workspace, need: int, in
     """(out, workspace) of a decode over packed or quantised pools: out checked or made, the workspace checked or made."""
     _, B, n_q, _ = q.shape
     dev = q.device
-    _native.refuse_derivatives("flash_decode over these caches", q, *(t for t in inputs if t.is_floating_point()))
+    _native.refuse_derivatives("flash_decode over these caches", q, inputs[0], inputs[1])
     if out_dtype not in _DTYPES:
         raise RuntimeError(f"out_dtype must be torch.float32 or torch.bfloat16, got {out_dtype}")
     made = workspace is None
@@ -454,7 +454,7 @@ def _step_out(q, n_kv: int, width: int, out_dtype, out, workspace, need: int, in
     _as_dev(out, "out", out_dtype, dev)
     if tuple(out.shape) != (1, B, n_q, width):
         raise RuntimeError(f"out must be [1, {B}, {n_q}, {width}]")
-    if any(_overlap(out, t) for t in (q, *inputs) + (() if made else (workspace,))):
+    if any(t is not None and _overlap(out, t) for t in (q, *inputs) + (() if made else (workspace,))):
         raise RuntimeError("out must be memory of its own: it overlaps an input or the workspace")
     return out, workspace
 
@@ -463,7 +463,7 @@ def _mx_decode(q, k, v, cp, pt, out, workspace, scale, n_kv, positions, n_pages,
     """flash_decode over the storages k, v of an MXCache pair."""
     _, B, n_q, _ = q.shape
     need = _native.load().palu_mx_decode_workspace_bytes(B, n_q, n_kv, width)
-    out, ws = _step_out(q, n_kv, width, out_dtype, out, workspace, need, [t for t in (k, v, cp, pt) if t is not None])
+    out, ws = _step_out(q, n_kv, width, out_dtype, out, workspace, need, (k, v, cp, pt))
     sc = float(HEAD_DIM ** -0.5 if scale is None else scale)
     if pt is None:
         _native.launch("flash_decode", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), cp.data_ptr(), out.data_ptr(), sc, B, n_q,
@@ -508,8 +508,7 @@ def flash_decode_shared(q, k, v, cur_pos_tensor, page_table_tensor, shared_len, 
     shared = _seq_ints(shared_len, "shared_len", n, dev)
     n_q = q.shape[2]
     need = _native.load().palu_flash_decode_shared_workspace_bytes(B, n, n_q, n_kv, width)
-    out, ws = _step_out(q, n_kv, width, out_dtype, out, workspace, need,
-                        [t for t in (k_store, v_store, cp, pt, cu, shared) if t is not None])
+    out, ws = _step_out(q, n_kv, width, out_dtype, out, workspace, need, (k_store, v_store, cp, pt, cu, shared))
     if B == 0:
         return out
     _native.launch("flash_decode_shared", dev, q.data_ptr(), k_store.data_ptr(), v_store.data_ptr(), cp.data_ptr(), pt.data_ptr(),
@@ -566,7 +565,7 @@ def _seq_ints(t, name: str, n: Optional[int], device) -> torch.Tensor:
         raise RuntimeError(f"{name} must be an integer tensor [{'B + 1' if n is None else n}]")
     if t.device != device or t.dtype != torch.int32:
         t = t.to(device=device, dtype=torch.int32)
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _strided_rows(t, name: str, width: Optional[int], device=None):

@@ -286,6 +286,16 @@ def test_batches(gpu, layout, B, groups, prefix, tail, nq, nkv):
     x.check(x.decode_shared(), rows=list(range(0, B, max(1, B // 24))) + [B - 1])
 
 
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("rows", [[4, 1, 1], [1, 3, 1, 1, 1], [2, 1], [1, 2, 1, 1], [1, 1, 1], [1]], ids=str)
+def test_lone_rows_beside_groups(gpu, layout, rows):
+    """Rows that are a group of their own: few enough that they are read with the larger groups, too many for that, only such."""
+    shared = [900 if n == 1 else 700 for n in rows]
+    lens = [s + 13 * i for i, (n, s) in enumerate(zip(rows, shared)) for _ in range(n)]
+    x = Batch(gpu, layout, lens, 8, 2, 64, 64, rows, shared, seed=len(lens))
+    x.check(x.decode_shared())
+
+
 @pytest.mark.parametrize("layout", ["rows", "tiled"])
 @pytest.mark.parametrize("w", [16, 32, 48, 80, 96, 112, 128])
 def test_shared_widths_bf16(gpu, layout, w):

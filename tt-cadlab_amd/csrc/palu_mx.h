@@ -5,7 +5,8 @@
 //
 // The scale of a block is the smallest power of two, from 2^-117 on, over which its largest value is at most 464 (7): it then
 // is within half a step of 448 (6) and no element is further than that from what it is held as. 2^-117 is where every held
-// value but 0 is a normal number; smaller blocks keep the absolute error of that scale (2^-127 in fp8, 2^-119 in fp4). Magnitudes past 1.75 2^127 are taken as that, so that what is read back is finite.
+// value but 0 is a normal number; smaller blocks keep the absolute error of that scale (2^-127 in fp8, 2^-119 in fp4).
+// Magnitudes past 1.75 2^127 are taken as that, so that what is read back is finite.
 //
 // A 32-position block of a cache w wide: its elements in the order that the attention's products take them, then the scales.
 //   K order, position 8 t + 4 c + i (t < 4, c < 2, i < 4), n = 4 t + i:
@@ -60,7 +61,8 @@ template <bool FP8>
 __device__ __forceinline__ unsigned mx_pair(unsigned word, int p, float scale) {
   bf16x2 r;
   if constexpr (FP8) {
-    r = p ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(word, scale, true) : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(word, scale, false);
+    r = p ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(word, scale, true)
+          : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(word, scale, false);
   } else {
     r = p == 0   ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 0)
         : p == 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 1)

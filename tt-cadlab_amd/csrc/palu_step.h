@@ -3,16 +3,24 @@
 //   out[b][h] = sum_{p <= cur[b]} softmax_p(scale q[b][h] . k[p][j]) v[p][j],   j = h / rep, rep = n_q / n_kv.
 // Included by one translation unit per family of layouts.
 //
-// A wave takes whole 32-position blocks, straight from memory into registers, the next block's loads under way while it
-// computes, and the four waves of a workgroup take every fourth block. Its columns are up to 16 C queries:
+// A wave takes whole 32-position blocks, the four waves of a workgroup every fourth (in fp4 every fourth pair). Its columns are
+// up to 16 C queries:
 //   S^T (keys x columns) = K Q^T, two v_mfma_f32_16x16x32_bf16 tiles of 16 keys, Q the B operand, in registers;
 //   P^T = 2^(S^T - m), the running maximum m refreshed when a score exceeds it by more than 2^8;
 //   O^T (channels x columns) += V^T P^T.
 // The rows of the K operand are the keys in the order of the caches' K tiles: the two accumulators then leave a lane with
 // the eight keys 8 g .. + 7 of its column, which is the B operand of the second product, and no value changes lanes. Tiled
 // and quantised caches hold both operands as they are taken, 8 bytes or more of a lane in one piece; a quantised value is
-// turned into bf16 (exactly) between memory and product, a lane's 32 channels of a key under one scale, two channels of a position
-// under one scale of V, which two byte permutations make pairs of positions. Row-major V is read in the same pairs.
+// turned into bf16 (exactly) between memory and product, a lane's 32 channels of a key under one scale, two channels of a
+// position under one scale of V, which two byte permutations make pairs of positions. Row-major V is read in the same pairs.
+//
+// Bound by memory for long batches: 32 rows of 8192 positions, 8 KV heads, in fp8 554 MB in 88 us, 6.3 TB/s (a copy of this card
+// reaches 4.9, a pure read 6.3), in fp4 285 MB in 52 us. For that a wave has a block of 8 KB or more on its way while it computes
+// another: copies straight to LDS, which take no registers, and not kept in the caches (kept there fp8 took 102 us); the next copy
+// goes out as soon as the block is in registers. A second block in registers spilled, and so did three workgroups a CU (115 us).
+// Page ids are uniform and read as scalars a turn early: as vector loads each was waited for together with the blocks before it.
+// Short ones are a chain of latencies: a launch 4 us, lengths, pages and queries 2, a first block 1 to 2, and where a row is cut, 3
+// for the pieces to meet (one row of 300 positions: 9 us; of 2048: 12; of 32768: 21 in fp4, 23 in fp8).
 //
 // Rounding: products of bf16 are exact in fp32, scores, statistics and sums are fp32; the probabilities are rounded to bf16
 // for the second product, by up to 2^-8 of each, and it is the rounded ones that are summed to divide by.
@@ -100,10 +108,14 @@ __device__ __forceinline__ void copy_block(char* to, const char* k, const char* 
   const unsigned l16 = lane * 16;
   if constexpr (L == PALU_LAYOUT_ROWS) {  // key (c, n), channels 32 s + 8 g .. + 7
 #pragma unroll
-    for (int i = 0; i < R::KI; ++i) one(k + (unsigned)((8 * (n >> 2) + 4 * (i >> 2) + (n & 3)) * (2 * HD) + (i & 3) * 64 + g * 16), i);
+    for (int i = 0; i < R::KI; ++i) {
+      const int key = 8 * (n >> 2) + 4 * (i >> 2) + (n & 3);
+      one(k + (unsigned)(key * (2 * HD) + (i & 3) * 64 + g * 16), i);
+    }
   } else {
 #pragma unroll
-    for (int i = 0; i < R::KI; i += 4) run(k + i * 1024 + l16, to + i * 1024, std::integral_constant<int, (R::KI > 4 ? 4 : R::KI)>());
+    for (int i = 0; i < R::KI; i += 4)
+      run(k + i * 1024 + l16, to + i * 1024, std::integral_constant<int, (R::KI > 4 ? 4 : R::KI)>());
   }
   char* tv = to + R::KI * 1024;
   if constexpr (L == PALU_LAYOUT_TILED || L == PALU_LAYOUT_ROWS) {
@@ -115,20 +127,25 @@ __device__ __forceinline__ void copy_block(char* to, const char* k, const char* 
     run(v + l16, tv, std::integral_constant<int, FULL>());
     if constexpr (FULL < R::VI) one(v + FULL * 1024 + min(l16, 512u - 16), R::KI + FULL);
     // 128 bytes of K's scales, then those of V
-    const char* from = lane < 32 ? k + mx_codes(R::FP8, HD) + 4 * lane : v + mx_codes(R::FP8, 32 * NB) + min(4 * (lane - 32), 32 * NB - 4);
+    const char *ks = k + mx_codes(R::FP8, HD), *vs = v + mx_codes(R::FP8, 32 * NB);
+    const char* from = lane < 32 ? ks + 4 * lane : vs + min(4 * (lane - 32), 32 * NB - 4);
     __builtin_amdgcn_global_load_lds((gvoid*)from, (lvoid*)(to + (R::KI + R::VI) * 1024), 4, 0, NT ? 2 : 0);
   }
 }
+// K's part of the registers out of its elements and scales (a copy in LDS, or all but row-major ones as they lie in memory), then
+// V's.
 template <int L, int NB>
-__device__ __forceinline__ void read_block(Raw<L, NB>& r, const char* s, int dv) {
-  using R = Raw<L, NB>;
-  const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+__device__ __forceinline__ void read_k(Raw<L, NB>& r, const char* k, const char* scales) {
+  const unsigned lane = threadIdx.x & 63;
 #pragma unroll
-  for (int i = 0; i < R::KI; ++i) r.k[i] = *reinterpret_cast<const u32x4*>(s + i * 1024 + lane * 16);
-  const char* v = s + R::KI * 1024;
+  for (int i = 0; i < Raw<L, NB>::KI; ++i) r.k[i] = *reinterpret_cast<const u32x4*>(k + i * 1024 + lane * 16);
+  if constexpr (is_mx(L)) r.ks = *reinterpret_cast<const unsigned short*>(scales + 2 * lane);
+}
+template <int L, int NB, bool LDS>
+__device__ __forceinline__ void read_v(Raw<L, NB>& r, const char* v, const char* scales, int dv) {
+  using R = Raw<L, NB>;
+  const unsigned lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   if constexpr (R::MX) {
-    const char* sc = s + (R::KI + R::VI) * 1024;
-    r.ks = *reinterpret_cast<const unsigned short*>(sc + 2 * lane);
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       if constexpr (R::FP8) {
@@ -138,18 +155,28 @@ __device__ __forceinline__ void read_block(Raw<L, NB>& r, const char* s, int dv)
         r.v[b / 2][2 * (b & 1)] = x[0];
         r.v[b / 2][2 * (b & 1) + 1] = x[1];
       }
-      r.vs[b] = *reinterpret_cast<const u32x2*>(sc + 128 + b * 32 + 8 * g);
+      r.vs[b] = *reinterpret_cast<const u32x2*>(scales + b * 32 + 8 * g);
     }
   } else if constexpr (L == PALU_LAYOUT_TILED) {
 #pragma unroll
-    for (int i = 0; i < R::VI; ++i) r.v[i] = *reinterpret_cast<const u32x4*>(v + i * 1024 + lane * 16);
+    for (int i = 0; i < R::VI; ++i)
+      r.v[i] = *reinterpret_cast<const u32x4*>(v + (LDS ? i : min(i, dv / 16 - 1)) * 1024 + lane * 16);
   } else {
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
-      for (int j = 0; j < 8; ++j)         // position 8 g + j, channels 32 b + 2 n and 2 n + 1
-        r.v[2 * b + j / 4][j & 3] = *reinterpret_cast<const unsigned*>(v + (8 * g + j) * (2 * dv) + min(64 * b + 4 * n, 2 * dv - 4));
+      for (int j = 0; j < 8; ++j) {       // position 8 g + j, channels 32 b + 2 n and 2 n + 1
+        const char* pair = v + (8 * g + j) * (2 * dv) + min(64 * b + 4 * n, 2u * dv - 4);
+        r.v[2 * b + j / 4][j & 3] = *reinterpret_cast<const unsigned*>(pair);
+      }
   }
+}
+template <int L, int NB>
+__device__ __forceinline__ void read_block(Raw<L, NB>& r, const char* s, int dv) {
+  using R = Raw<L, NB>;
+  const char* sc = s + (R::KI + R::VI) * 1024;
+  read_k<L, NB>(r, s, sc);
+  read_v<L, NB, true>(r, s + R::KI * 1024, sc + 128, dv);
 }
 
 // Neighbouring blocks that a wave takes together: some 8 KB or more on their way to it.
@@ -246,8 +273,8 @@ struct Wave {
   }
 
   // The block's positions 0 .. seen - 1 (MASK: the rest may hold anything).
-  template <bool MASK>
-  __device__ __forceinline__ void add(const Raw<L, NB>& r, float qscale, int seen) {
+  template <bool MASK, typename AK, typename AV>
+  __device__ __forceinline__ void add(const Raw<L, NB>& r, float qscale, int seen, AK&& after_k, AV&& after_v) {
     const int g = (threadIdx.x & 63) >> 4;
     f32x4 s[C][2];
 #pragma unroll
@@ -258,6 +285,7 @@ struct Wave {
 #pragma unroll
         for (int x = 0; x < C; ++x) s[x][c] = mfma16(k, q[x][i], i == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : s[x][c]);
       }
+    after_k();
     bf16x8 p[C];
 #pragma unroll
     for (int x = 0; x < C; ++x) {
@@ -300,6 +328,43 @@ struct Wave {
 #pragma unroll
         for (int x = 0; x < C; ++x) o[x][2 * b + t] = mfma16(__builtin_bit_cast(bf16x8, y[t]), p[x], o[x][2 * b + t]);
       }
+    }
+    after_v();
+  }
+  template <bool MASK>
+  __device__ __forceinline__ void add(const Raw<L, NB>& r, float qscale, int seen) {
+    add<MASK>(r, qscale, seen, [] {}, [] {});
+  }
+
+  // The same over whole blocks straight from memory into the registers, the next block's K as soon as this one's scores are done,
+  // its V after this one's products: for blocks that several workgroups read and the L2 holds, the way over LDS is the longer
+  // one (64 rows with a prefix of 8192 in bf16: 24.4 -> 22.3 us). Blocks that are read once are longer on their way.
+  template <int NW, typename P, typename F>
+  __device__ __forceinline__ void pass_direct(int first, int end, float qscale, int dv, P&& page_at, F&& where) {
+    first += __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    if (first >= end) return;
+    Raw<L, NB> r;
+    const char *k, *v;
+    constexpr int KS = is_mx(L) ? mx_codes(mx_fp8(L), HD) : 0, VS = is_mx(L) ? mx_codes(mx_fp8(L), 32 * NB) : 0;
+    where(page_at(first), first, k, v);
+    int page = page_at(min(first + NW, end - 1));
+    read_k<L, NB>(r, k, k + KS);
+    read_v<L, NB, false>(r, v, v + VS, dv);
+    for (int blk = first; blk < end; blk += NW) {
+      const int next = min(blk + NW, end - 1);
+      where(page, next, k, v);
+      page = page_at(min(blk + 2 * NW, end - 1));
+      add<false>(r, qscale, 32,
+          [&]() __attribute__((always_inline)) {
+            __builtin_amdgcn_sched_barrier(0);
+            read_k<L, NB>(r, k, k + KS);
+            __builtin_amdgcn_sched_barrier(0);
+          },
+          [&]() __attribute__((always_inline)) {
+            __builtin_amdgcn_sched_barrier(0);
+            read_v<L, NB, false>(r, v, v + VS, dv);
+            __builtin_amdgcn_sched_barrier(0);
+          });
     }
   }
 
@@ -443,7 +508,9 @@ __device__ __forceinline__ void wg_sum2(float& x, float& y, float* part) {
     part[4 + (threadIdx.x >> 6)] = y;
   }
   __syncthreads();
-  auto all = [&](const float* p) { return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, p[0] + p[1] + p[2] + p[3]))); };
+  auto all = [](const float* p) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, p[0] + p[1] + p[2] + p[3])));
+  };
   x = all(part);
   y = all(part + 4);
 }
@@ -454,8 +521,11 @@ __device__ __forceinline__ float wg_sum(float x, float* part) {
 }
 
 // How items are cut into pieces of up to len blocks, a workgroup each: the first of a few lengths, from an even share of all
-// blocks (total: in a float, since rows that share their pages can be more blocks than an int holds) on, of which the chip holds all pieces (`slots`) at once, and at least `least`. of(i) gives n items of some blocks each; a thread has
-// i0 .. i1 - 1. Its pieces are number before .. before + mine - 1 of all; where that never fits, at most slots + all items.
+// blocks on (total: a float, since rows that share their pages can be more blocks than an int holds), of which the chip holds
+// all pieces (`slots`) at once, and at least `least`. of(i) gives n items of some blocks each; a thread has i0 .. i1 - 1. Its
+// pieces are number before .. before + mine - 1 of all; where they never fit, they are at most slots + all items. Whole shares of
+// items, some workgroups with a little less to do, were faster than even shares that begin and end inside items and join more
+// parts (64 rows of up to 2304 positions in fp4: 33 us against 37).
 struct Cut {
   int len, before, mine, all;
   __device__ __forceinline__ int pieces(int blocks) const { return (blocks + len - 1) / len; }
@@ -465,7 +535,8 @@ struct Items {
 };
 template <typename F>
 __device__ __forceinline__ Cut cut_items(float total, int i0, int i1, int slots, int least, int* scan, F&& of) {
-  const int share = (int)ceilf(total / (float)slots * (total < 0x1p24f ? 1.f : 1.f + 0x1p-14f));   // (a little more where it is rounded)
+  const float up = total < 0x1p24f ? 1.f : 1.f + 0x1p-14f;    // (the total may be rounded)
+  const int share = (int)ceilf(total / (float)slots * up);
   Cut c;
   for (int t = 0; t < 4; ++t) {           // uniform
     c.len = max(least, share + share / 8 * t + share % 8 * t / 8);
@@ -496,7 +567,9 @@ __device__ __forceinline__ void place_of(const StepArgs& a, int page, int kvh, i
 // ---- the rows' own blocks -----------------------------------------------------------------------
 // An item is a row's KV head: its blocks, but for those that have been read with the group's prefix, cut into even pieces. The
 // pieces of an item are joined by the workgroup that finds all of them done.
-constexpr int STEP_LEAST = 16;            // blocks of a piece, at least
+// Blocks of a piece, at least: four turns of its waves (fp4: two). With 8 a row of 2048 positions is 1.5 us faster, rows of 300 and 512
+// 1.5 to 3 us slower, for they are cut then.
+constexpr int STEP_LEAST = 16;
 constexpr int STEP_WGS = 512;             // workgroups that the chip holds at once, by the kernel's LDS and registers
 inline int step_grid(int B, int n_kv) { return STEP_WGS + B * n_kv; }
 inline size_t step_bytes(int B, int n_kv, int rep, int dv) {
@@ -542,14 +615,18 @@ __device__ __forceinline__ void store4(const StepArgs& a, long long at, f32x4 y)
   }
 }
 
-// Parts of this launch go to memory and come from there, past the caches, whichever XCD wrote them: system-scope accesses of 4 and
-// of 16 bytes (a piece of 16 is not written or read as one, nor has it to be: a flag says that all of a part is there).
+// Parts of this launch go to memory and come from there, past the caches, whichever XCD wrote them: system-scope accesses of 4
+// and of 16 bytes (which need not be one piece: a flag says that all of a part is there).
 constexpr int SYSTEM_SCOPE = 1 | 16;      // sc0, sc1
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t parts_at(float* base) {
   return __builtin_amdgcn_make_buffer_rsrc(base, 0, 0x7fffffff, 0x00027000);   // plain bytes
 }
-__device__ __forceinline__ void store_part(float* p, float x) { __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM); }
-__device__ __forceinline__ float load_part(const float* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM); }
+__device__ __forceinline__ void store_part(float* p, float x) {
+  __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+}
+__device__ __forceinline__ float load_part(const float* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+}
 __device__ __forceinline__ void store_part4(__amdgpu_buffer_rsrc_t p, int at, f32x4 x) {
   __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), p, at * 4, 0, SYSTEM_SCOPE);
 }
@@ -601,7 +678,8 @@ __global__ __launch_bounds__(256, 2) void palu_step_kernel(const StepArgs a) {
   __syncthreads();
   const int b = __builtin_amdgcn_readfirstlane(found[0]), in = __builtin_amdgcn_readfirstlane(found[1]);
   const RowWork r = uniform(found_row);
-  const int chunks = uniform(cut.pieces(r.end - r.first)), kvh = uniform(in / chunks), chunk = in - kvh * chunks, wg0 = want - chunk;
+  const int chunks = uniform(cut.pieces(r.end - r.first)), kvh = uniform(in / chunks), chunk = in - kvh * chunks;
+  const int wg0 = want - chunk;           // the item's first piece
   const int len = uniform((r.end - r.first + chunks - 1) / chunks), lo = r.first + chunk * len, hi = min(r.end, lo + len);
   Wave<L, NB, 1> st;
   st.clear();
@@ -609,7 +687,9 @@ __global__ __launch_bounds__(256, 2) void palu_step_kernel(const StepArgs a) {
   st.template pass<false>(
       lo, min(hi, (r.seen + 31) >> 5), r.seen, fabsf(a.qscale), a.dv, smem + w * place_bytes<L, NB>(),
       [&](int blk) __attribute__((always_inline)) { return page_of(a, blk < r.pblocks ? r.lead : b, blk); },
-      [&](int page, int blk, const char*& k, const char*& v) __attribute__((always_inline)) { place_of(a, page, kvh, blk, k, v); });
+      [&](int page, int blk, const char*& k, const char*& v) __attribute__((always_inline)) {
+        place_of(a, page, kvh, blk, k, v);
+      });
   __syncthreads();                        // every wave is done with its places
   to_lds(lds, st, 0);
   __syncthreads();
@@ -634,8 +714,8 @@ __global__ __launch_bounds__(256, 2) void palu_step_kernel(const StepArgs a) {
     const f32x4 y = r.seen == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : j.y * inv;       // a row that sees nothing: zeros
     store4(a, ((long long)b * a.n_q + kvh * a.rep + h) * a.dv + d, y);
   };
-  // The parts: this workgroup's own (in LDS), or all workgroups' (one of which is its own), and the prefix's pieces, which the launch
-  // before wrote.
+  // The parts: this workgroup's own (in LDS), or all workgroups' (one of which is its own), and the prefix's pieces, which the
+  // launch before wrote.
   const __amdgpu_buffer_rsrc_t parts = parts_at(a.part + wg0 * part_size);
   const int pre_size = a.pre_cols * (a.dv + 2);
   auto pieces_of = [&](int h, int& x) {   // the pieces of a head, in column x of theirs
@@ -741,7 +821,9 @@ inline int pre_tile(int B, int n_groups, int rep) {         // C by the average 
 // Column tiles of all groups, at most, and pieces: tiles of n blocks are cut into at most n / len + 1 pieces, len at least the
 // workgroups' even share of all blocks.
 inline long long pre_tiles(int B, int n_groups, int rep, int C) { return (long long)B * rep / (16 * C) + std::min(B, n_groups); }
-inline long long pre_slots(int B, int n_groups, int rep, int n_kv, int C) { return PRE_WGS + pre_tiles(B, n_groups, rep, C) * n_kv; }
+inline long long pre_slots(int B, int n_groups, int rep, int n_kv, int C) {
+  return PRE_WGS + pre_tiles(B, n_groups, rep, C) * n_kv;
+}
 inline size_t pre_bytes(int B, int n_groups, int rep, int n_kv, int dv) {
   const int C = pre_tile(B, n_groups, rep);
   return (size_t)pre_slots(B, n_groups, rep, n_kv, C) * 16 * C * (dv + 2) * sizeof(float) + (size_t)B * sizeof(RowPrefix);
@@ -761,16 +843,16 @@ __device__ __forceinline__ Group group_of(const StepArgs& a, int gi, bool lone) 
 
 template <int L, int NB, int C>
 __global__ __launch_bounds__(256, 2) void palu_prefix_kernel(const StepArgs a) {
-  __shared__ __attribute__((aligned(1024))) char smem[step_lds<L, NB>()];
+  __shared__ __attribute__((aligned(1024))) char smem[L == PALU_LAYOUT_ROWS ? step_lds<L, NB>() : WaveLds<NB>::bytes(16)];
   const WaveLds<NB> lds{reinterpret_cast<float*>(smem), 16};
   __shared__ int scan[8], found[4], bases[256];
   constexpr int COLS = 16 * C;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int per = (a.n_groups + 255) / 256, g0 = min(tid * per, a.n_groups), g1 = min(g0 + per, a.n_groups);
   auto tiles_of = [&](const Group& g) { return g.blocks ? (g.rows * a.rep + COLS - 1) / COLS * a.n_kv : 0; };   // of all KV heads
-  // Lone rows' blocks that groups "share" are read here too if there are no more of them than of larger groups: then they do not keep a few
-  // workgroups of the second launch busy when all others are done (16 groups of 64 rows over 2048 positions, one of them of a single row:
-  // 39 -> 28 us). Else the second launch is the better place, which reads them past the L2.
+  // What a lone row shares with itself is read here too if it is no more than the larger groups' blocks: the second launch would
+  // have a few workgroups busy with it when all others are done (64 rows in 16 groups, one of them of a single row, over up to
+  // 2048 positions: 40 -> 31 us for both launches). Otherwise that launch is the better place, which reads past the caches.
   Group own{0, 0, 0};                     // a thread's only group
   float of_lone = 0.f, of_larger = 0.f;
   for (int i = g0; i < g1; ++i) {
@@ -833,7 +915,7 @@ __global__ __launch_bounds__(256, 2) void palu_prefix_kernel(const StepArgs a) {
   __syncthreads();
   const int in = __builtin_amdgcn_readfirstlane(found[0]);
   if (in < 0) return;                     // uniform: past the last piece
-  const Group g{__builtin_amdgcn_readfirstlane(found[1]), __builtin_amdgcn_readfirstlane(found[2]), __builtin_amdgcn_readfirstlane(found[3])};
+  const Group g{uniform(found[1]), uniform(found[2]), uniform(found[3])};
   const int pieces = uniform(cut.pieces(g.blocks)), tile = uniform(in / pieces), piece = in - tile * pieces;
   const int ct = uniform(tile / a.n_kv), kvh = tile - ct * a.n_kv;
   const int each = uniform((g.blocks + pieces - 1) / pieces), lo = piece * each, hi = min(g.blocks, lo + each);
@@ -841,12 +923,19 @@ __global__ __launch_bounds__(256, 2) void palu_prefix_kernel(const StepArgs a) {
   st.clear();
 #pragma unroll
   for (int x = 0; x < C; ++x) {
-    const int col = min(ct * COLS + 16 * x + (lane & 15), g.rows * a.rep - 1), row = col / a.rep;   // columns past the group repeat its last
+    const int col = min(ct * COLS + 16 * x + (lane & 15), g.rows * a.rep - 1);    // (those past the group repeat its last)
+    const int row = col / a.rep;
     st.query(x, a.q + ((long long)(g.row + row) * a.n_q + kvh * a.rep + (col - row * a.rep)) * HD, a.qscale < 0.f);
   }
-  st.template pass<true>(
-      lo, hi, 32 * g.blocks, fabsf(a.qscale), a.dv, smem + w * place_bytes<L, NB>(), [&](int blk) __attribute__((always_inline)) { return page_of(a, g.row, blk); },
-      [&](int page, int blk, const char*& k, const char*& v) __attribute__((always_inline)) { place_of(a, page, kvh, blk, k, v); });
+  auto page_at = [&](int blk) __attribute__((always_inline)) { return page_of(a, g.row, blk); };
+  auto where = [&](int page, int blk, const char*& k, const char*& v) __attribute__((always_inline)) {
+    place_of(a, page, kvh, blk, k, v);
+  };
+  if constexpr (L == PALU_LAYOUT_ROWS) {  // (V's operands are gathered: out of LDS)
+    st.template pass<true>(lo, hi, 32 * g.blocks, fabsf(a.qscale), a.dv, smem + w * place_bytes<L, NB>(), page_at, where);
+  } else {
+    st.template pass_direct<4>(lo, hi, fabsf(a.qscale), a.dv, page_at, where);
+  }
   float* po = a.pre + (long long)want * COLS * (a.dv + 2);
   const int vecs = a.dv / 4;
 #pragma unroll

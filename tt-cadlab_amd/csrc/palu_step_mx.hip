@@ -29,7 +29,7 @@ int step_setup(StepArgs& a, const void* q, const void* k, const void* v, const i
     return fail(PALU_EUNSUPPORTED, "%s: head_dim_v %d (multiples of %d up to %d)", who, dv, step, HD);
   if (positions % 32) return fail(PALU_EINVAL, "%s: a cache holds whole 32-position blocks, got %d positions", who, positions);
   const long long capacity = table ? (long long)pt_stride * positions : positions;
-  if ((long long)batch * n_kv > 65535) return fail(PALU_EUNSUPPORTED, "batch * n_kv = %d exceeds the grid limit", batch * n_kv);
+  if ((long long)batch * n_kv > 65535) return fail(PALU_EUNSUPPORTED, "batch * n_kv = %lld exceeds the grid limit", (long long)batch * n_kv);
   if (capacity > 65536) return fail(PALU_EUNSUPPORTED, "%s: %lld positions; this build covers 65536", who, capacity);
   if (!al16(q) || !al16(k) || !al16(v) || !al16(out)) return fail(PALU_EINVAL, "%s: 16-byte alignment required", who);
   memset(&a, 0, sizeof(a));

@@ -87,6 +87,7 @@ NOALLOC_SCRATCH_BYTES = 64 << 20     # PALU_NOALLOC_SCRATCH_BYTES
 
 _lock = threading.Lock()
 _lib = None
+_entries = {}                         # of the loaded library, by the names that launch() gives them
 
 
 def load() -> ctypes.CDLL:
@@ -143,9 +144,14 @@ def refuse_derivatives(what: str, *tensors) -> None:
 
 def launch(name: str, device, *args) -> None:
     """check(palu_<name>(*args, the current stream of `device`)) with that device current."""
-    fn = getattr(load(), "palu_" + name)
-    if torch._C._cuda_getDevice() == device.index:
-        check(fn(*args, stream_handle(device)))
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = getattr(load(), "palu_" + name)
+    index = device.index
+    if torch._C._cuda_getDevice() == index:
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+        if status != PALU_OK:
+            check(status)
     else:
         with torch.cuda.device(device):
             check(fn(*args, stream_handle(device)))

@@ -151,6 +151,9 @@ _DTYPES = {torch.float32: _native.DTYPE_F32, torch.bfloat16: _native.DTYPE_BF16}
 
 
 def _as_dev(t: torch.Tensor, name: str, dtype=None, device=None) -> torch.Tensor:
+    if isinstance(t, torch.Tensor) and t.is_cuda and (dtype is None or t.dtype is dtype) and t.is_contiguous() and \
+            (device is None or t.device == device):
+        return t
     if not isinstance(t, torch.Tensor):
         raise RuntimeError(f"{name} must be a torch.Tensor")
     if not t.is_cuda:
@@ -218,7 +221,7 @@ def _cur_pos(cur_pos_tensor: torch.Tensor, batch: int, device) -> torch.Tensor:
     cp = cur_pos_tensor if cur_pos_tensor.dim() == 1 else cur_pos_tensor.reshape(-1)
     if cp.numel() != batch:
         raise RuntimeError(f"cur_pos_tensor has {cp.numel()} entries for batch {batch}")
-    if cp.device != device or cp.dtype != torch.int32:
+    if cp.dtype is not torch.int32 or cp.device != device:
         cp = cp.to(device=device, dtype=torch.int32)
     return cp if cp.is_contiguous() else cp.contiguous()
 
@@ -229,7 +232,7 @@ def _page_table(page_table_tensor, batch: int, device) -> torch.Tensor:
     if page_table_tensor.shape[0] != batch:
         raise RuntimeError(f"page_table_tensor has {page_table_tensor.shape[0]} rows for batch {batch}")
     pt = page_table_tensor
-    if pt.device != device or pt.dtype != torch.int32:
+    if pt.dtype is not torch.int32 or pt.device != device:
         pt = pt.to(device=device, dtype=torch.int32)
     return pt if pt.is_contiguous() else pt.contiguous()
 
@@ -561,6 +564,9 @@ def naive_decode(q, k_latent, u_k, cos, sin, v_latent, cur_pos_tensor, recon_len
 
 def _seq_ints(t, name: str, n: Optional[int], device) -> torch.Tensor:
     """A contiguous int32 vector on the device (of n entries), converted where it is another integer type or elsewhere."""
+    if isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.dim() == 1 and t.device == device and t.is_contiguous() and \
+            (n is None or t.shape[0] == n):
+        return t
     if not isinstance(t, torch.Tensor) or t.is_floating_point() or t.dim() != 1 or (n is not None and t.numel() != n):
         raise RuntimeError(f"{name} must be an integer tensor [{'B + 1' if n is None else n}]")
     if t.device != device or t.dtype != torch.int32:

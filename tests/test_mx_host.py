@@ -290,6 +290,20 @@ def test_ops_of_bf16_caches_refuse_quantised_ones(launches):
     assert not launches
 
 
+def test_storage_that_was_replaced_is_looked_at(launches):
+    """A cache's data may be another tensor than at its start; blocks of another size would be read past their end."""
+    cu, table, pos, q = _ints([0, 3]), _ints([[0, 1]]), _ints([5]), _t(1, 1, 4, 128)
+    for other in (_mx(w=32), _mx(fmt="fp4")):
+        c, v = _mx(), _mx(role="v")
+        c.data = v.data = other.data
+        for call in [lambda: fused.paged_fill_cache(c, _t(3, 2, 64), cu, table), lambda: fused.paged_read_cache(c, 3, cu, table),
+                     lambda: fused.paged_update_cache(c, _t(1, 2, 64), pos, page_table=table),
+                     lambda: fused.flash_decode(q, _mx(w=128), v, pos, page_table_tensor=table)]:
+            with pytest.raises(RuntimeError, match="blocks of"):
+                call()
+    assert not launches
+
+
 def test_page_pools_take_quantised_pools(launches):
     k, v, rows = _mx(n=5, w=128), _mx(n=5, role="v", fmt="fp4"), _t(5, 2, 32, 32)
     PagePools([k, v, rows]).compact(_ints([[0, 1]]), _ints([3]))

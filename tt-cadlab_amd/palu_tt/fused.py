@@ -179,6 +179,8 @@ def _cache_arg(t, name: str, device, role: Optional[str] = None, mx: bool = Fals
         _as_dev(t.data, name, torch.uint8, device)
         if not (role is None or t.role == role):
             raise RuntimeError(f"{name} is an MXCache in {t.role!r} order; this argument reads a {role!r} cache")
+        if t.data.shape[-1] != MXCache.block_bytes(t.fmt, t.width):      # (data may have been replaced)
+            raise RuntimeError(f"{name}: blocks of {t.data.shape[-1]} bytes are not those of {t.fmt} and width {t.width}")
         layout = _native.LAYOUT_MX8 if t.fmt == "fp8" else _native.LAYOUT_MX4
         return t.data, t.shape, layout + (1 if role is None and t.role == "v" else 0)
     if isinstance(t, GroupedLatentCache):

@@ -155,6 +155,22 @@ def test_splits(gpu, fmt, B, longest, nkv):
 
 
 @pytest.mark.parametrize("fmt", ["fp8", "fp4"])
+@pytest.mark.parametrize("B,nkv,nq,short,long", [
+    (150, 4, 16, 60, []), (110, 5, 5, 256, []), (180, 3, 12, 200, [3000]), (400, 3, 3, 40, []), (300, 6, 18, 300, [20000, 700]),
+    (70, 8, 32, 257, [288, 289, 5000]), (1100, 1, 16, 33, [900])])
+def test_many_items(gpu, fmt, B, nkv, nq, short, long):
+    """More items than workgroups: a KV head of a short row to a wave (numbers of them that are no multiple of 4, too), pieces of long
+    rows between them, empty rows."""
+    g = torch.Generator().manual_seed(B)
+    lens = long + torch.randint(0, short + 1, (B - len(long),), generator=g).tolist()
+    lens = [lens[i] for i in torch.randperm(B, generator=g).tolist()]
+    x = Batch(gpu, fmt, lens, nq, nkv, 96 if nkv % 2 else 64, 64, seed=B)
+    got = x.decode()
+    x.check(got, rows=sorted({*range(0, B, max(1, B // 40)), *(b for b, n in enumerate(lens) if n > short), B - 1}))
+    assert torch.equal(got, x.decode())
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "fp4"])
 @pytest.mark.parametrize("S,lens", [(32, [1, 32, 0]), (160, [160, 33, 1, 97]), (8192, [8192, 5000, 31])], ids=str)
 def test_contiguous(gpu, fmt, S, lens):
     g = torch.Generator().manual_seed(S)
@@ -294,6 +310,18 @@ def test_lone_rows_beside_groups(gpu, layout, rows):
     lens = [s + 13 * i for i, (n, s) in enumerate(zip(rows, shared)) for _ in range(n)]
     x = Batch(gpu, layout, lens, 8, 2, 64, 64, rows, shared, seed=len(lens))
     x.check(x.decode_shared())
+
+
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("B,groups,prefix,tail,nq,nkv", [(150, 1, 700, 60, 16, 4), (180, 60, 300, 300, 9, 3), (270, 9, 96, 500, 20, 5)])
+def test_many_items_behind_prefixes(gpu, layout, B, groups, prefix, tail, nq, nkv):
+    g = torch.Generator().manual_seed(B)
+    cuts = sorted(torch.randperm(B - 1, generator=g)[:groups - 1].add(1).tolist())
+    rows = [b - a for a, b in zip([0] + cuts, cuts + [B])]
+    shared = [prefix] + torch.randint(1, prefix + 1, (groups - 1,), generator=g).tolist()
+    lens = [s + int(torch.randint(0, tail, (), generator=g)) for n, s in zip(rows, shared) for _ in range(n)]
+    x = Batch(gpu, layout, lens, nq, nkv, 48 if layout in ("rows", "tiled") else 64, 64, rows, shared, seed=B, garbage=0.0)
+    x.check(x.decode_shared(), rows=list(range(0, B, 7)) + [B - 1])
 
 
 @pytest.mark.parametrize("layout", ["rows", "tiled"])

@@ -368,15 +368,13 @@ struct Wave {
     }
   }
 
-  // This wave's blocks of first .. end - 1, of a sequence that is seen up to position seen - 1 (ALL: whole blocks only): every
-  // fourth group of them. page_at(blk) gives a block's page, where(page, blk, k, v) its places; s: the wave's place in LDS. While
+  // This wave's blocks of first .. end - 1, of a sequence that is seen up to position seen - 1 (ALL: whole blocks only): a group
+  // of them, then the one `waves` groups further, and so on. page_at(blk) gives a block's page, where(page, blk, k, v) its places; s: the wave's place in LDS. While
   // a group is computed the next one is on its way; its pages are asked for a turn earlier.
   template <bool ALL, typename P, typename F>
-  __device__ __forceinline__ void pass(int first, int end, int seen, float qscale, int dv, char* s, P&& page_at, F&& where) {
+  __device__ __forceinline__ void pass(int first, int waves, int end, int seen, float qscale, int dv, char* s, P&& page_at, F&& where) {
     using R = Raw<L, NB>;
     constexpr int G = step_group(L);
-    first += (int)(threadIdx.x >> 6) * G;
-    first = __builtin_amdgcn_readfirstlane(first);
     if (first >= end) return;
     int page[G];
     auto pages = [&](int blk) __attribute__((always_inline)) {
@@ -395,7 +393,7 @@ struct Wave {
     wait_copies();                        // the queries are here (the pages took as long)
     fetch(first);
     for (int blk = first; blk < end;) {
-      const int next = blk + 4 * G;
+      const int next = blk + waves * G;
       pages(min(next, end - 1));
       wait_copies();
       R r[G];
@@ -523,7 +521,8 @@ __device__ __forceinline__ float wg_sum(float x, float* part) {
 // How items are cut into pieces of up to len blocks, a workgroup each: the first of a few lengths, from an even share of all
 // blocks on (total: a float, since rows that share their pages can be more blocks than an int holds), of which the chip holds
 // all pieces (`slots`) at once, and at least `least`. of(i) gives n items of some blocks each; a thread has i0 .. i1 - 1. Its
-// pieces are number before .. before + mine - 1 of all; where they never fit, they are at most slots + all items. Whole shares of
+// pieces are number before .. before + mine - 1 of all; where they never fit, they are at most slots + all items (t: the first
+// length that is tried, of 0 to 3). Whole shares of
 // items, some workgroups with a little less to do, were faster than even shares that begin and end inside items and join more
 // parts (64 rows of up to 2304 positions in fp4: 33 us against 37).
 struct Cut {
@@ -534,11 +533,11 @@ struct Items {
   int n, blocks;
 };
 template <typename F>
-__device__ __forceinline__ Cut cut_items(float total, int i0, int i1, int slots, int least, int* scan, F&& of) {
+__device__ __forceinline__ Cut cut_items(float total, int i0, int i1, int slots, int least, int t, int* scan, F&& of) {
   const float up = total < 0x1p24f ? 1.f : 1.f + 0x1p-14f;    // (the total may be rounded)
   const int share = (int)ceilf(total / (float)slots * up);
   Cut c;
-  for (int t = 0; t < 4; ++t) {           // uniform
+  for (; t < 4; ++t) {                    // uniform
     c.len = max(least, share + share / 8 * t + share % 8 * t / 8);
     c.mine = 0;
     for (int i = i0; i < i1; ++i) {
@@ -571,9 +570,18 @@ __device__ __forceinline__ void place_of(const StepArgs& a, int page, int kvh, i
 // 1.5 to 3 us slower, for they are cut then.
 constexpr int STEP_LEAST = 16;
 constexpr int STEP_WGS = 512;             // workgroups that the chip holds at once, by the kernel's LDS and registers
-inline int step_grid(int B, int n_kv) { return STEP_WGS + B * n_kv; }
+// More items than those (MANY): rows of up to STEP_SHORT own blocks have four KV heads to a workgroup, one to a wave, and nothing to
+// join but a prefix; of longer ones a workgroup has a piece, as ever. Above 1024 items 512 workgroups take piece after piece, since
+// one that finds no piece costs 3 us of its place to find that out (512 rows of up to 64 positions, 8 KV heads, fp8: 77 -> 19 us; 256
+// of up to 200: 37 -> 21); up to there each piece has its own, which balances long rows better (66 rows of up to 4000: 68 us, 78 in
+// such a loop; 100 of up to 100: 17 -> 10.5). Limits of 4 and 16 blocks: 256 rows of 200 27 us, 32 rows of up to 1024 with 32 KV
+// heads 46 us against 35.
+constexpr int STEP_SHORT = 8;
+inline bool step_many(int B, int n_kv) { return (long long)B * n_kv > STEP_WGS; }
+inline int step_slots(int B, int n_kv) { return STEP_WGS + B * n_kv; }         // pieces, at most
+inline int step_grid(int B, int n_kv) { return B * n_kv > 1024 ? STEP_WGS : step_slots(B, n_kv); }
 inline size_t step_bytes(int B, int n_kv, int rep, int dv) {
-  return (size_t)step_grid(B, n_kv) * ((size_t)rep * (dv + 2) * sizeof(float) + sizeof(unsigned long long));
+  return (size_t)step_slots(B, n_kv) * ((size_t)rep * (dv + 2) * sizeof(float) + sizeof(unsigned long long));
 }
 
 struct RowWork {
@@ -634,7 +642,24 @@ __device__ __forceinline__ f32x4 load_part4(__amdgpu_buffer_rsrc_t p, int at) {
   return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(p, at * 4, 0, SYSTEM_SCOPE));
 }
 
+// A wave's own result (of column tile 0), not joined with any: out from element `at` on.
 template <int L, int NB>
+__device__ __forceinline__ void store_wave(const StepArgs& a, const Wave<L, NB, 1>& st, long long at, bool none) {
+  const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  const float l = wave_sum_xor48(st.l[0]), inv = none ? 0.f : 1.f / l;
+  if (n >= a.rep) return;
+  at += (long long)n * a.dv;
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    const f32x4 y = st.o[0][2 * b] * inv, z = st.o[0][2 * b + 1] * inv;        // as in to_lds
+    constexpr bool T = L == PALU_LAYOUT_TILED;
+    const int d0 = 32 * b + (T ? 4 : 8) * g, d1 = d0 + (T ? 16 : 4);
+    if (d0 < a.dv) store4(a, at + d0, T ? y : f32x4{y[0], z[0], y[1], z[1]});
+    if (d1 < a.dv) store4(a, at + d1, T ? z : f32x4{y[2], z[2], y[3], z[3]});
+  }
+}
+
+template <int L, int NB, bool MANY>
 __global__ __launch_bounds__(256, 2) void palu_step_kernel(const StepArgs a) {
   __shared__ __attribute__((aligned(1024))) char smem[step_lds<L, NB>()];
   const WaveLds<NB> lds{reinterpret_cast<float*>(smem), a.rep};
@@ -656,155 +681,173 @@ __global__ __launch_bounds__(256, 2) void palu_step_kernel(const StepArgs a) {
     const RowWork r = row(i);
     mine += (float)a.n_kv * (float)(r.end - r.first);
   }
-  const Cut cut = cut_items(wg_sum(mine, reinterpret_cast<float*>(scan)), r0, r1, STEP_WGS, STEP_LEAST, scan, [&](int i) {
-    const RowWork r = row(i);
-    return Items{a.n_kv, r.end - r.first};
-  });
-  const int want = blockIdx.x;
-  if (want >= cut.all) return;            // uniform
-  if (want >= cut.before && want < cut.before + cut.mine) {
-    int at = cut.before, b = r0;
-    RowWork r = row(b);
-    for (;;) {
-      const int n = cut.pieces(r.end - r.first) * a.n_kv;
-      if (want < at + n || b + 1 >= r1) break;
-      at += n;
-      r = row(++b);
-    }
-    found[0] = b;
-    found[1] = want - at;
-    found_row = r;
-  }
-  __syncthreads();
-  const int b = __builtin_amdgcn_readfirstlane(found[0]), in = __builtin_amdgcn_readfirstlane(found[1]);
-  const RowWork r = uniform(found_row);
-  const int chunks = uniform(cut.pieces(r.end - r.first)), kvh = uniform(in / chunks), chunk = in - kvh * chunks;
-  const int wg0 = want - chunk;           // the item's first piece
-  const int len = uniform((r.end - r.first + chunks - 1) / chunks), lo = r.first + chunk * len, hi = min(r.end, lo + len);
-  Wave<L, NB, 1> st;
-  st.clear();
-  st.query(0, a.q + ((long long)b * a.n_q + kvh * a.rep + min(lane & 15, a.rep - 1)) * HD, a.qscale < 0.f);
-  st.template pass<false>(
-      lo, min(hi, (r.seen + 31) >> 5), r.seen, fabsf(a.qscale), a.dv, smem + w * place_bytes<L, NB>(),
-      [&](int blk) __attribute__((always_inline)) { return page_of(a, blk < r.pblocks ? r.lead : b, blk); },
-      [&](int page, int blk, const char*& k, const char*& v) __attribute__((always_inline)) {
-        place_of(a, page, kvh, blk, k, v);
-      });
-  __syncthreads();                        // every wave is done with its places
-  to_lds(lds, st, 0);
-  __syncthreads();
-  const int vecs = a.dv / 4, units = a.rep * vecs;
-  const long long part_size = (long long)a.rep * (a.dv + 2);
-  if (chunks > 1) {
-    float* po = a.part + want * part_size;
-    const __amdgpu_buffer_rsrc_t p4 = parts_at(po);
-    for (int e = tid; e < units; e += 256) {
-      const int h = e / vecs, d = 4 * (e - h * vecs);
-      const Joined j = join_waves(lds, h, d);
-      store_part4(p4, h * a.dv + d, j.y);
-      if (d == 0) {
-        store_part(po + a.rep * a.dv + h, j.m);
-        store_part(po + a.rep * a.dv + a.rep + h, j.l);
-      }
-    }
-    if (!chunks_all_done(a.flags + wg0, a.epoch, chunks, chunk, found)) return;   // uniform
-  }
-  auto finish = [&](int h, int d, const Joined& j) __attribute__((always_inline)) {
-    const float inv = 1.f / j.l;
-    const f32x4 y = r.seen == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : j.y * inv;       // a row that sees nothing: zeros
-    store4(a, ((long long)b * a.n_q + kvh * a.rep + h) * a.dv + d, y);
+  auto items_of = [&](const RowWork& r) {   // MANY: four KV heads of a short row to a workgroup, one to a wave
+    const int blocks = r.end - r.first;
+    return MANY && blocks <= STEP_SHORT ? Items{(a.n_kv + 3) / 4, 1} : Items{a.n_kv, blocks};
   };
-  // The parts: this workgroup's own (in LDS), or all workgroups' (one of which is its own), and the prefix's pieces, which the
-  // launch before wrote.
-  const __amdgpu_buffer_rsrc_t parts = parts_at(a.part + wg0 * part_size);
-  const int pre_size = a.pre_cols * (a.dv + 2);
-  auto pieces_of = [&](int h, int& x) {   // the pieces of a head, in column x of theirs
-    const int col = r.local * a.rep + h, tile = r.pieces ? col / a.pre_cols : 0;
-    x = col - tile * a.pre_cols;
-    return a.pre + (r.base + (long long)(tile * a.n_kv + kvh) * r.pieces) * pre_size;
-  };
-  const int groups = min(max(1, 256 / units), MAX_GROUPS), grp = groups > 1 ? tid / units : 0, batch = U * groups;
-  for (int e0 = 0; e0 < units; e0 += 256) {                   // (uniform)
-    const int e = groups > 1 ? tid - grp * units : e0 + tid;
-    const bool on = e < units && grp < groups;
-    const int h = on ? e / vecs : 0, d = on ? 4 * (e - h * vecs) : 0;
-    Joined j = no_parts();
-    // n parts, U to each of 256 / units threads at a time, whose loads are all under way together: stat(c, x, m, l) loads the
-    // statistics of part c's column x, four(c) this thread's four channels.
-    auto gather = [&](int n, auto&& stat, auto&& four) __attribute__((always_inline)) {
-      for (int c0 = 0; c0 < n; c0 += batch) {                 // (uniform)
-        float m[MAX_GROUPS], l[MAX_GROUPS];
-#pragma unroll
-        for (int i = 0; i < MAX_GROUPS; ++i) {
-          if (16 * i >= batch || c0 + 16 * i >= n) break;     // (uniform)
-          stat(min(c0 + 16 * i + (tid >> 4), n - 1), min(tid & 15, a.rep - 1), m[i], l[i]);
-        }
-        f32x4 y[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          if (c0 + u * groups >= n) break;                    // (uniform)
-          y[u] = four(min(c0 + u * groups + min(grp, groups - 1), n - 1));
-        }
-        __syncthreads();                  // the batch before has been read
-#pragma unroll
-        for (int i = 0; i < MAX_GROUPS; ++i) {
-          const int c = 16 * i + (tid >> 4);
-          if (16 * i >= batch || c0 + 16 * i >= n) break;
-          joining.stats[0][c][tid & 15] = m[i];
-          joining.stats[1][c][tid & 15] = l[i];
-        }
-        __syncthreads();
-        if (!on) continue;
-        Joined b = no_parts();
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          if (c0 + u * groups + grp >= n) break;
-          b.m = fmaxf(b.m, joining.stats[0][u * groups + grp][h]);
-        }
-        const float ref = b.m == NEG_INF ? 0.f : b.m;
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          if (c0 + u * groups + grp >= n) break;
-          const float f = __builtin_amdgcn_exp2f(joining.stats[0][u * groups + grp][h] - ref);
-          b.l += f * joining.stats[1][u * groups + grp][h];
-          b.y += f * y[u];
-        }
-        j.add(b.y, b.m, b.l);
-      }
-    };
-    gather(chunks == 1 ? 0 : chunks, [&](int c, int x, float& m, float& l) __attribute__((always_inline)) {
-             const float* p = a.part + (wg0 + c) * part_size + a.rep * a.dv + x;
-             m = load_part(p);
-             l = load_part(p + a.rep);
-           }, [&](int c) __attribute__((always_inline)) { return load_part4(parts, c * (int)part_size + h * a.dv + d); });
-    int col, stat_col;
-    const float *pre = pieces_of(h, col), *stats = pieces_of(min(tid & 15, a.rep - 1), stat_col);
-    gather(r.pieces, [&](int c, int x, float& m, float& l) __attribute__((always_inline)) {
-             const float* p = stats + (long long)c * pre_size + a.pre_cols * a.dv + stat_col;
-             m = p[0];
-             l = p[a.pre_cols];
-           }, [&](int c) __attribute__((always_inline)) {
-             return *reinterpret_cast<const f32x4*>(pre + (long long)c * pre_size + col * a.dv + d);
-           });
-    if (on && chunks == 1 && grp == 0) {
-      const Joined mine = join_waves(lds, h, d);
-      j.add(mine.y, mine.m, mine.l);
+  const Cut cut = cut_items(wg_sum(mine, reinterpret_cast<float*>(scan)), r0, r1, STEP_WGS, STEP_LEAST, MANY ? 3 : 0, scan,
+                            [&](int i) { return items_of(row(i)); });
+  int want = blockIdx.x;
+  if (!MANY && want >= cut.all) return;   // uniform
+  do {
+    if (MANY) {
+      if (want >= cut.all) return;        // uniform
+      __syncthreads();                    // the piece before is done with LDS
     }
-    if (groups == 1) {
-      if (on) finish(h, d, j);
+    if (want >= cut.before && want < cut.before + cut.mine) {
+      int at = cut.before, b = r0;
+      RowWork r = row(b);
+      for (;;) {
+        const Items x = items_of(r);
+        const int n = x.n * cut.pieces(x.blocks);
+        if (want < at + n || b + 1 >= r1) break;
+        at += n;
+        r = row(++b);
+      }
+      found[0] = b;
+      found[1] = want - at;
+      found_row = r;
+    }
+    __syncthreads();
+    const int b = uniform(found[0]), in = uniform(found[1]);
+    const RowWork r = uniform(found_row);
+    const bool each = MANY && r.end - r.first <= STEP_SHORT;    // (uniform)
+    const int chunks = each ? 1 : uniform(cut.pieces(r.end - r.first)), head0 = each ? 4 * in : uniform(in / chunks);
+    const int chunk = each ? 0 : in - head0 * chunks, wg0 = want - chunk;      // wg0: the item's first piece
+    const int head = each ? min(head0 + w, a.n_kv - 1) : head0;                // this wave's
+    const int len = uniform((r.end - r.first + chunks - 1) / chunks), lo = r.first + chunk * len, hi = min(r.end, lo + len);
+    Wave<L, NB, 1> st;
+    st.clear();
+    st.query(0, a.q + ((long long)b * a.n_q + head * a.rep + min(lane & 15, a.rep - 1)) * HD, a.qscale < 0.f);
+    st.template pass<false>(
+        lo + (each ? 0 : w * step_group(L)), each ? 1 : 4, min(hi, (r.seen + 31) >> 5), r.seen, fabsf(a.qscale), a.dv, smem + w * place_bytes<L, NB>(),
+        [&](int blk) __attribute__((always_inline)) { return page_of(a, blk < r.pblocks ? r.lead : b, blk); },
+        [&](int page, int blk, const char*& k, const char*& v) __attribute__((always_inline)) {
+          place_of(a, page, head, blk, k, v);
+        });
+    if (each && !r.pieces) {                // (uniform) nothing to join
+      if (head0 + w < a.n_kv) store_wave<L, NB>(a, st, ((long long)b * a.n_q + head * a.rep) * a.dv, r.seen == 0);
       continue;
     }
-    __syncthreads();                      // the last batch has been read
-    if (on) joining.sums[tid] = j;
+    __syncthreads();                        // every wave is done with its places
+    to_lds(lds, st, 0);
     __syncthreads();
-    if (tid < units) {
-      for (int i = 1; i < groups; ++i) {
-        const Joined x = joining.sums[tid + i * units];
-        j.add(x.y, x.m, x.l);
+    const int vecs = a.dv / 4, units = a.rep * vecs;
+    const long long part_size = (long long)a.rep * (a.dv + 2);
+    if (chunks > 1) {
+      float* po = a.part + want * part_size;
+      const __amdgpu_buffer_rsrc_t p4 = parts_at(po);
+      for (int e = tid; e < units; e += 256) {
+        const int h = e / vecs, d = 4 * (e - h * vecs);
+        const Joined j = join_waves(lds, h, d);
+        store_part4(p4, h * a.dv + d, j.y);
+        if (d == 0) {
+          store_part(po + a.rep * a.dv + h, j.m);
+          store_part(po + a.rep * a.dv + a.rep + h, j.l);
+        }
       }
-      finish(h, d, j);
+      if (!chunks_all_done(a.flags + wg0, a.epoch, chunks, chunk, found)) continue; // uniform
     }
-  }
+    for (int x = 0, kvh = head0; x < (each ? 4 : 1) && kvh < a.n_kv; ++x, ++kvh) {   // (uniform)
+      auto finish = [&](int h, int d, const Joined& j) __attribute__((always_inline)) {
+        const float inv = 1.f / j.l;
+        const f32x4 y = r.seen == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : j.y * inv;       // a row that sees nothing: zeros
+        store4(a, ((long long)b * a.n_q + kvh * a.rep + h) * a.dv + d, y);
+      };
+      // The parts: this workgroup's own (in LDS), or all workgroups' (one of which is its own), and the prefix's pieces, which the
+      // launch before wrote.
+      const __amdgpu_buffer_rsrc_t parts = parts_at(a.part + wg0 * part_size);
+      const int pre_size = a.pre_cols * (a.dv + 2);
+      auto pieces_of = [&](int h, int& x) {   // the pieces of a head, in column x of theirs
+        const int col = r.local * a.rep + h, tile = r.pieces ? col / a.pre_cols : 0;
+        x = col - tile * a.pre_cols;
+        return a.pre + (r.base + (long long)(tile * a.n_kv + kvh) * r.pieces) * pre_size;
+      };
+      const int groups = min(max(1, 256 / units), MAX_GROUPS), grp = groups > 1 ? tid / units : 0, batch = U * groups;
+      for (int e0 = 0; e0 < units; e0 += 256) {                   // (uniform)
+        const int e = groups > 1 ? tid - grp * units : e0 + tid;
+        const bool on = e < units && grp < groups;
+        const int h = on ? e / vecs : 0, d = on ? 4 * (e - h * vecs) : 0;
+        Joined j = no_parts();
+        // n parts, U to each of 256 / units threads at a time, whose loads are all under way together: stat(c, x, m, l) loads the
+        // statistics of part c's column x, four(c) this thread's four channels.
+        auto gather = [&](int n, auto&& stat, auto&& four) __attribute__((always_inline)) {
+          for (int c0 = 0; c0 < n; c0 += batch) {                 // (uniform)
+            float m[MAX_GROUPS], l[MAX_GROUPS];
+#pragma unroll
+            for (int i = 0; i < MAX_GROUPS; ++i) {
+              if (16 * i >= batch || c0 + 16 * i >= n) break;     // (uniform)
+              stat(min(c0 + 16 * i + (tid >> 4), n - 1), min(tid & 15, a.rep - 1), m[i], l[i]);
+            }
+            f32x4 y[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+              if (c0 + u * groups >= n) break;                    // (uniform)
+              y[u] = four(min(c0 + u * groups + min(grp, groups - 1), n - 1));
+            }
+            __syncthreads();                  // the batch before has been read
+#pragma unroll
+            for (int i = 0; i < MAX_GROUPS; ++i) {
+              const int c = 16 * i + (tid >> 4);
+              if (16 * i >= batch || c0 + 16 * i >= n) break;
+              joining.stats[0][c][tid & 15] = m[i];
+              joining.stats[1][c][tid & 15] = l[i];
+            }
+            __syncthreads();
+            if (!on) continue;
+            Joined b = no_parts();
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+              if (c0 + u * groups + grp >= n) break;
+              b.m = fmaxf(b.m, joining.stats[0][u * groups + grp][h]);
+            }
+            const float ref = b.m == NEG_INF ? 0.f : b.m;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+              if (c0 + u * groups + grp >= n) break;
+              const float f = __builtin_amdgcn_exp2f(joining.stats[0][u * groups + grp][h] - ref);
+              b.l += f * joining.stats[1][u * groups + grp][h];
+              b.y += f * y[u];
+            }
+            j.add(b.y, b.m, b.l);
+          }
+        };
+        gather(chunks == 1 ? 0 : chunks, [&](int c, int x, float& m, float& l) __attribute__((always_inline)) {
+                 const float* p = a.part + (wg0 + c) * part_size + a.rep * a.dv + x;
+                 m = load_part(p);
+                 l = load_part(p + a.rep);
+               }, [&](int c) __attribute__((always_inline)) { return load_part4(parts, c * (int)part_size + h * a.dv + d); });
+        int col, stat_col;
+        const float *pre = pieces_of(h, col), *stats = pieces_of(min(tid & 15, a.rep - 1), stat_col);
+        gather(r.pieces, [&](int c, int x, float& m, float& l) __attribute__((always_inline)) {
+                 const float* p = stats + (long long)c * pre_size + a.pre_cols * a.dv + stat_col;
+                 m = p[0];
+                 l = p[a.pre_cols];
+               }, [&](int c) __attribute__((always_inline)) {
+                 return *reinterpret_cast<const f32x4*>(pre + (long long)c * pre_size + col * a.dv + d);
+               });
+        if (on && chunks == 1 && grp == 0) {
+          const Joined mine = each ? Joined{*reinterpret_cast<const f32x4*>(lds.row(x, h) + d), lds.m(x, h), lds.l(x, h)}
+                                   : join_waves(lds, h, d);
+          j.add(mine.y, mine.m, mine.l);
+        }
+        if (groups == 1) {
+          if (on) finish(h, d, j);
+          continue;
+        }
+        __syncthreads();                      // the last batch has been read
+        if (on) joining.sums[tid] = j;
+        __syncthreads();
+        if (tid < units) {
+          for (int i = 1; i < groups; ++i) {
+            const Joined x = joining.sums[tid + i * units];
+            j.add(x.y, x.m, x.l);
+          }
+          finish(h, d, j);
+        }
+      }
+    }
+  } while (MANY && (want += gridDim.x, true));
 }
 
 // ---- the groups' prefixes -----------------------------------------------------------------------
@@ -863,16 +906,18 @@ __global__ __launch_bounds__(256, 2) void palu_prefix_kernel(const StepArgs a) {
   const bool lone = of_lone <= of_larger;
   if (!lone && own.rows == 1) own.blocks = 0;
   auto group = [&](int i) { return per == 1 ? own : group_of(a, i, lone); };
-  const Cut cut = cut_items(of_larger + (lone ? of_lone : 0.f), g0, g1, PRE_WGS, PRE_LEAST, scan, [&](int i) {
+  const Cut cut = cut_items(of_larger + (lone ? of_lone : 0.f), g0, g1, PRE_WGS, PRE_LEAST, 0, scan, [&](int i) {
     const Group g = group(i);
     return Items{tiles_of(g), g.blocks};
   });
   const int row_wgs = (a.B + 255) / 256;
-  if ((int)blockIdx.x < row_wgs) {        // the rows' records, a thread each
+  // The rows' records, a thread each: the last workgroups, which are the first to have no piece.
+  const int rec = (int)(gridDim.x - 1 - blockIdx.x), b = rec * 256 + tid;
+  if (rec < row_wgs) {                    // (uniform)
     bases[tid] = cut.before;
     __syncthreads();
-    const int b = (int)blockIdx.x * 256 + tid;
-    if (b >= a.B) return;
+  }
+  if (rec < row_wgs && b < a.B) {
     int gi = 0;
     for (int end = a.n_groups; end - gi > 1;) {   // the last group that begins at b or before it
       const int mid = (gi + end) >> 1;
@@ -888,68 +933,71 @@ __global__ __launch_bounds__(256, 2) void palu_prefix_kernel(const StepArgs a) {
         base += tiles_of(x) * cut.pieces(x.blocks);
       }
       const int pieces = cut.pieces(g.blocks);
-      // (Groups that overlap, where the offsets make no sense, can be more pieces than the workspace was sized for.)
       r = RowPrefix{g.row, g.blocks, base >= 0 && base + tiles_of(g) * pieces <= a.pre_slots ? pieces : 0, base, b - g.row, {}};
     }
     a.rows[b] = r;
-    return;
   }
-  const int want = (int)blockIdx.x - row_wgs;
-  if (tid == 0) found[0] = -1;
-  __syncthreads();
-  if (want >= cut.before && want < cut.before + cut.mine) {
-    int at = cut.before;
-    for (int i = g0; i < g1; ++i) {
-      const Group g = group(i);
-      const int n = tiles_of(g) * cut.pieces(g.blocks);
-      if (want >= at && want < at + n) {
-        found[0] = want - at;
-        found[1] = g.row;
-        found[2] = g.rows;
-        found[3] = g.blocks;
-        break;
-      }
-      at += n;
-    }
-  }
-  __syncthreads();
-  const int in = __builtin_amdgcn_readfirstlane(found[0]);
-  if (in < 0) return;                     // uniform: past the last piece
-  const Group g{uniform(found[1]), uniform(found[2]), uniform(found[3])};
-  const int pieces = uniform(cut.pieces(g.blocks)), tile = uniform(in / pieces), piece = in - tile * pieces;
-  const int ct = uniform(tile / a.n_kv), kvh = tile - ct * a.n_kv;
-  const int each = uniform((g.blocks + pieces - 1) / pieces), lo = piece * each, hi = min(g.blocks, lo + each);
-  Wave<L, NB, C> st;
-  st.clear();
-#pragma unroll
-  for (int x = 0; x < C; ++x) {
-    const int col = min(ct * COLS + 16 * x + (lane & 15), g.rows * a.rep - 1);    // (those past the group repeat its last)
-    const int row = col / a.rep;
-    st.query(x, a.q + ((long long)(g.row + row) * a.n_q + kvh * a.rep + (col - row * a.rep)) * HD, a.qscale < 0.f);
-  }
-  auto page_at = [&](int blk) __attribute__((always_inline)) { return page_of(a, g.row, blk); };
-  auto where = [&](int page, int blk, const char*& k, const char*& v) __attribute__((always_inline)) {
-    place_of(a, page, kvh, blk, k, v);
-  };
-  if constexpr (L == PALU_LAYOUT_ROWS) {  // (V's operands are gathered: out of LDS)
-    st.template pass<true>(lo, hi, 32 * g.blocks, fabsf(a.qscale), a.dv, smem + w * place_bytes<L, NB>(), page_at, where);
-  } else {
-    st.template pass_direct<4>(lo, hi, fabsf(a.qscale), a.dv, page_at, where);
-  }
-  float* po = a.pre + (long long)want * COLS * (a.dv + 2);
-  const int vecs = a.dv / 4;
-#pragma unroll
-  for (int x = 0; x < C; ++x) {
-    __syncthreads();                      // every wave is done with its places, or with the results before
-    to_lds(lds, st, x);
+  // (Groups that overlap, where the offsets make no sense, can be more pieces than the workspace was sized for, or than can be
+  // counted: those are left out.)
+  for (int want = blockIdx.x; want < min(cut.all, a.pre_slots); want += gridDim.x) {   // (uniform)
+    __syncthreads();                      // the piece before is done with LDS
+    if (tid == 0) found[0] = -1;
     __syncthreads();
-    for (int e = tid; e < 16 * vecs; e += 256) {
-      const int n = e / vecs, d = 4 * (e - n * vecs), col = 16 * x + n;
-      const Joined j = join_waves(lds, n, d);
-      *reinterpret_cast<f32x4*>(po + col * a.dv + d) = j.y;
-      if (d == 0) {
-        po[COLS * a.dv + col] = j.m;
-        po[COLS * (a.dv + 1) + col] = j.l;
+    if (want >= cut.before && want < cut.before + cut.mine) {
+      int at = cut.before;
+      for (int i = g0; i < g1; ++i) {
+        const Group g = group(i);
+        const int n = tiles_of(g) * cut.pieces(g.blocks);
+        if (want >= at && want < at + n) {
+          found[0] = want - at;
+          found[1] = g.row;
+          found[2] = g.rows;
+          found[3] = g.blocks;
+          break;
+        }
+        at += n;
+      }
+    }
+    __syncthreads();
+    const int in = __builtin_amdgcn_readfirstlane(found[0]);
+    if (in < 0) continue;                   // (uniform)
+    const Group g{uniform(found[1]), uniform(found[2]), uniform(found[3])};
+    const int pieces = uniform(cut.pieces(g.blocks)), tile = uniform(in / pieces), piece = in - tile * pieces;
+    const int ct = uniform(tile / a.n_kv), kvh = tile - ct * a.n_kv;
+    const int each = uniform((g.blocks + pieces - 1) / pieces), lo = piece * each, hi = min(g.blocks, lo + each);
+    Wave<L, NB, C> st;
+    st.clear();
+#pragma unroll
+    for (int x = 0; x < C; ++x) {
+      const int col = min(ct * COLS + 16 * x + (lane & 15), g.rows * a.rep - 1);    // (those past the group repeat its last)
+      const int row = col / a.rep;
+      st.query(x, a.q + ((long long)(g.row + row) * a.n_q + kvh * a.rep + (col - row * a.rep)) * HD, a.qscale < 0.f);
+    }
+    auto page_at = [&](int blk) __attribute__((always_inline)) { return page_of(a, g.row, blk); };
+    auto where = [&](int page, int blk, const char*& k, const char*& v) __attribute__((always_inline)) {
+      place_of(a, page, kvh, blk, k, v);
+    };
+    if constexpr (L == PALU_LAYOUT_ROWS) {  // (V's operands are gathered: out of LDS)
+      st.template pass<true>(lo + w * step_group(L), 4, hi, 32 * g.blocks, fabsf(a.qscale), a.dv, smem + w * place_bytes<L, NB>(),
+                             page_at, where);
+    } else {
+      st.template pass_direct<4>(lo, hi, fabsf(a.qscale), a.dv, page_at, where);
+    }
+    float* po = a.pre + (long long)want * COLS * (a.dv + 2);
+    const int vecs = a.dv / 4;
+#pragma unroll
+    for (int x = 0; x < C; ++x) {
+      __syncthreads();                      // every wave is done with its places, or with the results before
+      to_lds(lds, st, x);
+      __syncthreads();
+      for (int e = tid; e < 16 * vecs; e += 256) {
+        const int n = e / vecs, d = 4 * (e - n * vecs), col = 16 * x + n;
+        const Joined j = join_waves(lds, n, d);
+        *reinterpret_cast<f32x4*>(po + col * a.dv + d) = j.y;
+        if (d == 0) {
+          po[COLS * a.dv + col] = j.m;
+          po[COLS * (a.dv + 1) + col] = j.l;
+        }
       }
     }
   }
@@ -966,12 +1014,13 @@ int step_launch(K kern, unsigned grid, int lds, const StepArgs& a, const char* w
 template <int L, int NB>
 int step_run_nb(const StepArgs& a, const char* who, hipStream_t s) {
   if (a.rows) {
-    const unsigned grid = (unsigned)((a.B + 255) / 256 + a.pre_slots);
-    const int rc = a.pre_cols == 16   ? step_launch(palu_prefix_kernel<L, NB, 1>, grid, 0, a, who, s)
-                                      : step_launch(palu_prefix_kernel<L, NB, 2>, grid, 0, a, who, s);
+    const int rc = a.pre_cols == 16   ? step_launch(palu_prefix_kernel<L, NB, 1>, PRE_WGS, 0, a, who, s)
+                                      : step_launch(palu_prefix_kernel<L, NB, 2>, PRE_WGS, 0, a, who, s);
     if (rc) return rc;
   }
-  return step_launch(palu_step_kernel<L, NB>, (unsigned)step_grid(a.B, a.n_kv), 0, a, who, s);
+  const unsigned grid = (unsigned)step_grid(a.B, a.n_kv);
+  return step_many(a.B, a.n_kv) ? step_launch(palu_step_kernel<L, NB, true>, grid, 0, a, who, s)
+                                : step_launch(palu_step_kernel<L, NB, false>, grid, 0, a, who, s);
 }
 
 template <int L>

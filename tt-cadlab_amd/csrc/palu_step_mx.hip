@@ -64,7 +64,7 @@ int step_workspace(StepArgs& a, void* workspace, size_t bytes, size_t need, cons
   if (!workspace || bytes < need || !al16(workspace))
     return fail(PALU_EINVAL, "%s: a 16-byte aligned workspace of %zu bytes needed (%s), got %zu", who, need, query,
                 workspace ? bytes : 0);
-  const long long slots = STEP_WGS + (long long)a.B * a.n_kv;
+  const long long slots = step_slots(a.B, a.n_kv);
   a.part = static_cast<float*>(workspace);
   a.flags = reinterpret_cast<unsigned long long*>(a.part + slots * a.rep * (a.dv + 2));
   a.epoch = next_epoch();

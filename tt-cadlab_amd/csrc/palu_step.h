@@ -369,10 +369,11 @@ struct Wave {
   }
 
   // This wave's blocks of first .. end - 1, of a sequence that is seen up to position seen - 1 (ALL: whole blocks only): a group
-  // of them, then the one `waves` groups further, and so on. page_at(blk) gives a block's page, where(page, blk, k, v) its places; s: the wave's place in LDS. While
-  // a group is computed the next one is on its way; its pages are asked for a turn earlier.
+  // of them, then the one `waves` groups further, and so on. page_at(blk) gives a block's page, where(page, blk, k, v) its places;
+  // s: the wave's place in LDS. While a group is computed the next one is on its way; its pages are asked for a turn earlier.
   template <bool ALL, typename P, typename F>
-  __device__ __forceinline__ void pass(int first, int waves, int end, int seen, float qscale, int dv, char* s, P&& page_at, F&& where) {
+  __device__ __forceinline__ void pass(int first, int waves, int end, int seen, float qscale, int dv, char* s, P&& page_at,
+                                       F&& where) {
     using R = Raw<L, NB>;
     constexpr int G = step_group(L);
     if (first >= end) return;
@@ -521,8 +522,8 @@ __device__ __forceinline__ float wg_sum(float x, float* part) {
 // How items are cut into pieces of up to len blocks, a workgroup each: the first of a few lengths, from an even share of all
 // blocks on (total: a float, since rows that share their pages can be more blocks than an int holds), of which the chip holds
 // all pieces (`slots`) at once, and at least `least`. of(i) gives n items of some blocks each; a thread has i0 .. i1 - 1. Its
-// pieces are number before .. before + mine - 1 of all; where they never fit, they are at most slots + all items (t: the first
-// length that is tried, of 0 to 3). Whole shares of
+// pieces are number before .. before + mine - 1 of all; where they never fit, they are at most slots + all items. fit: that
+// they can is likely, and lengths of up to 15/8 of a share are tried; otherwise 11/8 is taken. Whole shares of
 // items, some workgroups with a little less to do, were faster than even shares that begin and end inside items and join more
 // parts (64 rows of up to 2304 positions in fp4: 33 us against 37).
 struct Cut {
@@ -533,19 +534,19 @@ struct Items {
   int n, blocks;
 };
 template <typename F>
-__device__ __forceinline__ Cut cut_items(float total, int i0, int i1, int slots, int least, int t, int* scan, F&& of) {
+__device__ __forceinline__ Cut cut_items(float total, int i0, int i1, int slots, int least, bool fit, int* scan, F&& of) {
   const float up = total < 0x1p24f ? 1.f : 1.f + 0x1p-14f;    // (the total may be rounded)
-  const int share = (int)ceilf(total / (float)slots * up);
+  const int share = max(least, (int)ceilf(total / (float)slots * up));
   Cut c;
-  for (; t < 4; ++t) {                    // uniform
-    c.len = max(least, share + share / 8 * t + share % 8 * t / 8);
+  for (int t = fit ? 0 : 3; ; t += t < 3 ? 1 : 2) {           // (uniform)
+    c.len = share + share / 8 * t + share % 8 * t / 8;
     c.mine = 0;
     for (int i = i0; i < i1; ++i) {
       const Items x = of(i);
       c.mine += x.n * c.pieces(x.blocks);
     }
     c.before = wg_scan(c.mine, scan, c.all);
-    if (c.all <= slots) break;
+    if (c.all <= slots || !fit || t == 7) break;
   }
   return c;
 }
@@ -566,16 +567,17 @@ __device__ __forceinline__ void place_of(const StepArgs& a, int page, int kvh, i
 // ---- the rows' own blocks -----------------------------------------------------------------------
 // An item is a row's KV head: its blocks, but for those that have been read with the group's prefix, cut into even pieces. The
 // pieces of an item are joined by the workgroup that finds all of them done.
-// Blocks of a piece, at least: four turns of its waves (fp4: two). With 8 a row of 2048 positions is 1.5 us faster, rows of 300 and 512
-// 1.5 to 3 us slower, for they are cut then.
+// Blocks of a piece, at least: four turns of its waves (fp4: two). With 8 a row of 2048 positions is 1.5 us faster, rows of 300
+// and 512 are 1.5 to 3 us slower, for they are cut then.
 constexpr int STEP_LEAST = 16;
 constexpr int STEP_WGS = 512;             // workgroups that the chip holds at once, by the kernel's LDS and registers
-// More items than those (MANY): rows of up to STEP_SHORT own blocks have four KV heads to a workgroup, one to a wave, and nothing to
-// join but a prefix; of longer ones a workgroup has a piece, as ever. Above 1024 items 512 workgroups take piece after piece, since
-// one that finds no piece costs 3 us of its place to find that out (512 rows of up to 64 positions, 8 KV heads, fp8: 77 -> 19 us; 256
-// of up to 200: 37 -> 21); up to there each piece has its own, which balances long rows better (66 rows of up to 4000: 68 us, 78 in
-// such a loop; 100 of up to 100: 17 -> 10.5). Limits of 4 and 16 blocks: 256 rows of 200 27 us, 32 rows of up to 1024 with 32 KV
-// heads 46 us against 35.
+// More items than those (MANY): rows of up to STEP_SHORT own blocks have four KV heads to a workgroup, one to a wave, which adds the
+// prefix's pieces by itself; of longer ones a workgroup has a piece, as ever. Above 1024 items 512 workgroups take piece after
+// piece, since one that finds no piece holds a place for 3 us to find that out (512 rows of up to 64 positions, 8 KV heads, fp8:
+// 77 -> 18.5 us; 256 of up to 200: 37 -> 19; 256 behind a prefix of 2000: 37 -> 16). Up to there each piece has its own, which
+// balances long rows better (66 rows of up to 4000: 68 us, 78 in such a loop). With 4 blocks as the limit 256 rows of 200 take 27
+// us, with 16 32 rows of up to 1024 with 32 KV heads 46 against 37; with 256 items as the bound 64 rows of up to 250 take 13.8
+// against 11.6.
 constexpr int STEP_SHORT = 8;
 inline bool step_many(int B, int n_kv) { return (long long)B * n_kv > STEP_WGS; }
 inline int step_slots(int B, int n_kv) { return STEP_WGS + B * n_kv; }         // pieces, at most
@@ -642,20 +644,57 @@ __device__ __forceinline__ f32x4 load_part4(__amdgpu_buffer_rsrc_t p, int at) {
   return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(p, at * 4, 0, SYSTEM_SCOPE));
 }
 
-// A wave's own result (of column tile 0), not joined with any: out from element `at` on.
+// A wave's result (of column tile 0), joined with the prefix's pieces (few, where there are many items) and written: row b's
+// queries of a KV head. A lane has its channels of a piece as it has its own.
 template <int L, int NB>
-__device__ __forceinline__ void store_wave(const StepArgs& a, const Wave<L, NB, 1>& st, long long at, bool none) {
-  const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-  const float l = wave_sum_xor48(st.l[0]), inv = none ? 0.f : 1.f / l;
+__device__ __forceinline__ void store_wave(const StepArgs& a, Wave<L, NB, 1>& st, int b, int head, const RowWork& r) {
+  constexpr bool T = L == PALU_LAYOUT_TILED;
+  int lane = threadIdx.x & 63;
+  asm("" : "+v"(lane));                   // (what follows from it is not kept in registers from piece to piece)
+  const int n = lane & 15, g = lane >> 4, d0 = (T ? 4 : 8) * g, d1 = d0 + (T ? 16 : 4);   // as in to_lds
+  float l = wave_sum_xor48(st.l[0]), m = st.m[0];
   if (n >= a.rep) return;
-  at += (long long)n * a.dv;
+  f32x4 y[2 * NB];
 #pragma unroll
-  for (int b = 0; b < NB; ++b) {
-    const f32x4 y = st.o[0][2 * b] * inv, z = st.o[0][2 * b + 1] * inv;        // as in to_lds
-    constexpr bool T = L == PALU_LAYOUT_TILED;
-    const int d0 = 32 * b + (T ? 4 : 8) * g, d1 = d0 + (T ? 16 : 4);
-    if (d0 < a.dv) store4(a, at + d0, T ? y : f32x4{y[0], z[0], y[1], z[1]});
-    if (d1 < a.dv) store4(a, at + d1, T ? z : f32x4{y[2], z[2], y[3], z[3]});
+  for (int i = 0; i < NB; ++i) {
+    const f32x4 p = st.o[0][2 * i], q = st.o[0][2 * i + 1];
+    y[2 * i] = T ? p : f32x4{p[0], q[0], p[1], q[1]};
+    y[2 * i + 1] = T ? q : f32x4{p[2], q[2], p[3], q[3]};
+  }
+  if (r.pieces) {                         // (uniform)
+    const int size = a.pre_cols * (a.dv + 2), col = r.local * a.rep + n, tile = col / a.pre_cols, x = col - tile * a.pre_cols;
+    const float* pre = a.pre + (r.base + (long long)(tile * a.n_kv + head) * r.pieces) * size;
+    struct Part {
+      f32x4 y[2 * NB];
+      float m, l;
+    } part;
+    auto load = [&](Part& p, int c) __attribute__((always_inline)) {
+      const float* at = pre + (long long)c * size;
+      p.m = at[a.pre_cols * a.dv + x];
+      p.l = at[a.pre_cols * (a.dv + 1) + x];
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {      // (of an odd multiple of 16 the upper half again)
+        p.y[2 * i] = *reinterpret_cast<const f32x4*>(at + x * a.dv + min(32 * i + d0, a.dv - 4));
+        p.y[2 * i + 1] = *reinterpret_cast<const f32x4*>(at + x * a.dv + min(32 * i + d1, a.dv - 4));
+      }
+    };
+#pragma unroll 1
+    for (int c = 0; c < r.pieces; ++c) {
+      load(part, c);
+      const float mn = fmaxf(m, part.m), ref = mn == NEG_INF ? 0.f : mn;
+      const float wa = __builtin_amdgcn_exp2f(m - ref), wb = __builtin_amdgcn_exp2f(part.m - ref);
+#pragma unroll
+      for (int i = 0; i < 2 * NB; ++i) y[i] = y[i] * wa + part.y[i] * wb;
+      l = l * wa + part.l * wb;
+      m = mn;
+    }
+  }
+  const float inv = 1.f / l;
+  const long long at = ((long long)b * a.n_q + head * a.rep + n) * a.dv;
+#pragma unroll
+  for (int i = 0; i < 2 * NB; ++i) {
+    const int d = 32 * (i / 2) + (i & 1 ? d1 : d0);
+    if (d < a.dv) store4(a, at + d, r.seen == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : y[i] * inv);
   }
 }
 
@@ -685,7 +724,8 @@ __global__ __launch_bounds__(256, 2) void palu_step_kernel(const StepArgs a) {
     const int blocks = r.end - r.first;
     return MANY && blocks <= STEP_SHORT ? Items{(a.n_kv + 3) / 4, 1} : Items{a.n_kv, blocks};
   };
-  const Cut cut = cut_items(wg_sum(mine, reinterpret_cast<float*>(scan)), r0, r1, STEP_WGS, STEP_LEAST, MANY ? 3 : 0, scan,
+  const bool fit = a.B * a.n_kv <= STEP_WGS * 3 / 4;
+  const Cut cut = cut_items(wg_sum(mine, reinterpret_cast<float*>(scan)), r0, r1, STEP_WGS, STEP_LEAST, fit, scan,
                             [&](int i) { return items_of(row(i)); });
   int want = blockIdx.x;
   if (!MANY && want >= cut.all) return;   // uniform
@@ -720,18 +760,21 @@ __global__ __launch_bounds__(256, 2) void palu_step_kernel(const StepArgs a) {
     st.clear();
     st.query(0, a.q + ((long long)b * a.n_q + head * a.rep + min(lane & 15, a.rep - 1)) * HD, a.qscale < 0.f);
     st.template pass<false>(
-        lo + (each ? 0 : w * step_group(L)), each ? 1 : 4, min(hi, (r.seen + 31) >> 5), r.seen, fabsf(a.qscale), a.dv, smem + w * place_bytes<L, NB>(),
+        lo + (each ? 0 : w * step_group(L)), each ? 1 : 4, min(hi, (r.seen + 31) >> 5), r.seen, fabsf(a.qscale), a.dv,
+        smem + w * place_bytes<L, NB>(),
         [&](int blk) __attribute__((always_inline)) { return page_of(a, blk < r.pblocks ? r.lead : b, blk); },
         [&](int page, int blk, const char*& k, const char*& v) __attribute__((always_inline)) {
           place_of(a, page, head, blk, k, v);
         });
-    if (each && !r.pieces) {                // (uniform) nothing to join
-      if (head0 + w < a.n_kv) store_wave<L, NB>(a, st, ((long long)b * a.n_q + head * a.rep) * a.dv, r.seen == 0);
+    if (each) {                           // (uniform)
+      if (head0 + w < a.n_kv) store_wave<L, NB>(a, st, b, head, r);
       continue;
     }
     __syncthreads();                        // every wave is done with its places
     to_lds(lds, st, 0);
     __syncthreads();
+    int tid = threadIdx.x;
+    if (MANY) asm("" : "+v"(tid));        // (see store_wave)
     const int vecs = a.dv / 4, units = a.rep * vecs;
     const long long part_size = (long long)a.rep * (a.dv + 2);
     if (chunks > 1) {
@@ -748,103 +791,101 @@ __global__ __launch_bounds__(256, 2) void palu_step_kernel(const StepArgs a) {
       }
       if (!chunks_all_done(a.flags + wg0, a.epoch, chunks, chunk, found)) continue; // uniform
     }
-    for (int x = 0, kvh = head0; x < (each ? 4 : 1) && kvh < a.n_kv; ++x, ++kvh) {   // (uniform)
-      auto finish = [&](int h, int d, const Joined& j) __attribute__((always_inline)) {
-        const float inv = 1.f / j.l;
-        const f32x4 y = r.seen == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : j.y * inv;       // a row that sees nothing: zeros
-        store4(a, ((long long)b * a.n_q + kvh * a.rep + h) * a.dv + d, y);
-      };
-      // The parts: this workgroup's own (in LDS), or all workgroups' (one of which is its own), and the prefix's pieces, which the
-      // launch before wrote.
-      const __amdgpu_buffer_rsrc_t parts = parts_at(a.part + wg0 * part_size);
-      const int pre_size = a.pre_cols * (a.dv + 2);
-      auto pieces_of = [&](int h, int& x) {   // the pieces of a head, in column x of theirs
-        const int col = r.local * a.rep + h, tile = r.pieces ? col / a.pre_cols : 0;
-        x = col - tile * a.pre_cols;
-        return a.pre + (r.base + (long long)(tile * a.n_kv + kvh) * r.pieces) * pre_size;
-      };
-      const int groups = min(max(1, 256 / units), MAX_GROUPS), grp = groups > 1 ? tid / units : 0, batch = U * groups;
-      for (int e0 = 0; e0 < units; e0 += 256) {                   // (uniform)
-        const int e = groups > 1 ? tid - grp * units : e0 + tid;
-        const bool on = e < units && grp < groups;
-        const int h = on ? e / vecs : 0, d = on ? 4 * (e - h * vecs) : 0;
-        Joined j = no_parts();
-        // n parts, U to each of 256 / units threads at a time, whose loads are all under way together: stat(c, x, m, l) loads the
-        // statistics of part c's column x, four(c) this thread's four channels.
-        auto gather = [&](int n, auto&& stat, auto&& four) __attribute__((always_inline)) {
-          for (int c0 = 0; c0 < n; c0 += batch) {                 // (uniform)
-            float m[MAX_GROUPS], l[MAX_GROUPS];
+    const int kvh = head0;
+    auto finish = [&](int h, int d, const Joined& j) __attribute__((always_inline)) {
+      const float inv = 1.f / j.l;
+      const f32x4 y = r.seen == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : j.y * inv;       // a row that sees nothing: zeros
+      store4(a, ((long long)b * a.n_q + kvh * a.rep + h) * a.dv + d, y);
+    };
+    // The parts: this workgroup's own (in LDS), or all workgroups' (one of which is its own), and the prefix's pieces, which the
+    // launch before wrote.
+    const __amdgpu_buffer_rsrc_t parts = parts_at(a.part + wg0 * part_size);
+    const int pre_size = a.pre_cols * (a.dv + 2);
+    auto pieces_of = [&](int h, int& x) {   // the pieces of a head, in column x of theirs
+      const int col = r.local * a.rep + h, tile = r.pieces ? col / a.pre_cols : 0;
+      x = col - tile * a.pre_cols;
+      return a.pre + (r.base + (long long)(tile * a.n_kv + kvh) * r.pieces) * pre_size;
+    };
+    const int groups = min(max(1, 256 / units), MAX_GROUPS), grp = groups > 1 ? tid / units : 0, batch = U * groups;
+    for (int e0 = 0; e0 < units; e0 += 256) {                   // (uniform)
+      const int e = groups > 1 ? tid - grp * units : e0 + tid;
+      const bool on = e < units && grp < groups;
+      const int h = on ? e / vecs : 0, d = on ? 4 * (e - h * vecs) : 0;
+      Joined j = no_parts();
+      // n parts, U to each of 256 / units threads at a time, whose loads are all under way together: stat(c, x, m, l) loads the
+      // statistics of part c's column x, four(c) this thread's four channels.
+      auto gather = [&](int n, auto&& stat, auto&& four) __attribute__((always_inline)) {
+        for (int c0 = 0; c0 < n; c0 += batch) {                 // (uniform)
+          float m[MAX_GROUPS], l[MAX_GROUPS];
 #pragma unroll
-            for (int i = 0; i < MAX_GROUPS; ++i) {
-              if (16 * i >= batch || c0 + 16 * i >= n) break;     // (uniform)
-              stat(min(c0 + 16 * i + (tid >> 4), n - 1), min(tid & 15, a.rep - 1), m[i], l[i]);
-            }
-            f32x4 y[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-              if (c0 + u * groups >= n) break;                    // (uniform)
-              y[u] = four(min(c0 + u * groups + min(grp, groups - 1), n - 1));
-            }
-            __syncthreads();                  // the batch before has been read
-#pragma unroll
-            for (int i = 0; i < MAX_GROUPS; ++i) {
-              const int c = 16 * i + (tid >> 4);
-              if (16 * i >= batch || c0 + 16 * i >= n) break;
-              joining.stats[0][c][tid & 15] = m[i];
-              joining.stats[1][c][tid & 15] = l[i];
-            }
-            __syncthreads();
-            if (!on) continue;
-            Joined b = no_parts();
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-              if (c0 + u * groups + grp >= n) break;
-              b.m = fmaxf(b.m, joining.stats[0][u * groups + grp][h]);
-            }
-            const float ref = b.m == NEG_INF ? 0.f : b.m;
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-              if (c0 + u * groups + grp >= n) break;
-              const float f = __builtin_amdgcn_exp2f(joining.stats[0][u * groups + grp][h] - ref);
-              b.l += f * joining.stats[1][u * groups + grp][h];
-              b.y += f * y[u];
-            }
-            j.add(b.y, b.m, b.l);
+          for (int i = 0; i < MAX_GROUPS; ++i) {
+            if (16 * i >= batch || c0 + 16 * i >= n) break;     // (uniform)
+            stat(min(c0 + 16 * i + (tid >> 4), n - 1), min(tid & 15, a.rep - 1), m[i], l[i]);
           }
-        };
-        gather(chunks == 1 ? 0 : chunks, [&](int c, int x, float& m, float& l) __attribute__((always_inline)) {
-                 const float* p = a.part + (wg0 + c) * part_size + a.rep * a.dv + x;
-                 m = load_part(p);
-                 l = load_part(p + a.rep);
-               }, [&](int c) __attribute__((always_inline)) { return load_part4(parts, c * (int)part_size + h * a.dv + d); });
-        int col, stat_col;
-        const float *pre = pieces_of(h, col), *stats = pieces_of(min(tid & 15, a.rep - 1), stat_col);
-        gather(r.pieces, [&](int c, int x, float& m, float& l) __attribute__((always_inline)) {
-                 const float* p = stats + (long long)c * pre_size + a.pre_cols * a.dv + stat_col;
-                 m = p[0];
-                 l = p[a.pre_cols];
-               }, [&](int c) __attribute__((always_inline)) {
-                 return *reinterpret_cast<const f32x4*>(pre + (long long)c * pre_size + col * a.dv + d);
-               });
-        if (on && chunks == 1 && grp == 0) {
-          const Joined mine = each ? Joined{*reinterpret_cast<const f32x4*>(lds.row(x, h) + d), lds.m(x, h), lds.l(x, h)}
-                                   : join_waves(lds, h, d);
-          j.add(mine.y, mine.m, mine.l);
-        }
-        if (groups == 1) {
-          if (on) finish(h, d, j);
-          continue;
-        }
-        __syncthreads();                      // the last batch has been read
-        if (on) joining.sums[tid] = j;
-        __syncthreads();
-        if (tid < units) {
-          for (int i = 1; i < groups; ++i) {
-            const Joined x = joining.sums[tid + i * units];
-            j.add(x.y, x.m, x.l);
+          f32x4 y[U];
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            if (c0 + u * groups >= n) break;                    // (uniform)
+            y[u] = four(min(c0 + u * groups + min(grp, groups - 1), n - 1));
           }
-          finish(h, d, j);
+          __syncthreads();                  // the batch before has been read
+#pragma unroll
+          for (int i = 0; i < MAX_GROUPS; ++i) {
+            const int c = 16 * i + (tid >> 4);
+            if (16 * i >= batch || c0 + 16 * i >= n) break;
+            joining.stats[0][c][tid & 15] = m[i];
+            joining.stats[1][c][tid & 15] = l[i];
+          }
+          __syncthreads();
+          if (!on) continue;
+          Joined b = no_parts();
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            if (c0 + u * groups + grp >= n) break;
+            b.m = fmaxf(b.m, joining.stats[0][u * groups + grp][h]);
+          }
+          const float ref = b.m == NEG_INF ? 0.f : b.m;
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            if (c0 + u * groups + grp >= n) break;
+            const float f = __builtin_amdgcn_exp2f(joining.stats[0][u * groups + grp][h] - ref);
+            b.l += f * joining.stats[1][u * groups + grp][h];
+            b.y += f * y[u];
+          }
+          j.add(b.y, b.m, b.l);
         }
+      };
+      gather(chunks == 1 ? 0 : chunks, [&](int c, int x, float& m, float& l) __attribute__((always_inline)) {
+               const float* p = a.part + (wg0 + c) * part_size + a.rep * a.dv + x;
+               m = load_part(p);
+               l = load_part(p + a.rep);
+             }, [&](int c) __attribute__((always_inline)) { return load_part4(parts, c * (int)part_size + h * a.dv + d); });
+      int col, stat_col;
+      const float *pre = pieces_of(h, col), *stats = pieces_of(min(tid & 15, a.rep - 1), stat_col);
+      gather(r.pieces, [&](int c, int x, float& m, float& l) __attribute__((always_inline)) {
+               const float* p = stats + (long long)c * pre_size + a.pre_cols * a.dv + stat_col;
+               m = p[0];
+               l = p[a.pre_cols];
+             }, [&](int c) __attribute__((always_inline)) {
+               return *reinterpret_cast<const f32x4*>(pre + (long long)c * pre_size + col * a.dv + d);
+             });
+      if (on && chunks == 1 && grp == 0) {
+        const Joined mine = join_waves(lds, h, d);
+        j.add(mine.y, mine.m, mine.l);
+      }
+      if (groups == 1) {
+        if (on) finish(h, d, j);
+        continue;
+      }
+      __syncthreads();                      // the last batch has been read
+      if (on) joining.sums[tid] = j;
+      __syncthreads();
+      if (tid < units) {
+        for (int i = 1; i < groups; ++i) {
+          const Joined x = joining.sums[tid + i * units];
+          j.add(x.y, x.m, x.l);
+        }
+        finish(h, d, j);
       }
     }
   } while (MANY && (want += gridDim.x, true));
@@ -906,7 +947,7 @@ __global__ __launch_bounds__(256, 2) void palu_prefix_kernel(const StepArgs a) {
   const bool lone = of_lone <= of_larger;
   if (!lone && own.rows == 1) own.blocks = 0;
   auto group = [&](int i) { return per == 1 ? own : group_of(a, i, lone); };
-  const Cut cut = cut_items(of_larger + (lone ? of_lone : 0.f), g0, g1, PRE_WGS, PRE_LEAST, 0, scan, [&](int i) {
+  const Cut cut = cut_items(of_larger + (lone ? of_lone : 0.f), g0, g1, PRE_WGS, PRE_LEAST, true, scan, [&](int i) {
     const Group g = group(i);
     return Items{tiles_of(g), g.blocks};
   });

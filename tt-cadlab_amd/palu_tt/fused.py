@@ -176,13 +176,16 @@ def _cache_arg(t, name: str, device, role: Optional[str] = None, mx: bool = Fals
         if not mx:
             raise RuntimeError(f"{name} is an MXCache, which this op does not read or write (flash_decode, flash_decode_shared, "
                                "paged_fill_cache, paged_update_cache and paged_read_cache do)")
-        _as_dev(t.data, name, torch.uint8, device)
+        data, fp8 = t.data, t.fmt == "fp8"
+        if not (data.dtype is torch.uint8 and data.is_cuda and data.is_contiguous() and data.device == device):
+            _as_dev(data, name, torch.uint8, device)
         if not (role is None or t.role == role):
             raise RuntimeError(f"{name} is an MXCache in {t.role!r} order; this argument reads a {role!r} cache")
-        if t.data.shape[-1] != MXCache.block_bytes(t.fmt, t.width):      # (data may have been replaced)
-            raise RuntimeError(f"{name}: blocks of {t.data.shape[-1]} bytes are not those of {t.fmt} and width {t.width}")
-        layout = _native.LAYOUT_MX8 if t.fmt == "fp8" else _native.LAYOUT_MX4
-        return t.data, t.shape, layout + (1 if role is None and t.role == "v" else 0)
+        B, G, blocks, size = data.shape
+        if size != MXCache.block_bytes(t.fmt, t.width):      # (data may have been replaced)
+            raise RuntimeError(f"{name}: blocks of {size} bytes are not those of {t.fmt} and width {t.width}")
+        layout = _native.LAYOUT_MX8 if fp8 else _native.LAYOUT_MX4
+        return data, (B, G, 32 * blocks, t.width), layout + (1 if role is None and t.role == "v" else 0)
     if isinstance(t, GroupedLatentCache):
         _as_dev(t.data, name, torch.bfloat16, device)
         if not (role is not None and t.role == role):
@@ -455,7 +458,8 @@ def _step_out(q, n_kv: int, width: int, out_dtype, out, workspace, need: int, in
     else:
         _native.workspace_bytes(workspace, need, dev)
     if out is None:
-        return torch.empty(1, B, n_q, width, dtype=out_dtype, device=dev), workspace
+        like = width == HEAD_DIM and out_dtype is torch.bfloat16
+        return torch.empty_like(q) if like else torch.empty(1, B, n_q, width, dtype=out_dtype, device=dev), workspace
     _as_dev(out, "out", out_dtype, dev)
     if tuple(out.shape) != (1, B, n_q, width):
         raise RuntimeError(f"out must be [1, {B}, {n_q}, {width}]")

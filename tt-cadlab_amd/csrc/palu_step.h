@@ -664,28 +664,19 @@ __device__ __forceinline__ void store_wave(const StepArgs& a, Wave<L, NB, 1>& st
   if (r.pieces) {                         // (uniform)
     const int size = a.pre_cols * (a.dv + 2), col = r.local * a.rep + n, tile = col / a.pre_cols, x = col - tile * a.pre_cols;
     const float* pre = a.pre + (r.base + (long long)(tile * a.n_kv + head) * r.pieces) * size;
-    struct Part {
-      f32x4 y[2 * NB];
-      float m, l;
-    } part;
-    auto load = [&](Part& p, int c) __attribute__((always_inline)) {
-      const float* at = pre + (long long)c * size;
-      p.m = at[a.pre_cols * a.dv + x];
-      p.l = at[a.pre_cols * (a.dv + 1) + x];
-#pragma unroll
-      for (int i = 0; i < NB; ++i) {      // (of an odd multiple of 16 the upper half again)
-        p.y[2 * i] = *reinterpret_cast<const f32x4*>(at + x * a.dv + min(32 * i + d0, a.dv - 4));
-        p.y[2 * i + 1] = *reinterpret_cast<const f32x4*>(at + x * a.dv + min(32 * i + d1, a.dv - 4));
-      }
-    };
 #pragma unroll 1
     for (int c = 0; c < r.pieces; ++c) {
-      load(part, c);
-      const float mn = fmaxf(m, part.m), ref = mn == NEG_INF ? 0.f : mn;
-      const float wa = __builtin_amdgcn_exp2f(m - ref), wb = __builtin_amdgcn_exp2f(part.m - ref);
+      const float* piece = pre + (long long)c * size;
+      const float pm = piece[a.pre_cols * a.dv + x], pl = piece[a.pre_cols * (a.dv + 1) + x];
+      f32x4 py[2 * NB];
 #pragma unroll
-      for (int i = 0; i < 2 * NB; ++i) y[i] = y[i] * wa + part.y[i] * wb;
-      l = l * wa + part.l * wb;
+      for (int i = 0; i < 2 * NB; ++i)    // (past an odd multiple of 16 the last channels again)
+        py[i] = *reinterpret_cast<const f32x4*>(piece + x * a.dv + min(32 * (i / 2) + (i & 1 ? d1 : d0), a.dv - 4));
+      const float mn = fmaxf(m, pm), ref = mn == NEG_INF ? 0.f : mn;
+      const float wa = __builtin_amdgcn_exp2f(m - ref), wb = __builtin_amdgcn_exp2f(pm - ref);
+#pragma unroll
+      for (int i = 0; i < 2 * NB; ++i) y[i] = y[i] * wa + py[i] * wb;
+      l = l * wa + pl * wb;
       m = mn;
     }
   }

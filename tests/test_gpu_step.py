@@ -122,8 +122,12 @@ class Batch:
     def decode(self, **kw):
         return fused.flash_decode(self.q, self.k, self.v, self.pos, page_table_tensor=self.table.to(self.dev), **kw)
 
-    def decode_shared(self, **kw):
-        return fused.flash_decode_shared(self.q, self.k, self.v, self.pos, self.own.to(self.dev), self.shared, self.cu, **kw)
+    def decode_shared(self, wide=True, **kw):
+        """wide: over a table with room for 65536 positions, where prefixes are read ahead whatever the rows' lengths."""
+        own = self.own
+        if wide:
+            own = torch.nn.functional.pad(own, (0, 65536 // self.page - own.shape[1]), value=-1)
+        return fused.flash_decode_shared(self.q, self.k, self.v, self.pos, own.to(self.dev), self.shared, self.cu, **kw)
 
 
 # ---- quantised caches ----------------------------------------------------------------------------
@@ -285,6 +289,7 @@ _GROUPS = [
 def test_groups(gpu, layout, groups, shared, lens, nq, nkv):
     x = Batch(gpu, layout, lens, nq, nkv, groups=groups, shared=shared, seed=sum(lens), page=64 if sum(lens) % 2 else 32)
     x.check(x.decode_shared())
+    x.check(x.decode_shared(wide=False))                                 # little enough for a launch without the prefixes'
 
 
 @pytest.mark.parametrize("layout", LAYOUTS)
@@ -310,6 +315,7 @@ def test_lone_rows_beside_groups(gpu, layout, rows):
     lens = [s + 13 * i for i, (n, s) in enumerate(zip(rows, shared)) for _ in range(n)]
     x = Batch(gpu, layout, lens, 8, 2, 64, 64, rows, shared, seed=len(lens))
     x.check(x.decode_shared())
+    x.check(x.decode_shared(wide=False))
 
 
 @pytest.mark.parametrize("layout", LAYOUTS)
@@ -322,6 +328,7 @@ def test_many_items_behind_prefixes(gpu, layout, B, groups, prefix, tail, nq, nk
     lens = [s + int(torch.randint(0, tail, (), generator=g)) for n, s in zip(rows, shared) for _ in range(n)]
     x = Batch(gpu, layout, lens, nq, nkv, 48 if layout in ("rows", "tiled") else 64, 64, rows, shared, seed=B, garbage=0.0)
     x.check(x.decode_shared(), rows=list(range(0, B, 7)) + [B - 1])
+    x.check(x.decode_shared(wide=False), rows=list(range(0, B, 7)) + [B - 1])
 
 
 @pytest.mark.parametrize("layout", ["rows", "tiled"])
@@ -359,24 +366,29 @@ def test_shared_equal_values_come_back_exactly(gpu, layout, std):
 @pytest.mark.parametrize("layout", LAYOUTS)
 def test_shared_without_groups_and_rows_of_no_group(gpu, layout):
     x = Batch(gpu, layout, [100, 70, 65, 90], groups=[4], shared=[64])
-    got = x.decode_shared()
+    got = x.decode_shared(wide=False)
     assert torch.equal(got, fused.flash_decode_shared(x.q, x.k, x.v, x.pos, x.own.to(gpu), x.shared))   # no cu_groups: one group
+    cu, x.cu = x.cu, None
+    ahead, x.cu = x.decode_shared(), cu
+    assert torch.equal(x.decode_shared(), ahead)
     y = Batch(gpu, layout, [100, 70, 65, 90], groups=[1, 2], shared=[64, 64])     # groups of rows 1 and 2; row 0 alone, row 3 of none
     y.cu, y.shared = _ints([1, 3], gpu), _ints([64], gpu)
     y.lead, y.blocks, y.own = [0, 1, 1, 3], [0, 2, 2, 0], y.table.clone()
     y.check(y.decode_shared())
+    y.check(y.decode_shared(wide=False))
 
 
 @pytest.mark.parametrize("layout", LAYOUTS)
-def test_shared_nan_reaches_the_rows_that_see_it(gpu, layout):
+@pytest.mark.parametrize("wide", [True, False])
+def test_shared_nan_reaches_the_rows_that_see_it(gpu, layout, wide):
     """One inside the prefix, which a row of the group that ends before it does not see; one behind it."""
     x = Batch(gpu, layout, [200, 90, 180, 100], 8, 2, groups=[3, 1], shared=[160, 0], garbage=0.0)
-    clean = x.decode_shared()
+    clean = x.decode_shared(wide)
     for page, row, rows in ((3, 0, (0, 2)), (5, 2, (2,))):
         bad = x.krows.clone()
         bad[int(x.table[row, page]), 1, 5, 9] = math.nan
         k, x.k = x.k, _store(bad, "k", layout)[0]
-        got, x.k = x.decode_shared(), k
+        got, x.k = x.decode_shared(wide), k
         hit = torch.zeros_like(clean, dtype=torch.bool)
         hit[0, list(rows), 4:] = True
         assert got[hit].isnan().all() and torch.equal(got[~hit], clean[~hit])
@@ -389,10 +401,13 @@ def test_offsets_that_make_no_sense_stay_inside(gpu, layout):
     B, n = 24, 40
     x = Batch(gpu, layout, [300] * B, 16, 1, garbage=0.0)
     g = torch.Generator().manual_seed(1)
-    for cu in ([0, B] * (n // 2) + [0], torch.randint(-100, 200, (n + 1,), generator=g).tolist(), [2 ** 31 - 1] * n + [-2 ** 31], [B] * n + [0]):
+    wide = torch.nn.functional.pad(x.table, (0, 65536 // x.page - x.table.shape[1]), value=-1)
+    for cu, table in [(cu, table) for table in (wide, x.table) for cu in
+                      ([0, B] * (n // 2) + [0], torch.randint(-100, 200, (n + 1,), generator=g).tolist(), [2 ** 31 - 1] * n + [-2 ** 31],
+                       [B] * n + [0])]:
         need = _native.load().palu_flash_decode_shared_workspace_bytes(B, n, 16, 1, 64)
         ws, out = torch.full((need + 8192,), 77, dtype=torch.uint8, device=gpu), torch.full((1, B + 2, 16, 64), 7.0, dtype=BF, device=gpu)
-        fused.flash_decode_shared(x.q, x.k, x.v, x.pos, x.table.to(gpu), _ints([2 ** 31 - 1, 300, -2 ** 31, 64] * (n // 4), gpu), _ints(cu, gpu),
+        fused.flash_decode_shared(x.q, x.k, x.v, x.pos, table.to(gpu), _ints([2 ** 31 - 1, 300, -2 ** 31, 64] * (n // 4), gpu), _ints(cu, gpu),
                                   out=out[:, 1:-1], workspace=ws[4096:4096 + need])
         assert (ws[:4096] == 77).all() and (ws[4096 + need:] == 77).all() and (out[0, 0] == 7).all() and (out[0, -1] == 7).all()
     x.check(x.decode())                                                  # and nothing is left behind

@@ -54,7 +54,7 @@ struct StepArgs {
   float* part;
   unsigned long long* flags;
   unsigned long long epoch;
-  // Shared prefixes (rows null: none).
+  // Shared prefixes (shared null: none; rows null: not read ahead).
   const int32_t* cu;                      // [n_groups + 1] first row of every group; null: one group
   const int32_t* shared;                  // [n_groups] positions shared
   int n_groups;
@@ -586,6 +586,29 @@ inline size_t step_bytes(int B, int n_kv, int rep, int dv) {
   return (size_t)step_slots(B, n_kv) * ((size_t)rep * (dv + 2) * sizeof(float) + sizeof(unsigned long long));
 }
 
+struct Group {
+  int row, rows, blocks;                  // blocks: of the prefix, 0 where nothing is shared
+};
+__device__ __forceinline__ Group group_of(const StepArgs& a, int gi, bool lone) {
+  const int c0 = a.cu ? a.cu[gi] : 0, c1 = a.cu ? a.cu[gi + 1] : a.B;
+  Group g;
+  g.row = min(max(c0, 0), a.B);
+  g.rows = min(max(c1, g.row), a.B) - g.row;
+  g.blocks = g.rows > (lone ? 0 : 1) ? min(max(a.shared[gi], 0), a.capacity) >> 5 : 0;
+  return g;
+}
+
+// The last group that begins at row b or before it.
+__device__ __forceinline__ int last_group(const StepArgs& a, int b) {
+  int gi = 0;
+  for (int end = a.n_groups; end - gi > 1;) {
+    const int mid = (gi + end) >> 1;
+    if (a.cu[mid] <= b) gi = mid;
+    else end = mid;
+  }
+  return gi;
+}
+
 struct RowWork {
   int lead, first, end, seen, pieces;     // blocks first .. end - 1 (at least one, which may hold nothing), prefix pieces
   int base, local, pblocks;
@@ -603,6 +626,12 @@ __device__ __forceinline__ RowWork row_work(const StepArgs& a, int b) {
       r.pieces = p.pieces;
       r.base = p.base;
       r.local = p.local;
+    }
+  } else if (a.shared) {                  // nothing has been read: the prefix's blocks are the row's, by its group's table
+    const Group g = group_of(a, last_group(a, b), false);
+    if (b >= g.row && b < g.row + g.rows) {
+      r.lead = g.row;
+      r.pblocks = g.blocks;
     }
   }
   return r;
@@ -906,18 +935,6 @@ inline size_t pre_bytes(int B, int n_groups, int rep, int n_kv, int dv) {
   return (size_t)pre_slots(B, n_groups, rep, n_kv, C) * 16 * C * (dv + 2) * sizeof(float) + (size_t)B * sizeof(RowPrefix);
 }
 
-struct Group {
-  int row, rows, blocks;                  // blocks: of the prefix, 0 where nothing is shared
-};
-__device__ __forceinline__ Group group_of(const StepArgs& a, int gi, bool lone) {
-  const int c0 = a.cu ? a.cu[gi] : 0, c1 = a.cu ? a.cu[gi + 1] : a.B;
-  Group g;
-  g.row = min(max(c0, 0), a.B);
-  g.rows = min(max(c1, g.row), a.B) - g.row;
-  g.blocks = g.rows > (lone ? 0 : 1) ? min(max(a.shared[gi], 0), a.capacity) >> 5 : 0;
-  return g;
-}
-
 template <int L, int NB, int C>
 __global__ __launch_bounds__(256, 2) void palu_prefix_kernel(const StepArgs a) {
   __shared__ __attribute__((aligned(1024))) char smem[L == PALU_LAYOUT_ROWS ? step_lds<L, NB>() : WaveLds<NB>::bytes(16)];
@@ -952,12 +969,7 @@ __global__ __launch_bounds__(256, 2) void palu_prefix_kernel(const StepArgs a) {
     __syncthreads();
   }
   if (rec < row_wgs && b < a.B) {
-    int gi = 0;
-    for (int end = a.n_groups; end - gi > 1;) {   // the last group that begins at b or before it
-      const int mid = (gi + end) >> 1;
-      if (a.cu[mid] <= b) gi = mid;
-      else end = mid;
-    }
+    const int gi = last_group(a, b);
     RowPrefix r{b, 0, 0, 0, 0, {}};
     const Group g = group_of(a, gi, lone);
     if (g.blocks && b >= g.row && b < g.row + g.rows) {

@@ -123,7 +123,7 @@ class Batch:
         return fused.flash_decode(self.q, self.k, self.v, self.pos, page_table_tensor=self.table.to(self.dev), **kw)
 
     def decode_shared(self, wide=True, **kw):
-        """wide: over a table with room for 65536 positions, where prefixes are read ahead whatever the rows' lengths."""
+        """wide: over a table with room for 65536 positions, where prefixes are read ahead (but for a few rows in 4 bits)."""
         own = self.own
         if wide:
             own = torch.nn.functional.pad(own, (0, 65536 // self.page - own.shape[1]), value=-1)

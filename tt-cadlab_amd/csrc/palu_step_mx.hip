@@ -133,10 +133,12 @@ extern "C" int palu_flash_decode_shared(const void* q, const void* k_pages, cons
   a.pre_cols = 16 * C;
   a.pre_slots = (int)pre_slots(batch, n_groups, a.rep, n_kv, C);
   a.pre = reinterpret_cast<float*>(static_cast<char*>(workspace) + align16(step_bytes(batch, n_kv, a.rep, head_dim_v)));
-  // The prefixes are read ahead unless all that the tables can name is so little, read for each row by itself, that this takes less
-  // than a launch more: 16 MB, rows of 2048 positions (three rows of fp8 behind 100 positions 14.4 -> 11.4 us, behind 1000 16 -> 12).
+  // Where all that the tables can name is little, each row reads its prefix by itself, by its group's table: 64 MiB or less take less
+  // than a second launch and its join (both launches, and one: three rows of fp8 behind 100 positions 14.2 us, 7.8, behind 8000
+  // 19.1, 16.0; 64 rows of tiles behind 128 positions, 67 MB, 20.3, 12.9; 16 rows over 71 MB, the prefixes nearly all of it, 18.7,
+  // 21.2; 30 rows of fp4 over 65 MB 19.2, 19.2).
   const long long most = (long long)batch * n_kv * (a.capacity / 32) * (a.k_blk + a.v_blk);
-  if (most > (16 << 20) || a.capacity > 2048)
+  if (most > (64LL << 20))
     a.rows = reinterpret_cast<RowPrefix*>(a.pre + (long long)a.pre_slots * a.pre_cols * (head_dim_v + 2));
   return step_any(a, cache_layout, who, stream);
 }

@@ -493,9 +493,10 @@ size_t palu_mx_decode_workspace_bytes(int batch, int n_q, int n_kv, int head_dim
 /* palu_flash_decode_paged of a batch in groups of neighbouring rows that share a prefix: rows cu_groups[i] .. cu_groups[i + 1] - 1
  * (int32 [n_groups + 1], device memory, not decreasing; NULL: n_groups is 1 and all rows are one group) share their first
  * shared_len[i] positions (int32 [n_groups], device memory). Whole 32-position blocks of them are read through the page table of
- * the group's first row, once for all rows of the group that see them all (once for each where the tables name 64 MiB at most,
- * which takes less than reading ahead); the rest of a row is read through its own table
- * (whose entries before that are not looked at). Rows of no group stand alone. Layouts PALU_LAYOUT_ROWS, _TILED (head_dim_v
+ * the group's first row, or, where that table's first entry is no page of the pool (the row has ended: palu_pages_update leaves
+ * -1), of the first row behind it whose first entry is one; once for all rows of the group that see them all (once for each where
+ * the tables name 64 MiB at most, which takes less than reading ahead). The rest of a row is read through its own table
+ * (whose entries before that are not looked at, but for the first). Rows of no group stand alone. Layouts PALU_LAYOUT_ROWS, _TILED (head_dim_v
  * multiples of 16 up to 128), _MX8 and _MX4 (of 32). A row at a negative position sees nothing and gets zeros, one past the
  * table sees all of it; page ids are clamped into the pool. At most 4096 rows. Bit-reproducible. workspace:
  * palu_flash_decode_shared_workspace_bytes, any contents, 16-byte aligned; calls that share one must be ordered on one stream. */

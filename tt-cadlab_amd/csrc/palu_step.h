@@ -31,10 +31,11 @@
 
 namespace palu {
 
-// What a row has of a prefix: its blocks 0 .. blocks - 1 are read through row `lead`'s table; where pieces > 0 they have been
-// read, and the row's queries are columns local * rep .. of the group's, in slots base + (tile * n_kv + kv) * pieces ..
+// What a row has of a prefix: its blocks 0 .. blocks - 1 are read through the table of its group's lead (lead_of), one of `rows`
+// rows from `first` on; where pieces > 0 they have been read, and the row's queries are columns local * rep .. of the group's, in
+// slots base + (tile * n_kv + kv) * pieces ..
 struct RowPrefix {
-  int lead, blocks, pieces, base, local, unused[3];
+  int first, rows, blocks, pieces, base, local, unused[2];
 };
 
 struct StepArgs {
@@ -609,16 +610,31 @@ __device__ __forceinline__ int last_group(const StepArgs& a, int b) {
   return gi;
 }
 
+// The row through whose table a group's prefix is read: the first whose table begins with a page of the pool, since a row that
+// has ended has none, and its pages may be another request's; the group's first where there is no such row. Of a whole wave.
+__device__ __forceinline__ int lead_of(const StepArgs& a, int row, int rows) {
+  const auto there = [&](int id) { return id >= 0 && id < a.n_pages; };
+  if (rows == 1 || there(load_uniform(a.table, (long long)row * a.pt_stride))) return row;
+  for (int i = 0; i < rows; i += 64) {    // (uniform)
+    const int r = row + min(i + (int)(threadIdx.x & 63), rows - 1);
+    const unsigned long long m = __ballot(there(a.table[(long long)r * a.pt_stride]));
+    if (m) return row + min(i + __builtin_ctzll(m), rows - 1);
+  }
+  return row;
+}
+
 struct RowWork {
-  int lead, first, end, seen, pieces;     // blocks first .. end - 1 (at least one, which may hold nothing), prefix pieces
-  int base, local, pblocks;
+  int first, end, seen, pieces;           // blocks first .. end - 1 (at least one, which may hold nothing), prefix pieces
+  int base, local;
+  int pblocks, group, rows;               // blocks of the prefix, the group's first row and rows
 };
 __device__ __forceinline__ RowWork row_work(const StepArgs& a, int b) {
   const int seen = seen_of(a, a.cur[b]), end = (seen + 31) >> 5;
-  RowWork r{b, 0, max(end, 1), seen, 0, 0, 0, 0};
+  RowWork r{0, max(end, 1), seen, 0, 0, 0, 0, b, 1};
   if (a.rows) {
     const RowPrefix p = a.rows[b];
-    r.lead = p.lead;
+    r.group = p.first;
+    r.rows = p.rows;
     r.pblocks = p.blocks;
     if (p.pieces && seen >= 32 * p.blocks) {
       r.first = p.blocks;
@@ -630,7 +646,8 @@ __device__ __forceinline__ RowWork row_work(const StepArgs& a, int b) {
   } else if (a.shared) {                  // nothing has been read: the prefix's blocks are the row's, by its group's table
     const Group g = group_of(a, last_group(a, b), false);
     if (b >= g.row && b < g.row + g.rows) {
-      r.lead = g.row;
+      r.group = g.row;
+      r.rows = g.rows;
       r.pblocks = g.blocks;
     }
   }
@@ -639,8 +656,8 @@ __device__ __forceinline__ RowWork row_work(const StepArgs& a, int b) {
 
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ __forceinline__ RowWork uniform(const RowWork& r) {
-  return RowWork{uniform(r.lead), uniform(r.first), uniform(r.end),  uniform(r.seen),
-                 uniform(r.pieces), uniform(r.base), uniform(r.local), uniform(r.pblocks)};
+  return RowWork{uniform(r.first), uniform(r.end),     uniform(r.seen),  uniform(r.pieces), uniform(r.base),
+                 uniform(r.local), uniform(r.pblocks), uniform(r.group), uniform(r.rows)};
 }
 
 __device__ __forceinline__ void store4(const StepArgs& a, long long at, f32x4 y) {
@@ -779,10 +796,11 @@ __global__ __launch_bounds__(256, 2) void palu_step_kernel(const StepArgs a) {
     Wave<L, NB, 1> st;
     st.clear();
     st.query(0, a.q + ((long long)b * a.n_q + head * a.rep + min(lane & 15, a.rep - 1)) * HD, a.qscale < 0.f);
+    const int lead = r.first < r.pblocks ? lead_of(a, r.group, r.rows) : b;    // (uniform)
     st.template pass<false>(
         lo + (each ? 0 : w * step_group(L)), each ? 1 : 4, min(hi, (r.seen + 31) >> 5), r.seen, fabsf(a.qscale), a.dv,
         smem + w * place_bytes<L, NB>(),
-        [&](int blk) __attribute__((always_inline)) { return page_of(a, blk < r.pblocks ? r.lead : b, blk); },
+        [&](int blk) __attribute__((always_inline)) { return page_of(a, blk < r.pblocks ? lead : b, blk); },
         [&](int page, int blk, const char*& k, const char*& v) __attribute__((always_inline)) {
           place_of(a, page, head, blk, k, v);
         });
@@ -970,7 +988,7 @@ __global__ __launch_bounds__(256, 2) void palu_prefix_kernel(const StepArgs a) {
   }
   if (rec < row_wgs && b < a.B) {
     const int gi = last_group(a, b);
-    RowPrefix r{b, 0, 0, 0, 0, {}};
+    RowPrefix r{b, 1, 0, 0, 0, 0, {}};
     const Group g = group_of(a, gi, lone);
     if (g.blocks && b >= g.row && b < g.row + g.rows) {
       int base = bases[gi / per];
@@ -979,7 +997,7 @@ __global__ __launch_bounds__(256, 2) void palu_prefix_kernel(const StepArgs a) {
         base += tiles_of(x) * cut.pieces(x.blocks);
       }
       const int pieces = cut.pieces(g.blocks);
-      r = RowPrefix{g.row, g.blocks, base >= 0 && base + tiles_of(g) * pieces <= a.pre_slots ? pieces : 0, base, b - g.row, {}};
+      r = RowPrefix{g.row, g.rows, g.blocks, base >= 0 && base + tiles_of(g) * pieces <= a.pre_slots ? pieces : 0, base, b - g.row, {}};
     }
     a.rows[b] = r;
   }
@@ -1019,7 +1037,8 @@ __global__ __launch_bounds__(256, 2) void palu_prefix_kernel(const StepArgs a) {
       const int row = col / a.rep;
       st.query(x, a.q + ((long long)(g.row + row) * a.n_q + kvh * a.rep + (col - row * a.rep)) * HD, a.qscale < 0.f);
     }
-    auto page_at = [&](int blk) __attribute__((always_inline)) { return page_of(a, g.row, blk); };
+    const int lead = lead_of(a, g.row, g.rows);
+    auto page_at = [&](int blk) __attribute__((always_inline)) { return page_of(a, lead, blk); };
     auto where = [&](int page, int blk, const char*& k, const char*& v) __attribute__((always_inline)) {
       place_of(a, page, kvh, blk, k, v);
     };

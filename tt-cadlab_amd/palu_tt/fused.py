@@ -489,9 +489,10 @@ def flash_decode_shared(q, k, v, cur_pos_tensor, page_table_tensor, shared_len, 
     """flash_decode over page pools for a batch in which neighbouring rows share a prefix (samples of one prompt, beams, one
     system prompt in front of all): rows cu_groups[i] .. cu_groups[i + 1] - 1 (int32 [n + 1] on the device; None: all rows are
     one group) share their first shared_len[i] positions (int32 [n] on the device). The prefix's whole 32-position blocks are read
-    through the page table of the group's first row (which has to name them, also if that row has ended), once for all rows of
-    the group that see them all; what is behind them through each row's own, whose entries before that are not looked at. Rows of no group stand alone. q, cur_pos_tensor,
-    the pools (row-major tensors, LatentCache or MXCache pairs) and the result as for flash_decode; head_dim_v multiples of 16 (of
+    through the page table of the group's first row, once for all rows of the group that see them all; what is behind them through
+    each row's own, whose entries before that are not looked at. A row that has ended may stay in its group: where the first row's
+    table begins with no page of the pool (PagePools leaves -1), the first row behind it whose table does stands for it, and has to
+    name the prefix's pages. Rows of no group stand alone. q, cur_pos_tensor, the pools (row-major tensors, LatentCache or MXCache pairs) and the result as for flash_decode; head_dim_v multiples of 16 (of
     32 for MXCache). At most 4096 rows. Repeated calls are bit-identical. out must not overlap the inputs; workspace: uint8, of
     palu_flash_decode_shared_workspace_bytes bytes, not shared between calls that may overlap. Forward only."""
     if not (isinstance(q, torch.Tensor) and q.dim() == 4 and q.shape[0] == 1 and q.shape[3] == HEAD_DIM):

@@ -132,6 +132,14 @@ def test_a_long_prefix_beside_many_short_rows(gpu, layout, nq, nkv, prefix):
 
 
 @pytest.mark.parametrize("layout", LAYOUTS)
+def test_a_few_pieces_beside_many_short_rows(gpu, layout):
+    """More items than workgroups, each with seven pieces of the prefix, or up to three, to join."""
+    lens = [2000 + 3 * b for b in range(66)] + [100 + b for b in range(4)] + [30] * 4
+    x = Batch(gpu, layout, lens, 32, 8, 64, 64, [66, 4], [2000, 96], garbage=0.0)
+    x.check(_run(x))
+
+
+@pytest.mark.parametrize("layout", LAYOUTS)
 def test_offsets_past_32_bits(gpu, layout):
     """The same batch over pools whose pages lie past 4 GiB and over ones of three pages."""
     n = 140_000 if layout in ("fp8", "fp4") else 70_000

@@ -573,13 +573,17 @@ __device__ __forceinline__ void place_of(const StepArgs& a, int page, int kvh, i
 constexpr int STEP_LEAST = 16;
 constexpr int STEP_WGS = 512;             // workgroups that the chip holds at once, by the kernel's LDS and registers
 // More items than those (MANY): rows of up to STEP_SHORT own blocks have four KV heads to a workgroup, one to a wave, which adds the
-// prefix's pieces by itself; of longer ones a workgroup has a piece, as ever. Above 1024 items 512 workgroups take piece after
+// prefix's pieces by itself, one after the other, where they are STEP_PIECES at most (a prefix of few rows can be hundreds: 65
+// rows with 8 KV heads, two of them behind 32000 positions in fp8, 69 us if a wave joins its 63 pieces, 35 if a workgroup does; 600 rows
+// with one, two of them behind 65000, 147 and 43; with 4 as the limit 65 rows behind 30000 take 78 us, with 8 or 16 76); of others a
+// workgroup has a piece, as ever. Above 1024 items 512 workgroups take piece after
 // piece, since one that finds no piece holds a place for 3 us to find that out (512 rows of up to 64 positions, 8 KV heads, fp8:
 // 77 -> 18.5 us; 256 of up to 200: 37 -> 19; 256 behind a prefix of 2000: 37 -> 16). Up to there each piece has its own, which
 // balances long rows better (66 rows of up to 4000: 68 us, 78 in such a loop). With 4 blocks as the limit 256 rows of 200 take 27
 // us, with 16 32 rows of up to 1024 with 32 KV heads 46 against 37; with 256 items as the bound 64 rows of up to 250 take 13.8
 // against 11.6.
 constexpr int STEP_SHORT = 8;
+constexpr int STEP_PIECES = 8;
 inline bool step_many(int B, int n_kv) { return (long long)B * n_kv > STEP_WGS; }
 inline int step_slots(int B, int n_kv) { return STEP_WGS + B * n_kv; }         // pieces, at most
 inline int step_grid(int B, int n_kv) { return B * n_kv > 1024 ? STEP_WGS : step_slots(B, n_kv); }
@@ -690,7 +694,7 @@ __device__ __forceinline__ f32x4 load_part4(__amdgpu_buffer_rsrc_t p, int at) {
   return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(p, at * 4, 0, SYSTEM_SCOPE));
 }
 
-// A wave's result (of column tile 0), joined with the prefix's pieces (few, where there are many items) and written: row b's
+// A wave's result (of column tile 0), joined with the prefix's pieces (STEP_PIECES at most) and written: row b's
 // queries of a KV head. A lane has its channels of a piece as it has its own.
 template <int L, int NB>
 __device__ __forceinline__ void store_wave(const StepArgs& a, Wave<L, NB, 1>& st, int b, int head, const RowWork& r) {
@@ -757,10 +761,9 @@ __global__ __launch_bounds__(256, 2) void palu_step_kernel(const StepArgs a) {
     const RowWork r = row(i);
     mine += (float)a.n_kv * (float)(r.end - r.first);
   }
-  auto items_of = [&](const RowWork& r) {   // MANY: four KV heads of a short row to a workgroup, one to a wave
-    const int blocks = r.end - r.first;
-    return MANY && blocks <= STEP_SHORT ? Items{(a.n_kv + 3) / 4, 1} : Items{a.n_kv, blocks};
-  };
+  // MANY: four KV heads of a short row to a workgroup, one to a wave
+  auto to_waves = [&](const RowWork& r) { return MANY && r.end - r.first <= STEP_SHORT && r.pieces <= STEP_PIECES; };
+  auto items_of = [&](const RowWork& r) { return to_waves(r) ? Items{(a.n_kv + 3) / 4, 1} : Items{a.n_kv, r.end - r.first}; };
   const bool fit = a.B * a.n_kv <= STEP_WGS * 3 / 4;
   const Cut cut = cut_items(wg_sum(mine, reinterpret_cast<float*>(scan)), r0, r1, STEP_WGS, STEP_LEAST, fit, scan,
                             [&](int i) { return items_of(row(i)); });
@@ -788,7 +791,7 @@ __global__ __launch_bounds__(256, 2) void palu_step_kernel(const StepArgs a) {
     __syncthreads();
     const int b = uniform(found[0]), in = uniform(found[1]);
     const RowWork r = uniform(found_row);
-    const bool each = MANY && r.end - r.first <= STEP_SHORT;    // (uniform)
+    const bool each = to_waves(r);          // (uniform)
     const int chunks = each ? 1 : uniform(cut.pieces(r.end - r.first)), head0 = each ? 4 * in : uniform(in / chunks);
     const int chunk = each ? 0 : in - head0 * chunks, wg0 = want - chunk;      // wg0: the item's first piece
     const int head = each ? min(head0 + w, a.n_kv - 1) : head0;                // this wave's

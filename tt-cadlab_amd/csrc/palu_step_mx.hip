@@ -136,7 +136,9 @@ extern "C" int palu_flash_decode_shared(const void* q, const void* k_pages, cons
   // Where all that the tables can name is little, each row reads its prefix by itself, by its group's table: 64 MiB or less take less
   // than a second launch and its join (both launches, and one: three rows of fp8 behind 100 positions 14.2 us, 7.8, behind 8000
   // 19.1, 16.0; 64 rows of tiles behind 128 positions, 67 MB, 20.3, 12.9; 16 rows over 71 MB, the prefixes nearly all of it, 18.7,
-  // 21.2; 30 rows of fp4 over 65 MB 19.2, 19.2).
+  // 21.2; 30 rows of fp4 over 65 MB 19.2, 19.2). Those are tables as wide as their longest row. The host knows the width and not what
+  // is shared: under a table for 32768 positions short prefixes take both launches (the three rows behind 100 positions 13.7 us, 7.6
+  // under one of 128; 16 rows with 8 KV heads behind 700 17.1, 11.9).
   const long long most = (long long)batch * n_kv * (a.capacity / 32) * (a.k_blk + a.v_blk);
   if (most > (64LL << 20))
     a.rows = reinterpret_cast<RowPrefix*>(a.pre + (long long)a.pre_slots * a.pre_cols * (head_dim_v + 2));

@@ -294,27 +294,28 @@ class MXCache:
         codes, scales = mx_quantize(rows, fmt)
         if fmt == "fp4":
             codes = codes[..., 0::2] | (codes[..., 1::2] << 4)
-        nblk, nb = S // BLOCK, w // 32
+        nblk, nb, n = S // BLOCK, w // 32, 2 if fmt == "fp8" else 1
         if role == "k":
-            x = codes.reshape(B, G, nblk, 4, 2, 4, nb, -1, 16).permute(0, 1, 2, 4, 7, 6, 3, 5, 8)
+            x = codes.reshape(B, G, nblk, 4, 2, 4, nb, n, 16).permute(0, 1, 2, 4, 7, 6, 3, 5, 8)
             s = scales.reshape(B, G, nblk, 4, 2, 4, nb).permute(0, 1, 2, 6, 3, 5, 4)
         else:
-            x = codes.reshape(B, G, nblk, 4, 8, nb, 16, -1).permute(0, 1, 2, 5, 3, 6, 4, 7)
+            x = codes.reshape(B, G, nblk, 4, 8, nb, 16, n).permute(0, 1, 2, 5, 3, 6, 4, 7)
             s = scales.reshape(B, G, nblk, BLOCK, nb).transpose(3, 4)
-        return MXCache(torch.cat([x.reshape(B, G, nblk, -1), s.reshape(B, G, nblk, -1)], -1).contiguous(), role, fmt, w)
+        return MXCache(torch.cat([x.flatten(3), s.flatten(3)], -1).contiguous(), role, fmt, w)
 
     def parts(self) -> Tuple[torch.Tensor, torch.Tensor]:
         """(codes [B, n_groups, max_seq, width], scale bytes [B, n_groups, max_seq, width / 32]), uint8."""
         B, G, S, w = self.shape
-        nblk, nb, size = S // BLOCK, w // 32, (32 if self.fmt == "fp8" else 16) * w
+        nblk, nb, n = S // BLOCK, w // 32, 2 if self.fmt == "fp8" else 1
+        size = 16 * n * w
         x, s = self.data[..., :size], self.data[..., size:]
         if self.role == "k":
-            x = x.reshape(B, G, nblk, 2, -1, nb, 4, 4, 16).permute(0, 1, 2, 6, 3, 7, 5, 4, 8)
+            x = x.reshape(B, G, nblk, 2, n, nb, 4, 4, 16).permute(0, 1, 2, 6, 3, 7, 5, 4, 8)
             s = s.reshape(B, G, nblk, nb, 4, 4, 2).permute(0, 1, 2, 4, 6, 5, 3)
         else:
-            x = x.reshape(B, G, nblk, nb, 4, 16, 8, -1).permute(0, 1, 2, 4, 6, 3, 5, 7)
+            x = x.reshape(B, G, nblk, nb, 4, 16, 8, n).permute(0, 1, 2, 4, 6, 3, 5, 7)
             s = s.reshape(B, G, nblk, nb, BLOCK).transpose(3, 4)
-        x = x.reshape(B, G, S, -1)
+        x = x.reshape(B, G, S, n * w // 2)
         if self.fmt == "fp4":
             x = torch.stack([x & 15, x >> 4], -1).flatten(-2)
         return x, s.reshape(B, G, S, nb)

@@ -765,7 +765,8 @@ def paged_update_cache(cache, new_rows: torch.Tensor, update_idxs_tensor: torch.
     """Latent append (ttnn.experimental.paged_update_cache on a latent cache, attention.py:622-623):
     cache[b, g, update_idxs[b], :] = new_rows[..., b, g, :] for every b with 0 <= idx < S. ``cache`` is a
     [B, G, S, width] bf16 tensor, a LatentCache or an MXCache (the rows are quantised as they are written). With ``page_table`` [B, max_pages] int32 the cache is a
-    page pool [n_pages, G, page_size, width] and row b goes to page page_table[b, idx // page_size]."""
+    page pool [n_pages, G, page_size, width] and row b goes to page page_table[b, idx // page_size]. Rows of one call must not go to the
+    same place of a page that they share (what is held there then is of either, an MXCache's values perhaps under the other's scale)."""
     dev = cache.device
     if isinstance(cache, GroupedLatentCache):
         if page_table is not None:
